@@ -35,12 +35,17 @@ EXPORTED_SYMBOLS = (
     "fg_spmm_csr_f32_general", "fg_sddmm_coo_f32_general", "fg_next_launch_options",
     "fg_spmm_dds_plan_create", "fg_spmm_dds_plan_destroy", "fg_spmm_dds_plan_num_launches",
     "fg_spmm_dds_plan_status", "fg_spmm_dds_f32", "fg_sddmm_status",
+    "fg_embedding_lookup", "fg_embedding_grad_workspace_bytes", "fg_embedding_grad",
+    "fg_softmax_xent_workspace_bytes", "fg_softmax_xent", "fg_softmax_xent_grad",
+    "fg_gradient_clip_workspace_bytes", "fg_gradient_clip",
 )
 
 LAUNCH_PROGRAMMATIC, SPMM_GIANT_ROWS_ONLY, SPMM_SKIP_GIANT_ROWS, SDDMM_TMA_STAGING = 1, 2, 4, 8  # fg_launch_flags
 SPMM_LONG_ROWS_ONLY, SPMM_SKIP_LONG_ROWS, SDDMM_ROW_REGISTERS = 16, 32, 64
 MSG_OPS = ("mul", "add", "sub", "div", "copy_lhs", "copy_rhs")    # enum fg_msg_op
 REDUCE_OPS = ("sum", "max", "min")                                # enum fg_reduce_op
+DTYPES = ("float32", "bfloat16", "float16")                       # enum fg_dtype
+INDEX_TYPES = ("int32", "int64")                                  # enum fg_index_type
 
 
 def load():
@@ -89,6 +94,24 @@ def load():
     lib.fg_peer_barrier.argtypes = [ctypes.POINTER(c_void), i32, i32, ctypes.c_uint32, c_void,
                                     i64, i32, c_void]
     lib.fg_gather_probe.argtypes = [c_void, i64, i32, i64, i32, c_void, i32, c_void]
+    f32, f64 = ctypes.c_float, ctypes.c_double
+    lib.fg_embedding_lookup.argtypes = [c_void, i32, i64, i64, c_void, i32, i64, i64, f32, c_void,
+                                        i64, c_void, i32, c_void]
+    lib.fg_embedding_grad_workspace_bytes.argtypes = [i64, i64, i64]
+    lib.fg_embedding_grad_workspace_bytes.restype = i64
+    lib.fg_embedding_grad.argtypes = [c_void, i32, i64, c_void, i32, i64, i64, i64, f32, i64, i32,
+                                      c_void, c_void, i64, c_void, i32, c_void]
+    lib.fg_softmax_xent_workspace_bytes.argtypes = [i32, i64, i64, i64, i32]
+    lib.fg_softmax_xent_workspace_bytes.restype = i64
+    lib.fg_softmax_xent.argtypes = [c_void, i64, c_void, i64, i32, c_void, i32, i64, i64, i64, f32,
+                                    i64, c_void, c_void, c_void, i64, c_void, i32, c_void]
+    lib.fg_softmax_xent_grad.argtypes = [c_void, c_void, i64, c_void, i64, i32, c_void, i32, i64,
+                                         i64, i64, f32, i64, c_void, c_void, c_void, c_void, i64,
+                                         c_void, i32, c_void]
+    lib.fg_gradient_clip_workspace_bytes.argtypes = [i32]
+    lib.fg_gradient_clip_workspace_bytes.restype = i64
+    lib.fg_gradient_clip.argtypes = [c_void, c_void, c_void, c_void, i32, i32, f64, f64, c_void,
+                                     c_void, i64, i32, c_void]
     lib.fg_shard_rows_by_nnz.argtypes = [c_i32p, i64, i32, c_i64p]
     lib.fg_shard_edges.argtypes = [i64, i32, c_i64p]
     _lib = lib

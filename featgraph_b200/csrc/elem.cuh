@@ -1,0 +1,103 @@
+// Element and index types of the training operators (lookup, cross entropy, clip): vector
+// loads and stores of float32 / bfloat16 / float16 rows as fp32 values, index loads, and the
+// dispatch over the types the C ABI names (fg_dtype, fg_index_type).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace fg {
+
+inline size_t dtype_size(int32_t dtype) { return dtype == FG_FLOAT32 ? 4 : 2; }
+inline bool dtype_known(int32_t dtype) { return dtype >= FG_FLOAT32 && dtype <= FG_FLOAT16; }
+inline bool index_known(int32_t t) { return t == FG_INDEX_INT32 || t == FG_INDEX_INT64; }
+
+// The widest of 16, 8, 4 and 2 bytes that divides every listed address, pitch and row length.
+inline int common_vector_bytes(std::initializer_list<uint64_t> things) {
+  uint64_t all = 16;
+  for (uint64_t t : things) all |= t;
+  return (int)(all & (~all + 1));
+}
+
+#ifdef __CUDACC__
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v);
+template <>
+__device__ __forceinline__ float to_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+
+// Round to nearest even: the one rounding of a result to its type.
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+// N consecutive elements as one memory access of N * sizeof(T) = 2, 4, 8 or 16 bytes.
+template <int BYTES>
+struct RawVec;
+template <>
+struct RawVec<16> { using type = uint4; };
+template <>
+struct RawVec<8> { using type = uint2; };
+template <>
+struct RawVec<4> { using type = unsigned; };
+template <>
+struct RawVec<2> { using type = unsigned short; };
+
+template <typename T, int N>
+struct alignas(N * sizeof(T)) Vec {
+  using Raw = typename RawVec<N * (int)sizeof(T)>::type;
+  T v[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> load_vec(const T* p) {
+  using V = Vec<T, N>;
+  typename V::Raw r = __ldg(reinterpret_cast<const typename V::Raw*>(p));
+  V out;
+  memcpy(&out, &r, sizeof(out));
+  return out;
+}
+// Read-once data: evicted first.
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> load_vec_stream(const T* p) {
+  using V = Vec<T, N>;
+  typename V::Raw r = __ldcs(reinterpret_cast<const typename V::Raw*>(p));
+  V out;
+  memcpy(&out, &r, sizeof(out));
+  return out;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& v) {
+  typename Vec<T, N>::Raw r;
+  memcpy(&r, &v, sizeof(r));
+  *reinterpret_cast<typename Vec<T, N>::Raw*>(p) = r;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_vec_stream(T* p, const Vec<T, N>& v) {
+  typename Vec<T, N>::Raw r;
+  memcpy(&r, &v, sizeof(r));
+  __stcs(reinterpret_cast<typename Vec<T, N>::Raw*>(p), r);
+}
+
+#endif  // __CUDACC__
+
+// CALL(T) for the element type `dtype`, already checked with dtype_known.
+#define FG_DISPATCH_DTYPE(dtype, CALL)          \
+  switch (dtype) {                              \
+    case FG_FLOAT32: CALL(float); break;        \
+    case FG_BFLOAT16: CALL(__nv_bfloat16); break; \
+    default: CALL(__half); break;               \
+  }
+
+}  // namespace fg

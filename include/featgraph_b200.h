@@ -349,6 +349,89 @@ int fg_sddmm_num_launches(int64_t nnz, int32_t feat_len, int32_t num_heads);
 int fg_sddmm_describe(int64_t nnz, int32_t feat_len, int32_t num_heads,
                       char* buf, int64_t buf_len);
 
+/* ------------------------------------------------------ training operators -- */
+
+/* What a training step runs next to the two sparse kernels: the vertex embedding table
+ * that feeds the SpMM, the loss over all vertices (or classes) that reads its output, and
+ * the bound on the gradients before the optimiser.  The reference has none of them (its
+ * README.md:6 leaves the layers around its kernels to the caller).
+ *
+ * Rows are row-major with the last dimension contiguous; a *_ld is the distance between
+ * two rows in elements.  All calls are asynchronous on `stream`, allocate nothing and keep
+ * nothing between calls; the workspace is scratch of the call's own, so two calls that may
+ * overlap need two of them.  status_dev is an int32 that the caller zeroed: a kernel that
+ * meets an id or a label out of range sets it (FG_STATUS_BAD_INDEX) and reads nothing
+ * there. */
+enum fg_dtype { FG_FLOAT32 = 0, FG_BFLOAT16 = 1, FG_FLOAT16 = 2 };
+enum fg_index_type { FG_INDEX_INT32 = 0, FG_INDEX_INT64 = 1 };
+enum { FG_STATUS_BAD_INDEX = 1 };
+
+/* out[i, :] = scale * table[ids[i], :] with one rounding to dtype; table is (n_vertices,
+ * feat_len).  A row whose id is out of range is NaN.  ids that repeat, in any order. */
+int fg_embedding_lookup(const void* table_dev, int32_t dtype, int64_t table_ld,
+                        int64_t n_vertices, const void* ids_dev, int32_t index_type,
+                        int64_t n_ids, int64_t feat_len, float scale, void* out_dev,
+                        int64_t out_ld, int32_t* status_dev, int32_t device, void* stream);
+
+/* The gradient of the table: grad[v, :] = scale * sum of out_grad[i, :] over the i with
+ * ids[i] = v, for every v < n_vertices (zero where no id is v, and for v = padding_id;
+ * padding_id < 0: none).  The ids are sorted, stably, on the device and the rows of one
+ * vertex summed in fp32 in an order that only the ids fix: the same call gives the same
+ * bits.  accumulate != 0 adds onto what grad holds (and leaves the rows that no id names
+ * as they were) instead of overwriting it.  grad is (n_vertices, feat_len) without gaps.
+ * An id out of range adds nothing. */
+int64_t fg_embedding_grad_workspace_bytes(int64_t n_ids, int64_t n_vertices, int64_t feat_len);
+int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_t out_grad_ld,
+                      const void* ids_dev, int32_t index_type, int64_t n_ids,
+                      int64_t n_vertices, int64_t feat_len, float scale, int64_t padding_id,
+                      int32_t accumulate, void* grad_dev, void* workspace_dev,
+                      int64_t workspace_bytes, int32_t* status_dev, int32_t device,
+                      void* stream);
+
+/* Softmax cross entropy of n samples over `vocab` vertices or classes, without keeping the
+ * (n, vocab) logits z = scale * feat @ weight^T; feat is (n, feat_len), weight (vocab,
+ * feat_len):
+ *   lse[t] = log sum_v exp z[t, v],   loss[t] = lse[t] - z[t, labels[t]],
+ * both fp32.  loss is 0 where labels[t] = ignore_index (lse is still that row's), NaN where
+ * a label is out of range.  An infinite logit makes its row NaN, except -inf beside a
+ * finite one. */
+int64_t fg_softmax_xent_workspace_bytes(int32_t dtype, int64_t n, int64_t vocab,
+                                        int64_t feat_len, int32_t with_grad);
+int fg_softmax_xent(const void* feat_dev, int64_t feat_ld, const void* weight_dev,
+                    int64_t weight_ld, int32_t dtype, const void* labels_dev,
+                    int32_t index_type, int64_t n, int64_t vocab, int64_t feat_len, float scale,
+                    int64_t ignore_index, float* loss_dev, float* lse_dev, void* workspace_dev,
+                    int64_t workspace_bytes, int32_t* status_dev, int32_t device, void* stream);
+
+/* Its gradients, from the gradient of the losses and the lse of the forward call, with the
+ * logits computed again piece by piece of the vocabulary:
+ *   dz[t, v] = scale * loss_grad[t] * (exp(z[t, v] - lse[t]) - [v = labels[t]]),
+ *   feat_grad = dz @ weight,  weight_grad = dz^T @ feat,
+ * both in dtype, without gaps, every element overwritten; either may be NULL.  A row whose
+ * label is ignore_index (or out of range) has dz = 0 whatever feat, lse and loss_grad hold
+ * there. */
+int fg_softmax_xent_grad(const float* loss_grad_dev, const void* feat_dev, int64_t feat_ld,
+                         const void* weight_dev, int64_t weight_ld, int32_t dtype,
+                         const void* labels_dev, int32_t index_type, int64_t n, int64_t vocab,
+                         int64_t feat_len, float scale, int64_t ignore_index,
+                         const float* lse_dev, void* feat_grad_dev, void* weight_grad_dev,
+                         void* workspace_dev, int64_t workspace_bytes, int32_t* status_dev,
+                         int32_t device, void* stream);
+
+/* Global norm of n_tensors gradients (each of its own dtype and element count) and clipping:
+ *   norm = sqrt of the sum of all squares, or, with max_abs_norm != 0, the largest magnitude;
+ *   out_k = grad_k * min(1, max_norm / (norm + eps)),
+ * the norm summed in fp64 from fp32 pieces in a fixed order.  outs[k] may be grads[k] (in
+ * place: then nothing is written when nothing has to be scaled), else the two do not
+ * overlap.  The four arrays are host memory and are read before the call returns.  A NaN
+ * norm makes every output NaN, an infinite one scales by zero, max_norm = +inf scales by 1. */
+int64_t fg_gradient_clip_workspace_bytes(int32_t n_tensors);
+int fg_gradient_clip(const void* const* grads_host_array, void* const* outs_host_array,
+                     const int64_t* sizes_host_array, const int32_t* dtypes_host_array,
+                     int32_t n_tensors, int32_t max_abs_norm, double max_norm, double eps,
+                     float* norm_dev, void* workspace_dev, int64_t workspace_bytes,
+                     int32_t device, void* stream);
+
 /* ------------------------------------------------- multi-GPU partitioning -- */
 
 /* Splits the rows of a CSR matrix into `world` contiguous blocks holding about
