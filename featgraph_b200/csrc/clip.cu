@@ -215,16 +215,16 @@ extern "C" int fg_gradient_clip(const void* const* grads_host_array, void* const
          ((uintptr_t)grads_host_array[k] | (uintptr_t)outs_host_array[k]) % es != 0))
       return fail(FG_ERR_INVALID_ARGUMENT, "tensor %d: null or misaligned pointer", (int)k);
   }
-  DeviceGuard guard(device);
-  FG_CUDA_TRY(guard.status);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  double* partial = static_cast<double*>(workspace_dev);
   int64_t all_chunks = 0;
   for (int32_t k = 0; k < n_tensors; ++k)
     all_chunks += (sizes_host_array[k] + kClipChunk - 1) / kClipChunk;
   if (all_chunks > INT32_MAX)
     return fail(FG_ERR_UNSUPPORTED, "%lld chunks of %d elements are too many",
                 (long long)all_chunks, kClipChunk);
+  DeviceGuard guard(device);
+  FG_CUDA_TRY(guard.status);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  double* partial = static_cast<double*>(workspace_dev);
   // the tensors from `first` on that one launch can name; returns the first one left
   auto fill = [&](int32_t first, ClipTensors& t, int& grid) -> int32_t {
     t.n = 0;
