@@ -124,7 +124,9 @@ class _TrainingOp(object):
         if code:
             self._status.zero_()
             torch.cuda.synchronize(self._device)
-            raise _lib.FeatGraphError(code, "%s met an index out of range" % type(self).__name__)
+            raise _lib.FeatGraphError(code, "%s %s" % (
+                type(self).__name__, "met an index out of range" if code == 1
+                else "gave up a bounded wait: its results are not to be used"))
         return 0
 
     @property
