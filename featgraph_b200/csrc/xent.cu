@@ -58,19 +58,22 @@ constexpr int kTileRows = 128;
 constexpr int kTileBytes = kTileRows * 128;   // 128 rows of 64 16-bit elements
 constexpr int kMmaThreads = 384;              // loads, mma, TMEM, one idle; then 8 epilogue warps
 constexpr int kEpilogueWarp = 4;
-constexpr int kMaxStages = 8;
+constexpr int kMaxSlots = 14;
+constexpr int kMaxBuffers = 3;
 constexpr int kMaxResidentTiles = 4;          // 64-element tiles of a row that stay in shared memory
-constexpr int kSharedBudget = 12 * kTileBytes;
 
 struct MmaArgs {
   int64_t n_rows, n_cols;
   int kb;                 // 64-element tiles of a row (of one piece of it, for float32)
-  int row_tiles, splits, steps, steps_per_split, stages;
+  int row_tiles, splits, steps, steps_per_split;
+  int chunks;             // pieces of at most kChunkTiles tiles that the results are cut into
+  int slots;              // of the ring in shared memory
+  int buffers;            // S tiles in TMEM
   int feat_len, out_cols; // out_cols: feat_len rounded up to 16
   int negate;             // a negative scale: |scale| with -A
   float logit_scale;      // |scale| * log2(e)
   const float* unscale;   // float32: what undoes the operands' scaling; else null
-  float2* stats;          // loss: (maximum, sum) per row, split and epilogue group, base 2
+  float2* stats;          // loss: (maximum, sum) per row, split and half of a step, base 2
   const float* row_bias;  // feat_grad: log2(hot) - lse * log2(e) of a row, -inf: takes no part
   const int32_t* row_label;
   const float* col_bias;  // weight_grad: the same of a column, plus log2 |weight|
@@ -84,12 +87,20 @@ struct MmaArgs {
   int32_t* status;
 };
 
-template <int MODE, typename T>
+// kStream: the rows do not stay in shared memory but come along with every step (wide rows).
+template <int MODE, typename T, bool STREAM>
 struct MmaShape {
   static constexpr bool kSplit = sizeof(T) == 4;  // float32 as two fp16 pieces, three products
   static constexpr int kCols = MODE == kLoss ? 256 : 128;
-  static constexpr int kOutAt = 256;              // TMEM columns: S, S, then the accumulators
-  static constexpr int kLowAt = 384;              // and float32's low pieces of P
+  static constexpr int kChunkTiles = kSplit ? 2 : 4;
+  // tiles of 16 KB that a slot of the ring holds: a tile of the streamed operand, with one of
+  // the rows where these are streamed too (or, for the second product, two of the first)
+  static constexpr int kSlotTiles = MODE == kLoss ? (STREAM ? 3 : 2) : (STREAM ? 2 : 1);
+  // float32: steps after which the accumulators are added up in registers.  tcgen05.mma adds
+  // to fp32 by cutting, about 2^-26 of the sum each time and always towards zero: 64 of these
+  // (eight a step) are 2^-20, several thousand were 1.1e-5.
+  static constexpr int kSegment = kSplit ? 8 : 1 << 30;
+  static constexpr int kLowOut = 128;             // the accumulators of float32's low products
 };
 
 // Two probabilities in 16 bits each, the first in the low half.
@@ -108,22 +119,22 @@ __device__ __forceinline__ float2 unpack_half2(uint32_t r) {
   return __half22float2(h);
 }
 
-// P in 16 bits to TMEM: 32 columns of S become 16.  Rounding it to the operands' type (half a
-// step, 2^-9 for bfloat16 and 2^-12 for float16) is what the second product's rate costs;
-// float32 keeps a second piece, together 2^-22.
-template <int MODE, typename T>
-__device__ __forceinline__ void store_p(uint32_t s_at, uint32_t low_at, int chunk, const float (&p)[32]) {
+// 32 columns of S become 32 k of P in 16 of the same columns.  Rounding P to the operands' type
+// (half a step, 2^-9 for bfloat16 and 2^-12 for float16) is what the second product's rate
+// costs; float32 keeps a second piece in the other 16 columns, together 2^-22.
+template <typename T>
+__device__ __forceinline__ void store_p(uint32_t at, const float (&p)[32]) {
   uint32_t r[16];
 #pragma unroll
   for (int k = 0; k < 16; ++k) r[k] = pack2<T>(p[2 * k], p[2 * k + 1]);
-  tc::tmem_store16(s_at + chunk * 16, r);
-  if (MmaShape<MODE, T>::kSplit) {
+  tc::tmem_store16(at, r);
+  if (sizeof(T) == 4) {
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
       const float2 hi = unpack_half2(r[k]);
       r[k] = pack2<T>(p[2 * k] - hi.x, p[2 * k + 1] - hi.y);
     }
-    tc::tmem_store16(low_at + chunk * 16, r);
+    tc::tmem_store16(at + 16, r);
   }
 }
 
@@ -132,40 +143,97 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
   return __all_sync(0xffffffffu, tc::bar_wait(bar, parity));
 }
 
+// A place in a ring of `n` slots or buffers and the parity of its current round.
+struct Place {
+  uint32_t at = 0, parity = 0;
+  __device__ __forceinline__ void next(uint32_t n) {
+    if (++at == n) {
+      at = 0;
+      parity ^= 1;
+    }
+  }
+};
+
+// What one item of a CTA's work is: a tile of the rows, a range of steps over the streamed
+// operand, and (for the gradients of wide rows) a piece of the results' columns.  Row tiles run
+// fastest: CTAs beside each other stream the same part.
+struct Item {
+  int row_tile, split, chunk, first, steps;
+};
+__device__ __forceinline__ Item item_at(const MmaArgs& a, int i) {
+  Item it;
+  it.row_tile = i % a.row_tiles;
+  const int rest = i / a.row_tiles;
+  it.chunk = rest % a.chunks;
+  it.split = rest / a.chunks;
+  it.first = it.split * a.steps_per_split;
+  it.steps = min(a.steps_per_split, a.steps - it.first);
+  return it;
+}
+
+// Stores 16 columns of one row of the results.
 template <int MODE, typename T>
+__device__ __forceinline__ void store_out(const MmaArgs& a, const Item& item, int64_t row, int c,
+                                          const float (&v)[16], float factor, bool live) {
+  if (c >= a.out_cols) return;
+  if (a.splits > 1) {  // a partial sum, rows out_cols apart
+    float* to = a.partial + ((int64_t)item.split * a.n_rows + row) * a.out_cols + c;
+#pragma unroll
+    for (int k = 0; k < 16; k += 4)
+      *reinterpret_cast<float4*>(to + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+    return;
+  }
+  T* to = static_cast<T*>(a.out) + row * a.feat_len + c;
+  constexpr int N = 16 / sizeof(T);
+  if (a.feat_len % N == 0 && ((uintptr_t)a.out & 15) == 0) {
+#pragma unroll
+    for (int k = 0; k < 16; k += N) {
+      if (c + k >= a.feat_len) break;
+      Vec<T, N> piece;
+#pragma unroll
+      for (int i = 0; i < N; ++i) piece.v[i] = from_float<T>(live ? v[k + i] * factor : 0.f);
+      store_vec<T, N>(to + k, piece);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (c + k < a.feat_len) to[k] = from_float<T>(live ? v[k] * factor : 0.f);
+  }
+}
+
+template <int MODE, typename T, bool STREAM>
 __global__ void __launch_bounds__(kMmaThreads, 1)
 xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
                 const __grid_constant__ CUtensorMap col_map, const __grid_constant__ MmaArgs a) {
-  using Shape = MmaShape<MODE, T>;
+  using Shape = MmaShape<MODE, T, STREAM>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kPlanes = Shape::kSplit ? 2 : 1;
+  constexpr uint32_t kSlotBytes = Shape::kSlotTiles * kTileBytes;
   extern __shared__ uint8_t raw_smem[];
-  __shared__ uint64_t bars[2 * kMaxStages + 9];
+  __shared__ uint64_t bars[2 * kMaxSlots + 2 * kMaxBuffers + 5];
   __shared__ uint32_t tmem_where;
   __shared__ __align__(16) float col_bias_s[MODE == kWeightGrad ? 8 : 1][128];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem = (smem_u32(raw_smem) + 1023) & ~1023u;
-  const int planes = Shape::kSplit ? 2 : 1;
-  const int tiles = a.kb * planes;                       // tiles of a resident row
-  const int stage_tiles = MODE == kLoss ? 1 : tiles;     // tiles of a stage
-  const uint32_t stage_bytes = (uint32_t)stage_tiles * (Shape::kCols / 128) * kTileBytes;
-  const uint32_t rows_at = smem, ring_at = smem + tiles * kTileBytes;
-  const uint32_t full = smem_u32(bars), empty = full + 8 * kMaxStages;
-  const uint32_t rows_full = empty + 8 * kMaxStages, rows_empty = rows_full + 8;
-  const uint32_t s_full = rows_full + 16, s_done = rows_full + 32;   // two each
-  const uint32_t out_full = rows_full + 48, out_empty = rows_full + 56, drained = rows_full + 64;
+  const int tiles = a.kb * kPlanes;                      // tiles of a whole row
+  const uint32_t rows_at = smem, ring_at = smem + (STREAM ? 0 : tiles * kTileBytes);
+  const uint32_t full = smem_u32(bars), empty = full + 8 * kMaxSlots;
+  const uint32_t s_full = empty + 8 * kMaxSlots, s_done = s_full + 8 * kMaxBuffers;
+  const uint32_t rows_full = s_done + 8 * kMaxBuffers, rows_empty = rows_full + 8;
+  const uint32_t out_full = rows_full + 16, out_empty = rows_full + 24, drained = rows_full + 32;
 
   if (threadIdx.x == 0) {
-    for (int k = 0; k < a.stages; ++k) {
+    for (int k = 0; k < a.slots; ++k) {
       tc::bar_init(full + 8 * k, 1);
       tc::bar_init(empty + 8 * k, 1);
     }
+    for (int k = 0; k < a.buffers; ++k) {
+      tc::bar_init(s_full + 8 * k, 1);
+      tc::bar_init(s_done + 8 * k, MODE == kLoss ? 256 : 128);
+    }
     tc::bar_init(rows_full, 1);
     tc::bar_init(rows_empty, 1);
-    for (int k = 0; k < 2; ++k) {
-      tc::bar_init(s_full + 8 * k, 1);
-      tc::bar_init(s_done + 8 * k, 128);
-    }
     tc::bar_init(out_full, 1);
     tc::bar_init(out_empty, 256);
     tc::bar_init(drained, 1);
@@ -177,229 +245,386 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  const uint32_t tmem = tmem_where;
-  const int items = a.row_tiles * a.splits;
-  // item = (split, row tile), row tiles first: CTAs beside each other stream the same part
-  auto steps_of = [&](int item, int& first) {
-    first = item / a.row_tiles * a.steps_per_split;
-    return min(a.steps_per_split, a.steps - first);
-  };
+  // all 512 columns are this CTA's: they start at address 0, and the S tiles there
+  constexpr uint32_t tmem = 0;
+  const uint32_t out_at = tmem + a.buffers * Shape::kCols;
+  const int items = a.row_tiles * a.splits * a.chunks;
 
   if (warp == 0) {
     if (lane == 0) {
-      uint32_t stage = 0, it = 0;
-      bool ok = true;
-      for (int item = blockIdx.x; ok && item < items; item += gridDim.x, ++it) {
-        int first;
-        const int n = steps_of(item, first);
-        if (it > 0 && !(ok = tc::bar_wait(rows_empty, (it - 1) & 1))) break;
-        tc::bar_expect(rows_full, tiles * kTileBytes);
-        for (int q = 0; q < tiles; ++q)
-          tc::load_tile(rows_at + q * kTileBytes, &row_map, q * 64, item % a.row_tiles * kTileRows,
-                        rows_full);
-        for (int j = 0; ok && j < n; ++j) {
-          for (int q = 0; q < tiles; q += stage_tiles, ++stage) {
-            const uint32_t slot = stage % a.stages, round = stage / a.stages;
-            if (round > 0 && !(ok = tc::bar_wait(empty + 8 * slot, (round - 1) & 1))) break;
-            tc::bar_expect(full + 8 * slot, stage_bytes);
-            for (int k = 0; k < stage_tiles; ++k)
-              tc::load_tile(ring_at + slot * stage_bytes + k * kTileBytes, &col_map, (q + k) * 64,
-                            (first + j) * Shape::kCols, full + 8 * slot);
+      Place slot;
+      uint32_t loaded = 0, it = 0;
+      bool ok = tmem_where == tmem;
+      // the next slot, free, with `n` tiles announced; 0 if the wait expired
+      auto next_slot = [&](int n) -> uint32_t {
+        if (loaded >= (uint32_t)a.slots && !tc::bar_wait(empty + 8 * slot.at, slot.parity ^ 1)) {
+          ok = false;
+          return 0;
+        }
+        tc::bar_expect(full + 8 * slot.at, n * kTileBytes);
+        return ring_at + slot.at * kSlotBytes;
+      };
+      auto load = [&](uint32_t to, const CUtensorMap* map, int tile, int row) {
+        tc::load_tile(to, map, tile * 64, row, full + 8 * slot.at);
+      };
+      auto loaded_one = [&]() {
+        slot.next(a.slots);
+        ++loaded;
+      };
+      for (int i = blockIdx.x; ok && i < items; i += gridDim.x, ++it) {
+        const Item item = item_at(a, i);
+        const int row0 = item.row_tile * kTileRows;
+        if (!STREAM) {
+          if (it > 0 && !(ok = tc::bar_wait(rows_empty, (it - 1) & 1))) break;
+          tc::bar_expect(rows_full, tiles * kTileBytes);
+          for (int q = 0; q < tiles; ++q)
+            tc::load_tile(rows_at + q * kTileBytes, &row_map, q * 64, row0, rows_full);
+          for (int j = 0; ok && j < item.steps; ++j)
+            for (int q = 0; q < tiles; ++q) {
+              const uint32_t to = next_slot(Shape::kCols / 128);
+              if (!ok) break;
+              load(to, &col_map, q, (item.first + j) * Shape::kCols);
+              loaded_one();
+            }
+        } else {
+          // in the order in which the products below take them
+          auto load_s = [&](int j) {
+            for (int kb = 0; ok && kb < a.kb; ++kb)
+              for (int u = 0; u < (Shape::kSplit ? 3 : 1); ++u) {
+                const uint32_t to = next_slot(1 + Shape::kCols / 128);
+                if (!ok) break;
+                load(to, &row_map, u == 1 ? a.kb + kb : kb, row0);
+                load(to + kTileBytes, &col_map, u == 2 ? a.kb + kb : kb,
+                     (item.first + j) * Shape::kCols);
+                loaded_one();
+              }
+          };
+          auto load_o = [&](int j) {
+            const int t0 = item.chunk * Shape::kChunkTiles, t1 = min(a.kb, t0 + Shape::kChunkTiles);
+            for (int plane = 0; ok && plane < kPlanes; ++plane)
+              for (int t = t0; ok && t < t1; t += 2) {
+                const uint32_t to = next_slot(min(2, t1 - t));
+                if (!ok) break;
+                for (int k = 0; k < min(2, t1 - t); ++k)
+                  load(to + k * kTileBytes, &col_map, plane * a.kb + t + k,
+                       (item.first + j) * Shape::kCols);
+                loaded_one();
+              }
+          };
+          if (MODE == kLoss) {
+            for (int j = 0; ok && j < item.steps; ++j) load_s(j);
+          } else {
+            const int ahead = min(a.buffers - 1, item.steps);
+            for (int j = 0; ok && j < ahead; ++j) load_s(j);
+            for (int j = 0; ok && j < item.steps; ++j) {
+              if (j + ahead < item.steps) load_s(j + ahead);
+              if (ok) load_o(j);
+            }
           }
         }
       }
       if (!ok) {  // give up only once nothing is in flight into this CTA's shared memory
         *a.status = FG_STATUS_WAIT_EXPIRED;
-        tc::bar_wait(rows_full, it & 1);
-        for (uint32_t k = stage > (uint32_t)a.stages ? stage - a.stages : 0; k < stage; ++k)
-          tc::bar_wait(full + 8 * (k % a.stages), (k / a.stages) & 1);
+        if (!STREAM) tc::bar_wait(rows_full, it & 1);
+        for (uint32_t k = 0; k < min(loaded, (uint32_t)a.slots); ++k) {
+          // the slots behind `slot.at` belong to the round before
+          const uint32_t round = k < slot.at ? slot.parity : slot.parity ^ 1;
+          tc::bar_wait(full + 8 * k, round);
+        }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t s_desc = tc::mma_desc(kBf16, Shape::kCols, a.negate != 0, false);
-      const uint32_t o_desc = tc::mma_desc(kBf16, a.out_cols, false, true);
-      uint32_t stage = 0, step = 0, it = 0;
-      bool ok = true;
-      // one product of 64 k: a tile of the rows with a tile of the stage
-      auto product = [&](uint32_t d, int row_tile, uint32_t col_tile_at, bool add) {
-        const uint64_t da = tc::tile_desc(rows_at + row_tile * kTileBytes, 16);
-        const uint64_t db = tc::tile_desc(col_tile_at, 16);
+    const uint32_t leader = tc::elect_one();
+    const uint32_t s_desc = tc::mma_desc(kBf16, Shape::kCols, a.negate != 0, false);
+    Place slot, o_slot, buf, o_buf;     // of S, and of the second product
+    uint32_t used = 0, it = 0, segments = 0;
+    bool ok = true;
+    const uint64_t rows_desc = tc::tile_desc(rows_at, 16);
+    const uint64_t ring_desc = tc::tile_desc(ring_at, 16);        // K-major
+    const uint64_t ring_desc_mn = tc::tile_desc(ring_at, kTileBytes);  // 64 n per tile
+    // 64 k of S
+    auto product = [&](uint32_t d, uint64_t da, uint64_t db, bool add) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) tc::mma_ss(d, da + 2 * k, db + 2 * k, s_desc, add || k > 0);
-      };
-      // S of one step, tile q of the streamed operand at `at`
-      auto logits = [&](uint32_t d, int q, uint32_t at) {
-        if (!Shape::kSplit) {
-          product(d, q, at, q > 0);
-        } else if (q < a.kb) {              // high x high, low x high
-          product(d, q, at, q > 0);
-          product(d, a.kb + q, at, true);
-        } else {                            // high x low
-          product(d, q - a.kb, at, true);
+      for (int k = 0; k < 4; ++k) tc::mma_ss(leader, d, da + 2 * k, db + 2 * k, s_desc, add || k > 0);
+    };
+    auto slot_ready = [&](const Place& p) {
+      if (!warp_wait(full + 8 * p.at, p.parity)) return ok = false;
+      tc::fence_after();
+      return true;
+    };
+    // S of one step into its buffer, then its barrier; frees the slots only where the second
+    // product does not need them
+    auto issue_s = [&]() {
+      const uint32_t d = tmem + buf.at * Shape::kCols;
+      if (!STREAM) {
+        for (int q = 0; q < tiles; ++q) {
+          if (!slot_ready(slot)) return;
+          const uint64_t db = ring_desc + slot.at * (kSlotBytes >> 4);
+          if (!Shape::kSplit) {
+            product(d, rows_desc + q * (kTileBytes >> 4), db, q > 0);
+          } else if (q < a.kb) {           // high x high, low x high
+            product(d, rows_desc + q * (kTileBytes >> 4), db, q > 0);
+            product(d, rows_desc + (a.kb + q) * (kTileBytes >> 4), db, true);
+          } else {                         // high x low
+            product(d, rows_desc + (q - a.kb) * (kTileBytes >> 4), db, true);
+          }
+          if (MODE == kLoss) tc::mma_commit(leader, empty + 8 * slot.at);
+          slot.next(a.slots);
         }
-      };
-      for (int item = blockIdx.x; ok && item < items; item += gridDim.x, ++it) {
-        int first;
-        const int n = steps_of(item, first);
-        if (!(ok = tc::bar_wait(rows_full, it & 1))) break;
-        if (MODE == kLoss) {
-          for (int j = 0; ok && j < n; ++j, ++step) {
-            const uint32_t buf = step & 1, use = step >> 1;
-            if (use > 0 && !(ok = tc::bar_wait(s_done + 8 * buf, (use - 1) & 1))) break;
-            for (int q = 0; q < tiles; ++q, ++stage) {
-              const uint32_t slot = stage % a.stages;
-              if (!(ok = tc::bar_wait(full + 8 * slot, (stage / a.stages) & 1))) break;
-              tc::fence_after();
-              logits(tmem + buf * Shape::kCols, q, ring_at + slot * stage_bytes);
-              tc::mma_commit(empty + 8 * slot);
-            }
-            if (ok) tc::mma_commit(s_full + 8 * buf);
-          }
-          if (ok) tc::mma_commit(rows_empty);
-        } else {
-          // S of step j + 1 is issued before the second product of step j, so that the
-          // tensor cores work on it while the epilogue warps turn S of step j into P.  The
-          // products run in the order of their issue: S of step j + 2 may overwrite P of j.
-          auto issue_s = [&](uint32_t g) {
-            const uint32_t slot = g % a.stages, buf = g & 1;
-            if (!tc::bar_wait(full + 8 * slot, (g / a.stages) & 1)) return false;
-            tc::fence_after();
-            for (int q = 0; q < tiles; ++q)
-              logits(tmem + buf * Shape::kCols, q, ring_at + slot * stage_bytes + q * kTileBytes);
-            tc::mma_commit(s_full + 8 * buf);
-            return true;
-          };
-          auto issue_o = [&](uint32_t g, bool begin) {
-            const uint32_t slot = g % a.stages, buf = g & 1;
-            if (!tc::bar_wait(s_done + 8 * buf, (g >> 1) & 1)) return false;
-            tc::fence_after();
-            const uint32_t d = tmem + Shape::kOutAt, at = ring_at + slot * stage_bytes;
-            const uint32_t hi = tmem + buf * Shape::kCols, lo = tmem + Shape::kLowAt + buf * 64;
-            const uint64_t b_hi = tc::tile_desc(at, kTileBytes);
-            const uint64_t b_lo = tc::tile_desc(at + a.kb * kTileBytes, kTileBytes);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              tc::mma_ts(d, hi + 8 * k, b_hi + 128 * k, o_desc, !begin || k > 0);
-              if (Shape::kSplit) {
-                tc::mma_ts(d, lo + 8 * k, b_hi + 128 * k, o_desc, true);
-                tc::mma_ts(d, hi + 8 * k, b_lo + 128 * k, o_desc, true);
-              }
-            }
-            tc::mma_commit(empty + 8 * slot);
-            return true;
-          };
-          ok = issue_s(step);
-          for (int j = 0; ok && j < n; ++j, ++step) {
-            if (j + 1 < n) ok = issue_s(step + 1);
-            if (j + 1 == n) tc::mma_commit(rows_empty);
-            if (ok && j == 0 && it > 0) ok = tc::bar_wait(out_empty, (it - 1) & 1);
-            ok = ok && issue_o(step, j == 0);
-          }
-          if (ok) tc::mma_commit(out_full);
+      } else {
+        for (int q = 0; q < a.kb * (Shape::kSplit ? 3 : 1); ++q) {
+          if (!slot_ready(slot)) return;
+          const uint64_t da = ring_desc + slot.at * (kSlotBytes >> 4);
+          product(d, da, da + (kTileBytes >> 4), q > 0);
+          tc::mma_commit(leader, empty + 8 * slot.at);
+          slot.next(a.slots);
         }
       }
-      // the last barrier arrivals of the tensor cores land before this CTA's memory is freed
-      tc::mma_commit(drained);
-      if (!tc::bar_wait(drained, 0) || !ok) *a.status = FG_STATUS_WAIT_EXPIRED;
-    }
-  } else if (warp >= kEpilogueWarp) {
-    const uint32_t group = (warp - kEpilogueWarp) >> 2;   // serves the S buffer of this number
-    const int quarter = warp & 3;                         // TMEM lanes 32 * quarter ...
-    const uint32_t lanes_at = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t s_at = lanes_at + group * Shape::kCols;
-    const float scale = fmaxf(a.logit_scale * (a.unscale ? *a.unscale : 1.f), 1.17549435e-38f);
-    uint32_t step = 0, it = 0;
-    bool ok = true;
-    for (int item = blockIdx.x; ok && item < items; item += gridDim.x, ++it) {
-      int first;
-      const int n = steps_of(item, first);
-      const int64_t row0 = (int64_t)(item % a.row_tiles) * kTileRows;
-      const int64_t row = row0 + quarter * 32 + lane;
-      const bool warp_live = row0 + quarter * 32 < a.n_rows;
+      tc::mma_commit(leader, s_full + 8 * buf.at);
+      buf.next(a.buffers);
+    };
+    for (int i = blockIdx.x; ok && i < items; i += gridDim.x, ++it) {
+      const Item item = item_at(a, i);
+      if (!STREAM && !(ok = warp_wait(rows_full, it & 1))) break;
       if (MODE == kLoss) {
+        for (int j = 0; ok && j < item.steps; ++j, ++used) {
+          if (used >= (uint32_t)a.buffers && !(ok = warp_wait(s_done + 8 * buf.at, buf.parity ^ 1)))
+            break;
+          tc::fence_after();
+          issue_s();
+        }
+        if (ok && !STREAM) tc::mma_commit(leader, rows_empty);
+      } else {
+        // S of the next steps is issued before the second product of step j, so that the
+        // tensor cores work on it while the epilogue warps turn S of step j into P.  The
+        // products run in the order of their issue: a later S may overwrite P of step j.
+        const int c0 = item.chunk * Shape::kChunkTiles * 64;
+        const int cols = min(a.out_cols - c0, Shape::kChunkTiles * 64);
+        // columns n0 ... of the results += P (of one step) x the tiles at `db`
+        auto product_o = [&](int n0, int n, uint32_t p, uint64_t db, bool low, bool begin) {
+          const uint32_t d = out_at + n0;
+          const uint32_t o_desc = tc::mma_desc(kBf16, n, false, true);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t hi = p + 32 * (k >> 1) + 8 * (k & 1);
+            if (!Shape::kSplit) {
+              tc::mma_ts(leader, d, hi, db + 128 * k, o_desc, !begin || k > 0);
+            } else if (!low) {             // high x high; low x high
+              tc::mma_ts(leader, d, hi, db + 128 * k, o_desc, !begin || k > 0);
+              tc::mma_ts(leader, d + Shape::kLowOut, hi + 16, db + 128 * k, o_desc, !begin || k > 0);
+            } else {                       // high x low
+              tc::mma_ts(leader, d + Shape::kLowOut, hi, db + 128 * k, o_desc, true);
+            }
+          }
+        };
+        auto issue_o = [&](int j) {
+          const bool begin = j % Shape::kSegment == 0;
+          if (begin && segments > 0 && !(ok = warp_wait(out_empty, (segments - 1) & 1))) return;
+          if (!(ok = warp_wait(s_done + 8 * o_buf.at, o_buf.parity))) return;
+          tc::fence_after();
+          const uint32_t p = tmem + o_buf.at * Shape::kCols;
+          if (!STREAM) {
+            for (int q = 0; q < tiles; ++q) {
+              const int t = q < a.kb ? q : q - a.kb;
+              product_o(t * 64, min(64, cols - t * 64), p,
+                        ring_desc_mn + o_slot.at * (kSlotBytes >> 4), q >= a.kb, begin);
+              tc::mma_commit(leader, empty + 8 * o_slot.at);
+              o_slot.next(a.slots);
+            }
+          } else {
+            for (int plane = 0; plane < kPlanes; ++plane)
+              for (int n0 = 0; n0 < cols; n0 += 128) {
+                if (!slot_ready(slot)) return;
+                product_o(n0, min(128, cols - n0), p, ring_desc_mn + slot.at * (kSlotBytes >> 4),
+                          plane == 1, begin);
+                tc::mma_commit(leader, empty + 8 * slot.at);
+                slot.next(a.slots);
+              }
+          }
+          o_buf.next(a.buffers);
+          if (j + 1 == item.steps || (j + 1) % Shape::kSegment == 0) {
+            tc::mma_commit(leader, out_full);
+            ++segments;
+          }
+        };
+        const int ahead = min(a.buffers - 1, item.steps);
+        for (int j = 0; ok && j < ahead; ++j) issue_s();
+        for (int j = 0; ok && j < item.steps; ++j) {
+          if (j + ahead < item.steps) issue_s();
+          if (ok && j + ahead + 1 == item.steps && !STREAM) tc::mma_commit(leader, rows_empty);
+          if (ok) issue_o(j);
+        }
+        if (!STREAM && ok && ahead == item.steps) tc::mma_commit(leader, rows_empty);
+      }
+    }
+    // the last barrier arrivals of the tensor cores land before this CTA's memory is freed
+    tc::mma_commit(leader, drained);
+    if (!warp_wait(drained, 0) || !ok) *a.status = FG_STATUS_WAIT_EXPIRED;
+  } else if (warp >= kEpilogueWarp) {
+    const int group = (warp - kEpilogueWarp) >> 2;
+    const int quarter = warp & 3;                         // TMEM lanes 32 * quarter ...
+    const uint32_t lanes_at = (uint32_t)(quarter * 32) << 16;
+    const float scale = fmaxf(a.logit_scale * (a.unscale ? *a.unscale : 1.f), 1.17549435e-38f);
+    Place buf;
+    uint32_t step = 0, segments = 0;
+    bool ok = true;
+    for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+      const Item item = item_at(a, i);
+      const int64_t row0 = (int64_t)item.row_tile * kTileRows;
+      const int64_t row = row0 + quarter * 32 + lane;
+      if (MODE == kLoss) {
+        // Each group takes 128 of a step's 256 columns.  The exponentials are taken relative to
+        // `top`, a value of the row that an earlier step had as its maximum, so that they do
+        // not wait for this step's maximum; only where that turns out 2^60 above it (or there
+        // is none yet) is the step looked through again with the new one.
+        const bool warp_live = row0 + quarter * 32 < a.n_rows;
         float top = -INFINITY, sum = 0.f;
-        for (int j = 0; j < n; ++j, ++step) {
-          if ((step & 1) != group) continue;
-          if (!(ok = warp_wait(s_full + 8 * group, (step >> 1) & 1))) break;
+        for (int j = 0; j < item.steps; ++j) {
+          if (!(ok = warp_wait(s_full + 8 * buf.at, buf.parity))) break;
           if (warp_live) {
             tc::fence_after();
-            const int64_t left = a.n_cols - (int64_t)(first + j) * Shape::kCols;
-            float x[2][32];
-            tc::tmem_load32(s_at, x[0]);
+            const uint32_t s_at = lanes_at + tmem + buf.at * Shape::kCols + group * 128;
+            const int64_t left = a.n_cols - (int64_t)(item.first + j) * Shape::kCols - group * 128;
+            float largest[4], part[4];
+            auto pass = [&](bool with_sum) {
+              const float off = top == -INFINITY ? 0.f : -top * scale;
 #pragma unroll
-            for (int c = 0; c < Shape::kCols / 32; ++c) {
-              float(&v)[32] = x[c & 1];
-              tc::wait_ld32(v);
-              if (c + 1 < Shape::kCols / 32) tc::tmem_load32(s_at + (c + 1) * 32, x[(c + 1) & 1]);
-              if (left < (c + 1) * 32) {
-#pragma unroll
-                for (int k = 0; k < 32; ++k)
-                  if (c * 32 + k >= left) v[k] = -INFINITY;
+              for (int k = 0; k < 4; ++k) {
+                largest[k] = -INFINITY;
+                part[k] = 0.f;
               }
-              float m = top;
+              float x[2][32];
+              tc::tmem_load32(s_at, x[0]);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) m = fmaxf(m, v[k]);
-              const float base = m == -INFINITY ? 0.f : m;
-              sum *= exp2_fast((top - base) * scale);
-              top = m;
-              const float off = -base * scale;
-              float part[4] = {0.f, 0.f, 0.f, 0.f};
+              for (int c = 0; c < 4; ++c) {
+                float(&v)[32] = x[c & 1];
+                tc::wait_ld32(v);
+                if (c < 3) tc::tmem_load32(s_at + (c + 1) * 32, x[(c + 1) & 1]);
+                if (left < (c + 1) * 32) {
 #pragma unroll
-              for (int k = 0; k < 32; ++k) part[k & 3] += exp2_fast(fmaf(v[k], scale, off));
-              sum += (part[0] + part[1]) + (part[2] + part[3]);
+                  for (int k = 0; k < 32; ++k)
+                    if (c * 32 + k >= left) v[k] = -INFINITY;
+                }
+#pragma unroll
+                for (int k = 0; k < 32; ++k) largest[k & 3] = fmaxf(largest[k & 3], v[k]);
+                if (with_sum) {
+#pragma unroll
+                  for (int k = 0; k < 32; ++k) part[k & 3] += exp2_fast(fmaf(v[k], scale, off));
+                }
+              }
+              return fmaxf(fmaxf(largest[0], largest[1]), fmaxf(largest[2], largest[3]));
+            };
+            if (__any_sync(0xffffffffu, top == -INFINITY)) {
+              const float m = pass(false);
+              if (top == -INFINITY) top = m;
             }
+            const float m = pass(true);
+            const bool far = (m - top) * scale > 60.f;
+            if (__any_sync(0xffffffffu, far)) {
+              if (far) {
+                sum *= exp2_fast((top - m) * scale);
+                top = m;
+              }
+              pass(true);
+            }
+            sum += (part[0] + part[1]) + (part[2] + part[3]);
             tc::fence_before();
           }
-          tc::bar_arrive(s_done + 8 * group);
+          tc::bar_arrive(s_done + 8 * buf.at);
+          buf.next(a.buffers);
         }
         if (row < a.n_rows)
-          a.stats[row * (a.splits * 2) + item / a.row_tiles * 2 + group] =
+          a.stats[(row * a.splits + item.split) * 2 + group] =
               make_float2(top == -INFINITY ? -INFINITY : top * scale, sum);
       } else {
+        // The groups take turns with the steps.
+        const int32_t warp_row0 = (int32_t)row0 + quarter * 32;
         float bias = -INFINITY;
-        int64_t label = -1;
+        int32_t label = -1;
         if (MODE == kFeatGrad && row < a.n_rows) {
           bias = a.row_bias[row];
           label = a.row_label[row];
         }
-        for (int j = 0; j < n; ++j, ++step) {
+        const int c0 = item.chunk * Shape::kChunkTiles * 64;
+        float factor = 0.f;
+        if (a.splits == 1 && row < a.n_rows)
+          factor = (a.out_scale ? *a.out_scale : 1.f) * (MODE == kFeatGrad ? a.row_factor[row] : 1.f);
+        const bool live = MODE != kFeatGrad || label >= 0;
+        float acc[Shape::kSplit ? 4 : 1][16];
+#pragma unroll
+        for (int q = 0; q < (Shape::kSplit ? 4 : 1); ++q)
+#pragma unroll
+          for (int k = 0; k < 16; ++k) acc[q][k] = 0.f;
+        // adds a segment of accumulators up in registers and lets the tensor cores go on
+        int flushed = 0;
+        auto flush = [&]() {
+          if (!(ok = warp_wait(out_full, segments & 1))) return;
+          tc::fence_after();
+#pragma unroll
+          for (int q = 0; q < (Shape::kSplit ? 4 : 1); ++q) {
+            const int c = group * 16 + q * 32;
+            if (c0 + c >= a.out_cols) break;
+            float v[16];
+            tc::tmem_load16(lanes_at + out_at + c, v);
+            tc::wait_ld16(v);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) acc[q][k] += v[k];
+            tc::tmem_load16(lanes_at + out_at + Shape::kLowOut + c, v);
+            tc::wait_ld16(v);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) acc[q][k] += v[k];
+          }
+          tc::fence_before();
+          tc::bar_arrive(out_empty);
+          ++segments;
+          ++flushed;
+        };
+        for (int j = 0; j < item.steps; ++j, ++step) {
+          const Place at = buf;
+          buf.next(a.buffers);
           if ((step & 1) != group) continue;
-          const int64_t col0 = (int64_t)(first + j) * Shape::kCols;
-          // whether a column of this step can be the label of a row of the tile, or has a
-          // negative weight: rare where the vocabulary is large, and then looked at one by one
-          bool special;
-          if (MODE == kFeatGrad) {
-            special = label >= col0 && label < col0 + Shape::kCols;
-          } else {
-            special = false;
+          const int64_t col0 = (int64_t)(item.first + j) * Shape::kCols;
+          // weight_grad: lane c holds columns c, 32 + c, ... of the step; in `hits` those whose
+          // label is one of this warp's rows, in `negative` those of a negative weight
+          int32_t col_label[4];
+          float col_weight[4];
+          uint32_t hits[4] = {0, 0, 0, 0}, negative[4] = {0, 0, 0, 0};
+          if (MODE == kWeightGrad) {
             __syncwarp();
 #pragma unroll
-            for (int c = lane; c < 128; c += 32) {
-              const int32_t l = a.col_label[col0 + c];
-              special |= (l >= row0 && l < row0 + kTileRows) || a.col_weight[col0 + c] < 0.f;
-              col_bias_s[warp - kEpilogueWarp][c] = a.col_bias[col0 + c];
+            for (int c = 0; c < 4; ++c) {
+              col_label[c] = a.col_label[col0 + c * 32 + lane];
+              col_weight[c] = a.col_weight[col0 + c * 32 + lane];
+              col_bias_s[warp - kEpilogueWarp][c * 32 + lane] = a.col_bias[col0 + c * 32 + lane];
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              hits[c] = __ballot_sync(0xffffffffu, col_label[c] >= warp_row0 && col_label[c] < warp_row0 + 32);
+              negative[c] = __ballot_sync(0xffffffffu, col_weight[c] < 0.f);
             }
             __syncwarp();
           }
-          special = __any_sync(0xffffffffu, special);
           const int64_t left = a.n_cols - col0;
-          if (!(ok = warp_wait(s_full + 8 * group, (step >> 1) & 1))) break;
+          if (!(ok = warp_wait(s_full + 8 * at.at, at.parity))) break;
           tc::fence_after();
-          float x[2][32];
-          tc::tmem_load32(s_at, x[0]);
+          const uint32_t s_at = lanes_at + tmem + at.at * Shape::kCols;
+          constexpr int kAhead = Shape::kSplit ? 1 : 2;  // float32 needs the registers
+          float x[kAhead][32];
+          if (kAhead == 2) tc::tmem_load32(s_at, x[0]);
 #pragma unroll
-          for (int c = 0; c < Shape::kCols / 32; ++c) {
-            float(&v)[32] = x[c & 1];
+          for (int c = 0; c < 4; ++c) {
+            float(&v)[32] = x[c % kAhead];
+            if (kAhead == 1) tc::tmem_load32(s_at + c * 32, v);
             tc::wait_ld32(v);
-            if (c + 1 < Shape::kCols / 32) tc::tmem_load32(s_at + (c + 1) * 32, x[(c + 1) & 1]);
+            if (kAhead == 2 && c < 3) tc::tmem_load32(s_at + (c + 1) * 32, x[(c + 1) % kAhead]);
             if (MODE == kFeatGrad) {
 #pragma unroll
               for (int k = 0; k < 32; ++k) v[k] = exp2_fast(fmaf(v[k], scale, bias));
-              if (special) {
+              const int64_t at_label = label - (col0 + c * 32);
+              if (__any_sync(0xffffffffu, at_label >= 0 && at_label < 32)) {
 #pragma unroll
                 for (int k = 0; k < 32; ++k)
-                  if (label == col0 + c * 32 + k) v[k] -= a.hot;
+                  if (at_label == k) v[k] -= a.hot;
               }
               if (left < (c + 1) * 32) {  // behind the vocabulary: no probability, whatever lse
 #pragma unroll
@@ -409,71 +634,62 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
             } else {
 #pragma unroll
               for (int k = 0; k < 32; k += 4) {
-                const float4 e = *reinterpret_cast<const float4*>(&col_bias_s[warp - kEpilogueWarp][c * 32 + k]);
+                const float4 e =
+                    *reinterpret_cast<const float4*>(&col_bias_s[warp - kEpilogueWarp][c * 32 + k]);
                 v[k] = exp2_fast(fmaf(v[k], scale, e.x));
                 v[k + 1] = exp2_fast(fmaf(v[k + 1], scale, e.y));
                 v[k + 2] = exp2_fast(fmaf(v[k + 2], scale, e.z));
                 v[k + 3] = exp2_fast(fmaf(v[k + 3], scale, e.w));
               }
-              if (special) {
+              if (negative[c]) {
 #pragma unroll
-                for (int k = 0; k < 32; ++k) {
-                  const float w = a.col_weight[col0 + c * 32 + k];
-                  if (w < 0.f) v[k] = -v[k];
-                  if (a.col_label[col0 + c * 32 + k] == row) v[k] -= w * a.hot;
-                }
+                for (int k = 0; k < 32; ++k)
+                  if (negative[c] >> k & 1) v[k] = -v[k];
+              }
+              for (uint32_t left_hits = hits[c]; left_hits; left_hits &= left_hits - 1) {
+                const int from = __ffs(left_hits) - 1;
+                const int32_t hit = __shfl_sync(0xffffffffu, col_label[c], from) - warp_row0;
+                const float weight = __shfl_sync(0xffffffffu, col_weight[c], from) * a.hot;
+#pragma unroll
+                for (int k = 0; k < 32; ++k)
+                  if (k == from && lane == hit) v[k] -= weight;
               }
             }
-            store_p<MODE, T>(s_at, lanes_at + Shape::kLowAt + group * 64, c, v);
+            store_p<T>(s_at + c * 32, v);
           }
           tc::wait_st();
           tc::fence_before();
-          tc::bar_arrive(s_done + 8 * group);
+          tc::bar_arrive(s_done + 8 * at.at);
+          if (Shape::kSplit)
+            while (ok && (flushed + 1) * Shape::kSegment <= j + 1) flush();
+          if (!ok) break;
         }
-        if (!ok || !(ok = warp_wait(out_full, it & 1))) break;
-        tc::fence_after();
-        // the two groups take alternate 16-column pieces of the accumulators
-        float factor = 0.f;
-        if (a.splits == 1 && row < a.n_rows)
-          factor = (a.out_scale ? *a.out_scale : 1.f) * (MODE == kFeatGrad ? a.row_factor[row] : 1.f);
-        for (int c = group * 16; c < a.out_cols; c += 32) {
-          float v[16];
-          __syncwarp();
-          tc::tmem_load16(lanes_at + Shape::kOutAt + c, v);
-          tc::wait_ld16(v);
+        if (!ok) break;
+        if (Shape::kSplit) {
+          while (ok && flushed * Shape::kSegment < item.steps) flush();
+          if (!ok) break;
           if (row < a.n_rows) {
-            if (a.splits > 1) {  // a partial sum, rows out_cols apart
-              float* to = a.partial + ((int64_t)(item / a.row_tiles) * a.n_rows + row) * a.out_cols + c;
 #pragma unroll
-              for (int k = 0; k < 16; k += 4)
-                *reinterpret_cast<float4*>(to + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-            } else {
-              if (MODE == kFeatGrad && label < 0) {
-#pragma unroll
-                for (int k = 0; k < 16; ++k) v[k] = 0.f;
-              }
-              T* to = static_cast<T*>(a.out) + row * a.feat_len + c;
-              constexpr int N = 16 / sizeof(T);
-              if (a.feat_len % N == 0 && ((uintptr_t)a.out & 15) == 0) {
-#pragma unroll
-                for (int k = 0; k < 16; k += N) {
-                  if (c + k >= a.feat_len) break;
-                  Vec<T, N> piece;
-#pragma unroll
-                  for (int i = 0; i < N; ++i) piece.v[i] = from_float<T>(v[k + i] * factor);
-                  store_vec<T, N>(to + k, piece);
-                }
-              } else {
-#pragma unroll
-                for (int k = 0; k < 16; ++k)
-                  if (c + k < a.feat_len) to[k] = from_float<T>(v[k] * factor);
-              }
-            }
+            for (int q = 0; q < (Shape::kSplit ? 4 : 1); ++q)
+              store_out<MODE, T>(a, item, row, c0 + group * 16 + q * 32, acc[q], factor, live);
           }
+        } else {
+          // the two groups take alternate 16-column pieces of the accumulators
+          if (!(ok = warp_wait(out_full, segments & 1))) break;
+          tc::fence_after();
+          ++segments;
+          const int cols = min(a.out_cols - c0, Shape::kChunkTiles * 64);
+          for (int c = group * 16; c < cols; c += 32) {
+            float v[16];
+            __syncwarp();
+            tc::tmem_load16(lanes_at + out_at + c, v);
+            tc::wait_ld16(v);
+            if (row < a.n_rows) store_out<MODE, T>(a, item, row, c0 + c, v, factor, live);
+          }
+          __syncwarp();
+          tc::fence_before();
+          tc::bar_arrive(out_empty);
         }
-        __syncwarp();
-        tc::fence_before();
-        tc::bar_arrive(out_empty);
       }
     }
     if (!ok && lane == 0) *a.status = FG_STATUS_WAIT_EXPIRED;
@@ -481,159 +697,8 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
   __syncwarp();
   tc::fence_before();
   __syncthreads();
-  if (warp == 2) tc::tmem_free(tmem, 512);
+  if (warp == 2) tc::tmem_free(tmem_where, 512);
 }
-
-// ------------------------------------------- without tensor cores: wide features --
-constexpr int kTile = 32;
-constexpr int64_t kPiece = 8192;
-
-// One 32 x 32 tile of a product with fp32 accumulators, 256 threads, four results a thread:
-// row ty + 8 i, column tx.
-template <typename A, typename B>
-__device__ __forceinline__ void product_tile(float (&acc)[4], int64_t m0, int64_t n0, int64_t m,
-                                             int64_t n, int64_t k_len, const A* a, int64_t a_m,
-                                             int64_t a_k, const B* b, int64_t b_n, int64_t b_k) {
-  __shared__ float sa[kTile][kTile + 1], sb[kTile][kTile + 1];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  for (int i = 0; i < 4; ++i) acc[i] = 0.f;
-  for (int64_t k0 = 0; k0 < k_len; k0 += kTile) {
-    for (int i = 0; i < 4; ++i) {
-      const int r = ty + 8 * i;
-      const int64_t k = k0 + tx;
-      sa[r][tx] = m0 + r < m && k < k_len ? to_float<A>(a[(m0 + r) * a_m + k * a_k]) : 0.f;
-      sb[r][tx] = n0 + r < n && k < k_len ? to_float<B>(b[(n0 + r) * b_n + k * b_k]) : 0.f;
-    }
-    __syncthreads();
-    for (int k = 0; k < kTile; ++k)
-      for (int i = 0; i < 4; ++i) acc[i] = fmaf(sa[ty + 8 * i][k], sb[tx][k], acc[i]);
-    __syncthreads();
-  }
-}
-
-// Running maximum and sum of exponentials of a tile row; one pair per (row, vocabulary tile).
-template <typename T>
-__global__ void __launch_bounds__(256)
-logit_stats_kernel(Batch b, const T* feat, int64_t feat_ld, const T* weight, int64_t weight_ld,
-                   float2* stats, float* picked) {
-  const int64_t v0 = (int64_t)blockIdx.x * kTile, t0 = (int64_t)blockIdx.y * kTile;
-  float acc[4];
-  product_tile<T, T>(acc, t0, v0, b.n, b.vocab, b.feat_len, feat, feat_ld, 1, weight, weight_ld, 1);
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  for (int i = 0; i < 4; ++i) {
-    const int64_t t = t0 + ty + 8 * i, v = v0 + tx;
-    const float z = v < b.vocab ? acc[i] * b.scale : -INFINITY;
-    float top = z;
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    float s = top == -INFINITY ? (z != z ? z : 0.f) : expf(z - top);
-    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    if (t >= b.n) continue;
-    if (tx == 0) stats[t * gridDim.x + blockIdx.x] = make_float2(top, s);
-    if (v < b.vocab && load_label(b.labels, b.wide, t) == v) picked[t] = z;
-  }
-}
-
-__global__ void __launch_bounds__(256)
-join_stats_kernel(Batch b, const float2* stats, int64_t tiles, const float* picked, float* loss,
-                  float* lse, int32_t* status) {
-  const int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (t >= b.n) return;
-  const int lane = threadIdx.x & 31;
-  float top = -INFINITY, s = 0.f;
-  for (int64_t k = lane; k < tiles; k += 32) {
-    const float2 p = stats[t * tiles + k];
-    const float m = fmaxf(top, p.x);
-    if (m == -INFINITY) { s += p.y; continue; }
-    s = s * expf(top - m) + p.y * expf(p.x - m);
-    top = m;
-  }
-  for (int d = 16; d > 0; d >>= 1) {
-    const float top2 = __shfl_xor_sync(0xffffffffu, top, d), s2 = __shfl_xor_sync(0xffffffffu, s, d);
-    const float m = fmaxf(top, top2);
-    s = m == -INFINITY ? s + s2 : s * expf(top - m) + s2 * expf(top2 - m);
-    top = m;
-  }
-  if (lane != 0) return;
-  const float l = top + logf(s);
-  lse[t] = l;
-  const int64_t y = load_label(b.labels, b.wide, t);
-  if (y == b.ignore_index) {
-    loss[t] = 0.f;
-  } else if ((uint64_t)y >= (uint64_t)b.vocab) {
-    *status = FG_STATUS_BAD_INDEX;
-    loss[t] = __int_as_float(0x7fc00000);
-  } else {
-    loss[t] = l - picked[t];
-  }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256)
-logit_grad_kernel(Batch b, const T* feat, int64_t feat_ld, const T* weight, int64_t weight_ld,
-                  const float* lse, const float* loss_grad, int64_t v_begin, int64_t v_count,
-                  float* dz) {
-  const int64_t v0 = (int64_t)blockIdx.x * kTile, t0 = (int64_t)blockIdx.y * kTile;
-  float acc[4];
-  product_tile<T, T>(acc, t0, v0, b.n, v_count, b.feat_len, feat, feat_ld, 1,
-                     weight + v_begin * weight_ld, weight_ld, 1);
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  for (int i = 0; i < 4; ++i) {
-    const int64_t t = t0 + ty + 8 * i, v = v0 + tx;
-    if (t >= b.n || v >= v_count) continue;
-    const int64_t y = load_label(b.labels, b.wide, t);
-    const bool live = y != b.ignore_index && (uint64_t)y < (uint64_t)b.vocab;
-    const float p = expf(acc[i] * b.scale - lse[t]) - (y == v_begin + v ? 1.f : 0.f);
-    dz[t * v_count + v] = live ? p * loss_grad[t] * b.scale : 0.f;
-  }
-}
-
-// feat_grad += dz @ weight over one piece; the sum over the pieces waits in fp32.
-template <typename T>
-__global__ void __launch_bounds__(256)
-feat_grad_kernel(Batch b, const float* dz, const T* weight, int64_t weight_ld, int64_t v_begin,
-                 int64_t v_count, float* acc_out, T* feat_grad, int first, int last) {
-  const int64_t t0 = (int64_t)blockIdx.y * kTile, d0 = (int64_t)blockIdx.x * kTile;
-  float acc[4];
-  product_tile<float, T>(acc, t0, d0, b.n, b.feat_len, v_count, dz, v_count, 1,
-                         weight + v_begin * weight_ld, 1, weight_ld);
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  for (int i = 0; i < 4; ++i) {
-    const int64_t t = t0 + ty + 8 * i, d = d0 + tx;
-    if (t >= b.n || d >= b.feat_len) continue;
-    const float v = acc[i] + (first ? 0.f : acc_out[t * b.feat_len + d]);
-    if (last)
-      feat_grad[t * b.feat_len + d] = from_float<T>(v);
-    else
-      acc_out[t * b.feat_len + d] = v;
-  }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256)
-live_feat_kernel(Batch b, const T* feat, int64_t feat_ld, T* out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= b.n * b.feat_len) return;
-  const int64_t t = i / b.feat_len, d = i - t * b.feat_len;
-  const int64_t y = load_label(b.labels, b.wide, t);
-  const bool live = y != b.ignore_index && (uint64_t)y < (uint64_t)b.vocab;
-  out[i] = live ? feat[t * feat_ld + d] : from_float<T>(0.f);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256)
-weight_grad_kernel(Batch b, const float* dz, const T* feat, int64_t feat_ld, int64_t v_begin,
-                   int64_t v_count, T* weight_grad) {
-  const int64_t v0 = (int64_t)blockIdx.y * kTile, d0 = (int64_t)blockIdx.x * kTile;
-  float acc[4];
-  product_tile<float, T>(acc, v0, d0, v_count, b.feat_len, b.n, dz, 1, v_count, feat, 1, feat_ld);
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  for (int i = 0; i < 4; ++i) {
-    const int64_t v = v0 + ty + 8 * i, d = d0 + tx;
-    if (v < v_count && d < b.feat_len)
-      weight_grad[(v_begin + v) * b.feat_len + d] = from_float<T>(acc[i]);
-  }
-}
-
 
 // ------------------------------------------------------------ around the kernel --
 // Scalars of a call, on the device (setup_kernel).
@@ -847,11 +912,12 @@ constexpr int kSms = 148;  // the grids below are sized for B200's 148 SMs, one 
 struct Cut {
   int splits, steps_per_split;
 };
-Cut cut_steps(int64_t row_tiles, int64_t steps, int item_steps) {
+Cut cut_steps(int64_t row_tiles, int64_t steps, int item_steps, int64_t most_steps) {
   Cut best = {1, (int)steps};
   int64_t best_time = INT64_MAX;
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(steps, 4 * kSms / std::max<int64_t>(row_tiles, 1)));
-  for (int64_t s = 1; s <= most; ++s) {
+  const int64_t least = (steps + most_steps - 1) / most_steps;
+  const int64_t most = std::max(least, std::min<int64_t>(steps, 4 * kSms / std::max<int64_t>(row_tiles, 1)));
+  for (int64_t s = least; s <= most; ++s) {
     const int64_t per = (steps + s - 1) / s, used = (steps + per - 1) / per;
     const int64_t waves = (row_tiles * used + kSms - 1) / kSms;
     const int64_t time = waves * (per + item_steps);
@@ -864,7 +930,6 @@ Cut cut_steps(int64_t row_tiles, int64_t steps, int item_steps) {
 }
 
 struct XentLayout {
-  bool mma;                     // the tensor-core path
   int kb, tiles;                // 64-element tiles of a row: of one piece, of all
   int64_t pitch;                // elements of a packed row
   int64_t padded;               // n up to a whole tile
@@ -873,7 +938,6 @@ struct XentLayout {
   Cut loss, feat, weight;
   size_t consts, abs_max, packed_feat, packed_weight;
   size_t stats, row_bias, row_factor, col_bias, col_weight, label, partial;
-  size_t s_stats, s_picked, s_dz, s_live, s_acc;  // the path without tensor cores
   size_t total;
 };
 
@@ -882,47 +946,40 @@ XentLayout xent_layout(int32_t dtype, int64_t n, int64_t vocab, int64_t feat_len
   const int planes = dtype == FG_FLOAT32 ? 2 : 1;
   l.kb = (int)((feat_len + 63) / 64);
   l.tiles = l.kb * planes;
-  l.mma = l.tiles <= kMaxResidentTiles;
   l.pitch = (int64_t)l.tiles * 64;
   l.t_tiles = (n + kTileRows - 1) / kTileRows;
   l.v_tiles = (vocab + kTileRows - 1) / kTileRows;
   l.padded = l.t_tiles * kTileRows;
   l.out_cols = (int)((feat_len + 15) / 16 * 16);
-  l.loss = cut_steps(l.t_tiles, (vocab + 255) / 256, 2);
-  l.feat = cut_steps(l.t_tiles, l.v_tiles, 4);
-  l.weight = cut_steps(l.v_tiles, l.t_tiles, 4);
+  // 1024 steps of the 16-bit gradients are 8192 additions into the same accumulators, which
+  // cut (see kSegment): 1e-4, half a step of float16; the pieces are joined in fp32
+  const int64_t most_steps = dtype == FG_FLOAT32 ? INT32_MAX : 1024;
+  const int chunk_tiles = dtype == FG_FLOAT32 ? 2 : 4;
+  const int64_t chunks = (l.kb + chunk_tiles - 1) / chunk_tiles;
+  l.loss = cut_steps(l.t_tiles, (vocab + 255) / 256, 2, INT32_MAX);
+  l.feat = cut_steps(l.t_tiles * chunks, l.v_tiles, 4, most_steps);
+  l.weight = cut_steps(l.v_tiles * chunks, l.t_tiles, 4, most_steps);
   size_t at = 0;
   auto take = [&at](size_t bytes) {
     const size_t here = at;
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  if (l.mma) {
-    l.consts = take(sizeof(Consts));
-    l.abs_max = take(2 * kMaxPartials * 4);
-    l.packed_feat = take((size_t)n * l.pitch * 2);
-    l.packed_weight = take((size_t)vocab * l.pitch * 2);
-    l.stats = take((size_t)n * l.loss.splits * 2 * sizeof(float2));
-    if (with_grad) {
-      l.row_bias = take((size_t)l.padded * 4);
-      l.row_factor = take((size_t)l.padded * 4);
-      l.col_bias = take((size_t)l.padded * 4);
-      l.col_weight = take((size_t)l.padded * 4);
-      l.label = take((size_t)l.padded * 4);
-      size_t rows = 0;
-      if (l.feat.splits > 1) rows = (size_t)l.feat.splits * n;
-      if (l.weight.splits > 1) rows = std::max(rows, (size_t)l.weight.splits * vocab);
-      l.partial = take(rows * l.out_cols * 4);
-    }
-  } else {
-    const int64_t tiles = (vocab + kTile - 1) / kTile;
-    l.s_stats = take((size_t)n * tiles * sizeof(float2));
-    l.s_picked = take((size_t)n * 4);
-    if (with_grad) {
-      l.s_dz = take((size_t)n * std::min(vocab, kPiece) * 4);
-      l.s_live = take((size_t)n * feat_len * dtype_size(dtype));
-      l.s_acc = take((size_t)n * feat_len * 4);
-    }
+  l.consts = take(sizeof(Consts));
+  l.abs_max = take(2 * kMaxPartials * 4);
+  l.packed_feat = take((size_t)n * l.pitch * 2);
+  l.packed_weight = take((size_t)vocab * l.pitch * 2);
+  l.stats = take((size_t)n * l.loss.splits * 2 * sizeof(float2));
+  if (with_grad) {
+    l.row_bias = take((size_t)l.padded * 4);
+    l.row_factor = take((size_t)l.padded * 4);
+    l.col_bias = take((size_t)l.padded * 4);
+    l.col_weight = take((size_t)l.padded * 4);
+    l.label = take((size_t)l.padded * 4);
+    size_t rows = 0;
+    if (l.feat.splits > 1) rows = (size_t)l.feat.splits * n;
+    if (l.weight.splits > 1) rows = std::max(rows, (size_t)l.weight.splits * vocab);
+    l.partial = take(rows * l.out_cols * 4);
   }
   l.total = at;
   return l;
@@ -1004,9 +1061,10 @@ int prepare_operands(const Batch& b, const XentLayout& l, char* ws, const T* fea
   return FG_OK;
 }
 
-template <int MODE, typename T>
-int launch_mma(const Batch& b, const XentLayout& l, const Operands& o, const Cut& cut, MmaArgs a,
-               cudaStream_t s) {
+template <int MODE, typename T, bool STREAM>
+int launch_mma_as(const Batch& b, const XentLayout& l, const Operands& o, const Cut& cut, MmaArgs a,
+                  cudaStream_t s) {
+  using Shape = MmaShape<MODE, T, STREAM>;
   const bool rows_are_samples = MODE != kWeightGrad;
   const void* row_p = rows_are_samples ? o.feat : o.weight;
   const void* col_p = rows_are_samples ? o.weight : o.feat;
@@ -1017,7 +1075,7 @@ int launch_mma(const Batch& b, const XentLayout& l, const Operands& o, const Cut
   const int64_t col_cols = col_ld == l.pitch && sizeof(T) == 4 ? l.pitch : b.feat_len;
   a.n_rows = rows_are_samples ? b.n : b.vocab;
   a.n_cols = rows_are_samples ? b.vocab : b.n;
-  constexpr int kCols = MmaShape<MODE, T>::kCols;
+  constexpr int kCols = Shape::kCols;
   CUtensorMap row_map, col_map;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   if (!make_tile_map(&row_map, row_p, kBf16, a.n_rows, row_cols, row_ld, kTileRows) ||
@@ -1032,15 +1090,28 @@ int launch_mma(const Batch& b, const XentLayout& l, const Operands& o, const Cut
   a.out_cols = l.out_cols;
   a.negate = b.scale < 0.f;
   a.logit_scale = std::fabs(b.scale) * kLog2e;
-  const int stage_tiles = (MODE == kLoss ? 1 : l.tiles) * (kCols / 128);
-  a.stages = std::min(kMaxStages, (kSharedBudget / kTileBytes - l.tiles) / stage_tiles);
-  const size_t smem = (size_t)(l.tiles + a.stages * stage_tiles) * kTileBytes + 1024;
-  auto kernel = xent_mma_kernel<MODE, T>;
+  // shared memory: 14 tiles of 16 KB at most, 13 where the columns' biases need some of it
+  const int room = MODE == kWeightGrad ? 13 : 14;
+  const int resident = STREAM ? 0 : l.tiles;
+  a.slots = std::min(kMaxSlots, (room - resident) / Shape::kSlotTiles);
+  const size_t smem = (size_t)(resident + a.slots * Shape::kSlotTiles) * kTileBytes + 1024;
+  // TMEM: 512 columns, two S tiles, three where the accumulators need only 128 columns
+  a.buffers = MODE != kLoss && !Shape::kSplit && l.out_cols <= 128 ? 3 : 2;
+  a.chunks = MODE == kLoss ? 1 : (l.kb + Shape::kChunkTiles - 1) / Shape::kChunkTiles;
+  auto kernel = xent_mma_kernel<MODE, T, STREAM>;
   FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  const int64_t items = (int64_t)a.row_tiles * a.splits;
+  const int64_t items = (int64_t)a.row_tiles * a.splits * a.chunks;
+  if (items > INT32_MAX) return fail(FG_ERR_UNSUPPORTED, "too many tiles");
   kernel<<<(int)std::min<int64_t>(items, kSms), kMmaThreads, smem, s>>>(row_map, col_map, a);
   FG_CUDA_TRY(cudaGetLastError());
   return FG_OK;
+}
+
+template <int MODE, typename T>
+int launch_mma(const Batch& b, const XentLayout& l, const Operands& o, const Cut& cut, const MmaArgs& a,
+               cudaStream_t s) {
+  return l.tiles <= kMaxResidentTiles ? launch_mma_as<MODE, T, false>(b, l, o, cut, a, s)
+                                      : launch_mma_as<MODE, T, true>(b, l, o, cut, a, s);
 }
 
 template <typename T>
@@ -1146,30 +1217,13 @@ extern "C" int fg_softmax_xent(const void* feat_dev, int64_t feat_ld, const void
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace_dev);
   const Batch b = {labels_dev, index_type == FG_INDEX_INT64, n, vocab, feat_len, ignore_index, scale};
-  if (l.mma) {
-    int rc = FG_OK;
+  int rc = FG_OK;
 #define FG_LOSS(T)                                                                               \
   rc = loss_mma<T>(b, l, ws, static_cast<const T*>(feat_dev), feat_ld,                           \
                    static_cast<const T*>(weight_dev), weight_ld, dtype, loss_dev, lse_dev, status_dev, s)
-    FG_DISPATCH_DTYPE(dtype, FG_LOSS)
+  FG_DISPATCH_DTYPE(dtype, FG_LOSS)
 #undef FG_LOSS
-    return rc;
-  }
-  float2* stats = reinterpret_cast<float2*>(ws + l.s_stats);
-  float* picked = reinterpret_cast<float*>(ws + l.s_picked);
-  const int64_t tiles = (vocab + kTile - 1) / kTile;
-  const dim3 grid((unsigned)tiles, (unsigned)((n + kTile - 1) / kTile));
-#define FG_STATS(T)                                                                        \
-  logit_stats_kernel<T><<<grid, 256, 0, s>>>(b, static_cast<const T*>(feat_dev), feat_ld,  \
-                                             static_cast<const T*>(weight_dev), weight_ld, \
-                                             stats, picked)
-  FG_DISPATCH_DTYPE(dtype, FG_STATS)
-#undef FG_STATS
-  FG_CUDA_TRY(cudaGetLastError());
-  join_stats_kernel<<<(unsigned)((n + 7) / 8), 256, 0, s>>>(b, stats, tiles, picked, loss_dev,
-                                                            lse_dev, status_dev);
-  FG_CUDA_TRY(cudaGetLastError());
-  return FG_OK;
+  return rc;
 }
 
 extern "C" int fg_softmax_xent_grad(const float* loss_grad_dev, const void* feat_dev,
@@ -1204,46 +1258,12 @@ extern "C" int fg_softmax_xent_grad(const float* loss_grad_dev, const void* feat
   const XentLayout l = xent_layout(dtype, n, vocab, feat_len, true);
   char* ws = static_cast<char*>(workspace_dev);
   const Batch b = {labels_dev, index_type == FG_INDEX_INT64, n, vocab, feat_len, ignore_index, scale};
-  if (l.mma) {
-    int rc = FG_OK;
+  int rc = FG_OK;
 #define FG_GRAD(T)                                                                              \
   rc = grad_mma<T>(b, l, ws, loss_grad_dev, static_cast<const T*>(feat_dev), feat_ld,           \
                    static_cast<const T*>(weight_dev), weight_ld, dtype, lse_dev,                \
                    static_cast<T*>(feat_grad_dev), static_cast<T*>(weight_grad_dev), status_dev, s)
-    FG_DISPATCH_DTYPE(dtype, FG_GRAD)
+  FG_DISPATCH_DTYPE(dtype, FG_GRAD)
 #undef FG_GRAD
-    return rc;
-  }
-  float* dz = reinterpret_cast<float*>(ws + l.s_dz);
-  float* acc = reinterpret_cast<float*>(ws + l.s_acc);
-  const unsigned t_tiles = (unsigned)((n + kTile - 1) / kTile);
-  const unsigned d_tiles = (unsigned)((feat_len + kTile - 1) / kTile);
-#define FG_LIVE(T)                                                                         \
-  live_feat_kernel<T><<<(unsigned)((n * feat_len + 255) / 256), 256, 0, s>>>(              \
-      b, static_cast<const T*>(feat_dev), feat_ld, reinterpret_cast<T*>(ws + l.s_live))
-  FG_DISPATCH_DTYPE(dtype, FG_LIVE)
-#undef FG_LIVE
-  for (int64_t v0 = 0; v0 < vocab; v0 += kPiece) {
-    const int64_t count = std::min(kPiece, vocab - v0);
-    const unsigned v_tiles = (unsigned)((count + kTile - 1) / kTile);
-#define FG_PIECE(T)                                                                              \
-  {                                                                                              \
-    const T* w = static_cast<const T*>(weight_dev);                                              \
-    logit_grad_kernel<T><<<dim3(v_tiles, t_tiles), 256, 0, s>>>(                                 \
-        b, static_cast<const T*>(feat_dev), feat_ld, w, weight_ld, lse_dev, loss_grad_dev, v0,   \
-        count, dz);                                                                              \
-    if (feat_grad_dev)                                                                           \
-      feat_grad_kernel<T><<<dim3(d_tiles, t_tiles), 256, 0, s>>>(                                \
-          b, dz, w, weight_ld, v0, count, acc, static_cast<T*>(feat_grad_dev), v0 == 0,          \
-          v0 + count == vocab);                                                                  \
-    if (weight_grad_dev)                                                                         \
-      weight_grad_kernel<T><<<dim3(d_tiles, v_tiles), 256, 0, s>>>(                              \
-          b, dz, reinterpret_cast<const T*>(ws + l.s_live), feat_len, v0, count,              \
-          static_cast<T*>(weight_grad_dev));                                                     \
-  }
-    FG_DISPATCH_DTYPE(dtype, FG_PIECE)
-#undef FG_PIECE
-  }
-  FG_CUDA_TRY(cudaGetLastError());
-  return FG_OK;
+  return rc;
 }

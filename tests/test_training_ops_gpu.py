@@ -237,7 +237,8 @@ def xent_reference(feat, weight, labels, scale, ignore, dloss=None):
 
 XENT_SIZES = [(1, 1, 1), (1, 7, 3), (2, 33, 8), (5, 1000, 64), (31, 129, 16), (128, 256, 64),
               (129, 257, 65), (131, 2003, 100), (257, 517, 33), (64, 4097, 128), (300, 10007, 32),
-              (1, 20011, 130), (1027, 700, 24), (40, 90, 600)]
+              (1, 20011, 130), (1027, 700, 24), (40, 90, 600), (200, 1500, 192), (150, 700, 256),
+              (400, 2600, 260), (97, 3000, 448)]
 
 
 def xent_inputs(n, v, d, dtype, seed, spread=2.0):
