@@ -56,8 +56,7 @@ enum Mode { kLoss = 0, kFeatGrad = 1, kWeightGrad = 2 };
 
 constexpr int kTileRows = 128;
 constexpr int kTileBytes = kTileRows * 128;   // 128 rows of 64 16-bit elements
-constexpr int kMmaThreads = 384;              // loads, mma, TMEM, one idle; then 8 epilogue warps
-constexpr int kEpilogueWarp = 4;
+constexpr int kEpilogueWarp = 4;              // before them: loads, mma, TMEM, one idle
 constexpr int kMaxSlots = 14;
 constexpr int kMaxBuffers = 3;
 constexpr int kMaxResidentTiles = 4;          // 64-element tiles of a row that stay in shared memory
@@ -73,7 +72,7 @@ struct MmaArgs {
   int negate;             // a negative scale: |scale| with -A
   float logit_scale;      // |scale| * log2(e)
   const float* unscale;   // float32: what undoes the operands' scaling; else null
-  float2* stats;          // loss: (maximum, sum) per row, split and half of a step, base 2
+  float2* stats;          // loss: (maximum, sum) per row, split and group of warps, base 2
   const float* row_bias;  // feat_grad: log2(hot) - lse * log2(e) of a row, -inf: takes no part
   const int32_t* row_label;
   const float* col_bias;  // weight_grad: the same of a column, plus log2 |weight|
@@ -92,14 +91,19 @@ template <int MODE, typename T, bool STREAM>
 struct MmaShape {
   static constexpr bool kSplit = sizeof(T) == 4;  // float32 as two fp16 pieces, three products
   static constexpr int kCols = MODE == kLoss ? 256 : 128;
+  // Groups of four epilogue warps.  The loss only reads S, in 64 columns a group: with four
+  // warps on every scheduler the exponentials' unit stays busy across the waits of each.  The
+  // gradients' groups hold twice the registers and take turns with the steps.
+  static constexpr int kGroups = MODE == kLoss ? 4 : 2;
+  static constexpr int kThreads = 32 * (kEpilogueWarp + 4 * kGroups);
   static constexpr int kChunkTiles = kSplit ? 2 : 4;
   // tiles of 16 KB that a slot of the ring holds: a tile of the streamed operand, with one of
   // the rows where these are streamed too (or, for the second product, two of the first)
   static constexpr int kSlotTiles = MODE == kLoss ? (STREAM ? 3 : 2) : (STREAM ? 2 : 1);
   // float32: steps after which the accumulators are added up in registers.  tcgen05.mma adds
-  // to fp32 by cutting, about 2^-26 of the sum each time and always towards zero: 64 of these
-  // (eight a step) are 2^-20, several thousand were 1.1e-5.
-  static constexpr int kSegment = kSplit ? 8 : 1 << 30;
+  // to fp32 by cutting, about 2^-26 of the sum each time and always towards zero: 32 of these
+  // (eight a step) are 2^-21, several thousand were 1.1e-5.
+  static constexpr int kSegment = kSplit ? 4 : 1 << 30;
   static constexpr int kLowOut = 128;             // the accumulators of float32's low products
 };
 
@@ -202,7 +206,7 @@ __device__ __forceinline__ void store_out(const MmaArgs& a, const Item& item, in
 }
 
 template <int MODE, typename T, bool STREAM>
-__global__ void __launch_bounds__(kMmaThreads, 1)
+__global__ void __launch_bounds__((MmaShape<MODE, T, STREAM>::kThreads), 1)
 xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
                 const __grid_constant__ CUtensorMap col_map, const __grid_constant__ MmaArgs a) {
   using Shape = MmaShape<MODE, T, STREAM>;
@@ -230,7 +234,7 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
     }
     for (int k = 0; k < a.buffers; ++k) {
       tc::bar_init(s_full + 8 * k, 1);
-      tc::bar_init(s_done + 8 * k, MODE == kLoss ? 256 : 128);
+      tc::bar_init(s_done + 8 * k, MODE == kLoss ? 128 * Shape::kGroups : 128);
     }
     tc::bar_init(rows_full, 1);
     tc::bar_init(rows_empty, 1);
@@ -473,46 +477,51 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
       const int64_t row0 = (int64_t)item.row_tile * kTileRows;
       const int64_t row = row0 + quarter * 32 + lane;
       if (MODE == kLoss) {
-        // Each group takes 128 of a step's 256 columns.  The exponentials are taken relative to
+        // Each group takes 64 of a step's 256 columns.  The exponentials are taken relative to
         // `top`, a value of the row that an earlier step had as its maximum, so that they do
         // not wait for this step's maximum; only where that turns out 2^60 above it (or there
         // is none yet) is the step looked through again with the new one.
+        constexpr int kMine = Shape::kCols / Shape::kGroups;
         const bool warp_live = row0 + quarter * 32 < a.n_rows;
         float top = -INFINITY, sum = 0.f;
         for (int j = 0; j < item.steps; ++j) {
           if (!(ok = warp_wait(s_full + 8 * buf.at, buf.parity))) break;
           if (warp_live) {
             tc::fence_after();
-            const uint32_t s_at = lanes_at + tmem + buf.at * Shape::kCols + group * 128;
-            const int64_t left = a.n_cols - (int64_t)(item.first + j) * Shape::kCols - group * 128;
-            float largest[4], part[4];
+            const uint32_t s_at = lanes_at + tmem + buf.at * Shape::kCols + group * kMine;
+            const int64_t left = a.n_cols - (int64_t)(item.first + j) * Shape::kCols - group * kMine;
+            float2 part[2];
             auto pass = [&](bool with_sum) {
               const float off = top == -INFINITY ? 0.f : -top * scale;
+              float largest[2] = {-INFINITY, -INFINITY};
+              part[0] = part[1] = make_float2(0.f, 0.f);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                largest[k] = -INFINITY;
-                part[k] = 0.f;
-              }
-              float x[2][32];
-              tc::tmem_load32(s_at, x[0]);
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                float(&v)[32] = x[c & 1];
+              for (int c = 0; c < kMine / 32; ++c) {
+                float v[32];
+                tc::tmem_load32(s_at + c * 32, v);
                 tc::wait_ld32(v);
-                if (c < 3) tc::tmem_load32(s_at + (c + 1) * 32, x[(c + 1) & 1]);
                 if (left < (c + 1) * 32) {
 #pragma unroll
                   for (int k = 0; k < 32; ++k)
                     if (c * 32 + k >= left) v[k] = -INFINITY;
                 }
 #pragma unroll
-                for (int k = 0; k < 32; ++k) largest[k & 3] = fmaxf(largest[k & 3], v[k]);
+                for (int k = 0; k < 32; k += 4) {
+                  largest[0] = fmaxf(largest[0], fmaxf(v[k], v[k + 1]));
+                  largest[1] = fmaxf(largest[1], fmaxf(v[k + 2], v[k + 3]));
+                }
                 if (with_sum) {
 #pragma unroll
-                  for (int k = 0; k < 32; ++k) part[k & 3] += exp2_fast(fmaf(v[k], scale, off));
+                  for (int k = 0; k < 32; k += 2) {
+                    float2 x = __ffma2_rn(make_float2(v[k], v[k + 1]), make_float2(scale, scale),
+                                          make_float2(off, off));
+                    x.x = exp2_fast(x.x);
+                    x.y = exp2_fast(x.y);
+                    part[k >> 1 & 1] = __fadd2_rn(part[k >> 1 & 1], x);
+                  }
                 }
               }
-              return fmaxf(fmaxf(largest[0], largest[1]), fmaxf(largest[2], largest[3]));
+              return fmaxf(largest[0], largest[1]);
             };
             if (__any_sync(0xffffffffu, top == -INFINITY)) {
               const float m = pass(false);
@@ -527,14 +536,14 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
               }
               pass(true);
             }
-            sum += (part[0] + part[1]) + (part[2] + part[3]);
+            sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
             tc::fence_before();
           }
           tc::bar_arrive(s_done + 8 * buf.at);
           buf.next(a.buffers);
         }
         if (row < a.n_rows)
-          a.stats[(row * a.splits + item.split) * 2 + group] =
+          a.stats[(row * a.splits + item.split) * Shape::kGroups + group] =
               make_float2(top == -INFINITY ? -INFINITY : top * scale, sum);
       } else {
         // The groups take turns with the steps.
@@ -905,6 +914,7 @@ join_partial_kernel(const float* __restrict__ partial, int splits, int64_t rows,
 }
 
 // ------------------------------------------------------------------------- host --
+constexpr int kLossGroups = MmaShape<kLoss, float, false>::kGroups;
 constexpr int kSms = 148;  // the grids below are sized for B200's 148 SMs, one CTA each
 
 // How often the streamed operand is cut so that row_tiles x splits CTAs fill the machine: the
@@ -969,7 +979,7 @@ XentLayout xent_layout(int32_t dtype, int64_t n, int64_t vocab, int64_t feat_len
   l.abs_max = take(2 * kMaxPartials * 4);
   l.packed_feat = take((size_t)n * l.pitch * 2);
   l.packed_weight = take((size_t)vocab * l.pitch * 2);
-  l.stats = take((size_t)n * l.loss.splits * 2 * sizeof(float2));
+  l.stats = take((size_t)n * l.loss.splits * kLossGroups * sizeof(float2));
   if (with_grad) {
     l.row_bias = take((size_t)l.padded * 4);
     l.row_factor = take((size_t)l.padded * 4);
@@ -1102,7 +1112,7 @@ int launch_mma_as(const Batch& b, const XentLayout& l, const Operands& o, const 
   FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   const int64_t items = (int64_t)a.row_tiles * a.splits * a.chunks;
   if (items > INT32_MAX) return fail(FG_ERR_UNSUPPORTED, "too many tiles");
-  kernel<<<(int)std::min<int64_t>(items, kSms), kMmaThreads, smem, s>>>(row_map, col_map, a);
+  kernel<<<(int)std::min<int64_t>(items, kSms), Shape::kThreads, smem, s>>>(row_map, col_map, a);
   FG_CUDA_TRY(cudaGetLastError());
   return FG_OK;
 }
@@ -1128,7 +1138,7 @@ int loss_mma(const Batch& b, const XentLayout& l, char* ws, const T* feat, int64
   a.status = status;
   if (int rc = launch_mma<kLoss, T>(b, l, o, l.loss, a, s)) return rc;
   join_loss_kernel<T><<<(unsigned)((b.n + 7) / 8), 256, 0, s>>>(
-      b, feat, feat_ld, weight, weight_ld, a.stats, l.loss.splits * 2, loss, lse, status);
+      b, feat, feat_ld, weight, weight_ld, a.stats, l.loss.splits * kLossGroups, loss, lse, status);
   FG_CUDA_TRY(cudaGetLastError());
   return FG_OK;
 }
