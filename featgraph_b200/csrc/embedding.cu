@@ -19,11 +19,11 @@ __device__ __forceinline__ int64_t load_index(const void* ids, int wide, int64_t
 }
 
 // ------------------------------------------------------------------ lookup --
-// A group of `lanes` (a power of two, at most 32) lanes copies kRows rows side by side: their
-// ids first, then the kRows gathers, so that a lane has kRows loads of up to 16 bytes in
-// flight behind one round trip for the ids.
+// A group of `lanes` (a power of two, at most 32) lanes copies kLookupRows consecutive rows side
+// by side, so that a lane has that many loads of up to 16 bytes in flight, and has the ids of
+// its next rows on the way meanwhile.
 constexpr int kLookupThreads = 256;
-constexpr int kLookupRows = 4;
+constexpr int kLookupRows = 8;
 
 template <typename T, int N>
 __global__ void __launch_bounds__(kLookupThreads)
@@ -33,52 +33,42 @@ lookup_kernel(const T* __restrict__ table, int64_t table_ld, int64_t n_vertices,
   const int lanes = 1 << log_lanes;
   const int64_t group = ((int64_t)blockIdx.x * kLookupThreads + threadIdx.x) >> log_lanes;
   const int lane = threadIdx.x & (lanes - 1);
-  const int64_t n_groups = ((int64_t)gridDim.x * kLookupThreads) >> log_lanes;
-  for (int64_t first = group; first < n_ids; first += n_groups * kLookupRows) {
-    int64_t id[kLookupRows];
+  const int64_t stride = (((int64_t)gridDim.x * kLookupThreads) >> log_lanes) * kLookupRows;
+  int64_t first = group * kLookupRows;
+  int64_t id[kLookupRows];
+#pragma unroll
+  for (int u = 0; u < kLookupRows; ++u)
+    id[u] = first + u < n_ids ? load_index(ids, wide, first + u) : 0;
+  for (; first < n_ids; first += stride) {
+    bool ok[kLookupRows];
+    int64_t from[kLookupRows];
 #pragma unroll
     for (int u = 0; u < kLookupRows; ++u) {
-      const int64_t i = first + u * n_groups;
-      id[u] = i < n_ids ? load_index(ids, wide, i) : 0;
-    }
-    bool bad[kLookupRows];
-#pragma unroll
-    for (int u = 0; u < kLookupRows; ++u) {
-      bad[u] = (uint64_t)id[u] >= (uint64_t)n_vertices;
-      if (bad[u] && lane == 0) *status = FG_STATUS_BAD_INDEX;
+      const bool in = first + u < n_ids;
+      ok[u] = in && (uint64_t)id[u] < (uint64_t)n_vertices;
+      if (in && !ok[u] && lane == 0) *status = FG_STATUS_BAD_INDEX;
+      from[u] = id[u] * table_ld;
+      id[u] = first + stride + u < n_ids ? load_index(ids, wide, first + stride + u) : 0;
     }
     for (int c = lane * N; c < feat_len; c += lanes * N) {
       Vec<T, N> row[kLookupRows];
 #pragma unroll
       for (int u = 0; u < kLookupRows; ++u)
-        if (!bad[u] && first + u * n_groups < n_ids)
-          row[u] = load_vec<T, N>(table + id[u] * table_ld + c);
+        if (ok[u]) row[u] = load_vec<T, N>(table + from[u] + c);
 #pragma unroll
       for (int u = 0; u < kLookupRows; ++u) {
-        const int64_t i = first + u * n_groups;
-        if (i >= n_ids) break;
+        if (first + u >= n_ids) break;
 #pragma unroll
         for (int k = 0; k < N; ++k)
-          row[u].v[k] = from_float<T>(bad[u] ? __int_as_float(0x7fc00000)
-                                             : to_float<T>(row[u].v[k]) * scale);
-        store_vec_stream<T, N>(out + i * out_ld + c, row[u]);
+          row[u].v[k] = from_float<T>(ok[u] ? to_float<T>(row[u].v[k]) * scale
+                                            : __int_as_float(0x7fc00000));
+        store_vec_stream<T, N>(out + (first + u) * out_ld + c, row[u]);
       }
     }
   }
 }
 
 // ------------------------------------------------------- gradient: the sort --
-// Stable least-significant-digit radix sort of (id, position) pairs, at most 9 bits a pass:
-// per block of kSortTile keys a histogram (sort_count_kernel), per digit an exclusive sum over
-// the blocks (sort_scan_kernel), then every key to its place (sort_place_kernel).  Equal ids
-// keep the order of their positions, so the sums below run in an order that only the ids fix.
-constexpr int kSortThreads = 256;
-constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortItems = 16;
-constexpr int kSortTile = kSortThreads * kSortItems;
-constexpr int kMaxDigitBits = 9;
-constexpr int kMaxBins = 1 << kMaxDigitBits;
-
 // The key of position i: its id, or n_vertices for a row that gets no gradient (the padding
 // id, or an id out of range), which sorts behind every vertex.
 struct KeySource {
@@ -100,21 +90,103 @@ __device__ __forceinline__ uint32_t source_key(const KeySource& s, int64_t i) {
   return id == s.padding ? (uint32_t)s.n_vertices : (uint32_t)id;
 }
 
+// The table's gradient starts as zeros: CTAs of the sort's first kernel write them while the
+// others wait for memory anyway.  `bytes` of it at `to`.
+struct ZeroFill {
+  uint8_t* to;
+  int64_t bytes;
+};
+__device__ __forceinline__ void zero_fill(const ZeroFill& z, int block, int blocks, int threads) {
+  const int64_t head = min(z.bytes, (int64_t)((16 - (uintptr_t)z.to % 16) % 16));
+  const int64_t vecs = (z.bytes - head) / 16;
+  uint4* at = reinterpret_cast<uint4*>(z.to + head);
+  for (int64_t i = (int64_t)block * threads + threadIdx.x; i < vecs; i += (int64_t)blocks * threads)
+    at[i] = make_uint4(0, 0, 0, 0);
+  if (block == 0) {
+    for (int64_t i = threadIdx.x; i < head; i += threads) z.to[i] = 0;
+    for (int64_t i = head + vecs * 16 + threadIdx.x; i < z.bytes; i += threads) z.to[i] = 0;
+  }
+}
+
+// Up to kRankMost ids: every position counts the pairs before it, (id, position) in order, and
+// that is its place.  n^2 comparisons, but one launch of a few microseconds (5003 ids: 3 us)
+// where the six of the radix sort take 30.
+constexpr int64_t kRankMost = 8192;
+constexpr int kRankThreads = 256;
+constexpr int kRankParts = 8;              // threads that share one position's comparisons
+constexpr int kRankTile = kRankThreads / kRankParts;
+
+__global__ void __launch_bounds__(kRankThreads)
+rank_kernel(KeySource src, int n, int sort_blocks, ZeroFill zero, uint32_t* __restrict__ keys_out,
+            uint32_t* __restrict__ positions_out) {
+  if ((int)blockIdx.x >= sort_blocks) {
+    zero_fill(zero, blockIdx.x - sort_blocks, gridDim.x - sort_blocks, kRankThreads);
+    return;
+  }
+  __shared__ __align__(16) uint32_t keys[kRankMost];
+  const int whole = (n + 31) / 32 * 32;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < whole; i += kRankThreads)
+    keys[i] = i < n ? source_key(src, i) : 0xffffffffu;
+  __syncthreads();
+  const int i = blockIdx.x * kRankTile + threadIdx.x / kRankParts;
+  const int part = threadIdx.x % kRankParts;
+  const uint32_t mine = i < n ? keys[i] : 0;
+  uint32_t before = 0;
+#pragma unroll 4
+  for (int k = part * 4; k < whole; k += kRankParts * 4) {
+    const uint4 q = *reinterpret_cast<const uint4*>(&keys[k]);
+    // equal ids count where they stand earlier
+    before += q.x < mine + (k < i);
+    before += q.y < mine + (k + 1 < i);
+    before += q.z < mine + (k + 2 < i);
+    before += q.w < mine + (k + 3 < i);
+  }
+#pragma unroll
+  for (int d = 1; d < kRankParts; d <<= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
+  if (part == 0 && i < n) {
+    keys_out[before] = mine;
+    positions_out[before] = i;
+  }
+}
+
+// Stable least-significant-digit radix sort of (id, position) pairs, at most 9 bits a pass:
+// per block of kSortTile keys a histogram (sort_count_kernel), per digit an exclusive sum over
+// the blocks (sort_scan_kernel), then every key to its place (sort_place_kernel).  Equal ids
+// keep the order of their positions, so the sums below run in an order that only the ids fix.
+// All keys of a thread are loaded before the first is used: with the loads inside the ranking
+// rounds a block took 22 us for its sixteen.
+constexpr int kSortThreads = 256;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortItems = 16;
+constexpr int kSortTile = kSortThreads * kSortItems;
+constexpr int kMaxDigitBits = 9;
+constexpr int kMaxBins = 1 << kMaxDigitBits;
+
 __global__ void __launch_bounds__(kSortThreads)
-sort_count_kernel(KeySource src, int64_t n, int shift, int bits, uint32_t* __restrict__ counts) {
+sort_count_kernel(KeySource src, int64_t n, int shift, int bits, uint32_t* __restrict__ counts,
+                  int sort_blocks, ZeroFill zero) {
+  if ((int)blockIdx.x >= sort_blocks) {
+    zero_fill(zero, blockIdx.x - sort_blocks, gridDim.x - sort_blocks, kSortThreads);
+    return;
+  }
   __shared__ uint32_t hist[kMaxBins];
   const int bins = 1 << bits;
-  for (int b = threadIdx.x; b < bins; b += kSortThreads) hist[b] = 0;
-  __syncthreads();
   const int64_t base = (int64_t)blockIdx.x * kSortTile;
-#pragma unroll 4
+  uint32_t key[kSortItems];
+#pragma unroll
   for (int k = 0; k < kSortItems; ++k) {
     const int64_t i = base + k * kSortThreads + threadIdx.x;
-    if (i < n) atomicAdd(&hist[(source_key(src, i) >> shift) & (bins - 1)], 1u);
+    key[k] = i < n ? source_key(src, i) : 0;
   }
+  for (int b = threadIdx.x; b < bins; b += kSortThreads) hist[b] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kSortItems; ++k)
+    if (base + k * kSortThreads + threadIdx.x < n) atomicAdd(&hist[(key[k] >> shift) & (bins - 1)], 1u);
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += kSortThreads)
-    counts[(int64_t)b * gridDim.x + blockIdx.x] = hist[b];
+    counts[(int64_t)b * sort_blocks + blockIdx.x] = hist[b];
 }
 
 // One warp per digit: counts[digit][block] becomes the digit's count in the blocks before.
@@ -126,17 +198,21 @@ sort_scan_kernel(uint32_t* __restrict__ counts, int n_blocks, int bins,
   if (digit >= bins) return;
   uint32_t* row = counts + (int64_t)digit * n_blocks;
   uint32_t running = 0;
-  for (int b0 = 0; b0 < n_blocks; b0 += 32) {
-    const int b = b0 + lane;
-    const uint32_t c = b < n_blocks ? row[b] : 0;
-    uint32_t incl = c;
+  for (int b0 = 0; b0 < n_blocks; b0 += 256) {
+    uint32_t c[8];
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const uint32_t up = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += up;
+    for (int k = 0; k < 8; ++k) c[k] = b0 + k * 32 + lane < n_blocks ? row[b0 + k * 32 + lane] : 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      uint32_t incl = c[k];
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += up;
+      }
+      if (b0 + k * 32 + lane < n_blocks) row[b0 + k * 32 + lane] = running + incl - c[k];
+      running += __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (b < n_blocks) row[b] = running + incl - c;
-    running += __shfl_sync(0xffffffffu, incl, 31);
   }
   if (lane == 0) totals[digit] = running;
 }
@@ -146,19 +222,31 @@ sort_place_kernel(KeySource src, int64_t n, int shift, int bits,
                   const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals,
                   uint32_t* __restrict__ keys_out, uint32_t* __restrict__ positions_out) {
   __shared__ uint32_t warp_hist[kSortWarps][kMaxBins];
-  __shared__ uint32_t base[kMaxBins];
   __shared__ uint32_t warp_sum[kSortWarps];
   const int bins = 1 << bits;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // each warp takes kSortItems * 32 consecutive keys, 32 at a time and in order
+  const int64_t first = (int64_t)blockIdx.x * kSortTile + warp * (kSortItems * 32);
+  uint32_t key[kSortItems], position[kSortItems];
+#pragma unroll
+  for (int k = 0; k < kSortItems; ++k) {
+    const int64_t i = first + k * 32 + lane;
+    key[k] = i < n ? source_key(src, i) : 0;
+    position[k] = i < n && src.keys ? src.positions[i] : (uint32_t)i;
+  }
+  // this block's first place of the digits of a thread: what smaller digits take in all, and
+  // what the same digit takes in the blocks before
+  constexpr int kPer = kMaxBins / kSortThreads;
+  uint32_t total[kPer], ahead[kPer], mine = 0;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int b = threadIdx.x * kPer + k;
+    total[k] = b < bins ? totals[b] : 0;
+    ahead[k] = b < bins ? counts[(int64_t)b * gridDim.x + blockIdx.x] : 0;
+    mine += total[k];
+  }
   for (int b = threadIdx.x; b < kSortWarps * kMaxBins; b += kSortThreads)
     (&warp_hist[0][0])[b] = 0;
-  // exclusive sum of the digits' totals: bins / kSortThreads = at most two digits a thread
-  const int per = (bins + kSortThreads - 1) / kSortThreads;
-  uint32_t mine = 0;
-  for (int k = 0; k < per; ++k) {
-    const int b = threadIdx.x * per + k;
-    if (b < bins) mine += totals[b];
-  }
   uint32_t incl = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -167,23 +255,10 @@ sort_place_kernel(KeySource src, int64_t n, int shift, int bits,
   }
   if (lane == 31) warp_sum[warp] = incl;
   __syncthreads();
-  uint32_t before = incl - mine;
-  for (int w = 0; w < warp; ++w) before += warp_sum[w];
-  for (int k = 0; k < per; ++k) {
-    const int b = threadIdx.x * per + k;
-    if (b < bins) {
-      base[b] = before + counts[(int64_t)b * gridDim.x + blockIdx.x];
-      before += totals[b];
-    }
-  }
-  // each warp takes kSortItems * 32 consecutive keys, 32 at a time and in order
-  const int64_t first = (int64_t)blockIdx.x * kSortTile + warp * (kSortItems * 32);
-  uint32_t key[kSortItems], rank[kSortItems];
+  uint32_t rank[kSortItems];
 #pragma unroll
   for (int k = 0; k < kSortItems; ++k) {
-    const int64_t i = first + k * 32 + lane;
-    const bool live = i < n;
-    key[k] = live ? source_key(src, i) : 0;
+    const bool live = first + k * 32 + lane < n;
     const uint32_t digit = live ? (key[k] >> shift) & (bins - 1) : (uint32_t)bins;
     const uint32_t peers = __match_any_sync(0xffffffffu, digit);
     const uint32_t below = __popc(peers & ((1u << lane) - 1));
@@ -195,23 +270,29 @@ sort_place_kernel(KeySource src, int64_t n, int shift, int bits,
     rank[k] = old + below;
   }
   __syncthreads();
-  for (int b = threadIdx.x; b < bins; b += kSortThreads) {
-    uint32_t run = base[b];
+  uint32_t before = incl - mine;
+  for (int w = 0; w < warp; ++w) before += warp_sum[w];
 #pragma unroll
-    for (int w = 0; w < kSortWarps; ++w) {
-      const uint32_t c = warp_hist[w][b];
-      warp_hist[w][b] = run;
-      run += c;
+  for (int k = 0; k < kPer; ++k) {
+    const int b = threadIdx.x * kPer + k;
+    if (b < bins) {
+      uint32_t run = before + ahead[k];
+#pragma unroll
+      for (int w = 0; w < kSortWarps; ++w) {
+        const uint32_t c = warp_hist[w][b];
+        warp_hist[w][b] = run;
+        run += c;
+      }
     }
+    before += total[k];
   }
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kSortItems; ++k) {
-    const int64_t i = first + k * 32 + lane;
-    if (i >= n) continue;
+    if (first + k * 32 + lane >= n) continue;
     const uint32_t at = warp_hist[warp][(key[k] >> shift) & (bins - 1)] + rank[k];
     keys_out[at] = key[k];
-    positions_out[at] = src.keys ? src.positions[i] : (uint32_t)i;
+    positions_out[at] = position[k];
   }
 }
 
@@ -227,114 +308,211 @@ __device__ __forceinline__ void store_grad_row(T* p, const float (&acc)[N], floa
   store_vec<T, N>(p, v);
 }
 
-// The sorted list is cut into pieces of `piece` positions; a group of lanes walks one piece
-// and sums its rows.  A vertex whose rows all lie inside the piece is written at once; the sum
-// of one that began in an earlier piece goes to partial[piece][0], of one that goes on into
-// the next piece to partial[piece][1] (a piece that is one vertex throughout uses only [0]
-// unless the vertex begins there), and join_kernel adds those up in order.
+// The sorted list, a run of equal keys per vertex.  A run of up to `window` rows is summed by
+// one group of lanes; of a longer one every window of the list (positions that are a multiple
+// of `window` and those behind) sums its part in a CTA of its own, and join_kernel adds the
+// parts up in order.
+struct Runs {
+  const uint32_t *keys, *positions;
+  int64_t n;
+  uint32_t none;             // the key of rows that go nowhere
+  int window;
+};
 constexpr int kSumThreads = 256;
-constexpr int kSumAhead = 8;
+constexpr int kSumAhead = 8;   // rows in flight per lane
+constexpr int kSumPiece = 32;  // positions whose runs (those that begin there) a group sums
+
+// What part of long runs a window holds: its first `head` rows belong to one that began in an
+// earlier window or on its first row; the rows from `tail` on to one that begins later in it.
+struct WindowParts {
+  int head, tail, count;
+  bool head_begins;
+};
+__device__ WindowParts find_parts(const Runs& r, int64_t window_index) {
+  __shared__ int shared_head, shared_tail, shared_back;
+  const int64_t begin = window_index * r.window;
+  WindowParts p;
+  p.count = (int)(r.n - begin < r.window ? r.n - begin : r.window);
+  const uint32_t first = r.keys[begin], last = r.keys[begin + p.count - 1];
+  if (threadIdx.x == 0) {
+    shared_head = p.count;
+    shared_tail = -1;
+    shared_back = 0;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < r.window; i += kSumThreads) {
+    if (i < p.count) {
+      const uint32_t key = r.keys[begin + i];
+      if (key != first) atomicMin(&shared_head, i);
+      if (key != last) atomicMax(&shared_tail, i);
+    }
+    // rows of the first run in front of the window
+    if (begin - 1 - i >= 0 && r.keys[begin - 1 - i] == first) atomicMax(&shared_back, i + 1);
+  }
+  __syncthreads();
+  p.head = shared_head;
+  p.tail = shared_tail + 1;
+  const int64_t start = begin - shared_back;
+  // a run is long if the row `window` behind its first is of the same vertex
+  auto is_long = [&](int64_t s, uint32_t key) {
+    return key != r.none && s + r.window < r.n && r.keys[s + r.window] == key;
+  };
+  p.head_begins = shared_back == 0;
+  const bool long_head = shared_back == r.window ? first != r.none : is_long(start, first);
+  const bool long_tail = p.tail > 0 && is_long(begin + p.tail, last);
+  if (!long_head) p.head = 0;
+  if (!long_tail) p.tail = p.count;
+  return p;
+}
+
+// The sum of `count` rows from position `from` on, all threads of the CTA, into to[feat_len].
+template <typename T, int N>
+__device__ void sum_part(const Runs& r, int64_t from, int count, const T* out_grad,
+                         int64_t out_grad_ld, int feat_len, int log_lanes, float* to) {
+  __shared__ __align__(16) float sums[kSumThreads * N];
+  const int lanes = 1 << log_lanes, groups = kSumThreads >> log_lanes;
+  const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> log_lanes;
+  for (int c0 = 0; c0 < feat_len; c0 += lanes * N) {
+    const int c = c0 + lane * N;
+    float acc[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) acc[k] = 0.f;
+    if (c < feat_len) {
+#pragma unroll 8
+      for (int i = group; i < count; i += groups) {
+        const Vec<T, N> row =
+            load_vec_stream<T, N>(out_grad + (int64_t)r.positions[from + i] * out_grad_ld + c);
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] += to_float<T>(row.v[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) sums[threadIdx.x * N + k] = acc[k];
+    __syncthreads();
+    // a thread per column adds the groups' sums in order
+    for (int i = threadIdx.x; i < lanes * N; i += kSumThreads) {
+      float s = 0.f;
+      for (int g = 0; g < groups; ++g) s += sums[g * lanes * N + i];
+      if (c0 + i < feat_len) to[c0 + i] = s;
+    }
+    __syncthreads();
+  }
+}
 
 template <typename T, int N>
 __global__ void __launch_bounds__(kSumThreads)
-sum_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ positions, int64_t n,
-           int64_t n_vertices, const T* __restrict__ out_grad, int64_t out_grad_ld, int feat_len,
+sum_kernel(Runs r, int n_windows, const T* __restrict__ out_grad, int64_t out_grad_ld, int feat_len,
            float scale, int accumulate, T* __restrict__ grad, float* __restrict__ partial,
-           int piece, int log_lanes, int slabs) {
+           int log_lanes, int slabs) {
+  if ((int)blockIdx.x < n_windows) {  // the long runs' windows come first: they take longest
+    const int64_t w = blockIdx.x;
+    const WindowParts p = find_parts(r, w);
+    const int64_t begin = w * r.window;
+    if (p.head > 0)
+      sum_part<T, N>(r, begin, p.head, out_grad, out_grad_ld, feat_len, log_lanes,
+                     partial + (w * 2 + 0) * feat_len);
+    if (p.tail < p.count)
+      sum_part<T, N>(r, begin + p.tail, p.count - p.tail, out_grad, out_grad_ld, feat_len, log_lanes,
+                     partial + (w * 2 + 1) * feat_len);
+    return;
+  }
   const int lanes = 1 << log_lanes;
-  const int64_t item = ((int64_t)blockIdx.x * kSumThreads + threadIdx.x) >> log_lanes;
-  const int64_t p = item / slabs;
-  const int c = ((int)(item - p * slabs) * lanes + (threadIdx.x & (lanes - 1))) * N;
-  const int64_t begin = p * piece;
-  if (begin >= n || c >= feat_len) return;
-  const int64_t end = begin + piece < n ? begin + piece : n;
-  const uint32_t none = (uint32_t)n_vertices;
-  uint32_t current = keys[begin];
-  bool open_before = begin > 0 && keys[begin - 1] == current;
+  const int64_t item = ((int64_t)(blockIdx.x - n_windows) * kSumThreads + threadIdx.x) >> log_lanes;
+  const int64_t piece = item / slabs;
+  const int c = ((int)(item - piece * slabs) * lanes + (threadIdx.x & (lanes - 1))) * N;
+  const int64_t begin = piece * kSumPiece;
+  if (begin >= r.n || c >= feat_len) return;
+  const int64_t end = begin + kSumPiece < r.n ? begin + kSumPiece : r.n;
+  uint32_t current = r.none;
+  bool mine = false;                   // whether the current run is this group's to sum
+  if (begin > 0) current = r.keys[begin - 1];
   float acc[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) acc[k] = 0.f;
-  for (int64_t j = begin; j < end; j += kSumAhead) {
-    uint32_t key[kSumAhead];
+  // behind the piece's end only the run that is under way goes on
+  for (int64_t j = begin; j < end || (mine && j < r.n && r.keys[j] == current); j += kSumAhead) {
+    uint32_t key[kSumAhead], position[kSumAhead];
+    // the arrays are padded to a multiple of kSumAhead; what lies behind n is not looked at
+#pragma unroll
+    for (int u = 0; u < kSumAhead; u += 4) {
+      *reinterpret_cast<uint4*>(&key[u]) = *reinterpret_cast<const uint4*>(r.keys + j + u);
+      *reinterpret_cast<uint4*>(&position[u]) = *reinterpret_cast<const uint4*>(r.positions + j + u);
+    }
+    // which of these rows count: those of runs that begin in the piece and are not long
+    bool take[kSumAhead], starts[kSumAhead];
+    uint32_t at = current;
+    bool is_mine = mine;
+#pragma unroll
+    for (int u = 0; u < kSumAhead; ++u) {
+      starts[u] = j + u < r.n && key[u] != at;
+      if (starts[u]) {
+        at = key[u];
+        is_mine = j + u < end && at != r.none;
+        if (is_mine && j + u + r.window < r.n && r.keys[j + u + r.window] == at) is_mine = false;
+      }
+      take[u] = is_mine && j + u < r.n;
+    }
     Vec<T, N> row[kSumAhead];
 #pragma unroll
-    for (int u = 0; u < kSumAhead; ++u) {
-      key[u] = j + u < end ? keys[j + u] : none;
-      if (key[u] != none)
-        row[u] = load_vec_stream<T, N>(out_grad + (int64_t)positions[j + u] * out_grad_ld + c);
-    }
+    for (int u = 0; u < kSumAhead; ++u)
+      if (take[u]) row[u] = load_vec_stream<T, N>(out_grad + (int64_t)position[u] * out_grad_ld + c);
 #pragma unroll
     for (int u = 0; u < kSumAhead; ++u) {
-      if (j + u >= end) break;
-      if (key[u] != current) {
-        if (current != none) {
-          if (open_before) {
-            float* to = partial + (p * 2 + 0) * feat_len + c;
-#pragma unroll
-            for (int k = 0; k < N; ++k) to[k] = acc[k];
-          } else {
-            store_grad_row<T, N>(grad + (int64_t)current * feat_len + c, acc, scale, accumulate);
-          }
-        }
-        open_before = false;
+      if (starts[u]) {
+        if (mine) store_grad_row<T, N>(grad + (int64_t)current * feat_len + c, acc, scale, accumulate);
         current = key[u];
+        mine = take[u];
 #pragma unroll
         for (int k = 0; k < N; ++k) acc[k] = 0.f;
       }
-      if (key[u] != none) {
+      if (take[u]) {
 #pragma unroll
         for (int k = 0; k < N; ++k) acc[k] += to_float<T>(row[u].v[k]);
       }
     }
   }
-  if (current == none) return;
-  const bool open_after = end < n && keys[end] == current;
-  if (!open_before && !open_after) {
-    store_grad_row<T, N>(grad + (int64_t)current * feat_len + c, acc, scale, accumulate);
-  } else {
-    float* to = partial + (p * 2 + (open_before ? 0 : 1)) * feat_len + c;
-#pragma unroll
-    for (int k = 0; k < N; ++k) to[k] = acc[k];
-  }
+  if (mine) store_grad_row<T, N>(grad + (int64_t)current * feat_len + c, acc, scale, accumulate);
 }
 
-// One CTA per piece; works only where a vertex begins in the piece and goes on behind it.  Its
-// partial sums are partial[piece][1], then partial[q][0] of the pieces q that it reaches:
-// every column's are cut into kJoinParts runs, summed in order, and the runs added in order.
+// A CTA per window; works only where a long run begins in it.  Its parts are this window's and
+// the heads of the windows behind: cut into kJoinParts runs, each summed in order, and these
+// added in order.
 constexpr int kJoinParts = 8;
 constexpr int kJoinColumns = 32;
 
 template <typename T>
-__global__ void __launch_bounds__(kJoinParts * kJoinColumns)
-join_kernel(const uint32_t* __restrict__ keys, int64_t n, int64_t n_vertices, int feat_len,
-            float scale, int accumulate, T* __restrict__ grad, const float* __restrict__ partial,
-            int piece) {
-  const int64_t p = blockIdx.x;
-  const int64_t end = (p + 1) * piece;
-  if (end >= n) return;
-  const uint32_t key = keys[end - 1];
-  if (key == (uint32_t)n_vertices || keys[end] != key) return;
-  const int64_t begin = p * piece;
-  if (begin > 0 && keys[begin] == key && keys[begin - 1] == key) return;  // it began earlier
-  // the last piece that the vertex reaches: the first position behind it, by bisection
-  int64_t lo = end, hi = n;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (keys[mid] == key) lo = mid + 1; else hi = mid;
+__global__ void __launch_bounds__(kSumThreads)
+join_kernel(Runs r, int feat_len, float scale, int accumulate, T* __restrict__ grad,
+            const float* __restrict__ partial) {
+  static_assert(kJoinParts * kJoinColumns == kSumThreads, "one thread per part and column");
+  const int64_t w = blockIdx.x;
+  const int64_t behind = (w + 1) * r.window;   // a long run goes on in the next window
+  if (behind >= r.n || r.keys[behind - 1] == r.none || r.keys[behind] != r.keys[behind - 1]) return;
+  const WindowParts p = find_parts(r, w);
+  int slot;
+  if (p.tail < p.count) slot = 1;
+  else if (p.head > 0 && p.head_begins) slot = 0;
+  else return;
+  const uint32_t key = r.keys[behind - 1];
+  // how many windows behind this one begin with the same vertex
+  int64_t terms = 1;
+  for (bool more = true; more;) {
+    const int64_t at = (w + terms + threadIdx.x) * r.window;
+    const int same = __syncthreads_count(at < r.n && r.keys[at] == key);
+    terms += same;
+    more = same == kSumThreads;
   }
-  const int64_t last = (lo - 1) / piece;
-  const int64_t terms = last - p + 1;
   const int part = threadIdx.x / kJoinColumns, lane = threadIdx.x % kJoinColumns;
   const int64_t per = (terms + kJoinParts - 1) / kJoinParts;
+  const int64_t t1 = (part + 1) * per < terms ? (part + 1) * per : terms;
   __shared__ float sums[kJoinParts][kJoinColumns];
   for (int c0 = 0; c0 < feat_len; c0 += kJoinColumns) {
     const int c = c0 + lane;
     float s = 0.f;
     if (c < feat_len) {
-      const int64_t t1 = (part + 1) * per < terms ? (part + 1) * per : terms;
 #pragma unroll 8
       for (int64_t t = part * per; t < t1; ++t)
-        s += partial[((p + t) * 2 + (t == 0 ? 1 : 0)) * feat_len + c];
+        s += partial[((w + t) * 2 + (t == 0 ? slot : 0)) * feat_len + c];
     }
     sums[part][lane] = s;
     __syncthreads();
@@ -357,16 +535,19 @@ int ceil_log2(int64_t v) {
 }
 
 struct GradLayout {
-  int piece;
-  int64_t pieces, blocks;
+  bool rank;                 // few ids: rank_kernel instead of the radix sort
+  int window;
+  int64_t windows, blocks;
   int passes, digit_bits;
   size_t keys[2], positions[2], counts, totals, partial, total;
 };
 
 GradLayout grad_layout(int64_t n, int64_t n_vertices, int64_t feat_len) {
   GradLayout l;
-  l.piece = 32;
-  l.pieces = (n + l.piece - 1) / l.piece;
+  l.rank = n <= kRankMost;
+  // few rows: short windows, so that no group of lanes walks a long run alone
+  l.window = l.rank ? 64 : 256;
+  l.windows = (n + l.window - 1) / l.window;
   l.blocks = (n + kSortTile - 1) / kSortTile;
   const int bits = std::max(1, ceil_log2(n_vertices + 1));  // n_vertices itself is a key
   l.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
@@ -377,13 +558,15 @@ GradLayout grad_layout(int64_t n, int64_t n_vertices, int64_t feat_len) {
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < (l.rank ? 1 : 2); ++k) {
     l.keys[k] = take((size_t)n * 4);
     l.positions[k] = take((size_t)n * 4);
   }
-  l.counts = take(((size_t)l.blocks << l.digit_bits) * 4);
-  l.totals = take(kMaxBins * 4);
-  l.partial = take((size_t)l.pieces * 2 * feat_len * 4);
+  if (!l.rank) {
+    l.counts = take(((size_t)l.blocks << l.digit_bits) * 4);
+    l.totals = take(kMaxBins * 4);
+  }
+  l.partial = take((size_t)l.windows * 2 * feat_len * 4);
   l.total = at;
   return l;
 }
@@ -431,7 +614,7 @@ extern "C" int fg_embedding_lookup(const void* table_dev, int32_t dtype, int64_t
   const int log_lanes = std::min(5, ceil_log2(per_row));
   const int64_t groups_per_block = kLookupThreads >> log_lanes;
   const int64_t want = (n_ids + groups_per_block * kLookupRows - 1) / (groups_per_block * kLookupRows);
-  const int grid = (int)std::min<int64_t>(std::max<int64_t>(want, 1), 1 << 20);
+  const int grid = (int)std::min<int64_t>(std::max<int64_t>(want, 1), 148 * 4);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
 #define FG_LOOKUP(T, N)                                                                        \
   lookup_kernel<T, N><<<grid, kLookupThreads, 0, s>>>(                                         \
@@ -489,42 +672,56 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
                                       (uint64_t)(uintptr_t)grad_dev, (uint64_t)(out_grad_ld * es),
                                       (uint64_t)(feat_len * es)});
   if (vb < (int)es) return fail(FG_ERR_INVALID_ARGUMENT, "a pointer is not aligned to its type");
-  if (!accumulate && n_vertices > 0)
-    FG_CUDA_TRY(cudaMemsetAsync(grad_dev, 0, (size_t)n_vertices * feat_len * es, s));
-  if (n_ids == 0) return FG_OK;
+  const ZeroFill zero = {static_cast<uint8_t*>(grad_dev),
+                         accumulate ? 0 : (int64_t)((size_t)n_vertices * feat_len * es)};
+  if (n_ids == 0) {
+    if (zero.bytes > 0) FG_CUDA_TRY(cudaMemsetAsync(grad_dev, 0, zero.bytes, s));
+    return FG_OK;
+  }
+  const int zero_blocks = (int)std::min<int64_t>(4 * 148, (zero.bytes + 65535) / 65536);
 
   char* ws = static_cast<char*>(workspace_dev);
   uint32_t* keys[2] = {reinterpret_cast<uint32_t*>(ws + l.keys[0]),
                        reinterpret_cast<uint32_t*>(ws + l.keys[1])};
   uint32_t* positions[2] = {reinterpret_cast<uint32_t*>(ws + l.positions[0]),
                             reinterpret_cast<uint32_t*>(ws + l.positions[1])};
-  uint32_t* counts = reinterpret_cast<uint32_t*>(ws + l.counts);
-  uint32_t* totals = reinterpret_cast<uint32_t*>(ws + l.totals);
   float* partial = reinterpret_cast<float*>(ws + l.partial);
   KeySource src = {ids_dev, nullptr, nullptr, index_type == FG_INDEX_INT64, n_vertices,
                    padding_id < 0 ? -1 : padding_id, status_dev};
-  const int bins = 1 << l.digit_bits;
-  for (int pass = 0; pass < l.passes; ++pass) {
-    const int shift = pass * l.digit_bits;
-    sort_count_kernel<<<(int)l.blocks, kSortThreads, 0, s>>>(src, n_ids, shift, l.digit_bits, counts);
-    sort_scan_kernel<<<(bins + kSortWarps - 1) / kSortWarps, kSortThreads, 0, s>>>(
-        counts, (int)l.blocks, bins, totals);
-    sort_place_kernel<<<(int)l.blocks, kSortThreads, 0, s>>>(
-        src, n_ids, shift, l.digit_bits, counts, totals, keys[pass & 1], positions[pass & 1]);
-    src.keys = keys[pass & 1];
-    src.positions = positions[pass & 1];
+  if (l.rank) {
+    const int blocks = (int)((n_ids + kRankTile - 1) / kRankTile);
+    rank_kernel<<<blocks + zero_blocks, kRankThreads, 0, s>>>(src, (int)n_ids, blocks, zero, keys[0],
+                                                              positions[0]);
+    src.keys = keys[0];
+    src.positions = positions[0];
+  } else {
+    uint32_t* counts = reinterpret_cast<uint32_t*>(ws + l.counts);
+    uint32_t* totals = reinterpret_cast<uint32_t*>(ws + l.totals);
+    const int bins = 1 << l.digit_bits;
+    for (int pass = 0; pass < l.passes; ++pass) {
+      const int shift = pass * l.digit_bits;
+      sort_count_kernel<<<(int)l.blocks + (pass == 0 ? zero_blocks : 0), kSortThreads, 0, s>>>(
+          src, n_ids, shift, l.digit_bits, counts, (int)l.blocks, zero);
+      sort_scan_kernel<<<(bins + kSortWarps - 1) / kSortWarps, kSortThreads, 0, s>>>(
+          counts, (int)l.blocks, bins, totals);
+      sort_place_kernel<<<(int)l.blocks, kSortThreads, 0, s>>>(
+          src, n_ids, shift, l.digit_bits, counts, totals, keys[pass & 1], positions[pass & 1]);
+      src.keys = keys[pass & 1];
+      src.positions = positions[pass & 1];
+    }
   }
+  const Runs runs = {src.keys, src.positions, n_ids, (uint32_t)n_vertices, l.window};
   const int per_row = (int)((feat_len * es + vb - 1) / vb);
   const int log_lanes = std::min(5, ceil_log2(per_row));
   const int slabs = (per_row + (1 << log_lanes) - 1) >> log_lanes;
-  const int64_t threads = (l.pieces * slabs) << log_lanes;
-  const int64_t grid = (threads + kSumThreads - 1) / kSumThreads;
+  const int64_t pieces = (n_ids + kSumPiece - 1) / kSumPiece;
+  const int64_t threads = (pieces * slabs) << log_lanes;
+  const int64_t grid = l.windows + (threads + kSumThreads - 1) / kSumThreads;
   if (grid > INT32_MAX) return fail(FG_ERR_UNSUPPORTED, "n_ids x feat_len is too large");
 #define FG_SUM(T, N)                                                                          \
   sum_kernel<T, N><<<(int)grid, kSumThreads, 0, s>>>(                                         \
-      src.keys, src.positions, n_ids, n_vertices, static_cast<const T*>(out_grad_dev),        \
-      out_grad_ld, (int)feat_len, scale, accumulate, static_cast<T*>(grad_dev), partial,      \
-      l.piece, log_lanes, slabs)
+      runs, (int)l.windows, static_cast<const T*>(out_grad_dev), out_grad_ld, (int)feat_len,  \
+      scale, accumulate, static_cast<T*>(grad_dev), partial, log_lanes, slabs)
 #define FG_SUM_T(T)                                                       \
   switch (vb / (int)sizeof(T)) {                                          \
     case 8: if constexpr (sizeof(T) == 2) FG_SUM(T, 8 / (sizeof(T) / 2)); break; \
@@ -532,9 +729,9 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
     case 2: FG_SUM(T, 2); break;                                          \
     default: FG_SUM(T, 1); break;                                         \
   }                                                                       \
-  join_kernel<T><<<(int)l.pieces, kJoinParts * kJoinColumns, 0, s>>>(     \
-      src.keys, n_ids, n_vertices, (int)feat_len, scale, accumulate,      \
-      static_cast<T*>(grad_dev), partial, l.piece);
+  if (n_ids > l.window)                                                   \
+    join_kernel<T><<<(int)l.windows, kSumThreads, 0, s>>>(                \
+        runs, (int)feat_len, scale, accumulate, static_cast<T*>(grad_dev), partial);
   FG_DISPATCH_DTYPE(dtype, FG_SUM_T)
 #undef FG_SUM_T
 #undef FG_SUM
