@@ -23,10 +23,10 @@ __device__ __forceinline__ int64_t load_index(const void* ids, int wide, int64_t
 // by side, so that a lane has that many loads of up to 16 bytes in flight, and has the ids of
 // its next rows on the way meanwhile.
 constexpr int kLookupThreads = 256;
-constexpr int kLookupRows = 8;
+constexpr int kLookupRows = 4;
 
 template <typename T, int N>
-__global__ void __launch_bounds__(kLookupThreads)
+__global__ void __launch_bounds__(kLookupThreads, 6)
 lookup_kernel(const T* __restrict__ table, int64_t table_ld, int64_t n_vertices,
               const void* __restrict__ ids, int wide, int64_t n_ids, int feat_len, float scale,
               T* __restrict__ out, int64_t out_ld, int log_lanes, int32_t* status) {
@@ -73,15 +73,14 @@ lookup_kernel(const T* __restrict__ table, int64_t table_ld, int64_t n_vertices,
 // id, or an id out of range), which sorts behind every vertex.
 struct KeySource {
   const void* ids;           // first pass: the caller's ids
-  const uint32_t* keys;      // later passes: the pairs of the pass before
-  const uint32_t* positions;
+  const uint2* pairs;        // later passes: (key, position) as the pass before left them
   int wide;
   int64_t n_vertices;
   int64_t padding;           // -1: none
   int32_t* status;
 };
 __device__ __forceinline__ uint32_t source_key(const KeySource& s, int64_t i) {
-  if (s.keys) return s.keys[i];
+  if (s.pairs) return s.pairs[i].x;
   const int64_t id = load_index(s.ids, s.wide, i);
   if ((uint64_t)id >= (uint64_t)s.n_vertices) {
     *s.status = FG_STATUS_BAD_INDEX;
@@ -90,8 +89,8 @@ __device__ __forceinline__ uint32_t source_key(const KeySource& s, int64_t i) {
   return id == s.padding ? (uint32_t)s.n_vertices : (uint32_t)id;
 }
 
-// The table's gradient starts as zeros: CTAs of the sort's first kernel write them while the
-// others wait for memory anyway.  `bytes` of it at `to`.
+// The table's gradient starts as zeros: spare CTAs of the sort's kernels write a part of them
+// each while the others wait for memory anyway.  `bytes` of it at `to`.
 struct ZeroFill {
   uint8_t* to;
   int64_t bytes;
@@ -117,8 +116,7 @@ constexpr int kRankParts = 8;              // threads that share one position's 
 constexpr int kRankTile = kRankThreads / kRankParts;
 
 __global__ void __launch_bounds__(kRankThreads)
-rank_kernel(KeySource src, int n, int sort_blocks, ZeroFill zero, uint32_t* __restrict__ keys_out,
-            uint32_t* __restrict__ positions_out) {
+rank_kernel(KeySource src, int n, int sort_blocks, ZeroFill zero, uint2* __restrict__ pairs_out) {
   if ((int)blockIdx.x >= sort_blocks) {
     zero_fill(zero, blockIdx.x - sort_blocks, gridDim.x - sort_blocks, kRankThreads);
     return;
@@ -144,24 +142,22 @@ rank_kernel(KeySource src, int n, int sort_blocks, ZeroFill zero, uint32_t* __re
   }
 #pragma unroll
   for (int d = 1; d < kRankParts; d <<= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
-  if (part == 0 && i < n) {
-    keys_out[before] = mine;
-    positions_out[before] = i;
-  }
+  if (part == 0 && i < n) pairs_out[before] = make_uint2(mine, i);
 }
 
 // Stable least-significant-digit radix sort of (id, position) pairs, at most 9 bits a pass:
 // per block of kSortTile keys a histogram (sort_count_kernel), per digit an exclusive sum over
-// the blocks (sort_scan_kernel), then every key to its place (sort_place_kernel).  Equal ids
+// the blocks (sort_scan_kernel), then every pair to its place (sort_place_kernel).  Equal ids
 // keep the order of their positions, so the sums below run in an order that only the ids fix.
 // All keys of a thread are loaded before the first is used: with the loads inside the ranking
-// rounds a block took 22 us for its sixteen.
-constexpr int kSortThreads = 256;
+// rounds a block took 22 us.
+constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortItems = 16;
+constexpr int kSortItems = 8;
 constexpr int kSortTile = kSortThreads * kSortItems;
 constexpr int kMaxDigitBits = 9;
 constexpr int kMaxBins = 1 << kMaxDigitBits;
+static_assert(kMaxBins == kSortThreads, "one thread per digit");
 
 __global__ void __launch_bounds__(kSortThreads)
 sort_count_kernel(KeySource src, int64_t n, int shift, int bits, uint32_t* __restrict__ counts,
@@ -179,14 +175,13 @@ sort_count_kernel(KeySource src, int64_t n, int shift, int bits, uint32_t* __res
     const int64_t i = base + k * kSortThreads + threadIdx.x;
     key[k] = i < n ? source_key(src, i) : 0;
   }
-  for (int b = threadIdx.x; b < bins; b += kSortThreads) hist[b] = 0;
+  hist[threadIdx.x] = 0;
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kSortItems; ++k)
     if (base + k * kSortThreads + threadIdx.x < n) atomicAdd(&hist[(key[k] >> shift) & (bins - 1)], 1u);
   __syncthreads();
-  for (int b = threadIdx.x; b < bins; b += kSortThreads)
-    counts[(int64_t)b * sort_blocks + blockIdx.x] = hist[b];
+  if ((int)threadIdx.x < bins) counts[(int64_t)threadIdx.x * sort_blocks + blockIdx.x] = hist[threadIdx.x];
 }
 
 // One warp per digit: counts[digit][block] becomes the digit's count in the blocks before.
@@ -217,82 +212,106 @@ sort_scan_kernel(uint32_t* __restrict__ counts, int n_blocks, int bins,
   if (lane == 0) totals[digit] = running;
 }
 
+// A block orders its pairs in shared memory first, so that those of one digit (eight on
+// average with 512 digits) are written side by side.
+struct PlaceShared {
+  uint2 pairs[kSortTile];
+  uint16_t warp_hist[kSortWarps][kMaxBins];  // counts, then places within the block
+  uint32_t base[kMaxBins];                   // where the digit's pairs go, less their place here
+  uint32_t warp_sum[2][kSortWarps];
+};
+
 __global__ void __launch_bounds__(kSortThreads)
 sort_place_kernel(KeySource src, int64_t n, int shift, int bits,
                   const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals,
-                  uint32_t* __restrict__ keys_out, uint32_t* __restrict__ positions_out) {
-  __shared__ uint32_t warp_hist[kSortWarps][kMaxBins];
-  __shared__ uint32_t warp_sum[kSortWarps];
+                  uint2* __restrict__ pairs_out, int sort_blocks, ZeroFill zero) {
+  if ((int)blockIdx.x >= sort_blocks) {
+    zero_fill(zero, blockIdx.x - sort_blocks, gridDim.x - sort_blocks, kSortThreads);
+    return;
+  }
+  extern __shared__ __align__(16) uint8_t raw[];
+  PlaceShared& sh = *reinterpret_cast<PlaceShared*>(raw);
   const int bins = 1 << bits;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t block_first = (int64_t)blockIdx.x * kSortTile;
   // each warp takes kSortItems * 32 consecutive keys, 32 at a time and in order
-  const int64_t first = (int64_t)blockIdx.x * kSortTile + warp * (kSortItems * 32);
-  uint32_t key[kSortItems], position[kSortItems];
+  const int64_t first = block_first + warp * (kSortItems * 32);
+  uint2 pair[kSortItems];
 #pragma unroll
   for (int k = 0; k < kSortItems; ++k) {
     const int64_t i = first + k * 32 + lane;
-    key[k] = i < n ? source_key(src, i) : 0;
-    position[k] = i < n && src.keys ? src.positions[i] : (uint32_t)i;
+    if (i >= n) pair[k] = make_uint2(0, 0);
+    else if (src.pairs) pair[k] = src.pairs[i];
+    else pair[k] = make_uint2(source_key(src, i), (uint32_t)i);
   }
-  // this block's first place of the digits of a thread: what smaller digits take in all, and
-  // what the same digit takes in the blocks before
-  constexpr int kPer = kMaxBins / kSortThreads;
-  uint32_t total[kPer], ahead[kPer], mine = 0;
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const int b = threadIdx.x * kPer + k;
-    total[k] = b < bins ? totals[b] : 0;
-    ahead[k] = b < bins ? counts[(int64_t)b * gridDim.x + blockIdx.x] : 0;
-    mine += total[k];
-  }
-  for (int b = threadIdx.x; b < kSortWarps * kMaxBins; b += kSortThreads)
-    (&warp_hist[0][0])[b] = 0;
-  uint32_t incl = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const uint32_t up = __shfl_up_sync(0xffffffffu, incl, d);
-    if (lane >= d) incl += up;
-  }
-  if (lane == 31) warp_sum[warp] = incl;
+  // a thread per digit: what it takes in all, and in the blocks before
+  const int digit_here = threadIdx.x;
+  const uint32_t total = digit_here < bins ? totals[digit_here] : 0;
+  const uint32_t ahead = digit_here < bins ? counts[(int64_t)digit_here * sort_blocks + blockIdx.x] : 0;
+  for (int b = threadIdx.x; b < kSortWarps * kMaxBins / 2; b += kSortThreads)
+    reinterpret_cast<uint32_t*>(&sh.warp_hist[0][0])[b] = 0;
   __syncthreads();
   uint32_t rank[kSortItems];
 #pragma unroll
   for (int k = 0; k < kSortItems; ++k) {
     const bool live = first + k * 32 + lane < n;
-    const uint32_t digit = live ? (key[k] >> shift) & (bins - 1) : (uint32_t)bins;
+    const uint32_t digit = live ? (pair[k].x >> shift) & (bins - 1) : (uint32_t)bins;
     const uint32_t peers = __match_any_sync(0xffffffffu, digit);
     const uint32_t below = __popc(peers & ((1u << lane) - 1));
     uint32_t old = 0;
-    if (live) old = warp_hist[warp][digit];
+    if (live) old = sh.warp_hist[warp][digit];
     __syncwarp();
-    if (live && below == 0) warp_hist[warp][digit] = old + __popc(peers);
+    if (live && below == 0) sh.warp_hist[warp][digit] = (uint16_t)(old + __popc(peers));
     __syncwarp();
     rank[k] = old + below;
   }
   __syncthreads();
-  uint32_t before = incl - mine;
-  for (int w = 0; w < warp; ++w) before += warp_sum[w];
+  // exclusive sums over the digits, of their totals and of this block's counts
+  uint32_t here = 0;
+  if (digit_here < bins)
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const int b = threadIdx.x * kPer + k;
-    if (b < bins) {
-      uint32_t run = before + ahead[k];
+    for (int w = 0; w < kSortWarps; ++w) here += sh.warp_hist[w][digit_here];
+  uint32_t sum_total = total, sum_here = here;
 #pragma unroll
-      for (int w = 0; w < kSortWarps; ++w) {
-        const uint32_t c = warp_hist[w][b];
-        warp_hist[w][b] = run;
-        run += c;
-      }
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint32_t a = __shfl_up_sync(0xffffffffu, sum_total, d);
+    const uint32_t b = __shfl_up_sync(0xffffffffu, sum_here, d);
+    if (lane >= d) {
+      sum_total += a;
+      sum_here += b;
     }
-    before += total[k];
+  }
+  if (lane == 31) {
+    sh.warp_sum[0][warp] = sum_total;
+    sh.warp_sum[1][warp] = sum_here;
+  }
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) {
+    sum_total += sh.warp_sum[0][w];
+    sum_here += sh.warp_sum[1][w];
+  }
+  if (digit_here < bins) {
+    uint32_t run = sum_here - here;
+    sh.base[digit_here] = sum_total - total + ahead - run;
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) {
+      const uint32_t c = sh.warp_hist[w][digit_here];
+      sh.warp_hist[w][digit_here] = (uint16_t)run;
+      run += c;
+    }
   }
   __syncthreads();
 #pragma unroll
+  for (int k = 0; k < kSortItems; ++k)
+    if (first + k * 32 + lane < n)
+      sh.pairs[sh.warp_hist[warp][(pair[k].x >> shift) & (bins - 1)] + rank[k]] = pair[k];
+  __syncthreads();
+#pragma unroll
   for (int k = 0; k < kSortItems; ++k) {
-    if (first + k * 32 + lane >= n) continue;
-    const uint32_t at = warp_hist[warp][(key[k] >> shift) & (bins - 1)] + rank[k];
-    keys_out[at] = key[k];
-    positions_out[at] = position[k];
+    const int i = k * kSortThreads + threadIdx.x;
+    if (block_first + i >= n) continue;
+    const uint2 p = sh.pairs[i];
+    pairs_out[sh.base[(p.x >> shift) & (bins - 1)] + i] = p;
   }
 }
 
@@ -308,19 +327,21 @@ __device__ __forceinline__ void store_grad_row(T* p, const float (&acc)[N], floa
   store_vec<T, N>(p, v);
 }
 
-// The sorted list, a run of equal keys per vertex.  A run of up to `window` rows is summed by
-// one group of lanes; of a longer one every window of the list (positions that are a multiple
-// of `window` and those behind) sums its part in a CTA of its own, and join_kernel adds the
-// parts up in order.
+// The sorted list, a run of equal keys per vertex.  A run of up to kWindow rows is summed by
+// one group of lanes.  Of a longer one every window of the list (positions that are a multiple
+// of kWindow and those behind) is summed by a warp of its own, and join_kernel adds the windows
+// up in order.  64: a group walks 80 rows at most; with 256 the longest of them held its CTA
+// for 40 us (1M skewed ids: 221 us for the sums).
+constexpr int kWindow = 64;
 struct Runs {
-  const uint32_t *keys, *positions;
+  const uint2* pairs;        // (key, position)
   int64_t n;
   uint32_t none;             // the key of rows that go nowhere
-  int window;
 };
 constexpr int kSumThreads = 256;
+constexpr int kSumWarps = kSumThreads / 32;
 constexpr int kSumAhead = 8;   // rows in flight per lane
-constexpr int kSumPiece = 32;  // positions whose runs (those that begin there) a group sums
+constexpr int kSumPiece = 16;  // positions whose runs (those that begin there) a group sums
 
 // What part of long runs a window holds: its first `head` rows belong to one that began in an
 // earlier window or on its first row; the rows from `tail` on to one that begins later in it.
@@ -328,86 +349,84 @@ struct WindowParts {
   int head, tail, count;
   bool head_begins;
 };
-__device__ WindowParts find_parts(const Runs& r, int64_t window_index) {
-  __shared__ int shared_head, shared_tail, shared_back;
-  const int64_t begin = window_index * r.window;
+// All lanes of a warp, two positions each.
+__device__ __forceinline__ WindowParts find_parts(const Runs& r, int64_t window_index) {
+  static_assert(kWindow == 64, "two positions a lane");
+  const int lane = threadIdx.x & 31;
+  const int64_t begin = window_index * kWindow;
   WindowParts p;
-  p.count = (int)(r.n - begin < r.window ? r.n - begin : r.window);
-  const uint32_t first = r.keys[begin], last = r.keys[begin + p.count - 1];
-  if (threadIdx.x == 0) {
-    shared_head = p.count;
-    shared_tail = -1;
-    shared_back = 0;
+  p.count = (int)(r.n - begin < kWindow ? r.n - begin : kWindow);
+  const uint32_t first = r.pairs[begin].x, last = r.pairs[begin + p.count - 1].x;
+  uint64_t is_first = 0, is_last = 0, is_back = 0;  // bit i: position i; back: begin - 1 - i
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int i = h * 32 + lane;
+    const uint32_t key = i < p.count ? r.pairs[begin + i].x : r.none;
+    const uint32_t before = begin - 1 - i >= 0 ? r.pairs[begin - 1 - i].x : r.none;
+    is_first |= (uint64_t)__ballot_sync(0xffffffffu, i < p.count && key == first) << (32 * h);
+    is_last |= (uint64_t)__ballot_sync(0xffffffffu, i < p.count && key == last) << (32 * h);
+    is_back |= (uint64_t)__ballot_sync(0xffffffffu, begin - 1 - i >= 0 && before == first) << (32 * h);
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < r.window; i += kSumThreads) {
-    if (i < p.count) {
-      const uint32_t key = r.keys[begin + i];
-      if (key != first) atomicMin(&shared_head, i);
-      if (key != last) atomicMax(&shared_tail, i);
-    }
-    // rows of the first run in front of the window
-    if (begin - 1 - i >= 0 && r.keys[begin - 1 - i] == first) atomicMax(&shared_back, i + 1);
-  }
-  __syncthreads();
-  p.head = shared_head;
-  p.tail = shared_tail + 1;
-  const int64_t start = begin - shared_back;
-  // a run is long if the row `window` behind its first is of the same vertex
+  p.head = __popcll(is_first);       // equal keys stand together
+  p.tail = p.count - __popcll(is_last);
+  const int back = __popcll(is_back);
+  // a run is long if the row kWindow behind its first is of the same vertex
   auto is_long = [&](int64_t s, uint32_t key) {
-    return key != r.none && s + r.window < r.n && r.keys[s + r.window] == key;
+    return key != r.none && s + kWindow < r.n && r.pairs[s + kWindow].x == key;
   };
-  p.head_begins = shared_back == 0;
-  const bool long_head = shared_back == r.window ? first != r.none : is_long(start, first);
-  const bool long_tail = p.tail > 0 && is_long(begin + p.tail, last);
-  if (!long_head) p.head = 0;
-  if (!long_tail) p.tail = p.count;
+  p.head_begins = back == 0;
+  if (back == kWindow ? first == r.none : !is_long(begin - back, first)) p.head = 0;
+  if (p.tail == 0 || !is_long(begin + p.tail, last)) p.tail = p.count;
   return p;
 }
 
-// The sum of `count` rows from position `from` on, all threads of the CTA, into to[feat_len].
+// The sum of `count` rows from position `from` on, all lanes of a warp, into to[feat_len].
 template <typename T, int N>
-__device__ void sum_part(const Runs& r, int64_t from, int count, const T* out_grad,
-                         int64_t out_grad_ld, int feat_len, int log_lanes, float* to) {
-  __shared__ __align__(16) float sums[kSumThreads * N];
-  const int lanes = 1 << log_lanes, groups = kSumThreads >> log_lanes;
-  const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> log_lanes;
+__device__ __forceinline__ void sum_part(const Runs& r, int64_t from, int count, const T* out_grad,
+                                         int64_t out_grad_ld, int feat_len, int log_lanes, float* to) {
+  const int lanes = 1 << log_lanes, groups = 32 >> log_lanes;
+  const int lane = threadIdx.x & (lanes - 1), group = (threadIdx.x & 31) >> log_lanes;
   for (int c0 = 0; c0 < feat_len; c0 += lanes * N) {
     const int c = c0 + lane * N;
     float acc[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] = 0.f;
-    if (c < feat_len) {
-#pragma unroll 8
-      for (int i = group; i < count; i += groups) {
-        const Vec<T, N> row =
-            load_vec_stream<T, N>(out_grad + (int64_t)r.positions[from + i] * out_grad_ld + c);
+    for (int i0 = group; i0 < count; i0 += groups * kSumAhead) {
+      Vec<T, N> row[kSumAhead];
 #pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] += to_float<T>(row.v[k]);
+      for (int u = 0; u < kSumAhead; ++u) {
+        const int i = i0 + u * groups;
+        if (i < count && c < feat_len)
+          row[u] = load_vec_stream<T, N>(out_grad + (int64_t)r.pairs[from + i].y * out_grad_ld + c);
       }
-    }
 #pragma unroll
-    for (int k = 0; k < N; ++k) sums[threadIdx.x * N + k] = acc[k];
-    __syncthreads();
-    // a thread per column adds the groups' sums in order
-    for (int i = threadIdx.x; i < lanes * N; i += kSumThreads) {
-      float s = 0.f;
-      for (int g = 0; g < groups; ++g) s += sums[g * lanes * N + i];
-      if (c0 + i < feat_len) to[c0 + i] = s;
+      for (int u = 0; u < kSumAhead; ++u)
+        if (i0 + u * groups < count && c < feat_len) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) acc[k] += to_float<T>(row[u].v[k]);
+        }
     }
-    __syncthreads();
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      for (int d = lanes; d < 32; d <<= 1) acc[k] += __shfl_xor_sync(0xffffffffu, acc[k], d);
+    if (group == 0 && c < feat_len) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) to[c + k] = acc[k];
+    }
   }
 }
 
 template <typename T, int N>
 __global__ void __launch_bounds__(kSumThreads)
-sum_kernel(Runs r, int n_windows, const T* __restrict__ out_grad, int64_t out_grad_ld, int feat_len,
-           float scale, int accumulate, T* __restrict__ grad, float* __restrict__ partial,
-           int log_lanes, int slabs) {
-  if ((int)blockIdx.x < n_windows) {  // the long runs' windows come first: they take longest
-    const int64_t w = blockIdx.x;
+sum_kernel(Runs r, int n_windows, int window_blocks, const T* __restrict__ out_grad,
+           int64_t out_grad_ld, int feat_len, float scale, int accumulate, T* __restrict__ grad,
+           float* __restrict__ partial, int log_lanes, int slabs) {
+  if ((int)blockIdx.x < window_blocks) {
+    const int64_t w = (int64_t)blockIdx.x * kSumWarps + (threadIdx.x >> 5);
+    if (w >= n_windows) return;
     const WindowParts p = find_parts(r, w);
-    const int64_t begin = w * r.window;
+    const int64_t begin = w * kWindow;
     if (p.head > 0)
       sum_part<T, N>(r, begin, p.head, out_grad, out_grad_ld, feat_len, log_lanes,
                      partial + (w * 2 + 0) * feat_len);
@@ -417,7 +436,7 @@ sum_kernel(Runs r, int n_windows, const T* __restrict__ out_grad, int64_t out_gr
     return;
   }
   const int lanes = 1 << log_lanes;
-  const int64_t item = ((int64_t)(blockIdx.x - n_windows) * kSumThreads + threadIdx.x) >> log_lanes;
+  const int64_t item = ((int64_t)(blockIdx.x - window_blocks) * kSumThreads + threadIdx.x) >> log_lanes;
   const int64_t piece = item / slabs;
   const int c = ((int)(item - piece * slabs) * lanes + (threadIdx.x & (lanes - 1))) * N;
   const int64_t begin = piece * kSumPiece;
@@ -425,18 +444,21 @@ sum_kernel(Runs r, int n_windows, const T* __restrict__ out_grad, int64_t out_gr
   const int64_t end = begin + kSumPiece < r.n ? begin + kSumPiece : r.n;
   uint32_t current = r.none;
   bool mine = false;                   // whether the current run is this group's to sum
-  if (begin > 0) current = r.keys[begin - 1];
+  if (begin > 0) current = r.pairs[begin - 1].x;
   float acc[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) acc[k] = 0.f;
   // behind the piece's end only the run that is under way goes on
-  for (int64_t j = begin; j < end || (mine && j < r.n && r.keys[j] == current); j += kSumAhead) {
+  for (int64_t j = begin; j < end || (mine && j < r.n && r.pairs[j].x == current); j += kSumAhead) {
     uint32_t key[kSumAhead], position[kSumAhead];
-    // the arrays are padded to a multiple of kSumAhead; what lies behind n is not looked at
+    // the list is padded to a multiple of kSumAhead; what lies behind n is not looked at
 #pragma unroll
-    for (int u = 0; u < kSumAhead; u += 4) {
-      *reinterpret_cast<uint4*>(&key[u]) = *reinterpret_cast<const uint4*>(r.keys + j + u);
-      *reinterpret_cast<uint4*>(&position[u]) = *reinterpret_cast<const uint4*>(r.positions + j + u);
+    for (int u = 0; u < kSumAhead; u += 2) {
+      const uint4 two = *reinterpret_cast<const uint4*>(r.pairs + j + u);
+      key[u] = two.x;
+      position[u] = two.y;
+      key[u + 1] = two.z;
+      position[u + 1] = two.w;
     }
     // which of these rows count: those of runs that begin in the piece and are not long
     bool take[kSumAhead], starts[kSumAhead];
@@ -448,7 +470,7 @@ sum_kernel(Runs r, int n_windows, const T* __restrict__ out_grad, int64_t out_gr
       if (starts[u]) {
         at = key[u];
         is_mine = j + u < end && at != r.none;
-        if (is_mine && j + u + r.window < r.n && r.keys[j + u + r.window] == at) is_mine = false;
+        if (is_mine && j + u + kWindow < r.n && r.pairs[j + u + kWindow].x == at) is_mine = false;
       }
       take[u] = is_mine && j + u < r.n;
     }
@@ -474,56 +496,84 @@ sum_kernel(Runs r, int n_windows, const T* __restrict__ out_grad, int64_t out_gr
   if (mine) store_grad_row<T, N>(grad + (int64_t)current * feat_len + c, acc, scale, accumulate);
 }
 
-// A CTA per window; works only where a long run begins in it.  Its parts are this window's and
-// the heads of the windows behind: cut into kJoinParts runs, each summed in order, and these
-// added in order.
-constexpr int kJoinParts = 8;
-constexpr int kJoinColumns = 32;
+// A warp per window; works only where a long run begins in it.  The run's parts are this
+// window's and the heads of the windows behind.  A run of up to kJoinAlone windows is added up
+// by that warp, a longer one by all warps of the CTA: cut into as many stretches, each summed
+// in order, and these added in order.
+constexpr int kJoinAlone = 32;
+
+// The sum of parts t0 <= t < t1 of the run that begins in window w, for column c (a lane's).
+__device__ __forceinline__ float join_terms(const float* partial, int64_t w, int slot, int64_t t0,
+                                            int64_t t1, int feat_len, int c) {
+  float s = 0.f;
+#pragma unroll 8
+  for (int64_t t = t0; t < t1; ++t) s += partial[((w + t) * 2 + (t == 0 ? slot : 0)) * feat_len + c];
+  return s;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kSumThreads)
-join_kernel(Runs r, int feat_len, float scale, int accumulate, T* __restrict__ grad,
+join_kernel(Runs r, int n_windows, int feat_len, float scale, int accumulate, T* __restrict__ grad,
             const float* __restrict__ partial) {
-  static_assert(kJoinParts * kJoinColumns == kSumThreads, "one thread per part and column");
-  const int64_t w = blockIdx.x;
-  const int64_t behind = (w + 1) * r.window;   // a long run goes on in the next window
-  if (behind >= r.n || r.keys[behind - 1] == r.none || r.keys[behind] != r.keys[behind - 1]) return;
-  const WindowParts p = find_parts(r, w);
-  int slot;
-  if (p.tail < p.count) slot = 1;
-  else if (p.head > 0 && p.head_begins) slot = 0;
-  else return;
-  const uint32_t key = r.keys[behind - 1];
-  // how many windows behind this one begin with the same vertex
-  int64_t terms = 1;
-  for (bool more = true; more;) {
-    const int64_t at = (w + terms + threadIdx.x) * r.window;
-    const int same = __syncthreads_count(at < r.n && r.keys[at] == key);
-    terms += same;
-    more = same == kSumThreads;
+  __shared__ int slots[kSumWarps];         // -1: no long run begins in the warp's window
+  __shared__ int64_t all_terms[kSumWarps];
+  __shared__ float sums[kSumWarps][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t w = (int64_t)blockIdx.x * kSumWarps + warp;
+  const int64_t behind = (w + 1) * kWindow;   // a long run goes on in the next window
+  int slot = -1;
+  uint32_t key = r.none;
+  if (w < n_windows && behind < r.n) {
+    key = r.pairs[behind - 1].x;
+    if (key != r.none && r.pairs[behind].x == key) {
+      const WindowParts p = find_parts(r, w);
+      if (p.tail < p.count) slot = 1;
+      else if (p.head > 0 && p.head_begins) slot = 0;
+    }
   }
-  const int part = threadIdx.x / kJoinColumns, lane = threadIdx.x % kJoinColumns;
-  const int64_t per = (terms + kJoinParts - 1) / kJoinParts;
-  const int64_t t1 = (part + 1) * per < terms ? (part + 1) * per : terms;
-  __shared__ float sums[kJoinParts][kJoinColumns];
-  for (int c0 = 0; c0 < feat_len; c0 += kJoinColumns) {
-    const int c = c0 + lane;
-    float s = 0.f;
-    if (c < feat_len) {
-#pragma unroll 8
-      for (int64_t t = part * per; t < t1; ++t)
-        s += partial[((w + t) * 2 + (t == 0 ? slot : 0)) * feat_len + c];
-    }
-    sums[part][lane] = s;
-    __syncthreads();
-    if (part == 0 && c < feat_len) {
-      float total = 0.f;
+  int64_t terms = 0;
+  if (slot >= 0) {  // how many windows behind this one begin with the same vertex
+    terms = 1;
+    for (bool more = true; more;) {
+      uint32_t same[4];
 #pragma unroll
-      for (int q = 0; q < kJoinParts; ++q) total += sums[q][lane];
-      float one[1] = {total};
-      store_grad_row<T, 1>(grad + (int64_t)key * feat_len + c, one, scale, accumulate);
+      for (int k = 0; k < 4; ++k) {
+        const int64_t at = (w + terms + k * 32 + lane) * kWindow;
+        same[k] = __ballot_sync(0xffffffffu, at < r.n && r.pairs[at < r.n ? at : 0].x == key);
+      }
+      const int count = __popc(same[0]) + __popc(same[1]) + __popc(same[2]) + __popc(same[3]);
+      terms += count;
+      more = count == 128;
     }
-    __syncthreads();
+    if (terms <= kJoinAlone)
+      for (int c = lane; c < feat_len; c += 32) {
+        const float one[1] = {join_terms(partial, w, slot, 0, terms, feat_len, c)};
+        store_grad_row<T, 1>(grad + (int64_t)key * feat_len + c, one, scale, accumulate);
+      }
+  }
+  if (lane == 0) {
+    slots[warp] = terms > kJoinAlone ? slot : -1;
+    all_terms[warp] = terms;
+  }
+  __syncthreads();
+  for (int q = 0; q < kSumWarps; ++q) {
+    if (slots[q] < 0) continue;
+    const int64_t from = (int64_t)blockIdx.x * kSumWarps + q, n = all_terms[q];
+    const int64_t per = (n + kSumWarps - 1) / kSumWarps;
+    const int64_t t0 = min(n, warp * per), t1 = min(n, (warp + 1) * per);
+    const uint32_t vertex = r.pairs[(from + 1) * kWindow].x;
+    for (int c0 = 0; c0 < feat_len; c0 += 32) {
+      const int c = c0 + lane;
+      sums[warp][lane] = c < feat_len ? join_terms(partial, from, slots[q], t0, t1, feat_len, c) : 0.f;
+      __syncthreads();
+      if (warp == 0 && c < feat_len) {
+        float one[1] = {0.f};
+#pragma unroll
+        for (int k = 0; k < kSumWarps; ++k) one[0] += sums[k][lane];
+        store_grad_row<T, 1>(grad + (int64_t)vertex * feat_len + c, one, scale, accumulate);
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -536,18 +586,15 @@ int ceil_log2(int64_t v) {
 
 struct GradLayout {
   bool rank;                 // few ids: rank_kernel instead of the radix sort
-  int window;
   int64_t windows, blocks;
   int passes, digit_bits;
-  size_t keys[2], positions[2], counts, totals, partial, total;
+  size_t pairs[2], counts, totals, partial, total;
 };
 
 GradLayout grad_layout(int64_t n, int64_t n_vertices, int64_t feat_len) {
   GradLayout l;
   l.rank = n <= kRankMost;
-  // few rows: short windows, so that no group of lanes walks a long run alone
-  l.window = l.rank ? 64 : 256;
-  l.windows = (n + l.window - 1) / l.window;
+  l.windows = (n + kWindow - 1) / kWindow;
   l.blocks = (n + kSortTile - 1) / kSortTile;
   const int bits = std::max(1, ceil_log2(n_vertices + 1));  // n_vertices itself is a key
   l.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
@@ -558,11 +605,9 @@ GradLayout grad_layout(int64_t n, int64_t n_vertices, int64_t feat_len) {
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  for (int k = 0; k < (l.rank ? 1 : 2); ++k) {
-    l.keys[k] = take((size_t)n * 4);
-    l.positions[k] = take((size_t)n * 4);
-  }
+  l.pairs[0] = take((size_t)n * 8);
   if (!l.rank) {
+    l.pairs[1] = take((size_t)n * 8);
     l.counts = take(((size_t)l.blocks << l.digit_bits) * 4);
     l.totals = take(kMaxBins * 4);
   }
@@ -614,7 +659,7 @@ extern "C" int fg_embedding_lookup(const void* table_dev, int32_t dtype, int64_t
   const int log_lanes = std::min(5, ceil_log2(per_row));
   const int64_t groups_per_block = kLookupThreads >> log_lanes;
   const int64_t want = (n_ids + groups_per_block * kLookupRows - 1) / (groups_per_block * kLookupRows);
-  const int grid = (int)std::min<int64_t>(std::max<int64_t>(want, 1), 148 * 4);
+  const int grid = (int)std::min<int64_t>(std::max<int64_t>(want, 1), 148 * 6);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
 #define FG_LOOKUP(T, N)                                                                        \
   lookup_kernel<T, N><<<grid, kLookupThreads, 0, s>>>(                                         \
@@ -678,50 +723,55 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
     if (zero.bytes > 0) FG_CUDA_TRY(cudaMemsetAsync(grad_dev, 0, zero.bytes, s));
     return FG_OK;
   }
-  const int zero_blocks = (int)std::min<int64_t>(4 * 148, (zero.bytes + 65535) / 65536);
+  // the zeros in `parts` equal parts (multiples of 64 KB, the last may be shorter)
+  auto zero_part = [&](int part, int parts) {
+    const int64_t each = (zero.bytes / parts + 65535) / 65536 * 65536;
+    const int64_t from = std::min(zero.bytes, part * each);
+    return ZeroFill{zero.to + from, std::min(zero.bytes - from, part + 1 == parts ? zero.bytes : each)};
+  };
+  auto zero_blocks = [](const ZeroFill& z) { return (int)std::min<int64_t>(2 * 148, (z.bytes + 65535) / 65536); };
 
   char* ws = static_cast<char*>(workspace_dev);
-  uint32_t* keys[2] = {reinterpret_cast<uint32_t*>(ws + l.keys[0]),
-                       reinterpret_cast<uint32_t*>(ws + l.keys[1])};
-  uint32_t* positions[2] = {reinterpret_cast<uint32_t*>(ws + l.positions[0]),
-                            reinterpret_cast<uint32_t*>(ws + l.positions[1])};
+  uint2* pairs[2] = {reinterpret_cast<uint2*>(ws + l.pairs[0]), reinterpret_cast<uint2*>(ws + l.pairs[1])};
   float* partial = reinterpret_cast<float*>(ws + l.partial);
-  KeySource src = {ids_dev, nullptr, nullptr, index_type == FG_INDEX_INT64, n_vertices,
+  KeySource src = {ids_dev, nullptr, index_type == FG_INDEX_INT64, n_vertices,
                    padding_id < 0 ? -1 : padding_id, status_dev};
   if (l.rank) {
     const int blocks = (int)((n_ids + kRankTile - 1) / kRankTile);
-    rank_kernel<<<blocks + zero_blocks, kRankThreads, 0, s>>>(src, (int)n_ids, blocks, zero, keys[0],
-                                                              positions[0]);
-    src.keys = keys[0];
-    src.positions = positions[0];
+    rank_kernel<<<blocks + zero_blocks(zero), kRankThreads, 0, s>>>(src, (int)n_ids, blocks, zero, pairs[0]);
+    src.pairs = pairs[0];
   } else {
     uint32_t* counts = reinterpret_cast<uint32_t*>(ws + l.counts);
     uint32_t* totals = reinterpret_cast<uint32_t*>(ws + l.totals);
-    const int bins = 1 << l.digit_bits;
+    const int bins = 1 << l.digit_bits, blocks = (int)l.blocks;
+    FG_CUDA_TRY(cudaFuncSetAttribute(sort_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)sizeof(PlaceShared)));
     for (int pass = 0; pass < l.passes; ++pass) {
       const int shift = pass * l.digit_bits;
-      sort_count_kernel<<<(int)l.blocks + (pass == 0 ? zero_blocks : 0), kSortThreads, 0, s>>>(
-          src, n_ids, shift, l.digit_bits, counts, (int)l.blocks, zero);
-      sort_scan_kernel<<<(bins + kSortWarps - 1) / kSortWarps, kSortThreads, 0, s>>>(
-          counts, (int)l.blocks, bins, totals);
-      sort_place_kernel<<<(int)l.blocks, kSortThreads, 0, s>>>(
-          src, n_ids, shift, l.digit_bits, counts, totals, keys[pass & 1], positions[pass & 1]);
-      src.keys = keys[pass & 1];
-      src.positions = positions[pass & 1];
+      const ZeroFill z0 = zero_part(2 * pass, 2 * l.passes), z1 = zero_part(2 * pass + 1, 2 * l.passes);
+      sort_count_kernel<<<blocks + zero_blocks(z0), kSortThreads, 0, s>>>(src, n_ids, shift, l.digit_bits,
+                                                                        counts, blocks, z0);
+      sort_scan_kernel<<<(bins + kSortWarps - 1) / kSortWarps, kSortThreads, 0, s>>>(counts, blocks, bins,
+                                                                                   totals);
+      sort_place_kernel<<<blocks + zero_blocks(z1), kSortThreads, sizeof(PlaceShared), s>>>(
+          src, n_ids, shift, l.digit_bits, counts, totals, pairs[pass & 1], blocks, z1);
+      src.pairs = pairs[pass & 1];
     }
   }
-  const Runs runs = {src.keys, src.positions, n_ids, (uint32_t)n_vertices, l.window};
+  const Runs runs = {src.pairs, n_ids, (uint32_t)n_vertices};
   const int per_row = (int)((feat_len * es + vb - 1) / vb);
   const int log_lanes = std::min(5, ceil_log2(per_row));
   const int slabs = (per_row + (1 << log_lanes) - 1) >> log_lanes;
   const int64_t pieces = (n_ids + kSumPiece - 1) / kSumPiece;
   const int64_t threads = (pieces * slabs) << log_lanes;
-  const int64_t grid = l.windows + (threads + kSumThreads - 1) / kSumThreads;
+  const int64_t window_blocks = (l.windows + kSumWarps - 1) / kSumWarps;
+  const int64_t grid = window_blocks + (threads + kSumThreads - 1) / kSumThreads;
   if (grid > INT32_MAX) return fail(FG_ERR_UNSUPPORTED, "n_ids x feat_len is too large");
 #define FG_SUM(T, N)                                                                          \
   sum_kernel<T, N><<<(int)grid, kSumThreads, 0, s>>>(                                         \
-      runs, (int)l.windows, static_cast<const T*>(out_grad_dev), out_grad_ld, (int)feat_len,  \
-      scale, accumulate, static_cast<T*>(grad_dev), partial, log_lanes, slabs)
+      runs, (int)l.windows, (int)window_blocks, static_cast<const T*>(out_grad_dev),          \
+      out_grad_ld, (int)feat_len, scale, accumulate, static_cast<T*>(grad_dev), partial,      \
+      log_lanes, slabs)
 #define FG_SUM_T(T)                                                       \
   switch (vb / (int)sizeof(T)) {                                          \
     case 8: if constexpr (sizeof(T) == 2) FG_SUM(T, 8 / (sizeof(T) / 2)); break; \
@@ -729,9 +779,9 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
     case 2: FG_SUM(T, 2); break;                                          \
     default: FG_SUM(T, 1); break;                                         \
   }                                                                       \
-  if (n_ids > l.window)                                                   \
-    join_kernel<T><<<(int)l.windows, kSumThreads, 0, s>>>(                \
-        runs, (int)feat_len, scale, accumulate, static_cast<T*>(grad_dev), partial);
+  if (n_ids > kWindow)                                                    \
+    join_kernel<T><<<(int)window_blocks, kSumThreads, 0, s>>>(            \
+        runs, (int)l.windows, (int)feat_len, scale, accumulate, static_cast<T*>(grad_dev), partial);
   FG_DISPATCH_DTYPE(dtype, FG_SUM_T)
 #undef FG_SUM_T
 #undef FG_SUM
