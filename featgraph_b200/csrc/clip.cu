@@ -75,8 +75,7 @@ __device__ __forceinline__ void chunk_norm(const T* __restrict__ p, int count, b
     for (int i = threadIdx.x; i < vecs; i += kClipThreads) {
       const Vec<T, N> v = load_vec<T, N>(p + (int64_t)i * N);
       float x[N];
-#pragma unroll
-      for (int k = 0; k < N; ++k) x[k] = to_float<T>(v.v[k]);
+      unpack<T, N>(v, x);
       add_group<MAX_NORM, N>(x, acc, top, nan);
     }
     done = vecs * N;
@@ -137,10 +136,11 @@ __device__ __forceinline__ void chunk_scale(const T* p, T* q, int count, bool ve
     const int vecs = count / N;
 #pragma unroll 4
     for (int i = threadIdx.x; i < vecs; i += kClipThreads) {
-      Vec<T, N> v = load_vec_stream<T, N>(p + (int64_t)i * N);
+      float x[N];
+      unpack<T, N>(load_vec_stream<T, N>(p + (int64_t)i * N), x);
 #pragma unroll
-      for (int k = 0; k < N; ++k) v.v[k] = from_float<T>(to_float<T>(v.v[k]) * share);
-      store_vec_stream<T, N>(q + (int64_t)i * N, v);
+      for (int k = 0; k < N; ++k) x[k] *= share;
+      store_vec_stream<T, N>(q + (int64_t)i * N, pack<T, N>(x));
     }
     done = vecs * N;
   }

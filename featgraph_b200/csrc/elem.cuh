@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace fg {
@@ -42,7 +44,9 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { re
 template <>
 __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// N consecutive elements as one memory access of N * sizeof(T) = 2, 4, 8 or 16 bytes.
+// N consecutive elements as one memory access of N * sizeof(T) = 2, 4, 8 or 16 bytes.  They
+// stay as loaded until they are unpacked: taken apart at the load, every load waited for the
+// one before.
 template <int BYTES>
 struct RawVec;
 template <>
@@ -55,39 +59,63 @@ template <>
 struct RawVec<2> { using type = unsigned short; };
 
 template <typename T, int N>
-struct alignas(N * sizeof(T)) Vec {
+struct Vec {
   using Raw = typename RawVec<N * (int)sizeof(T)>::type;
-  T v[N];
+  Raw raw;
 };
 
 template <typename T, int N>
+__device__ __forceinline__ void unpack(const Vec<T, N>& v, float (&x)[N]) {
+  if constexpr (sizeof(T) == 4) {
+    memcpy(x, &v.raw, sizeof(v.raw));
+  } else if constexpr (N == 1) {
+    T one;
+    memcpy(&one, &v.raw, 2);
+    x[0] = to_float<T>(one);
+  } else {
+    uint32_t w[N / 2];
+    memcpy(w, &v.raw, sizeof(v.raw));
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        x[2 * k] = __uint_as_float(w[k] << 16);
+        x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+      } else {
+        __half2 h;
+        memcpy(&h, &w[k], 4);
+        const float2 f = __half22float2(h);
+        x[2 * k] = f.x;
+        x[2 * k + 1] = f.y;
+      }
+    }
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> pack(const float (&x)[N]) {
+  T t[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) t[k] = from_float<T>(x[k]);
+  Vec<T, N> v;
+  memcpy(&v.raw, t, sizeof(v.raw));
+  return v;
+}
+
+template <typename T, int N>
 __device__ __forceinline__ Vec<T, N> load_vec(const T* p) {
-  using V = Vec<T, N>;
-  typename V::Raw r = __ldg(reinterpret_cast<const typename V::Raw*>(p));
-  V out;
-  memcpy(&out, &r, sizeof(out));
-  return out;
+  return {__ldg(reinterpret_cast<const typename Vec<T, N>::Raw*>(p))};
 }
 // Read-once data: evicted first.
 template <typename T, int N>
 __device__ __forceinline__ Vec<T, N> load_vec_stream(const T* p) {
-  using V = Vec<T, N>;
-  typename V::Raw r = __ldcs(reinterpret_cast<const typename V::Raw*>(p));
-  V out;
-  memcpy(&out, &r, sizeof(out));
-  return out;
+  return {__ldcs(reinterpret_cast<const typename Vec<T, N>::Raw*>(p))};
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& v) {
-  typename Vec<T, N>::Raw r;
-  memcpy(&r, &v, sizeof(r));
-  *reinterpret_cast<typename Vec<T, N>::Raw*>(p) = r;
+  *reinterpret_cast<typename Vec<T, N>::Raw*>(p) = v.raw;
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_vec_stream(T* p, const Vec<T, N>& v) {
-  typename Vec<T, N>::Raw r;
-  memcpy(&r, &v, sizeof(r));
-  __stcs(reinterpret_cast<typename Vec<T, N>::Raw*>(p), r);
+  __stcs(reinterpret_cast<typename Vec<T, N>::Raw*>(p), v.raw);
 }
 
 #endif  // __CUDACC__

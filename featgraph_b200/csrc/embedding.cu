@@ -23,10 +23,10 @@ __device__ __forceinline__ int64_t load_index(const void* ids, int wide, int64_t
 // by side, so that a lane has that many loads of up to 16 bytes in flight, and has the ids of
 // its next rows on the way meanwhile.
 constexpr int kLookupThreads = 256;
-constexpr int kLookupRows = 4;
+constexpr int kLookupRows = 8;
 
 template <typename T, int N>
-__global__ void __launch_bounds__(kLookupThreads, 6)
+__global__ void __launch_bounds__(kLookupThreads)
 lookup_kernel(const T* __restrict__ table, int64_t table_ld, int64_t n_vertices,
               const void* __restrict__ ids, int wide, int64_t n_ids, int feat_len, float scale,
               T* __restrict__ out, int64_t out_ld, int log_lanes, int32_t* status) {
@@ -58,11 +58,11 @@ lookup_kernel(const T* __restrict__ table, int64_t table_ld, int64_t n_vertices,
 #pragma unroll
       for (int u = 0; u < kLookupRows; ++u) {
         if (first + u >= n_ids) break;
+        float x[N];
+        unpack<T, N>(row[u], x);
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-          row[u].v[k] = from_float<T>(ok[u] ? to_float<T>(row[u].v[k]) * scale
-                                            : __int_as_float(0x7fc00000));
-        store_vec_stream<T, N>(out + (first + u) * out_ld + c, row[u]);
+        for (int k = 0; k < N; ++k) x[k] = ok[u] ? x[k] * scale : __int_as_float(0x7fc00000);
+        store_vec_stream<T, N>(out + (first + u) * out_ld + c, pack<T, N>(x));
       }
     }
   }
@@ -319,12 +319,16 @@ sort_place_kernel(KeySource src, int64_t n, int shift, int bits,
 template <typename T, int N>
 __device__ __forceinline__ void store_grad_row(T* p, const float (&acc)[N], float scale,
                                                int accumulate) {
-  Vec<T, N> v;
-  if (accumulate) v = *reinterpret_cast<const Vec<T, N>*>(p);
+  float x[N];
 #pragma unroll
-  for (int k = 0; k < N; ++k)
-    v.v[k] = from_float<T>(accumulate ? to_float<T>(v.v[k]) + acc[k] * scale : acc[k] * scale);
-  store_vec<T, N>(p, v);
+  for (int k = 0; k < N; ++k) x[k] = acc[k] * scale;
+  if (accumulate) {
+    float before[N];
+    unpack<T, N>(*reinterpret_cast<const Vec<T, N>*>(p), before);
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] += before[k];
+  }
+  store_vec<T, N>(p, pack<T, N>(x));
 }
 
 // The sorted list, a run of equal keys per vertex.  A run of up to kWindow rows is summed by
@@ -342,6 +346,7 @@ constexpr int kSumThreads = 256;
 constexpr int kSumWarps = kSumThreads / 32;
 constexpr int kSumAhead = 8;   // rows in flight per lane
 constexpr int kSumPiece = 16;  // positions whose runs (those that begin there) a group sums
+constexpr int kSumLeastLanes = 4;  // of a group, also where a row has less to load
 
 // What part of long runs a window holds: its first `head` rows belong to one that began in an
 // earlier window or on its first row; the rows from `tail` on to one that begins later in it.
@@ -402,8 +407,10 @@ __device__ __forceinline__ void sum_part(const Runs& r, int64_t from, int count,
 #pragma unroll
       for (int u = 0; u < kSumAhead; ++u)
         if (i0 + u * groups < count && c < feat_len) {
+          float x[N];
+          unpack<T, N>(row[u], x);
 #pragma unroll
-          for (int k = 0; k < N; ++k) acc[k] += to_float<T>(row[u].v[k]);
+          for (int k = 0; k < N; ++k) acc[k] += x[k];
         }
     }
     __syncwarp();
@@ -421,75 +428,75 @@ template <typename T, int N>
 __global__ void __launch_bounds__(kSumThreads)
 sum_kernel(Runs r, int n_windows, int window_blocks, const T* __restrict__ out_grad,
            int64_t out_grad_ld, int feat_len, float scale, int accumulate, T* __restrict__ grad,
-           float* __restrict__ partial, int log_lanes, int slabs) {
+           float* __restrict__ partial, int pitch, int log_lanes) {
   if ((int)blockIdx.x < window_blocks) {
+    if (blockIdx.y > 0) return;
     const int64_t w = (int64_t)blockIdx.x * kSumWarps + (threadIdx.x >> 5);
     if (w >= n_windows) return;
     const WindowParts p = find_parts(r, w);
     const int64_t begin = w * kWindow;
     if (p.head > 0)
       sum_part<T, N>(r, begin, p.head, out_grad, out_grad_ld, feat_len, log_lanes,
-                     partial + (w * 2 + 0) * feat_len);
+                     partial + (w * 2 + 0) * pitch);
     if (p.tail < p.count)
       sum_part<T, N>(r, begin + p.tail, p.count - p.tail, out_grad, out_grad_ld, feat_len, log_lanes,
-                     partial + (w * 2 + 1) * feat_len);
+                     partial + (w * 2 + 1) * pitch);
     return;
   }
-  const int lanes = 1 << log_lanes;
-  const int64_t item = ((int64_t)(blockIdx.x - window_blocks) * kSumThreads + threadIdx.x) >> log_lanes;
-  const int64_t piece = item / slabs;
-  const int c = ((int)(item - piece * slabs) * lanes + (threadIdx.x & (lanes - 1))) * N;
-  const int64_t begin = piece * kSumPiece;
-  if (begin >= r.n || c >= feat_len) return;
-  const int64_t end = begin + kSumPiece < r.n ? begin + kSumPiece : r.n;
-  uint32_t current = r.none;
+  // A group of lanes per piece of kSumPiece positions.  The CTA's stretch of the list, the row
+  // in front of it and all that its groups may look at behind it come into shared memory in one
+  // round trip, so that a group's only waits are for its rows.
+  constexpr int kBehind = kSumPiece + 2 * kWindow;
+  __shared__ uint2 list[1 + (kSumThreads / kSumLeastLanes) * kSumPiece + kBehind];
+  const int lanes = 1 << log_lanes, groups = kSumThreads >> log_lanes;
+  const int64_t block_first = (int64_t)(blockIdx.x - window_blocks) * groups * kSumPiece;
+  for (int i = threadIdx.x; i < 1 + groups * kSumPiece + kBehind; i += kSumThreads) {
+    const int64_t at = block_first - 1 + i;
+    list[i] = at >= 0 && at < r.n ? r.pairs[at] : make_uint2(r.none, 0);
+  }
+  __syncthreads();
+  const int c = ((int)blockIdx.y * lanes + (threadIdx.x & (lanes - 1))) * N;
+  const int begin = 1 + (threadIdx.x >> log_lanes) * kSumPiece, end = begin + kSumPiece;
+  if (c >= feat_len) return;
+  uint32_t current = list[begin - 1].x;
   bool mine = false;                   // whether the current run is this group's to sum
-  if (begin > 0) current = r.pairs[begin - 1].x;
   float acc[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) acc[k] = 0.f;
-  // behind the piece's end only the run that is under way goes on
-  for (int64_t j = begin; j < end || (mine && j < r.n && r.pairs[j].x == current); j += kSumAhead) {
-    uint32_t key[kSumAhead], position[kSumAhead];
-    // the list is padded to a multiple of kSumAhead; what lies behind n is not looked at
-#pragma unroll
-    for (int u = 0; u < kSumAhead; u += 2) {
-      const uint4 two = *reinterpret_cast<const uint4*>(r.pairs + j + u);
-      key[u] = two.x;
-      position[u] = two.y;
-      key[u + 1] = two.z;
-      position[u + 1] = two.w;
-    }
+  // behind the piece's end only the run that is under way goes on, by kWindow rows at most
+  for (int j = begin; j < end || (mine && list[j].x == current); j += kSumAhead) {
     // which of these rows count: those of runs that begin in the piece and are not long
-    bool take[kSumAhead], starts[kSumAhead];
+    uint32_t take = 0, starts = 0;
     uint32_t at = current;
     bool is_mine = mine;
-#pragma unroll
-    for (int u = 0; u < kSumAhead; ++u) {
-      starts[u] = j + u < r.n && key[u] != at;
-      if (starts[u]) {
-        at = key[u];
-        is_mine = j + u < end && at != r.none;
-        if (is_mine && j + u + kWindow < r.n && r.pairs[j + u + kWindow].x == at) is_mine = false;
-      }
-      take[u] = is_mine && j + u < r.n;
-    }
     Vec<T, N> row[kSumAhead];
 #pragma unroll
-    for (int u = 0; u < kSumAhead; ++u)
-      if (take[u]) row[u] = load_vec_stream<T, N>(out_grad + (int64_t)position[u] * out_grad_ld + c);
+    for (int u = 0; u < kSumAhead; ++u) {
+      const uint2 p = list[j + u];
+      if (p.x != at) {
+        at = p.x;
+        starts |= 1u << u;
+        is_mine = j + u < end && at != r.none && list[j + u + kWindow].x != at;
+      }
+      if (is_mine) {
+        take |= 1u << u;
+        row[u] = load_vec_stream<T, N>(out_grad + (int64_t)p.y * out_grad_ld + c);
+      }
+    }
 #pragma unroll
     for (int u = 0; u < kSumAhead; ++u) {
-      if (starts[u]) {
+      if (starts >> u & 1) {
         if (mine) store_grad_row<T, N>(grad + (int64_t)current * feat_len + c, acc, scale, accumulate);
-        current = key[u];
-        mine = take[u];
+        current = list[j + u].x;
+        mine = take >> u & 1;
 #pragma unroll
         for (int k = 0; k < N; ++k) acc[k] = 0.f;
       }
-      if (take[u]) {
+      if (take >> u & 1) {
+        float x[N];
+        unpack<T, N>(row[u], x);
 #pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] += to_float<T>(row[u].v[k]);
+        for (int k = 0; k < N; ++k) acc[k] += x[k];
       }
     }
   }
@@ -502,22 +509,36 @@ sum_kernel(Runs r, int n_windows, int window_blocks, const T* __restrict__ out_g
 // in order, and these added in order.
 constexpr int kJoinAlone = 32;
 
-// The sum of parts t0 <= t < t1 of the run that begins in window w, for column c (a lane's).
-__device__ __forceinline__ float join_terms(const float* partial, int64_t w, int slot, int64_t t0,
-                                            int64_t t1, int feat_len, int c) {
-  float s = 0.f;
+// The sum of parts t0 <= t < t1 of the run that begins in window w, for four columns from c on.
+__device__ __forceinline__ float4 join_terms(const float* partial, int64_t w, int slot, int64_t t0,
+                                             int64_t t1, int pitch, int c) {
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-  for (int64_t t = t0; t < t1; ++t) s += partial[((w + t) * 2 + (t == 0 ? slot : 0)) * feat_len + c];
+  for (int64_t t = t0; t < t1; ++t) {
+    const float4 v = *reinterpret_cast<const float4*>(
+        partial + ((w + t) * 2 + (t == 0 ? slot : 0)) * pitch + c);
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
   return s;
+}
+template <typename T>
+__device__ __forceinline__ void store_joined(T* row, int feat_len, int c, float4 s, float scale,
+                                             int accumulate) {
+  const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float one[1] = {v[k]};
+    if (c + k < feat_len) store_grad_row<T, 1>(row + c + k, one, scale, accumulate);
+  }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kSumThreads)
 join_kernel(Runs r, int n_windows, int feat_len, float scale, int accumulate, T* __restrict__ grad,
-            const float* __restrict__ partial) {
+            const float* __restrict__ partial, int pitch) {
   __shared__ int slots[kSumWarps];         // -1: no long run begins in the warp's window
   __shared__ int64_t all_terms[kSumWarps];
-  __shared__ float sums[kSumWarps][32];
+  __shared__ float4 sums[kSumWarps][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t w = (int64_t)blockIdx.x * kSumWarps + warp;
   const int64_t behind = (w + 1) * kWindow;   // a long run goes on in the next window
@@ -546,10 +567,9 @@ join_kernel(Runs r, int n_windows, int feat_len, float scale, int accumulate, T*
       more = count == 128;
     }
     if (terms <= kJoinAlone)
-      for (int c = lane; c < feat_len; c += 32) {
-        const float one[1] = {join_terms(partial, w, slot, 0, terms, feat_len, c)};
-        store_grad_row<T, 1>(grad + (int64_t)key * feat_len + c, one, scale, accumulate);
-      }
+      for (int c = lane * 4; c < feat_len; c += 128)
+        store_joined<T>(grad + (int64_t)key * feat_len, feat_len, c,
+                        join_terms(partial, w, slot, 0, terms, pitch, c), scale, accumulate);
   }
   if (lane == 0) {
     slots[warp] = terms > kJoinAlone ? slot : -1;
@@ -562,15 +582,18 @@ join_kernel(Runs r, int n_windows, int feat_len, float scale, int accumulate, T*
     const int64_t per = (n + kSumWarps - 1) / kSumWarps;
     const int64_t t0 = min(n, warp * per), t1 = min(n, (warp + 1) * per);
     const uint32_t vertex = r.pairs[(from + 1) * kWindow].x;
-    for (int c0 = 0; c0 < feat_len; c0 += 32) {
-      const int c = c0 + lane;
-      sums[warp][lane] = c < feat_len ? join_terms(partial, from, slots[q], t0, t1, feat_len, c) : 0.f;
+    for (int c0 = 0; c0 < feat_len; c0 += 128) {
+      const int c = c0 + lane * 4;
+      if (c < feat_len) sums[warp][lane] = join_terms(partial, from, slots[q], t0, t1, pitch, c);
       __syncthreads();
       if (warp == 0 && c < feat_len) {
-        float one[1] = {0.f};
+        float4 s = sums[0][lane];
 #pragma unroll
-        for (int k = 0; k < kSumWarps; ++k) one[0] += sums[k][lane];
-        store_grad_row<T, 1>(grad + (int64_t)vertex * feat_len + c, one, scale, accumulate);
+        for (int k = 1; k < kSumWarps; ++k) {
+          const float4 v = sums[k][lane];
+          s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+        store_joined<T>(grad + (int64_t)vertex * feat_len, feat_len, c, s, scale, accumulate);
       }
       __syncthreads();
     }
@@ -588,6 +611,7 @@ struct GradLayout {
   bool rank;                 // few ids: rank_kernel instead of the radix sort
   int64_t windows, blocks;
   int passes, digit_bits;
+  int pitch;                 // of a partial sum, in floats
   size_t pairs[2], counts, totals, partial, total;
 };
 
@@ -611,7 +635,8 @@ GradLayout grad_layout(int64_t n, int64_t n_vertices, int64_t feat_len) {
     l.counts = take(((size_t)l.blocks << l.digit_bits) * 4);
     l.totals = take(kMaxBins * 4);
   }
-  l.partial = take((size_t)l.windows * 2 * feat_len * 4);
+  l.pitch = (int)((feat_len + 3) / 4 * 4);
+  l.partial = take((size_t)l.windows * 2 * l.pitch * 4);
   l.total = at;
   return l;
 }
@@ -659,7 +684,7 @@ extern "C" int fg_embedding_lookup(const void* table_dev, int32_t dtype, int64_t
   const int log_lanes = std::min(5, ceil_log2(per_row));
   const int64_t groups_per_block = kLookupThreads >> log_lanes;
   const int64_t want = (n_ids + groups_per_block * kLookupRows - 1) / (groups_per_block * kLookupRows);
-  const int grid = (int)std::min<int64_t>(std::max<int64_t>(want, 1), 148 * 6);
+  const int grid = (int)std::min<int64_t>(std::max<int64_t>(want, 1), 148 * 4);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
 #define FG_LOOKUP(T, N)                                                                        \
   lookup_kernel<T, N><<<grid, kLookupThreads, 0, s>>>(                                         \
@@ -760,18 +785,19 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
   }
   const Runs runs = {src.pairs, n_ids, (uint32_t)n_vertices};
   const int per_row = (int)((feat_len * es + vb - 1) / vb);
-  const int log_lanes = std::min(5, ceil_log2(per_row));
-  const int slabs = (per_row + (1 << log_lanes) - 1) >> log_lanes;
+  const int log_lanes = std::max(ceil_log2(kSumLeastLanes), std::min(5, ceil_log2(per_row)));
+  const int64_t slabs = (per_row + (1 << log_lanes) - 1) >> log_lanes;
   const int64_t pieces = (n_ids + kSumPiece - 1) / kSumPiece;
-  const int64_t threads = (pieces * slabs) << log_lanes;
   const int64_t window_blocks = (l.windows + kSumWarps - 1) / kSumWarps;
-  const int64_t grid = window_blocks + (threads + kSumThreads - 1) / kSumThreads;
-  if (grid > INT32_MAX) return fail(FG_ERR_UNSUPPORTED, "n_ids x feat_len is too large");
+  const int64_t blocks_x = window_blocks + ((pieces << log_lanes) + kSumThreads - 1) / kSumThreads;
+  if (blocks_x > INT32_MAX || slabs > 65535)
+    return fail(FG_ERR_UNSUPPORTED, "n_ids x feat_len is too large");
+  const dim3 grid((unsigned)blocks_x, (unsigned)slabs);
 #define FG_SUM(T, N)                                                                          \
-  sum_kernel<T, N><<<(int)grid, kSumThreads, 0, s>>>(                                         \
+  sum_kernel<T, N><<<grid, kSumThreads, 0, s>>>(                                              \
       runs, (int)l.windows, (int)window_blocks, static_cast<const T*>(out_grad_dev),          \
       out_grad_ld, (int)feat_len, scale, accumulate, static_cast<T*>(grad_dev), partial,      \
-      log_lanes, slabs)
+      l.pitch, log_lanes)
 #define FG_SUM_T(T)                                                       \
   switch (vb / (int)sizeof(T)) {                                          \
     case 8: if constexpr (sizeof(T) == 2) FG_SUM(T, 8 / (sizeof(T) / 2)); break; \
@@ -781,7 +807,7 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
   }                                                                       \
   if (n_ids > kWindow)                                                    \
     join_kernel<T><<<(int)window_blocks, kSumThreads, 0, s>>>(            \
-        runs, (int)l.windows, (int)feat_len, scale, accumulate, static_cast<T*>(grad_dev), partial);
+        runs, (int)l.windows, (int)feat_len, scale, accumulate, static_cast<T*>(grad_dev), partial, l.pitch);
   FG_DISPATCH_DTYPE(dtype, FG_SUM_T)
 #undef FG_SUM_T
 #undef FG_SUM

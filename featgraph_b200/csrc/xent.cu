@@ -193,10 +193,10 @@ __device__ __forceinline__ void store_out(const MmaArgs& a, const Item& item, in
 #pragma unroll
     for (int k = 0; k < 16; k += N) {
       if (c + k >= a.feat_len) break;
-      Vec<T, N> piece;
+      float x[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) piece.v[i] = from_float<T>(live ? v[k + i] * factor : 0.f);
-      store_vec<T, N>(to + k, piece);
+      for (int i = 0; i < N; ++i) x[i] = live ? v[k + i] * factor : 0.f;
+      store_vec<T, N>(to + k, pack<T, N>(x));
     }
   } else {
 #pragma unroll
