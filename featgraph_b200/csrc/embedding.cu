@@ -79,9 +79,13 @@ struct KeySource {
   int64_t padding;           // -1: none
   int32_t* status;
 };
-__device__ __forceinline__ uint32_t source_key(const KeySource& s, int64_t i) {
-  if (s.pairs) return s.pairs[i].x;
-  const int64_t id = load_index(s.ids, s.wide, i);
+// What a key is made of, as it lies in memory, and the key.  Apart, so that a thread can have
+// all its loads on the way before it looks at the first (and may have to report it).
+__device__ __forceinline__ int64_t load_source(const KeySource& s, int64_t i) {
+  return s.pairs ? (int64_t)s.pairs[i].x : load_index(s.ids, s.wide, i);
+}
+__device__ __forceinline__ uint32_t make_key(const KeySource& s, int64_t id) {
+  if (s.pairs) return (uint32_t)id;
   if ((uint64_t)id >= (uint64_t)s.n_vertices) {
     *s.status = FG_STATUS_BAD_INDEX;
     return (uint32_t)s.n_vertices;
@@ -112,7 +116,7 @@ __device__ __forceinline__ void zero_fill(const ZeroFill& z, int block, int bloc
 // where the six of the radix sort take 30.
 constexpr int64_t kRankMost = 8192;
 constexpr int kRankThreads = 256;
-constexpr int kRankParts = 8;              // threads that share one position's comparisons
+constexpr int kRankParts = 16;             // threads that share one position's comparisons
 constexpr int kRankTile = kRankThreads / kRankParts;
 
 __global__ void __launch_bounds__(kRankThreads)
@@ -123,22 +127,46 @@ rank_kernel(KeySource src, int n, int sort_blocks, ZeroFill zero, uint2* __restr
   }
   __shared__ __align__(16) uint32_t keys[kRankMost];
   const int whole = (n + 31) / 32 * 32;
-#pragma unroll 8
-  for (int i = threadIdx.x; i < whole; i += kRankThreads)
-    keys[i] = i < n ? source_key(src, i) : 0xffffffffu;
+  for (int i0 = threadIdx.x; i0 < whole; i0 += kRankThreads * 16) {
+    int64_t id[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int i = i0 + k * kRankThreads;
+      id[k] = i < n ? load_source(src, i) : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int i = i0 + k * kRankThreads;
+      if (i < whole) keys[i] = i < n ? make_key(src, id[k]) : 0xffffffffu;
+    }
+  }
   __syncthreads();
   const int i = blockIdx.x * kRankTile + threadIdx.x / kRankParts;
   const int part = threadIdx.x % kRankParts;
   const uint32_t mine = i < n ? keys[i] : 0;
   uint32_t before = 0;
+  // equal ids count where they stand earlier: in front of this CTA's positions (whole steps of
+  // the loop) all do, behind them none
+  constexpr int kStep = kRankParts * 4;
+  const int tile0 = blockIdx.x * kRankTile / kStep * kStep;
+  const int tile1 = min(whole, ((int)blockIdx.x * kRankTile + kRankTile + kStep - 1) / kStep * kStep);
+  auto four = [&](int k) { return *reinterpret_cast<const uint4*>(&keys[k]); };
 #pragma unroll 4
-  for (int k = part * 4; k < whole; k += kRankParts * 4) {
-    const uint4 q = *reinterpret_cast<const uint4*>(&keys[k]);
-    // equal ids count where they stand earlier
+  for (int k = part * 4; k < tile0; k += kStep) {
+    const uint4 q = four(k);
+    before += (q.x <= mine) + (q.y <= mine) + (q.z <= mine) + (q.w <= mine);
+  }
+  for (int k = tile0 + part * 4; k < tile1; k += kStep) {
+    const uint4 q = four(k);
     before += q.x < mine + (k < i);
     before += q.y < mine + (k + 1 < i);
     before += q.z < mine + (k + 2 < i);
     before += q.w < mine + (k + 3 < i);
+  }
+#pragma unroll 4
+  for (int k = tile1 + part * 4; k < whole; k += kStep) {
+    const uint4 q = four(k);
+    before += (q.x < mine) + (q.y < mine) + (q.z < mine) + (q.w < mine);
   }
 #pragma unroll
   for (int d = 1; d < kRankParts; d <<= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
@@ -169,17 +197,18 @@ sort_count_kernel(KeySource src, int64_t n, int shift, int bits, uint32_t* __res
   __shared__ uint32_t hist[kMaxBins];
   const int bins = 1 << bits;
   const int64_t base = (int64_t)blockIdx.x * kSortTile;
-  uint32_t key[kSortItems];
+  int64_t id[kSortItems];
 #pragma unroll
   for (int k = 0; k < kSortItems; ++k) {
     const int64_t i = base + k * kSortThreads + threadIdx.x;
-    key[k] = i < n ? source_key(src, i) : 0;
+    id[k] = i < n ? load_source(src, i) : 0;
   }
   hist[threadIdx.x] = 0;
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kSortItems; ++k)
-    if (base + k * kSortThreads + threadIdx.x < n) atomicAdd(&hist[(key[k] >> shift) & (bins - 1)], 1u);
+    if (base + k * kSortThreads + threadIdx.x < n)
+      atomicAdd(&hist[(make_key(src, id[k]) >> shift) & (bins - 1)], 1u);
   __syncthreads();
   if ((int)threadIdx.x < bins) counts[(int64_t)threadIdx.x * sort_blocks + blockIdx.x] = hist[threadIdx.x];
 }
@@ -237,12 +266,24 @@ sort_place_kernel(KeySource src, int64_t n, int shift, int bits,
   // each warp takes kSortItems * 32 consecutive keys, 32 at a time and in order
   const int64_t first = block_first + warp * (kSortItems * 32);
   uint2 pair[kSortItems];
+  if (src.pairs) {
 #pragma unroll
-  for (int k = 0; k < kSortItems; ++k) {
-    const int64_t i = first + k * 32 + lane;
-    if (i >= n) pair[k] = make_uint2(0, 0);
-    else if (src.pairs) pair[k] = src.pairs[i];
-    else pair[k] = make_uint2(source_key(src, i), (uint32_t)i);
+    for (int k = 0; k < kSortItems; ++k) {
+      const int64_t i = first + k * 32 + lane;
+      pair[k] = i < n ? src.pairs[i] : make_uint2(0, 0);
+    }
+  } else {
+    int64_t id[kSortItems];
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+      const int64_t i = first + k * 32 + lane;
+      id[k] = i < n ? load_source(src, i) : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+      const int64_t i = first + k * 32 + lane;
+      pair[k] = i < n ? make_uint2(make_key(src, id[k]), (uint32_t)i) : make_uint2(0, 0);
+    }
   }
   // a thread per digit: what it takes in all, and in the blocks before
   const int digit_here = threadIdx.x;
@@ -256,7 +297,15 @@ sort_place_kernel(KeySource src, int64_t n, int shift, int bits,
   for (int k = 0; k < kSortItems; ++k) {
     const bool live = first + k * 32 + lane < n;
     const uint32_t digit = live ? (pair[k].x >> shift) & (bins - 1) : (uint32_t)bins;
-    const uint32_t peers = __match_any_sync(0xffffffffu, digit);
+    // the lanes with the same digit, bit by bit (__match_any_sync waits on the shared-memory
+    // pipe: 17 us a pass of 1M keys)
+    uint32_t peers = __ballot_sync(0xffffffffu, live);
+    if (!live) peers = ~peers;
+    for (int b = 0; b < bits; ++b) {
+      const bool set = digit >> b & 1;
+      const uint32_t votes = __ballot_sync(0xffffffffu, set);
+      peers &= set ? votes : ~votes;
+    }
     const uint32_t below = __popc(peers & ((1u << lane) - 1));
     uint32_t old = 0;
     if (live) old = sh.warp_hist[warp][digit];
@@ -335,7 +384,8 @@ __device__ __forceinline__ void store_grad_row(T* p, const float (&acc)[N], floa
 // one group of lanes.  Of a longer one every window of the list (positions that are a multiple
 // of kWindow and those behind) is summed by a warp of its own, and join_kernel adds the windows
 // up in order.  64: a group walks 80 rows at most; with 256 the longest of them held its CTA
-// for 40 us (1M skewed ids: 221 us for the sums).
+// for 40 us (1M skewed ids: 221 us for the sums), with 32 the joining took longer (43 us
+// against 28).  A CTA whose windows lie whole in one run leaves one sum for all of them.
 constexpr int kWindow = 64;
 struct Runs {
   const uint2* pairs;        // (key, position)
@@ -344,7 +394,7 @@ struct Runs {
 };
 constexpr int kSumThreads = 256;
 constexpr int kSumWarps = kSumThreads / 32;
-constexpr int kSumAhead = 8;   // rows in flight per lane
+constexpr int kSumAhead = 4;   // rows in flight per lane; with 8, fewer CTAs fit (182 us against 159)
 constexpr int kSumPiece = 16;  // positions whose runs (those that begin there) a group sums
 constexpr int kSumLeastLanes = 4;  // of a group, also where a row has less to load
 
@@ -361,20 +411,27 @@ __device__ __forceinline__ WindowParts find_parts(const Runs& r, int64_t window_
   const int64_t begin = window_index * kWindow;
   WindowParts p;
   p.count = (int)(r.n - begin < kWindow ? r.n - begin : kWindow);
-  const uint32_t first = r.pairs[begin].x, last = r.pairs[begin + p.count - 1].x;
-  uint64_t is_first = 0, is_last = 0, is_back = 0;  // bit i: position i; back: begin - 1 - i
+  uint32_t key[2], before[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int i = h * 32 + lane;
-    const uint32_t key = i < p.count ? r.pairs[begin + i].x : r.none;
-    const uint32_t before = begin - 1 - i >= 0 ? r.pairs[begin - 1 - i].x : r.none;
-    is_first |= (uint64_t)__ballot_sync(0xffffffffu, i < p.count && key == first) << (32 * h);
-    is_last |= (uint64_t)__ballot_sync(0xffffffffu, i < p.count && key == last) << (32 * h);
-    is_back |= (uint64_t)__ballot_sync(0xffffffffu, begin - 1 - i >= 0 && before == first) << (32 * h);
+    key[h] = i < p.count ? r.pairs[begin + i].x : r.none;
+    before[h] = begin - 1 - i >= 0 ? r.pairs[begin - 1 - i].x : r.none;
   }
-  p.head = __popcll(is_first);       // equal keys stand together
-  p.tail = p.count - __popcll(is_last);
-  const int back = __popcll(is_back);
+  const uint32_t first = __shfl_sync(0xffffffffu, key[0], 0);
+  const uint32_t last0 = __shfl_sync(0xffffffffu, key[0], (p.count - 1) & 31);
+  const uint32_t last1 = __shfl_sync(0xffffffffu, key[1], (p.count - 1) & 31);
+  const uint32_t last = p.count > 32 ? last1 : last0;
+  int back = 0, same_last = 0;
+  p.head = 0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {  // equal keys stand together
+    const int i = h * 32 + lane;
+    p.head += __popc(__ballot_sync(0xffffffffu, i < p.count && key[h] == first));
+    same_last += __popc(__ballot_sync(0xffffffffu, i < p.count && key[h] == last));
+    back += __popc(__ballot_sync(0xffffffffu, begin - 1 - i >= 0 && before[h] == first));
+  }
+  p.tail = p.count - same_last;
   // a run is long if the row kWindow behind its first is of the same vertex
   auto is_long = [&](int64_t s, uint32_t key) {
     return key != r.none && s + kWindow < r.n && r.pairs[s + kWindow].x == key;
@@ -384,6 +441,13 @@ __device__ __forceinline__ WindowParts find_parts(const Runs& r, int64_t window_
   if (p.tail == 0 || !is_long(begin + p.tail, last)) p.tail = p.count;
   return p;
 }
+
+// Whether the kSumWarps windows from `w` on lie whole in one run (which is long then).
+__device__ __forceinline__ bool whole_block(const Runs& r, int64_t w) {
+  const int64_t begin = w * kWindow, end = begin + kSumWarps * kWindow;
+  return end <= r.n && r.pairs[begin].x != r.none && r.pairs[begin].x == r.pairs[end - 1].x;
+}
+__device__ __forceinline__ int ceil_log2_device(int v) { return v <= 1 ? 0 : 32 - __clz(v - 1); }
 
 // The sum of `count` rows from position `from` on, all lanes of a warp, into to[feat_len].
 template <typename T, int N>
@@ -425,16 +489,36 @@ __device__ __forceinline__ void sum_part(const Runs& r, int64_t from, int count,
 }
 
 template <typename T, int N>
-__global__ void __launch_bounds__(kSumThreads)
+__global__ void __launch_bounds__(kSumThreads, 5)
 sum_kernel(Runs r, int n_windows, int window_blocks, const T* __restrict__ out_grad,
            int64_t out_grad_ld, int feat_len, float scale, int accumulate, T* __restrict__ grad,
            float* __restrict__ partial, int pitch, int log_lanes) {
   if ((int)blockIdx.x < window_blocks) {
     if (blockIdx.y > 0) return;
     const int64_t w = (int64_t)blockIdx.x * kSumWarps + (threadIdx.x >> 5);
+    const int64_t begin = w * kWindow;
+    const int64_t block_w = (int64_t)blockIdx.x * kSumWarps;
+    if (whole_block(r, block_w)) {
+      // one long run throughout: the warps' sums, added up in order, at the first window
+      __shared__ float whole[kSumWarps][128];
+      for (int c0 = 0; c0 < feat_len; c0 += 128) {
+        const int span = min(128, feat_len - c0);
+        const int span_lanes = min(log_lanes, ceil_log2_device((span + N - 1) / N));
+        sum_part<T, N>(r, begin, kWindow, out_grad + c0, out_grad_ld, span, span_lanes,
+                       whole[threadIdx.x >> 5]);
+        __syncthreads();
+        for (int c = threadIdx.x; c < span; c += kSumThreads) {
+          float s = 0.f;
+#pragma unroll
+          for (int k = 0; k < kSumWarps; ++k) s += whole[k][c];
+          partial[(block_w * 2 + 0) * pitch + c0 + c] = s;
+        }
+        __syncthreads();
+      }
+      return;
+    }
     if (w >= n_windows) return;
     const WindowParts p = find_parts(r, w);
-    const int64_t begin = w * kWindow;
     if (p.head > 0)
       sum_part<T, N>(r, begin, p.head, out_grad, out_grad_ld, feat_len, log_lanes,
                      partial + (w * 2 + 0) * pitch);
@@ -504,19 +588,50 @@ sum_kernel(Runs r, int n_windows, int window_blocks, const T* __restrict__ out_g
 }
 
 // A warp per window; works only where a long run begins in it.  The run's parts are this
-// window's and the heads of the windows behind.  A run of up to kJoinAlone windows is added up
+// window's and the heads of the windows behind.  A run of up to kJoinAlone parts is added up
 // by that warp, a longer one by all warps of the CTA: cut into as many stretches, each summed
 // in order, and these added in order.
 constexpr int kJoinAlone = 32;
 
-// The sum of parts t0 <= t < t1 of the run that begins in window w, for four columns from c on.
-__device__ __forceinline__ float4 join_terms(const float* partial, int64_t w, int slot, int64_t t0,
+// The parts of a long run: `count` windows from `first` on, of which those in whole blocks
+// have one sum between them.  Part t is that of window first + t up to the first block that is
+// whole, then of a block each, then of the windows behind the last.
+struct RunParts {
+  int64_t first, whole0, whole1, last;  // windows; blocks [whole0, whole1) are whole
+  int slot;
+  __device__ __forceinline__ int64_t count() const {
+    return whole1 > whole0 ? (whole0 - first) + (whole1 - whole0) / kSumWarps + (last + 1 - whole1)
+                           : last + 1 - first;
+  }
+  __device__ __forceinline__ int64_t window(int64_t t) const {
+    if (whole1 <= whole0 || t < whole0 - first) return first + t;
+    t -= whole0 - first;
+    const int64_t blocks = (whole1 - whole0) / kSumWarps;
+    return t < blocks ? whole0 + t * kSumWarps : whole1 + (t - blocks);
+  }
+};
+__device__ __forceinline__ RunParts run_parts(const Runs& r, int64_t first, int64_t windows, int slot) {
+  RunParts p;
+  p.first = first;
+  p.slot = slot;
+  p.last = first + windows - 1;
+  // whole blocks begin on a multiple of kSumWarps windows; the run's own first window counts
+  // only if the run begins on its first row, and the last block only if it is full of the run
+  p.whole0 = (first + kSumWarps - 1) / kSumWarps * kSumWarps;
+  if (p.whole0 == first && slot == 1) p.whole0 += kSumWarps;
+  p.whole1 = (p.last + 1) / kSumWarps * kSumWarps;
+  if (p.whole1 > p.whole0 && !whole_block(r, p.whole1 - kSumWarps)) p.whole1 -= kSumWarps;
+  return p;
+}
+
+// The sum of parts t0 <= t < t1, for four columns from c on.
+__device__ __forceinline__ float4 join_terms(const float* partial, const RunParts& p, int64_t t0,
                                              int64_t t1, int pitch, int c) {
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
   for (int64_t t = t0; t < t1; ++t) {
     const float4 v = *reinterpret_cast<const float4*>(
-        partial + ((w + t) * 2 + (t == 0 ? slot : 0)) * pitch + c);
+        partial + (p.window(t) * 2 + (t == 0 ? p.slot : 0)) * pitch + c);
     s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
   }
   return s;
@@ -536,8 +651,7 @@ template <typename T>
 __global__ void __launch_bounds__(kSumThreads)
 join_kernel(Runs r, int n_windows, int feat_len, float scale, int accumulate, T* __restrict__ grad,
             const float* __restrict__ partial, int pitch) {
-  __shared__ int slots[kSumWarps];         // -1: no long run begins in the warp's window
-  __shared__ int64_t all_terms[kSumWarps];
+  __shared__ RunParts runs[kSumWarps];     // those that the whole CTA adds up; slot -1: none
   __shared__ float4 sums[kSumWarps][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t w = (int64_t)blockIdx.x * kSumWarps + warp;
@@ -552,39 +666,41 @@ join_kernel(Runs r, int n_windows, int feat_len, float scale, int accumulate, T*
       else if (p.head > 0 && p.head_begins) slot = 0;
     }
   }
-  int64_t terms = 0;
+  RunParts parts;
+  parts.slot = -1;
   if (slot >= 0) {  // how many windows behind this one begin with the same vertex
-    terms = 1;
+    int64_t windows = 1;
     for (bool more = true; more;) {
       uint32_t same[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int64_t at = (w + terms + k * 32 + lane) * kWindow;
+        const int64_t at = (w + windows + k * 32 + lane) * kWindow;
         same[k] = __ballot_sync(0xffffffffu, at < r.n && r.pairs[at < r.n ? at : 0].x == key);
       }
       const int count = __popc(same[0]) + __popc(same[1]) + __popc(same[2]) + __popc(same[3]);
-      terms += count;
+      windows += count;
       more = count == 128;
     }
-    if (terms <= kJoinAlone)
+    parts = run_parts(r, w, windows, slot);
+    const int64_t terms = parts.count();
+    if (terms <= kJoinAlone) {
       for (int c = lane * 4; c < feat_len; c += 128)
         store_joined<T>(grad + (int64_t)key * feat_len, feat_len, c,
-                        join_terms(partial, w, slot, 0, terms, pitch, c), scale, accumulate);
+                        join_terms(partial, parts, 0, terms, pitch, c), scale, accumulate);
+      parts.slot = -1;
+    }
   }
-  if (lane == 0) {
-    slots[warp] = terms > kJoinAlone ? slot : -1;
-    all_terms[warp] = terms;
-  }
+  if (lane == 0) runs[warp] = parts;
   __syncthreads();
   for (int q = 0; q < kSumWarps; ++q) {
-    if (slots[q] < 0) continue;
-    const int64_t from = (int64_t)blockIdx.x * kSumWarps + q, n = all_terms[q];
-    const int64_t per = (n + kSumWarps - 1) / kSumWarps;
+    const RunParts run = runs[q];
+    if (run.slot < 0) continue;
+    const int64_t n = run.count(), per = (n + kSumWarps - 1) / kSumWarps;
     const int64_t t0 = min(n, warp * per), t1 = min(n, (warp + 1) * per);
-    const uint32_t vertex = r.pairs[(from + 1) * kWindow].x;
+    const uint32_t vertex = r.pairs[(run.first + 1) * kWindow].x;
     for (int c0 = 0; c0 < feat_len; c0 += 128) {
       const int c = c0 + lane * 4;
-      if (c < feat_len) sums[warp][lane] = join_terms(partial, from, slots[q], t0, t1, pitch, c);
+      if (c < feat_len) sums[warp][lane] = join_terms(partial, run, t0, t1, pitch, c);
       __syncthreads();
       if (warp == 0 && c < feat_len) {
         float4 s = sums[0][lane];
