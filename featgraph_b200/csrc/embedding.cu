@@ -111,68 +111,6 @@ __device__ __forceinline__ void zero_fill(const ZeroFill& z, int block, int bloc
   }
 }
 
-// Up to kRankMost ids: every position counts the pairs before it, (id, position) in order, and
-// that is its place.  n^2 comparisons, but one launch of a few microseconds (5003 ids: 3 us)
-// where the six of the radix sort take 30.
-constexpr int64_t kRankMost = 8192;
-constexpr int kRankThreads = 256;
-constexpr int kRankParts = 16;             // threads that share one position's comparisons
-constexpr int kRankTile = kRankThreads / kRankParts;
-
-__global__ void __launch_bounds__(kRankThreads)
-rank_kernel(KeySource src, int n, int sort_blocks, ZeroFill zero, uint2* __restrict__ pairs_out) {
-  if ((int)blockIdx.x >= sort_blocks) {
-    zero_fill(zero, blockIdx.x - sort_blocks, gridDim.x - sort_blocks, kRankThreads);
-    return;
-  }
-  __shared__ __align__(16) uint32_t keys[kRankMost];
-  const int whole = (n + 31) / 32 * 32;
-  for (int i0 = threadIdx.x; i0 < whole; i0 += kRankThreads * 16) {
-    int64_t id[16];
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const int i = i0 + k * kRankThreads;
-      id[k] = i < n ? load_source(src, i) : 0;
-    }
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const int i = i0 + k * kRankThreads;
-      if (i < whole) keys[i] = i < n ? make_key(src, id[k]) : 0xffffffffu;
-    }
-  }
-  __syncthreads();
-  const int i = blockIdx.x * kRankTile + threadIdx.x / kRankParts;
-  const int part = threadIdx.x % kRankParts;
-  const uint32_t mine = i < n ? keys[i] : 0;
-  uint32_t before = 0;
-  // equal ids count where they stand earlier: in front of this CTA's positions (whole steps of
-  // the loop) all do, behind them none
-  constexpr int kStep = kRankParts * 4;
-  const int tile0 = blockIdx.x * kRankTile / kStep * kStep;
-  const int tile1 = min(whole, ((int)blockIdx.x * kRankTile + kRankTile + kStep - 1) / kStep * kStep);
-  auto four = [&](int k) { return *reinterpret_cast<const uint4*>(&keys[k]); };
-#pragma unroll 4
-  for (int k = part * 4; k < tile0; k += kStep) {
-    const uint4 q = four(k);
-    before += (q.x <= mine) + (q.y <= mine) + (q.z <= mine) + (q.w <= mine);
-  }
-  for (int k = tile0 + part * 4; k < tile1; k += kStep) {
-    const uint4 q = four(k);
-    before += q.x < mine + (k < i);
-    before += q.y < mine + (k + 1 < i);
-    before += q.z < mine + (k + 2 < i);
-    before += q.w < mine + (k + 3 < i);
-  }
-#pragma unroll 4
-  for (int k = tile1 + part * 4; k < whole; k += kStep) {
-    const uint4 q = four(k);
-    before += (q.x < mine) + (q.y < mine) + (q.z < mine) + (q.w < mine);
-  }
-#pragma unroll
-  for (int d = 1; d < kRankParts; d <<= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
-  if (part == 0 && i < n) pairs_out[before] = make_uint2(mine, i);
-}
-
 // Stable least-significant-digit radix sort of (id, position) pairs, at most 9 bits a pass:
 // per block of kSortTile keys a histogram (sort_count_kernel), per digit an exclusive sum over
 // the blocks (sort_scan_kernel), then every pair to its place (sort_place_kernel).  Equal ids
@@ -716,6 +654,225 @@ join_kernel(Runs r, int n_windows, int feat_len, float scale, int accumulate, T*
   }
 }
 
+// ------------------------------------------------------ gradient: few ids --
+// Up to kFewIds ids the whole gradient is one launch.  The vertices are dealt out to kSlices
+// CTAs (times the slabs of columns): each looks through all ids for its own, keeps them in
+// order, ranks the few it has by (vertex, position), and sums.  A slice has one vertex of
+// every kSlices neighbours, at a place that changes from one such stretch to the next, so that neither
+// neighbouring nor evenly spaced popular vertices meet in one.  5003 skewed ids: the sort, sums
+// and join in launches of their own took 29 us.
+constexpr int64_t kFewIds = 8192;
+constexpr int kSliceBits = 7;
+constexpr int kSlices = 1 << kSliceBits;
+constexpr int kSliceThreads = 512;
+constexpr int kSliceAhead = 8;
+constexpr int kSliceAlone = 32;   // rows that one group of lanes sums alone
+constexpr int kSliceRank = 64;   // rows that are ranked by comparing each with each
+
+__device__ __forceinline__ uint32_t slice_shift(uint32_t high) {
+  return (high ^ high >> kSliceBits ^ high >> 2 * kSliceBits) & (kSlices - 1);
+}
+__device__ __forceinline__ uint32_t slice_of(uint32_t v) {
+  return (v & (kSlices - 1)) ^ slice_shift(v >> kSliceBits);
+}
+
+inline size_t slice_shared_bytes(int64_t n) { return (size_t)((n + 31) / 32 * 32) * 12; }
+
+template <typename T, int N>
+__global__ void __launch_bounds__(kSliceThreads)
+slice_kernel(KeySource src, int n, const T* __restrict__ out_grad, int64_t out_grad_ld, int feat_len,
+             float scale, int accumulate, T* __restrict__ grad, int log_lanes) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  const int room = (n + 31) / 32 * 32;
+  uint32_t* keys = reinterpret_cast<uint32_t*>(raw);            // of all ids
+  uint32_t* mine = keys + room;                                 // of this slice's, in order
+  uint16_t* found = reinterpret_cast<uint16_t*>(mine + room);   // their positions
+  uint16_t* sorted = found + room;                              // and these by (vertex, position)
+  __shared__ int warp_count[kSliceThreads / 32];
+  __shared__ int n_long, long_start[kFewIds / kSliceAlone];
+  __shared__ float sums[kSliceThreads * N];
+  const int warp = threadIdx.x >> 5, lane32 = threadIdx.x & 31;
+  const int lanes = 1 << log_lanes, groups = kSliceThreads >> log_lanes;
+  const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> log_lanes;
+  const int c = ((int)blockIdx.y * lanes + lane) * N;
+  const bool in = c < feat_len;
+
+  for (int i0 = threadIdx.x; i0 < room; i0 += kSliceThreads * 8) {
+    int64_t id[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = i0 + k * kSliceThreads;
+      id[k] = i < n ? load_source(src, i) : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = i0 + k * kSliceThreads;
+      if (i < room) keys[i] = i < n ? make_key(src, id[k]) : (uint32_t)src.n_vertices;
+    }
+  }
+  // zeros first; the sums overwrite them behind the barriers below
+  if (!accumulate && in) {
+    float zeros[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) zeros[k] = 0.f;
+    const Vec<T, N> zero = pack<T, N>(zeros);
+    for (int64_t high = group; high * kSlices < src.n_vertices; high += groups) {
+      const int64_t v = high * kSlices + (blockIdx.x ^ slice_shift((uint32_t)high));
+      if (v < src.n_vertices) store_vec<T, N>(grad + v * feat_len + c, zero);
+    }
+  }
+  if (threadIdx.x == 0) n_long = 0;
+  __syncthreads();
+  // each warp looks through a stretch of whole 32s
+  const int per = (room / 32 + kSliceThreads / 32 - 1) / (kSliceThreads / 32) * 32;
+  const int from = min(room, warp * per), to = min(room, from + per);
+  auto is_mine = [&](uint32_t key) {
+    return key < (uint32_t)src.n_vertices && slice_of(key) == blockIdx.x;
+  };
+  int count = 0;
+  for (int i = from + lane32; i < to; i += 32)
+    count += __popc(__ballot_sync(0xffffffffu, is_mine(keys[i])));
+  if (lane32 == 0) warp_count[warp] = count;
+  __syncthreads();
+  int at = 0, m = 0;
+#pragma unroll
+  for (int w = 0; w < kSliceThreads / 32; ++w) {
+    if (w == warp) at = m;
+    m += warp_count[w];
+  }
+  if (m == 0) return;
+  for (int i = from + lane32; i < to; i += 32) {
+    const uint32_t key = keys[i];
+    const uint32_t hits = __ballot_sync(0xffffffffu, is_mine(key));
+    if (is_mine(key)) {
+      const int e = at + __popc(hits & ((1u << lane32) - 1));
+      found[e] = (uint16_t)i;
+      mine[e] = key;
+    }
+    at += __popc(hits);
+  }
+  __syncthreads();
+  // While there are many: the rows of one vertex of theirs after the other are taken out, in
+  // order.  The vertex in the middle of the list is most likely the one that has most rows.
+  int left = m, out = 0;
+  __shared__ int warp_taken[kSliceThreads / 32];
+  for (int round = 0; left > kSliceRank && round < 64; ++round) {
+    const uint32_t pivot = mine[left / 2];
+    __syncthreads();
+    int kept = 0;
+    for (int e0 = 0; e0 < left; e0 += kSliceThreads) {
+      const int e = e0 + threadIdx.x;
+      const uint32_t key = e < left ? mine[e] : 0;
+      const uint16_t position = e < left ? found[e] : 0;
+      const uint32_t take = __ballot_sync(0xffffffffu, e < left && key == pivot);
+      const uint32_t keep = __ballot_sync(0xffffffffu, e < left && key != pivot);
+      if (lane32 == 0) {
+        warp_taken[warp] = __popc(take);
+        warp_count[warp] = __popc(keep);
+      }
+      __syncthreads();
+      int to_taken = out, to_kept = kept;
+#pragma unroll
+      for (int w = 0; w < kSliceThreads / 32; ++w) {
+        if (w < warp) {
+          to_taken += warp_taken[w];
+          to_kept += warp_count[w];
+        }
+        out += warp_taken[w];
+        kept += warp_count[w];
+      }
+      const uint32_t below = (1u << lane32) - 1;
+      if (take >> lane32 & 1) sorted[to_taken + __popc(take & below)] = position;
+      if (keep >> lane32 & 1) {
+        mine[to_kept + __popc(keep & below)] = key;
+        found[to_kept + __popc(keep & below)] = position;
+      }
+      __syncthreads();
+    }
+    left = kept;
+  }
+  // the others by counting what stands before them
+  for (int e = threadIdx.x; e < left; e += kSliceThreads) {
+    const uint32_t key = mine[e];
+    int rank = 0;
+    for (int f = 0; f < left; ++f) rank += mine[f] < key + (f < e);
+    sorted[out + rank] = found[e];
+  }
+  __syncthreads();
+  // a run per vertex: short ones to a group of lanes each
+  auto row_of = [&](int e) { return out_grad + (int64_t)sorted[e] * out_grad_ld + c; };
+  for (int e = group; e < m; e += groups) {
+    const uint32_t key = keys[sorted[e]];
+    if (e > 0 && keys[sorted[e - 1]] == key) continue;
+    int end = e + 1;
+    while (end < m && end - e <= kSliceAlone && keys[sorted[end]] == key) ++end;
+    if (end - e > kSliceAlone) {
+      if (lane == 0) long_start[atomicAdd(&n_long, 1)] = e;
+      continue;
+    }
+    if (!in) continue;
+    float acc[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) acc[k] = 0.f;
+    for (int j = e; j < end; j += kSliceAhead) {
+      Vec<T, N> row[kSliceAhead];
+#pragma unroll
+      for (int u = 0; u < kSliceAhead; ++u)
+        if (j + u < end) row[u] = load_vec_stream<T, N>(row_of(j + u));
+#pragma unroll
+      for (int u = 0; u < kSliceAhead; ++u)
+        if (j + u < end) {
+          float x[N];
+          unpack<T, N>(row[u], x);
+#pragma unroll
+          for (int k = 0; k < N; ++k) acc[k] += x[k];
+        }
+    }
+    store_grad_row<T, N>(grad + (int64_t)key * feat_len + c, acc, scale, accumulate);
+  }
+  __syncthreads();
+  // long ones to all groups, a stretch each, and their sums added up in order
+  for (int q = 0; q < n_long; ++q) {
+    const int e = long_start[q];
+    const uint32_t key = keys[sorted[e]];
+    int lo = e + kSliceAlone, hi = m;
+    while (lo < hi) {  // the first behind the run
+      const int mid = (lo + hi) >> 1;
+      if (keys[sorted[mid]] == key) lo = mid + 1; else hi = mid;
+    }
+    const int stretch = (lo - e + groups - 1) / groups;
+    const int j0 = min(lo, e + group * stretch), j1 = min(lo, j0 + stretch);
+    float acc[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) acc[k] = 0.f;
+    if (in)
+      for (int j = j0; j < j1; j += kSliceAhead) {
+        Vec<T, N> row[kSliceAhead];
+#pragma unroll
+        for (int u = 0; u < kSliceAhead; ++u)
+          if (j + u < j1) row[u] = load_vec_stream<T, N>(row_of(j + u));
+#pragma unroll
+        for (int u = 0; u < kSliceAhead; ++u)
+          if (j + u < j1) {
+            float x[N];
+            unpack<T, N>(row[u], x);
+#pragma unroll
+            for (int k = 0; k < N; ++k) acc[k] += x[k];
+          }
+      }
+#pragma unroll
+    for (int k = 0; k < N; ++k) sums[threadIdx.x * N + k] = acc[k];
+    __syncthreads();
+    if (group == 0 && in) {
+      for (int g = 1; g < groups; ++g)
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] += sums[((g << log_lanes) + lane) * N + k];
+      store_grad_row<T, N>(grad + (int64_t)key * feat_len + c, acc, scale, accumulate);
+    }
+    __syncthreads();
+  }
+}
+
 // ------------------------------------------------------------------- host --
 int ceil_log2(int64_t v) {
   int b = 0;
@@ -724,7 +881,7 @@ int ceil_log2(int64_t v) {
 }
 
 struct GradLayout {
-  bool rank;                 // few ids: rank_kernel instead of the radix sort
+  bool few;                  // one launch of slice_kernel
   int64_t windows, blocks;
   int passes, digit_bits;
   int pitch;                 // of a partial sum, in floats
@@ -732,8 +889,12 @@ struct GradLayout {
 };
 
 GradLayout grad_layout(int64_t n, int64_t n_vertices, int64_t feat_len) {
-  GradLayout l;
-  l.rank = n <= kRankMost;
+  GradLayout l = {};
+  l.few = n <= kFewIds;
+  if (l.few) {
+    l.total = 256;           // the kernel needs none; a caller always brings some
+    return l;
+  }
   l.windows = (n + kWindow - 1) / kWindow;
   l.blocks = (n + kSortTile - 1) / kSortTile;
   const int bits = std::max(1, ceil_log2(n_vertices + 1));  // n_vertices itself is a key
@@ -746,11 +907,9 @@ GradLayout grad_layout(int64_t n, int64_t n_vertices, int64_t feat_len) {
     return here;
   };
   l.pairs[0] = take((size_t)n * 8);
-  if (!l.rank) {
-    l.pairs[1] = take((size_t)n * 8);
-    l.counts = take(((size_t)l.blocks << l.digit_bits) * 4);
-    l.totals = take(kMaxBins * 4);
-  }
+  l.pairs[1] = take((size_t)n * 8);
+  l.counts = take(((size_t)l.blocks << l.digit_bits) * 4);
+  l.totals = take(kMaxBins * 4);
   l.pitch = (int)((feat_len + 3) / 4 * 4);
   l.partial = take((size_t)l.windows * 2 * l.pitch * 4);
   l.total = at;
@@ -877,30 +1036,53 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
   float* partial = reinterpret_cast<float*>(ws + l.partial);
   KeySource src = {ids_dev, nullptr, index_type == FG_INDEX_INT64, n_vertices,
                    padding_id < 0 ? -1 : padding_id, status_dev};
-  if (l.rank) {
-    const int blocks = (int)((n_ids + kRankTile - 1) / kRankTile);
-    rank_kernel<<<blocks + zero_blocks(zero), kRankThreads, 0, s>>>(src, (int)n_ids, blocks, zero, pairs[0]);
-    src.pairs = pairs[0];
-  } else {
-    uint32_t* counts = reinterpret_cast<uint32_t*>(ws + l.counts);
-    uint32_t* totals = reinterpret_cast<uint32_t*>(ws + l.totals);
-    const int bins = 1 << l.digit_bits, blocks = (int)l.blocks;
-    FG_CUDA_TRY(cudaFuncSetAttribute(sort_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     (int)sizeof(PlaceShared)));
-    for (int pass = 0; pass < l.passes; ++pass) {
-      const int shift = pass * l.digit_bits;
-      const ZeroFill z0 = zero_part(2 * pass, 2 * l.passes), z1 = zero_part(2 * pass + 1, 2 * l.passes);
-      sort_count_kernel<<<blocks + zero_blocks(z0), kSortThreads, 0, s>>>(src, n_ids, shift, l.digit_bits,
-                                                                        counts, blocks, z0);
-      sort_scan_kernel<<<(bins + kSortWarps - 1) / kSortWarps, kSortThreads, 0, s>>>(counts, blocks, bins,
-                                                                                   totals);
-      sort_place_kernel<<<blocks + zero_blocks(z1), kSortThreads, sizeof(PlaceShared), s>>>(
-          src, n_ids, shift, l.digit_bits, counts, totals, pairs[pass & 1], blocks, z1);
-      src.pairs = pairs[pass & 1];
-    }
+  const int per_row = (int)((feat_len * es + vb - 1) / vb);
+  if (l.few) {
+    // slabs of 256 bytes where the rows allow 16-byte accesses: a popular vertex of long rows is
+    // then the work of several CTAs
+    const int log_lanes = std::min(vb == 16 ? 4 : 5, ceil_log2(per_row));
+    const int64_t slabs = (per_row + (1 << log_lanes) - 1) >> log_lanes;
+    if (slabs > 65535) return fail(FG_ERR_UNSUPPORTED, "feat_len is too large");
+    const size_t smem = slice_shared_bytes(n_ids);
+    const dim3 grid(kSlices, (unsigned)slabs);
+#define FG_SLICE(T, N)                                                                             \
+  {                                                                                                \
+    FG_CUDA_TRY(cudaFuncSetAttribute(slice_kernel<T, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
+                                     (int)slice_shared_bytes(kFewIds)));                           \
+    slice_kernel<T, N><<<grid, kSliceThreads, smem, s>>>(                                          \
+        src, (int)n_ids, static_cast<const T*>(out_grad_dev), out_grad_ld, (int)feat_len, scale,   \
+        accumulate, static_cast<T*>(grad_dev), log_lanes);                                         \
+  }
+#define FG_SLICE_T(T)                                                       \
+  switch (vb / (int)sizeof(T)) {                                            \
+    case 8: if constexpr (sizeof(T) == 2) FG_SLICE(T, 8 / (sizeof(T) / 2)); break; \
+    case 4: FG_SLICE(T, 4); break;                                          \
+    case 2: FG_SLICE(T, 2); break;                                          \
+    default: FG_SLICE(T, 1); break;                                         \
+  }
+    FG_DISPATCH_DTYPE(dtype, FG_SLICE_T)
+#undef FG_SLICE_T
+#undef FG_SLICE
+    FG_CUDA_TRY(cudaGetLastError());
+    return FG_OK;
+  }
+  uint32_t* counts = reinterpret_cast<uint32_t*>(ws + l.counts);
+  uint32_t* totals = reinterpret_cast<uint32_t*>(ws + l.totals);
+  const int bins = 1 << l.digit_bits, blocks = (int)l.blocks;
+  FG_CUDA_TRY(cudaFuncSetAttribute(sort_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   (int)sizeof(PlaceShared)));
+  for (int pass = 0; pass < l.passes; ++pass) {
+    const int shift = pass * l.digit_bits;
+    const ZeroFill z0 = zero_part(2 * pass, 2 * l.passes), z1 = zero_part(2 * pass + 1, 2 * l.passes);
+    sort_count_kernel<<<blocks + zero_blocks(z0), kSortThreads, 0, s>>>(src, n_ids, shift, l.digit_bits,
+                                                                      counts, blocks, z0);
+    sort_scan_kernel<<<(bins + kSortWarps - 1) / kSortWarps, kSortThreads, 0, s>>>(counts, blocks, bins,
+                                                                                 totals);
+    sort_place_kernel<<<blocks + zero_blocks(z1), kSortThreads, sizeof(PlaceShared), s>>>(
+        src, n_ids, shift, l.digit_bits, counts, totals, pairs[pass & 1], blocks, z1);
+    src.pairs = pairs[pass & 1];
   }
   const Runs runs = {src.pairs, n_ids, (uint32_t)n_vertices};
-  const int per_row = (int)((feat_len * es + vb - 1) / vb);
   const int log_lanes = std::max(ceil_log2(kSumLeastLanes), std::min(5, ceil_log2(per_row)));
   const int64_t slabs = (per_row + (1 << log_lanes) - 1) >> log_lanes;
   const int64_t pieces = (n_ids + kSumPiece - 1) / kSumPiece;
@@ -921,8 +1103,7 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
     case 2: FG_SUM(T, 2); break;                                          \
     default: FG_SUM(T, 1); break;                                         \
   }                                                                       \
-  if (n_ids > kWindow)                                                    \
-    join_kernel<T><<<(int)window_blocks, kSumThreads, 0, s>>>(            \
+  join_kernel<T><<<(int)window_blocks, kSumThreads, 0, s>>>(            \
         runs, (int)l.windows, (int)feat_len, scale, accumulate, static_cast<T*>(grad_dev), partial, l.pitch);
   FG_DISPATCH_DTYPE(dtype, FG_SUM_T)
 #undef FG_SUM_T

@@ -127,7 +127,8 @@ def make_ids(kind, n, v, g):
     (1, 1, 1, "flat"), (1, 70001, 12, "flat"), (2, 3, 5, "same"), (31, 4, 8, "flat"), (32, 1, 64, "same"),
     (33, 600, 33, "skewed"), (65, 40, 128, "same"), (4096, 511, 16, "skewed"), (4097, 512, 100, "skewed"),
     (5003, 10007, 100, "skewed"), (20011, 262144, 64, "flat"), (30000, 3, 130, "skewed"),
-    (100003, 1000, 24, "skewed"), (66000, 70000, 260, "skewed")])
+    (100003, 1000, 24, "skewed"), (66000, 70000, 260, "skewed"), (8192, 5, 40, "flat"), (8192, 7, 136, "same"),
+    (8193, 9, 72, "skewed"), (8000, 3, 33, "skewed"), (7000, 1500000, 4, "flat"), (3000, 64, 700, "skewed")])
 def test_lookup_grad(dtype, n, v, f, kind):
     g = gen(n + v + f)
     ids = make_ids(kind, n, v, g).to(torch.int32 if n % 2 else torch.int64)
@@ -167,6 +168,21 @@ def test_lookup_grad_padding_accumulate_and_strides(dtype):
         check(into, want, bound, dy.dtype)
         if padding is not None:
             assert torch.equal(into[padding], before[padding])
+
+
+@pytest.mark.parametrize("n, distinct", [(8192, 8192), (6000, 500), (8192, 1000)])
+def test_lookup_grad_of_ids_that_meet_in_one_slice(n, distinct):
+    # vertices that the kernel for few ids deals to one and the same CTA
+    high = torch.arange(distinct, device="cuda")
+    vertices = high * 128 + ((high ^ (high >> 7) ^ (high >> 14)) & 127)
+    g = gen(n)
+    ids = vertices[torch.randint(distinct, (n,), generator=g, device="cuda")]
+    v = distinct * 128
+    dy = torch.randn((n, 4), generator=g, device="cuda")
+    m = module.EmbeddingLookupcuda()
+    m.build([te.placeholder((v, 4), "float32")] + like(ids), {"with_grad": True}, {})
+    want, bound = grad_reference(dy, ids, v, 1.0)
+    check(m.run_grad([dy, ids]).torch, want, bound, dy.dtype)
 
 
 def test_lookup_grad_without_ids():
