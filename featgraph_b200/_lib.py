@@ -37,7 +37,7 @@ EXPORTED_SYMBOLS = (
     "fg_spmm_dds_plan_status", "fg_spmm_dds_f32", "fg_sddmm_status",
     "fg_embedding_lookup", "fg_embedding_grad_workspace_bytes", "fg_embedding_grad",
     "fg_softmax_xent_workspace_bytes", "fg_softmax_xent", "fg_softmax_xent_grad",
-    "fg_gradient_clip_workspace_bytes", "fg_gradient_clip",
+    "fg_gradient_clip_workspace_bytes", "fg_gradient_clip", "fg_training_call",
 )
 
 LAUNCH_PROGRAMMATIC, SPMM_GIANT_ROWS_ONLY, SPMM_SKIP_GIANT_ROWS, SDDMM_TMA_STAGING = 1, 2, 4, 8  # fg_launch_flags
@@ -46,6 +46,7 @@ MSG_OPS = ("mul", "add", "sub", "div", "copy_lhs", "copy_rhs")    # enum fg_msg_
 REDUCE_OPS = ("sum", "max", "min")                                # enum fg_reduce_op
 DTYPES = ("float32", "bfloat16", "float16")                       # enum fg_dtype
 INDEX_TYPES = ("int32", "int64")                                  # enum fg_index_type
+OP_LOOKUP, OP_LOOKUP_GRAD, OP_XENT, OP_XENT_GRAD, OP_CLIP = range(5)   # enum fg_training_op
 
 
 def load():
@@ -108,6 +109,7 @@ def load():
     lib.fg_softmax_xent_grad.argtypes = [c_void, c_void, i64, c_void, i64, i32, c_void, i32, i64,
                                          i64, i64, f32, i64, c_void, c_void, c_void, c_void, i64,
                                          c_void, i32, c_void]
+    lib.fg_training_call.argtypes = [i32, ctypes.c_char_p, i32]
     lib.fg_gradient_clip_workspace_bytes.argtypes = [i32]
     lib.fg_gradient_clip_workspace_bytes.restype = i64
     lib.fg_gradient_clip.argtypes = [c_void, c_void, c_void, c_void, i32, i32, f64, f64, c_void,

@@ -1,5 +1,7 @@
 // Error reporting, version and the host-only partitioning helpers of the C ABI.
 #include <algorithm>
+#include <cstring>
+#include <utility>
 
 #include "common.cuh"
 
@@ -84,4 +86,44 @@ extern "C" int fg_shard_edges(int64_t nnz, int32_t world, int64_t* bounds) {
   const int64_t chunk = ((nnz + world - 1) / world + 31) / 32 * 32;
   for (int32_t k = 0; k <= world; ++k) bounds[k] = std::min<int64_t>(nnz, chunk * k);
   return FG_OK;
+}
+
+namespace {
+// An argument of fg_training_call: whatever the callee's parameter is.
+struct Word {
+  int64_t w;
+  template <typename T>
+  operator T*() const { return reinterpret_cast<T*>(static_cast<uintptr_t>(w)); }
+  operator int64_t() const { return w; }
+  operator int32_t() const { return static_cast<int32_t>(w); }
+  operator double() const {
+    double d;
+    memcpy(&d, &w, sizeof(d));
+    return d;
+  }
+  operator float() const { return static_cast<float>(static_cast<double>(*this)); }
+};
+template <typename... P, size_t... I>
+int call_with(int (*f)(P...), const int64_t* words, std::index_sequence<I...>) {
+  return f(static_cast<P>(Word{words[I]})...);
+}
+template <typename... P>
+int call(int (*f)(P...), const int64_t* words, int32_t n_words) {
+  if (n_words != (int32_t)sizeof...(P))
+    return fg::fail(FG_ERR_INVALID_ARGUMENT, "%d argument words, this call takes %d", (int)n_words,
+                    (int)sizeof...(P));
+  return call_with(f, words, std::index_sequence_for<P...>());
+}
+}  // namespace
+
+extern "C" int fg_training_call(int32_t training_op, const int64_t* words, int32_t n_words) {
+  if (!words) return fg::fail(FG_ERR_INVALID_ARGUMENT, "null words");
+  switch (training_op) {
+    case FG_OP_EMBEDDING_LOOKUP: return call(fg_embedding_lookup, words, n_words);
+    case FG_OP_EMBEDDING_GRAD: return call(fg_embedding_grad, words, n_words);
+    case FG_OP_SOFTMAX_XENT: return call(fg_softmax_xent, words, n_words);
+    case FG_OP_SOFTMAX_XENT_GRAD: return call(fg_softmax_xent_grad, words, n_words);
+    case FG_OP_GRADIENT_CLIP: return call(fg_gradient_clip, words, n_words);
+  }
+  return fg::fail(FG_ERR_INVALID_ARGUMENT, "unknown training_op=%d", (int)training_op);
 }

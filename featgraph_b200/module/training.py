@@ -9,8 +9,9 @@ another stream than the module's last one waits for that one first; while a stre
 captured nothing is waited for, so two graphs that hold calls of one module must not be
 replayed side by side.
 """
-import ctypes
+import array
 import math
+import struct
 
 import torch
 
@@ -23,6 +24,14 @@ _TORCH_DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16"
                  "int32": torch.int32, "int64": torch.int64}
 
 
+# The argument words of the C calls (fg_training_call): q an integer or a pointer, d a number.
+_LOOKUP = struct.Struct("=8qd5q")
+_LOOKUP_GRAD = struct.Struct("=8qd8q")
+_XENT = struct.Struct("=10qd8q")
+_XENT_GRAD = struct.Struct("=11qd9q")
+_CLIP = struct.Struct("=6qdd5q")
+
+
 class _TrainingOp(object):
     """What the three modules share: device, workspace, status word, stream hand-over."""
     _compute_func = None
@@ -32,10 +41,11 @@ class _TrainingOp(object):
         if not torch.cuda.is_available():
             raise RuntimeError("%s needs a CUDA device; there is no CPU fallback"
                                % type(self).__name__)
-        _lib.load()
         self._target = "cuda"
+        self._call = _lib.load().fg_training_call
         self._ctx = gpu(int(device_id))
         self._device = self._ctx.torch_device
+        self._index = self._ctx.device_id
         self._spec = None
         self.out_tvm = None
 
@@ -53,7 +63,10 @@ class _TrainingOp(object):
         size = max(self._workspace_bytes(out), 16)
         self._workspace = self._own(torch.empty(size, dtype=torch.uint8, device=self._device))
         self._workspace_size = size
+        self._workspace_at = self._workspace.data_ptr()
+        self._status_at = self._status.data_ptr()
         self._last_stream = torch.cuda.current_stream(self._device)
+        self._last_handle = self._last_stream.cuda_stream
         self._spec = out
 
     def _own(self, tensor):
@@ -72,14 +85,19 @@ class _TrainingOp(object):
 
     def _stream(self):
         """The current stream's handle, ordered behind the module's last call."""
+        handle = torch._C._cuda_getCurrentRawStream(self._index)
+        if handle != self._last_handle:
+            self._change_stream(handle)
+        return handle
+
+    def _change_stream(self, handle):
+        if torch.cuda.is_current_stream_capturing():
+            return
         stream = torch.cuda.current_stream(self._device)
-        if stream != self._last_stream:
-            if not torch.cuda.is_current_stream_capturing():
-                stream.wait_stream(self._last_stream)
-                for t in self._owned:
-                    t.record_stream(stream)
-                self._last_stream = stream
-        return ctypes.c_void_p(stream.cuda_stream)
+        stream.wait_stream(self._last_stream)
+        for t in self._owned:
+            t.record_stream(stream)
+        self._last_stream, self._last_handle = stream, handle
 
     def _need(self, count, inputs, what):
         if self._spec is None:
@@ -87,13 +105,26 @@ class _TrainingOp(object):
         if len(inputs) != count:
             raise ValueError("%s takes exactly %d input arrays, got %d" % (what, count, len(inputs)))
 
-    def _tensor(self, x, shape, dtype, what, rows=False):
-        """Check one input against its placeholder; ``rows``: a 2-D array whose rows may lie
+    @staticmethod
+    def _expect(placeholder, what, rows=False, dtype=None):
+        """What ``_tensor`` checks an input against; ``rows``: a 2-D array whose rows may lie
         apart (each row itself contiguous)."""
+        return (placeholder.shape, _TORCH_DTYPES[dtype or placeholder.dtype], what, rows)
+
+    def _tensor(self, x, expected):
+        """One input as a torch tensor, checked (this runs in every call: the usual case is
+        one line)."""
+        t = x.torch if type(x) is NDArray else x
+        if isinstance(t, torch.Tensor) and t.dtype is expected[1] and t.shape == expected[0] \
+                and t.get_device() == self._index and t.is_contiguous():
+            return t
+        return self._odd_tensor(x, *expected)
+
+    def _odd_tensor(self, x, shape, dtype, what, rows):
         t = x.torch if isinstance(x, NDArray) else x
         if not isinstance(t, torch.Tensor):
             raise TypeError("%s: expected an NDArray or a torch.Tensor, got %r" % (what, type(x)))
-        if t.dtype != _TORCH_DTYPES[dtype]:
+        if t.dtype != dtype:
             raise TypeError("%s: dtype %s does not match the placeholder's %s" % (what, t.dtype,
                                                                                  dtype))
         if tuple(t.shape) != shape:
@@ -110,9 +141,11 @@ class _TrainingOp(object):
                                  "strides %r" % (what, t.stride()))
         return t
 
-    @staticmethod
-    def _pitch(t):
-        return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+    def _rows(self, x, expected):
+        """``_tensor`` and the distance between its rows in elements."""
+        t = self._tensor(x, expected)
+        width = expected[0][1]
+        return t, width if t.is_contiguous() or expected[0][0] < 2 else t.stride(0)
 
     def device_status(self):
         """Synchronise and return the status word: 0 when every id and label so far was in
@@ -159,6 +192,14 @@ class EmbeddingLookupcuda(_TrainingOp):
         if out.attrs["with_grad"]:
             self.grad_tvm = self._own_zeros(table.shape, table.dtype)
         self._codes = (_lib.DTYPES.index(table.dtype), _lib.INDEX_TYPES.index(ids.dtype))
+        self._table = self._expect(table, "Table", rows=True)
+        self._ids = self._expect(ids, "Ids")
+        self._into = self._expect(table, "accumulate_into")
+        self._out_grad = (out.shape, self._table[1], "OutGrad", True)
+        a = out.attrs
+        self._sizes = (out.shape[0], a["num_vertices"], a["feat_len"], a["scale"])
+        self._padding = -1 if a["padding_idx"] is None else a["padding_idx"]
+        self._out_at = self.out_tvm.torch.data_ptr()
 
     def _workspace_bytes(self, out):
         if not out.attrs["with_grad"]:
@@ -166,19 +207,18 @@ class EmbeddingLookupcuda(_TrainingOp):
         return int(_lib.load().fg_embedding_grad_workspace_bytes(
             out.shape[0], out.attrs["num_vertices"], out.attrs["feat_len"]))
 
-    def _launch(self, table, ids):
-        a = self._spec.attrs
-        _lib.check(_lib.load().fg_embedding_lookup(
-            table.data_ptr(), self._codes[0], self._pitch(table), a["num_vertices"],
-            ids.data_ptr(), self._codes[1], self._spec.shape[0], a["feat_len"], a["scale"],
-            self.out_tvm.torch.data_ptr(), a["feat_len"], self._status.data_ptr(),
-            self._ctx.device_id, self._stream()))
+    def _launch(self, table, pitch, ids):
+        n, vertices, feat_len, scale = self._sizes
+        code = self._call(_lib.OP_LOOKUP, _LOOKUP.pack(
+            table.data_ptr(), self._codes[0], pitch, vertices, ids.data_ptr(), self._codes[1], n,
+            feat_len, scale, self._out_at, feat_len, self._status_at, self._index,
+            self._stream()), 14)
+        if code:
+            _lib.check(code)
 
     def _checked_inputs(self, inputs):
         self._need(2, inputs, "run()")
-        tp, ip = self._spec.inputs
-        return (self._tensor(inputs[0], tp.shape, tp.dtype, "Table", rows=True),
-                self._tensor(inputs[1], ip.shape, ip.dtype, "Ids"))
+        return self._rows(inputs[0], self._table) + (self._tensor(inputs[1], self._ids),)
 
     def run(self, input_tvm_ndarrays):
         """[Table, Ids] -> ``self.out_tvm``, the same array every call."""
@@ -187,8 +227,8 @@ class EmbeddingLookupcuda(_TrainingOp):
 
     def measure_average_time(self, input_tvm_ndarrays, num_runs):
         """Mean seconds of the lookup over ``num_runs`` launches."""
-        table, ids = self._checked_inputs(input_tvm_ndarrays)
-        return time_launches(self._ctx, lambda: self._launch(table, ids), num_runs)
+        inputs = self._checked_inputs(input_tvm_ndarrays)
+        return time_launches(self._ctx, lambda: self._launch(*inputs), num_runs)
 
     def run_grad(self, input_tvm_ndarrays, accumulate_into=None):
         """[OutGrad (n, F), Ids] -> the table's gradient (V, F): ``self.grad_tvm``, the same
@@ -196,23 +236,22 @@ class EmbeddingLookupcuda(_TrainingOp):
         array of the table's type (say, the gradient that a loss with tied weights left) that
         the sums are added onto instead; it is returned."""
         self._need(2, input_tvm_ndarrays, "run_grad()")
-        a = self._spec.attrs
-        if not a["with_grad"]:
+        if self.grad_tvm is None:
             raise RuntimeError("run_grad() needs build(..., {'with_grad': True}, ...)")
-        tp, ip = self._spec.inputs
-        dy = self._tensor(input_tvm_ndarrays[0], self._spec.shape, tp.dtype, "OutGrad", rows=True)
-        ids = self._tensor(input_tvm_ndarrays[1], ip.shape, ip.dtype, "Ids")
+        dy, pitch = self._rows(input_tvm_ndarrays[0], self._out_grad)
+        ids = self._tensor(input_tvm_ndarrays[1], self._ids)
         if accumulate_into is None:
             result, grad = self.grad_tvm, self.grad_tvm.torch
         else:
-            result = accumulate_into
-            grad = self._tensor(accumulate_into, tp.shape, tp.dtype, "accumulate_into")
-        padding = -1 if a["padding_idx"] is None else a["padding_idx"]
-        _lib.check(_lib.load().fg_embedding_grad(
-            dy.data_ptr(), self._codes[0], self._pitch(dy), ids.data_ptr(), self._codes[1],
-            self._spec.shape[0], a["num_vertices"], a["feat_len"], a["scale"], padding,
-            accumulate_into is not None, grad.data_ptr(), self._workspace.data_ptr(),
-            self._workspace_size, self._status.data_ptr(), self._ctx.device_id, self._stream()))
+            result, grad = accumulate_into, self._tensor(accumulate_into, self._into)
+        n, vertices, feat_len, scale = self._sizes
+        code = self._call(_lib.OP_LOOKUP_GRAD, _LOOKUP_GRAD.pack(
+            dy.data_ptr(), self._codes[0], pitch, ids.data_ptr(), self._codes[1], n, vertices,
+            feat_len, scale, self._padding, accumulate_into is not None, grad.data_ptr(),
+            self._workspace_at, self._workspace_size, self._status_at, self._index,
+            self._stream()), 17)
+        if code:
+            _lib.check(code)
         return result
 
 
@@ -240,6 +279,13 @@ class SoftmaxCrossEntropycuda(_TrainingOp):
             self.feat_grad_tvm = self._own_zeros(feat.shape, feat.dtype)
             self.weight_grad_tvm = self._own_zeros(weight.shape, weight.dtype)
         self._codes = (_lib.DTYPES.index(feat.dtype), _lib.INDEX_TYPES.index(labels.dtype))
+        self._inputs = (self._expect(feat, "Feat", rows=True),
+                        self._expect(weight, "Weight", rows=True), self._expect(labels, "Labels"))
+        self._loss_grad = (out.shape, torch.float32, "LossGrad", False)
+        self._lse = (out.shape, torch.float32, "Lse", False)
+        a = out.attrs
+        self._sizes = (out.shape[0], a["vocab"], a["feat_len"], a["scale"], a["ignore_index"])
+        self._loss_at, self._lse_at = self.out_tvm.torch.data_ptr(), self.lse_tvm.torch.data_ptr()
 
     def _workspace_bytes(self, out):
         return int(_lib.load().fg_softmax_xent_workspace_bytes(
@@ -247,19 +293,19 @@ class SoftmaxCrossEntropycuda(_TrainingOp):
             out.attrs["feat_len"], out.attrs["with_grad"]))
 
     def _checked_inputs(self, inputs):
-        fp, wp, lp = self._spec.inputs
-        return (self._tensor(inputs[0], fp.shape, fp.dtype, "Feat", rows=True),
-                self._tensor(inputs[1], wp.shape, wp.dtype, "Weight", rows=True),
-                self._tensor(inputs[2], lp.shape, lp.dtype, "Labels"))
+        e = self._inputs
+        return (self._rows(inputs[0], e[0]) + self._rows(inputs[1], e[1])
+                + (self._tensor(inputs[2], e[2]),))
 
-    def _launch(self, feat, weight, labels):
-        a = self._spec.attrs
-        _lib.check(_lib.load().fg_softmax_xent(
-            feat.data_ptr(), self._pitch(feat), weight.data_ptr(), self._pitch(weight),
-            self._codes[0], labels.data_ptr(), self._codes[1], self._spec.shape[0], a["vocab"],
-            a["feat_len"], a["scale"], a["ignore_index"], self.out_tvm.torch.data_ptr(),
-            self.lse_tvm.torch.data_ptr(), self._workspace.data_ptr(), self._workspace_size,
-            self._status.data_ptr(), self._ctx.device_id, self._stream()))
+    def _launch(self, feat, feat_pitch, weight, weight_pitch, labels):
+        n, vocab, feat_len, scale, ignore = self._sizes
+        code = self._call(_lib.OP_XENT, _XENT.pack(
+            feat.data_ptr(), feat_pitch, weight.data_ptr(), weight_pitch, self._codes[0],
+            labels.data_ptr(), self._codes[1], n, vocab, feat_len, scale, ignore, self._loss_at,
+            self._lse_at, self._workspace_at, self._workspace_size, self._status_at, self._index,
+            self._stream()), 19)
+        if code:
+            _lib.check(code)
 
     def run(self, input_tvm_ndarrays):
         """[Feat, Weight, Labels] -> (``self.out_tvm``, ``self.lse_tvm``): the losses and the
@@ -279,19 +325,21 @@ class SoftmaxCrossEntropycuda(_TrainingOp):
         ``self.weight_grad_tvm``), the same arrays every call, every element overwritten.
         ``Lse`` is what ``run`` returned for these inputs."""
         self._need(5, input_tvm_ndarrays, "run_grad()")
-        a = self._spec.attrs
-        if not a["with_grad"]:
+        if self.feat_grad_tvm is None:
             raise RuntimeError("run_grad() needs build(..., {'with_grad': True}, ...)")
-        dl = self._tensor(input_tvm_ndarrays[0], self._spec.shape, "float32", "LossGrad")
-        feat, weight, labels = self._checked_inputs(input_tvm_ndarrays[1:4])
-        lse = self._tensor(input_tvm_ndarrays[4], self._spec.shape, "float32", "Lse")
-        _lib.check(_lib.load().fg_softmax_xent_grad(
-            dl.data_ptr(), feat.data_ptr(), self._pitch(feat), weight.data_ptr(),
-            self._pitch(weight), self._codes[0], labels.data_ptr(), self._codes[1],
-            self._spec.shape[0], a["vocab"], a["feat_len"], a["scale"], a["ignore_index"],
+        dl = self._tensor(input_tvm_ndarrays[0], self._loss_grad)
+        feat, feat_pitch, weight, weight_pitch, labels = \
+            self._checked_inputs(input_tvm_ndarrays[1:4])
+        lse = self._tensor(input_tvm_ndarrays[4], self._lse)
+        n, vocab, feat_len, scale, ignore = self._sizes
+        code = self._call(_lib.OP_XENT_GRAD, _XENT_GRAD.pack(
+            dl.data_ptr(), feat.data_ptr(), feat_pitch, weight.data_ptr(), weight_pitch,
+            self._codes[0], labels.data_ptr(), self._codes[1], n, vocab, feat_len, scale, ignore,
             lse.data_ptr(), self.feat_grad_tvm.torch.data_ptr(),
-            self.weight_grad_tvm.torch.data_ptr(), self._workspace.data_ptr(),
-            self._workspace_size, self._status.data_ptr(), self._ctx.device_id, self._stream()))
+            self.weight_grad_tvm.torch.data_ptr(), self._workspace_at, self._workspace_size,
+            self._status_at, self._index, self._stream()), 21)
+        if code:
+            _lib.check(code)
         return self.feat_grad_tvm, self.weight_grad_tvm
 
 
@@ -314,32 +362,34 @@ class GradientClipcuda(_TrainingOp):
         self.clipped_tvm = None
         if not out.attrs["in_place"]:
             self.clipped_tvm = [self._own_zeros(p.shape, p.dtype) for p in out.inputs]
-        sizes = [int(math.prod(p.shape)) for p in out.inputs]
-        self._sizes = (ctypes.c_int64 * n)(*sizes)
-        self._codes = (ctypes.c_int32 * n)(*[_lib.DTYPES.index(p.dtype) for p in out.inputs])
-        self._ins = (ctypes.c_void_p * n)()
-        if out.attrs["in_place"]:
-            self._outs = self._ins
-        else:
-            self._outs = (ctypes.c_void_p * n)(*[a.torch.data_ptr() for a in self.clipped_tvm])
+        # host arrays of the C call; what address they lie at is asked for once
+        self._sizes = array.array("q", [int(math.prod(p.shape)) for p in out.inputs] or [0])
+        self._codes = array.array("i", [_lib.DTYPES.index(p.dtype) for p in out.inputs] or [0])
+        self._outs = None
+        if not out.attrs["in_place"]:
+            self._outs = array.array("Q", [a.torch.data_ptr() for a in self.clipped_tvm] or [0])
+            self._outs_at = self._outs.buffer_info()[0]
+        self._sizes_at, self._codes_at = (a.buffer_info()[0] for a in (self._sizes, self._codes))
+        self._inputs = [self._expect(p, "Grads[%d]" % k) for k, p in enumerate(out.inputs)]
+        self._args = (n, out.attrs["norm_type"] == math.inf, out.attrs["max_norm"],
+                      out.attrs["eps"], self.out_tvm.torch.data_ptr())
 
     def _workspace_bytes(self, out):
         return int(_lib.load().fg_gradient_clip_workspace_bytes(len(out.inputs)))
 
     def _launch(self, tensors):
-        a = self._spec.attrs
-        for k, t in enumerate(tensors):
-            self._ins[k] = t.data_ptr()
-        _lib.check(_lib.load().fg_gradient_clip(
-            self._ins, self._outs, self._sizes, self._codes, len(tensors),
-            a["norm_type"] == math.inf, a["max_norm"], a["eps"], self.out_tvm.torch.data_ptr(),
-            self._workspace.data_ptr(), self._workspace_size, self._ctx.device_id,
-            self._stream()))
+        ins = array.array("Q", [t.data_ptr() for t in tensors])
+        ins_at = ins.buffer_info()[0]
+        code = self._call(_lib.OP_CLIP, _CLIP.pack(
+            ins_at, ins_at if self._outs is None else self._outs_at, self._sizes_at,
+            self._codes_at, *self._args, self._workspace_at, self._workspace_size, self._index,
+            self._stream()), 13)
+        if code:
+            _lib.check(code)
 
     def _checked_inputs(self, inputs):
         self._need(len(self._spec.inputs) if self._spec else 0, inputs, "run()")
-        tensors = [self._tensor(x, p.shape, p.dtype, "Grads[%d]" % k)
-                   for k, (x, p) in enumerate(zip(inputs, self._spec.inputs))]
+        tensors = [self._tensor(x, e) for x, e in zip(inputs, self._inputs)]
         if self._spec.attrs["in_place"]:
             spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
                            for t in tensors if t.numel())

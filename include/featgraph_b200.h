@@ -433,6 +433,19 @@ int fg_gradient_clip(const void* const* grads_host_array, void* const* outs_host
                      float* norm_dev, void* workspace_dev, int64_t workspace_bytes,
                      int32_t device, void* stream);
 
+/* The five calls above with their arguments as 64-bit words: word i is argument i in the
+ * order of the declaration, a pointer or an integer as such, a float or a double as the
+ * bits of a double.  For callers whose language spends more on passing an argument than
+ * a small kernel takes (ctypes: 5 us for fourteen). */
+enum fg_training_op {
+  FG_OP_EMBEDDING_LOOKUP = 0,
+  FG_OP_EMBEDDING_GRAD = 1,
+  FG_OP_SOFTMAX_XENT = 2,
+  FG_OP_SOFTMAX_XENT_GRAD = 3,
+  FG_OP_GRADIENT_CLIP = 4
+};
+int fg_training_call(int32_t training_op, const int64_t* words, int32_t n_words);
+
 /* ------------------------------------------------- multi-GPU partitioning -- */
 
 /* Splits the rows of a CSR matrix into `world` contiguous blocks holding about

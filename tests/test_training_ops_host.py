@@ -162,3 +162,19 @@ def test_workspace_sizes_grow_with_the_work(lib):
     assert sizes == sorted(sizes) and sizes[0] > 0
     assert lib.fg_gradient_clip_workspace_bytes(5000) > lib.fg_gradient_clip_workspace_bytes(1) > 0
     assert np.iinfo(np.int32).max < lib.fg_embedding_grad_workspace_bytes(2000000000, 1000, 64)
+
+
+def test_calls_by_words(lib):
+    import struct
+    words = struct.pack("=8qd5q", 4096, 0, 8, 10, 4096, 0, 0, 8, 1.0, 4096, 8, 4096, 0, 0)
+    assert lib.fg_training_call(_lib.OP_LOOKUP, words, 14) == 0        # no ids: nothing to do
+    _refused(lib, lib.fg_training_call(_lib.OP_LOOKUP, words, 13), 1, "takes 14")
+    _refused(lib, lib.fg_training_call(9, words, 14), 1, "training_op")
+    _refused(lib, lib.fg_training_call(_lib.OP_LOOKUP, None, 14), 1, "null")
+    bad = struct.pack("=8qd5q", 4096, 0, 7, 10, 4096, 0, 5, 8, 1.0, 4096, 8, 4096, 0, 0)
+    _refused(lib, lib.fg_training_call(_lib.OP_LOOKUP, bad, 14), 1, "pitch")
+    # a number arrives as such: max_norm = -1.5 is refused by its value
+    clip = struct.pack("=6qdd5q", 4096, 4096, 4096, 4096, 0, 0, -1.5, 1e-6, 4096, 4096, 1 << 20, 0, 0)
+    _refused(lib, lib.fg_training_call(_lib.OP_CLIP, clip, 13), 1, "-1.5")
+    for op, fields in ((_lib.OP_LOOKUP_GRAD, 17), (_lib.OP_XENT, 19), (_lib.OP_XENT_GRAD, 21)):
+        _refused(lib, lib.fg_training_call(op, words, 1), 1, "takes %d" % fields)
