@@ -109,6 +109,7 @@ __device__ double block_norm(double v, double* shared) {
 template <bool MAX_NORM>
 __global__ void __launch_bounds__(kClipThreads)
 partial_norm_kernel(const __grid_constant__ ClipTensors t, double* __restrict__ partial) {
+  begin_chained();
   __shared__ double shared[kClipThreads / 32];
   double acc = 0.0;
   float top = 0.f;
@@ -152,6 +153,7 @@ template <bool MAX_NORM>
 __global__ void __launch_bounds__(kClipThreads)
 scale_kernel(const __grid_constant__ ClipTensors t, const double* __restrict__ partial,
              int n_partial, double max_norm, double eps, float* __restrict__ norm_out) {
+  begin_chained();
   __shared__ double shared[kClipThreads / 32];
   double acc = 0.0;
   for (int i = threadIdx.x; i < n_partial; i += kClipThreads)
@@ -249,21 +251,15 @@ extern "C" int fg_gradient_clip(const void* const* grads_host_array, void* const
   int32_t next = 0;
   do {
     next = fill(next, t, grid);
-    if (max_abs_norm)
-      partial_norm_kernel<true><<<grid, kClipThreads, 0, s>>>(t, partial + n_partial);
-    else
-      partial_norm_kernel<false><<<grid, kClipThreads, 0, s>>>(t, partial + n_partial);
-    FG_CUDA_TRY(cudaGetLastError());
+    FG_CUDA_TRY(launch(n_partial > 0, max_abs_norm ? partial_norm_kernel<true> : partial_norm_kernel<false>,
+                       grid, kClipThreads, 0, s, t, partial + n_partial));
     n_partial += grid;
   } while (next < n_tensors);
   next = 0;
   do {
     next = fill(next, t, grid);
-    if (max_abs_norm)
-      scale_kernel<true><<<grid, kClipThreads, 0, s>>>(t, partial, n_partial, max_norm, eps, norm_dev);
-    else
-      scale_kernel<false><<<grid, kClipThreads, 0, s>>>(t, partial, n_partial, max_norm, eps, norm_dev);
-    FG_CUDA_TRY(cudaGetLastError());
+    FG_CUDA_TRY(launch(true, max_abs_norm ? scale_kernel<true> : scale_kernel<false>, grid, kClipThreads,
+                       0, s, t, partial, n_partial, max_norm, eps, norm_dev));
   } while (next < n_tensors);
   return FG_OK;
 }

@@ -128,4 +128,31 @@ __device__ __forceinline__ void store_vec_stream(T* p, const Vec<T, N>& v) {
     default: CALL(__half); break;               \
   }
 
+// Launches a kernel; `chained`: programmatically behind the one before it in the stream, a
+// kernel of the same call, so that its launch overlaps that one's run.  Every kernel that is
+// launched this way begins with wait_for_prior_grids() before it touches memory, and lets the
+// next one be launched (launch_dependents) only behind that, so nothing overtakes anything.
+template <typename... P, typename... A>
+cudaError_t launch(bool chained, void (*kernel)(P...), dim3 grid, int threads, size_t smem,
+                   cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = chained ? 1 : 0;
+  return cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
+}
+
+#ifdef __CUDACC__
+__device__ __forceinline__ void begin_chained() {
+  wait_for_prior_grids();
+  launch_dependents();
+}
+#endif
+
 }  // namespace fg

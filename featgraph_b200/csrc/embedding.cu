@@ -128,6 +128,7 @@ static_assert(kMaxBins == kSortThreads, "one thread per digit");
 __global__ void __launch_bounds__(kSortThreads)
 sort_count_kernel(KeySource src, int64_t n, int shift, int bits, uint32_t* __restrict__ counts,
                   int sort_blocks, ZeroFill zero) {
+  begin_chained();
   if ((int)blockIdx.x >= sort_blocks) {
     zero_fill(zero, blockIdx.x - sort_blocks, gridDim.x - sort_blocks, kSortThreads);
     return;
@@ -155,6 +156,7 @@ sort_count_kernel(KeySource src, int64_t n, int shift, int bits, uint32_t* __res
 __global__ void __launch_bounds__(kSortThreads)
 sort_scan_kernel(uint32_t* __restrict__ counts, int n_blocks, int bins,
                  uint32_t* __restrict__ totals) {
+  begin_chained();
   const int digit = blockIdx.x * kSortWarps + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (digit >= bins) return;
@@ -192,6 +194,7 @@ __global__ void __launch_bounds__(kSortThreads)
 sort_place_kernel(KeySource src, int64_t n, int shift, int bits,
                   const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals,
                   uint2* __restrict__ pairs_out, int sort_blocks, ZeroFill zero) {
+  begin_chained();
   if ((int)blockIdx.x >= sort_blocks) {
     zero_fill(zero, blockIdx.x - sort_blocks, gridDim.x - sort_blocks, kSortThreads);
     return;
@@ -431,6 +434,7 @@ __global__ void __launch_bounds__(kSumThreads, 5)
 sum_kernel(Runs r, int n_windows, int window_blocks, const T* __restrict__ out_grad,
            int64_t out_grad_ld, int feat_len, float scale, int accumulate, T* __restrict__ grad,
            float* __restrict__ partial, int pitch, int log_lanes) {
+  begin_chained();
   if ((int)blockIdx.x < window_blocks) {
     if (blockIdx.y > 0) return;
     const int64_t w = (int64_t)blockIdx.x * kSumWarps + (threadIdx.x >> 5);
@@ -589,6 +593,7 @@ template <typename T>
 __global__ void __launch_bounds__(kSumThreads)
 join_kernel(Runs r, int n_windows, int feat_len, float scale, int accumulate, T* __restrict__ grad,
             const float* __restrict__ partial, int pitch) {
+  begin_chained();
   __shared__ RunParts runs[kSumWarps];     // those that the whole CTA adds up; slot -1: none
   __shared__ float4 sums[kSumWarps][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1074,12 +1079,12 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
   for (int pass = 0; pass < l.passes; ++pass) {
     const int shift = pass * l.digit_bits;
     const ZeroFill z0 = zero_part(2 * pass, 2 * l.passes), z1 = zero_part(2 * pass + 1, 2 * l.passes);
-    sort_count_kernel<<<blocks + zero_blocks(z0), kSortThreads, 0, s>>>(src, n_ids, shift, l.digit_bits,
-                                                                      counts, blocks, z0);
-    sort_scan_kernel<<<(bins + kSortWarps - 1) / kSortWarps, kSortThreads, 0, s>>>(counts, blocks, bins,
-                                                                                 totals);
-    sort_place_kernel<<<blocks + zero_blocks(z1), kSortThreads, sizeof(PlaceShared), s>>>(
-        src, n_ids, shift, l.digit_bits, counts, totals, pairs[pass & 1], blocks, z1);
+    FG_CUDA_TRY(launch(pass > 0, sort_count_kernel, blocks + zero_blocks(z0), kSortThreads, 0, s, src, n_ids,
+                       shift, l.digit_bits, counts, blocks, z0));
+    FG_CUDA_TRY(launch(true, sort_scan_kernel, (bins + kSortWarps - 1) / kSortWarps, kSortThreads, 0, s,
+                       counts, blocks, bins, totals));
+    FG_CUDA_TRY(launch(true, sort_place_kernel, blocks + zero_blocks(z1), kSortThreads, sizeof(PlaceShared),
+                       s, src, n_ids, shift, l.digit_bits, counts, totals, pairs[pass & 1], blocks, z1));
     src.pairs = pairs[pass & 1];
   }
   const Runs runs = {src.pairs, n_ids, (uint32_t)n_vertices};
@@ -1091,20 +1096,21 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
   if (blocks_x > INT32_MAX || slabs > 65535)
     return fail(FG_ERR_UNSUPPORTED, "n_ids x feat_len is too large");
   const dim3 grid((unsigned)blocks_x, (unsigned)slabs);
-#define FG_SUM(T, N)                                                                          \
-  sum_kernel<T, N><<<grid, kSumThreads, 0, s>>>(                                              \
-      runs, (int)l.windows, (int)window_blocks, static_cast<const T*>(out_grad_dev),          \
-      out_grad_ld, (int)feat_len, scale, accumulate, static_cast<T*>(grad_dev), partial,      \
-      l.pitch, log_lanes)
+#define FG_SUM(T, N)                                                                             \
+  FG_CUDA_TRY(launch(true, sum_kernel<T, N>, grid, kSumThreads, 0, s, runs, (int)l.windows,      \
+                     (int)window_blocks, static_cast<const T*>(out_grad_dev), out_grad_ld,       \
+                     (int)feat_len, scale, accumulate, static_cast<T*>(grad_dev), partial, l.pitch, \
+                     log_lanes))
 #define FG_SUM_T(T)                                                       \
   switch (vb / (int)sizeof(T)) {                                          \
     case 8: if constexpr (sizeof(T) == 2) FG_SUM(T, 8 / (sizeof(T) / 2)); break; \
     case 4: FG_SUM(T, 4); break;                                          \
     case 2: FG_SUM(T, 2); break;                                          \
-    default: FG_SUM(T, 1); break;                                         \
-  }                                                                       \
-  join_kernel<T><<<(int)window_blocks, kSumThreads, 0, s>>>(            \
-        runs, (int)l.windows, (int)feat_len, scale, accumulate, static_cast<T*>(grad_dev), partial, l.pitch);
+    default: FG_SUM(T, 1); break;                                                                \
+  }                                                                                              \
+  FG_CUDA_TRY(launch(true, join_kernel<T>, (int)window_blocks, kSumThreads, 0, s, runs,          \
+                     (int)l.windows, (int)feat_len, scale, accumulate, static_cast<T*>(grad_dev), \
+                     partial, l.pitch));
   FG_DISPATCH_DTYPE(dtype, FG_SUM_T)
 #undef FG_SUM_T
 #undef FG_SUM

@@ -69,6 +69,7 @@ struct MmaArgs {
   int slots;              // of the ring in shared memory
   int buffers;            // S tiles in TMEM
   int feat_len, out_cols; // out_cols: feat_len rounded up to 16
+  int out_vec;            // bytes of an aligned access to the results' rows
   int negate;             // a negative scale: |scale| with -A
   float logit_scale;      // |scale| * log2(e)
   const float* unscale;   // float32: what undoes the operands' scaling; else null
@@ -175,6 +176,19 @@ __device__ __forceinline__ Item item_at(const MmaArgs& a, int i) {
   return it;
 }
 
+// x[0 ... min(16, left)), N (a divisor of what `left` can be) at a time.
+template <typename T, int N>
+__device__ __forceinline__ void store_pieces(T* to, int left, const float (&x)[16]) {
+#pragma unroll
+  for (int k = 0; k < 16; k += N) {
+    if (k >= left) break;
+    float piece[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) piece[i] = x[k + i];
+    store_vec<T, N>(to + k, pack<T, N>(piece));
+  }
+}
+
 // Stores 16 columns of one row of the results.
 template <int MODE, typename T>
 __device__ __forceinline__ void store_out(const MmaArgs& a, const Item& item, int64_t row, int c,
@@ -188,21 +202,14 @@ __device__ __forceinline__ void store_out(const MmaArgs& a, const Item& item, in
     return;
   }
   T* to = static_cast<T*>(a.out) + row * a.feat_len + c;
-  constexpr int N = 16 / sizeof(T);
-  if (a.feat_len % N == 0 && ((uintptr_t)a.out & 15) == 0) {
+  float x[16];
 #pragma unroll
-    for (int k = 0; k < 16; k += N) {
-      if (c + k >= a.feat_len) break;
-      float x[N];
-#pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = live ? v[k + i] * factor : 0.f;
-      store_vec<T, N>(to + k, pack<T, N>(x));
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-      if (c + k < a.feat_len) to[k] = from_float<T>(live ? v[k] * factor : 0.f);
-  }
+  for (int k = 0; k < 16; ++k) x[k] = live ? v[k] * factor : 0.f;
+  // as wide as every row of the results is aligned
+  if (a.out_vec == 16) store_pieces<T, 16 / sizeof(T)>(to, a.feat_len - c, x);
+  else if (a.out_vec == 8) store_pieces<T, 8 / sizeof(T)>(to, a.feat_len - c, x);
+  else if (a.out_vec == 4) store_pieces<T, 4 / sizeof(T)>(to, a.feat_len - c, x);
+  else store_pieces<T, 1>(to, a.feat_len - c, x);
 }
 
 template <int MODE, typename T, bool STREAM>
@@ -249,6 +256,7 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
+  begin_chained();
   // all 512 columns are this CTA's: they start at address 0, and the S tiles there
   constexpr uint32_t tmem = 0;
   const uint32_t out_at = tmem + a.buffers * Shape::kCols;
@@ -717,30 +725,43 @@ struct Consts {
   float out_feat, out_weight;       // factors of the two gradients
   float inv_weight_max;             // 1 / the largest |loss_grad|
 };
-constexpr int kMaxPartials = 256;
+constexpr int kMaxPartials = 592;
 
-// Largest finite magnitude per CTA of the rows that take part, for both float32 operands.
+// Largest finite magnitude per CTA of the rows that take part, for both float32 operands
+// (blockIdx.y).  A warp a row, four loads a lane ahead.
 __global__ void __launch_bounds__(256)
 abs_max_kernel(Batch b, const float* __restrict__ feat, int64_t feat_ld,
                const float* __restrict__ weight, int64_t weight_ld, float* __restrict__ partial) {
+  begin_chained();
   float top = 0.f;
   const bool second = blockIdx.y == 1;
   const float* p = second ? weight : feat;
   const int64_t rows = second ? b.vocab : b.n, ld = second ? weight_ld : feat_ld;
-  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8) {
-    if (!second && live_label(b, r) < 0) continue;
-#pragma unroll 4
-    for (int64_t c = threadIdx.x & 31; c < b.feat_len; c += 32) {
-      const float v = fabsf(p[r * ld + c]);
-      if (v < INFINITY) top = fmaxf(top, v);
+  // 32 lanes take whole rows of up to 128 elements four at a time, longer rows one at a time
+  const int per_row = (int)min((int64_t)4, (b.feat_len + 31) / 32), together = 4 / per_row;
+  const int64_t warps = (int64_t)gridDim.x * 8;
+  for (int64_t r0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * together; r0 < rows;
+       r0 += warps * together) {
+    for (int64_t c0 = threadIdx.x & 31; c0 < b.feat_len; c0 += 32 * per_row) {
+      float v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t r = r0 + k / per_row, c = c0 + (k % per_row) * 32;
+        const bool in = k < together * per_row && r < rows && c < b.feat_len;
+        v[k] = in ? fabsf(p[r * ld + c]) : 0.f;
+        if (!second && in && live_label(b, r) < 0) v[k] = 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (v[k] < INFINITY) top = fmaxf(top, v[k]);
     }
   }
-  __shared__ float warps[8];
+  __shared__ float warps_top[8];
   for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = top;
+  if ((threadIdx.x & 31) == 0) warps_top[threadIdx.x >> 5] = top;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < 8; ++w) top = fmaxf(top, warps[w]);
+    for (int w = 1; w < 8; ++w) top = fmaxf(top, warps_top[w]);
     partial[blockIdx.y * kMaxPartials + blockIdx.x] = top;
   }
 }
@@ -762,82 +783,111 @@ __device__ __forceinline__ int operand_exponent(float top) {
   return min(60, max(-60, 13 - e));
 }
 
+// What the gradients' kernels need of a sample, and of the padding up to a whole tile.
+struct SampleArrays {
+  const float *lse, *loss_grad;
+  float *row_bias, *row_factor, *col_bias, *col_weight;
+  int32_t* label;
+  int64_t padded;
+  float hot;
+};
+__device__ __forceinline__ void sample(const Batch& b, const SampleArrays& s, float inv_weight_max,
+                                       int64_t t) {
+  const int32_t y = live_label(b, t);
+  float bias = -INFINITY, weight = 0.f, g = 0.f;
+  if (y >= 0) {
+    g = s.loss_grad[t];
+    weight = g * inv_weight_max;
+    bias = log2f(s.hot) - s.lse[t] * kLog2e;
+  }
+  s.label[t] = y;
+  s.row_bias[t] = bias;
+  s.row_factor[t] = g * b.scale / s.hot;
+  s.col_weight[t] = weight;
+  s.col_bias[t] = weight == 0.f ? -INFINITY : bias + log2f(fabsf(weight));
+}
+
+// The scalars, by one CTA; it also makes the sample arrays of a batch of up to kSetupSamples.
+constexpr int64_t kSetupSamples = 8192;
 __global__ void __launch_bounds__(1024)
-setup_kernel(Batch b, const float* __restrict__ loss_grad, const float* __restrict__ abs_max,
-             int n_abs_max, float hot, Consts* consts) {
+setup_kernel(Batch b, SampleArrays s, const float* __restrict__ abs_max, Consts* consts) {
+  begin_chained();
   __shared__ float shared[32];
   float top = 0.f;
-  if (loss_grad)
+  if (s.loss_grad)
     for (int64_t t = threadIdx.x; t < b.n; t += 1024)
-      if (live_label(b, t) >= 0) top = fmaxf(top, fabsf(loss_grad[t]));
+      if (live_label(b, t) >= 0) top = fmaxf(top, fabsf(s.loss_grad[t]));
   top = block_max(top, shared);
   int ef = 0, ew = 0;
   if (abs_max) {
-    const bool in = threadIdx.x < n_abs_max;
+    const bool in = threadIdx.x < kMaxPartials;
     ef = operand_exponent(block_max(in ? abs_max[threadIdx.x] : 0.f, shared));
     ew = operand_exponent(block_max(in ? abs_max[kMaxPartials + threadIdx.x] : 0.f, shared));
   }
+  const float inv = top >= 1.17549435e-38f ? 1.f / top : 0.f;
   if (threadIdx.x == 0) {
     Consts c;
     c.scale_feat = ldexpf(1.f, ef);
     c.scale_weight = ldexpf(1.f, ew);
     c.unscale = ldexpf(1.f, -ef - ew);
     c.out_feat = ldexpf(1.f, -ew);
-    c.out_weight = top * b.scale / hot * ldexpf(1.f, -ef);
-    c.inv_weight_max = top >= 1.17549435e-38f ? 1.f / top : 0.f;
+    c.out_weight = top * b.scale / s.hot * ldexpf(1.f, -ef);
+    c.inv_weight_max = inv;
     *consts = c;
   }
+  if (s.loss_grad && s.padded <= kSetupSamples)
+    for (int64_t t = threadIdx.x; t < s.padded; t += 1024) sample(b, s, inv, t);
+}
+__global__ void __launch_bounds__(256)
+sample_kernel(Batch b, SampleArrays s, const Consts* __restrict__ consts) {
+  begin_chained();
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t < s.padded) sample(b, s, consts->inv_weight_max, t);
 }
 
-// An operand as the tensor maps want it: rows of `pitch` 16-bit elements, zero behind feat_len.
+// Operands as the tensor maps want them: rows of `pitch` 16-bit elements, zero behind feat_len.
 // float32 becomes two fp16 pieces, the second behind the first.  A row whose label is out of
-// play (`masked`) becomes zero, whatever it held.
+// play (`masked`) becomes zero, whatever it held.  The first `blocks` CTAs pack one operand, the
+// others the second.
+template <typename T>
+struct PackJob {
+  const T* from;
+  int64_t ld, rows;
+  int blocks, masked;
+  const float* factor;
+  uint16_t* to;
+};
 template <typename T>
 __global__ void __launch_bounds__(256)
-pack_kernel(Batch b, const T* __restrict__ from, int64_t ld, int64_t rows, int64_t pitch,
-            int masked, const float* __restrict__ factor, uint16_t* __restrict__ to) {
+pack_kernel(Batch b, PackJob<T> first, PackJob<T> second, int64_t pitch) {
+  begin_chained();
+  const bool is_second = (int)blockIdx.x >= first.blocks;
+  const PackJob<T> j = is_second ? second : first;
+  const int64_t block = is_second ? blockIdx.x - first.blocks : blockIdx.x;
   const int64_t piece = sizeof(T) == 4 ? pitch / 2 : pitch;
-  const float f = sizeof(T) == 4 ? *factor : 1.f;
-  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8) {
-    const bool live = !masked || live_label(b, r) >= 0;
-    for (int64_t c = threadIdx.x & 31; c < piece; c += 32) {
-      const bool in = live && c < b.feat_len;
-      if (sizeof(T) == 4) {
-        const float x = in ? to_float<T>(from[r * ld + c]) * f : 0.f;
-        const __half hi = __float2half_rn(x);
-        to[r * pitch + c] = __half_as_ushort(hi);
-        to[r * pitch + piece + c] = __half_as_ushort(__float2half_rn(x - __half2float(hi)));
+  const float f = sizeof(T) == 4 ? *j.factor : 1.f;
+  for (int64_t r = block * 8 + (threadIdx.x >> 5); r < j.rows; r += (int64_t)j.blocks * 8) {
+    const bool live = !j.masked || live_label(b, r) >= 0;
+    // two neighbouring elements a lane, so that the 16-bit pieces are written as 32 bits
+#pragma unroll 2
+    for (int64_t c = (threadIdx.x & 31) * 2; c < piece; c += 64) {
+      T x[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        x[k] = live && c + k < b.feat_len ? j.from[r * j.ld + c + k] : from_float<T>(0.f);
+      if constexpr (sizeof(T) == 4) {
+        const __half2 hi = __floats2half2_rn(x[0] * f, x[1] * f);
+        const float2 back = __half22float2(hi);
+        const __half2 lo = __floats2half2_rn(x[0] * f - back.x, x[1] * f - back.y);
+        *reinterpret_cast<__half2*>(j.to + r * pitch + c) = hi;
+        *reinterpret_cast<__half2*>(j.to + r * pitch + piece + c) = lo;
       } else {
-        uint16_t raw = 0;
-        if (in) memcpy(&raw, &from[r * ld + c], 2);
-        to[r * pitch + c] = raw;
+        uint32_t raw;
+        memcpy(&raw, x, 4);
+        *reinterpret_cast<uint32_t*>(j.to + r * pitch + c) = raw;
       }
     }
   }
-}
-
-struct SampleArrays {
-  float *row_bias, *row_factor, *col_bias, *col_weight;
-  int32_t* label;
-};
-// Per sample, and for the padding up to a whole tile: what the gradients' kernels need of it.
-__global__ void __launch_bounds__(256)
-sample_kernel(Batch b, const float* __restrict__ lse, const float* __restrict__ loss_grad, float hot,
-              const Consts* __restrict__ consts, int64_t padded, SampleArrays s) {
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= padded) return;
-  const int32_t y = live_label(b, t);
-  float bias = -INFINITY, weight = 0.f, g = 0.f;
-  if (y >= 0) {
-    g = loss_grad[t];
-    weight = g * consts->inv_weight_max;
-    bias = log2f(hot) - lse[t] * kLog2e;
-  }
-  s.label[t] = y;
-  s.row_bias[t] = bias;
-  s.row_factor[t] = g * b.scale / hot;
-  s.col_weight[t] = weight;
-  s.col_bias[t] = weight == 0.f ? -INFINITY : bias + log2f(fabsf(weight));
 }
 
 // loss and lse of a sample from its partial maxima and sums (base 2); the label's logit is
@@ -847,6 +897,7 @@ __global__ void __launch_bounds__(256)
 join_loss_kernel(Batch b, const T* __restrict__ feat, int64_t feat_ld, const T* __restrict__ weight,
                  int64_t weight_ld, const float2* __restrict__ stats, int parts,
                  float* __restrict__ loss, float* __restrict__ lse, int32_t* status) {
+  begin_chained();
   const int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (t >= b.n) return;
   const int lane = threadIdx.x & 31;
@@ -887,22 +938,36 @@ join_loss_kernel(Batch b, const T* __restrict__ feat, int64_t feat_ld, const T* 
   }
 }
 
-// A gradient from the partial sums of its splits, added in order.
+// A gradient from the partial sums of its splits.  A thread adds every kJoinParts-th of them,
+// and the first thread of a result those sums in order.
+constexpr int kJoinParts = 8;
 template <typename T>
 __global__ void __launch_bounds__(256)
 join_partial_kernel(const float* __restrict__ partial, int splits, int64_t rows, int out_cols,
                     int feat_len, const float* __restrict__ row_factor,
                     const int32_t* __restrict__ row_label, const float* __restrict__ out_scale,
                     T* __restrict__ out) {
+  begin_chained();
+  constexpr int kQuads = 256 / kJoinParts;
+  __shared__ float4 sums[kJoinParts][kQuads];
   const int quads = out_cols / 4;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int part = threadIdx.x / kQuads, at = threadIdx.x % kQuads;
+  const int64_t i = (int64_t)blockIdx.x * kQuads + at;
   const int64_t row = i / quads;
   const int c = (int)(i - row * quads) * 4;
-  if (row >= rows) return;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (row < rows)
 #pragma unroll 4
-  for (int k = 0; k < splits; ++k) {
-    const float4 p = *reinterpret_cast<const float4*>(partial + (k * rows + row) * out_cols + c);
+    for (int k = part; k < splits; k += kJoinParts) {
+      const float4 p = *reinterpret_cast<const float4*>(partial + (k * rows + row) * out_cols + c);
+      sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
+    }
+  sums[part][at] = sum;
+  __syncthreads();
+  if (part != 0 || row >= rows) return;
+#pragma unroll
+  for (int k = 1; k < kJoinParts; ++k) {
+    const float4 p = sums[k][at];
     sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
   }
   const float factor = (out_scale ? *out_scale : 1.f) * (row_factor ? row_factor[row] : 1.f);
@@ -1027,53 +1092,54 @@ bool fits_map(int32_t dtype, const void* p, int64_t ld) {
   return dtype != FG_FLOAT32 && ((uintptr_t)p & 15) == 0 && ld % 8 == 0;
 }
 
-template <typename T>
-int pack_operand(const Batch& b, const T* from, int64_t ld, int64_t rows, int64_t pitch, int masked,
-                 const float* factor, void* to, cudaStream_t s) {
-  const int grid = (int)std::min<int64_t>((rows + 7) / 8, 8 * kSms);
-  pack_kernel<T><<<grid, 256, 0, s>>>(b, from, ld, rows, pitch, masked, factor,
-                                      static_cast<uint16_t*>(to));
-  FG_CUDA_TRY(cudaGetLastError());
-  return FG_OK;
-}
-
-// Scales of float32 operands, consts, packed copies where they are needed.
+// Scalars, sample arrays (with loss_grad), scales of float32 operands, and packed copies where
+// they are needed.  `chained`: whether this call has launched something before.
 template <typename T>
 int prepare_operands(const Batch& b, const XentLayout& l, char* ws, const T* feat, int64_t feat_ld,
-                     const T* weight, int64_t weight_ld, int32_t dtype, const float* loss_grad,
-                     float hot, bool masked, cudaStream_t s, Operands* o) {
+                     const T* weight, int64_t weight_ld, int32_t dtype, const SampleArrays& samples,
+                     cudaStream_t s, Operands* o, bool* chained) {
   Consts* consts = reinterpret_cast<Consts*>(ws + l.consts);
   float* abs_max = reinterpret_cast<float*>(ws + l.abs_max);
+  const bool grad = samples.loss_grad != nullptr;
   if constexpr (sizeof(T) == 4) {
-    abs_max_kernel<<<dim3(kMaxPartials, 2), 256, 0, s>>>(b, feat, feat_ld, weight, weight_ld, abs_max);
-    FG_CUDA_TRY(cudaGetLastError());
+    FG_CUDA_TRY(launch(*chained, abs_max_kernel, dim3(kMaxPartials, 2), 256, 0, s, b, feat, feat_ld, weight,
+                       weight_ld, abs_max));
+    *chained = true;
   }
-  if (sizeof(T) == 4 || loss_grad) {
-    setup_kernel<<<1, 1024, 0, s>>>(b, loss_grad, sizeof(T) == 4 ? abs_max : nullptr, kMaxPartials,
-                                    hot, consts);
-    FG_CUDA_TRY(cudaGetLastError());
+  if (sizeof(T) == 4 || grad) {
+    FG_CUDA_TRY(launch(*chained, setup_kernel, 1, 1024, 0, s, b, samples,
+                       sizeof(T) == 4 ? abs_max : nullptr, consts));
+    *chained = true;
+    if (grad && samples.padded > kSetupSamples)
+      FG_CUDA_TRY(launch(true, sample_kernel, (unsigned)((samples.padded + 255) / 256), 256, 0, s, b, samples,
+                         consts));
   }
   *o = {feat, weight, feat_ld, weight_ld};
-  if (masked || !fits_map(dtype, feat, feat_ld)) {
-    if (int rc = pack_operand<T>(b, feat, feat_ld, b.n, l.pitch, masked, &consts->scale_feat,
-                                 ws + l.packed_feat, s))
-      return rc;
+  auto blocks = [](int64_t rows) { return (int)std::min<int64_t>((rows + 7) / 8, 8 * kSms); };
+  PackJob<T> jobs[2] = {};
+  if (grad || !fits_map(dtype, feat, feat_ld)) {
+    jobs[0] = {feat, feat_ld, b.n, blocks(b.n), grad, &consts->scale_feat,
+               reinterpret_cast<uint16_t*>(ws + l.packed_feat)};
     o->feat = ws + l.packed_feat;
     o->feat_ld = l.pitch;
   }
   if (!fits_map(dtype, weight, weight_ld)) {
-    if (int rc = pack_operand<T>(b, weight, weight_ld, b.vocab, l.pitch, 0, &consts->scale_weight,
-                                 ws + l.packed_weight, s))
-      return rc;
+    jobs[1] = {weight, weight_ld, b.vocab, blocks(b.vocab), 0, &consts->scale_weight,
+               reinterpret_cast<uint16_t*>(ws + l.packed_weight)};
     o->weight = ws + l.packed_weight;
     o->weight_ld = l.pitch;
+  }
+  if (jobs[0].blocks + jobs[1].blocks > 0) {
+    FG_CUDA_TRY(launch(*chained, pack_kernel<T>, jobs[0].blocks + jobs[1].blocks, 256, 0, s, b, jobs[0],
+                       jobs[1], l.pitch));
+    *chained = true;
   }
   return FG_OK;
 }
 
 template <int MODE, typename T, bool STREAM>
 int launch_mma_as(const Batch& b, const XentLayout& l, const Operands& o, const Cut& cut, MmaArgs a,
-                  cudaStream_t s) {
+                  bool chained, cudaStream_t s) {
   using Shape = MmaShape<MODE, T, STREAM>;
   const bool rows_are_samples = MODE != kWeightGrad;
   const void* row_p = rows_are_samples ? o.feat : o.weight;
@@ -1099,6 +1165,7 @@ int launch_mma_as(const Batch& b, const XentLayout& l, const Operands& o, const 
   a.feat_len = (int)b.feat_len;
   a.out_cols = l.out_cols;
   a.negate = b.scale < 0.f;
+  a.out_vec = common_vector_bytes({(uint64_t)(uintptr_t)a.out, (uint64_t)b.feat_len * sizeof(T)});
   a.logit_scale = std::fabs(b.scale) * kLog2e;
   // shared memory: 14 tiles of 16 KB at most, 13 where the columns' biases need some of it
   const int room = MODE == kWeightGrad ? 13 : 14;
@@ -1112,16 +1179,16 @@ int launch_mma_as(const Batch& b, const XentLayout& l, const Operands& o, const 
   FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   const int64_t items = (int64_t)a.row_tiles * a.splits * a.chunks;
   if (items > INT32_MAX) return fail(FG_ERR_UNSUPPORTED, "too many tiles");
-  kernel<<<(int)std::min<int64_t>(items, kSms), Shape::kThreads, smem, s>>>(row_map, col_map, a);
-  FG_CUDA_TRY(cudaGetLastError());
+  FG_CUDA_TRY(launch(chained, kernel, (unsigned)std::min<int64_t>(items, kSms), Shape::kThreads, smem, s,
+                     row_map, col_map, a));
   return FG_OK;
 }
 
 template <int MODE, typename T>
 int launch_mma(const Batch& b, const XentLayout& l, const Operands& o, const Cut& cut, const MmaArgs& a,
-               cudaStream_t s) {
-  return l.tiles <= kMaxResidentTiles ? launch_mma_as<MODE, T, false>(b, l, o, cut, a, s)
-                                      : launch_mma_as<MODE, T, true>(b, l, o, cut, a, s);
+               bool chained, cudaStream_t s) {
+  return l.tiles <= kMaxResidentTiles ? launch_mma_as<MODE, T, false>(b, l, o, cut, a, chained, s)
+                                      : launch_mma_as<MODE, T, true>(b, l, o, cut, a, chained, s);
 }
 
 template <typename T>
@@ -1129,17 +1196,18 @@ int loss_mma(const Batch& b, const XentLayout& l, char* ws, const T* feat, int64
              const T* weight, int64_t weight_ld, int32_t dtype, float* loss, float* lse,
              int32_t* status, cudaStream_t s) {
   Operands o;
-  if (int rc = prepare_operands<T>(b, l, ws, feat, feat_ld, weight, weight_ld, dtype, nullptr, 1.f,
-                                   false, s, &o))
+  SampleArrays none = {};
+  none.hot = 1.f;
+  bool chained = false;
+  if (int rc = prepare_operands<T>(b, l, ws, feat, feat_ld, weight, weight_ld, dtype, none, s, &o, &chained))
     return rc;
   MmaArgs a = {};
   a.unscale = sizeof(T) == 4 ? &reinterpret_cast<Consts*>(ws + l.consts)->unscale : nullptr;
   a.stats = reinterpret_cast<float2*>(ws + l.stats);
   a.status = status;
-  if (int rc = launch_mma<kLoss, T>(b, l, o, l.loss, a, s)) return rc;
-  join_loss_kernel<T><<<(unsigned)((b.n + 7) / 8), 256, 0, s>>>(
-      b, feat, feat_ld, weight, weight_ld, a.stats, l.loss.splits * kLossGroups, loss, lse, status);
-  FG_CUDA_TRY(cudaGetLastError());
+  if (int rc = launch_mma<kLoss, T>(b, l, o, l.loss, a, chained, s)) return rc;
+  FG_CUDA_TRY(launch(true, join_loss_kernel<T>, (unsigned)((b.n + 7) / 8), 256, 0, s, b, feat, feat_ld,
+                     weight, weight_ld, a.stats, l.loss.splits * kLossGroups, loss, lse, status));
   return FG_OK;
 }
 
@@ -1150,19 +1218,17 @@ int grad_mma(const Batch& b, const XentLayout& l, char* ws, const float* loss_gr
   // fp16 holds down to 2^-24: a probability of 1 is held as 2^14, so that the smallest that
   // count are 2^-38
   const float hot = dtype == FG_BFLOAT16 ? 1.f : 16384.f;
+  const SampleArrays arrays = {lse, loss_grad,
+                               reinterpret_cast<float*>(ws + l.row_bias),
+                               reinterpret_cast<float*>(ws + l.row_factor),
+                               reinterpret_cast<float*>(ws + l.col_bias),
+                               reinterpret_cast<float*>(ws + l.col_weight),
+                               reinterpret_cast<int32_t*>(ws + l.label), l.padded, hot};
   Operands o;
-  if (int rc = prepare_operands<T>(b, l, ws, feat, feat_ld, weight, weight_ld, dtype, loss_grad, hot,
-                                   true, s, &o))
+  bool chained = false;
+  if (int rc = prepare_operands<T>(b, l, ws, feat, feat_ld, weight, weight_ld, dtype, arrays, s, &o, &chained))
     return rc;
   Consts* consts = reinterpret_cast<Consts*>(ws + l.consts);
-  SampleArrays arrays = {reinterpret_cast<float*>(ws + l.row_bias),
-                         reinterpret_cast<float*>(ws + l.row_factor),
-                         reinterpret_cast<float*>(ws + l.col_bias),
-                         reinterpret_cast<float*>(ws + l.col_weight),
-                         reinterpret_cast<int32_t*>(ws + l.label)};
-  sample_kernel<<<(unsigned)((l.padded + 255) / 256), 256, 0, s>>>(b, lse, loss_grad, hot, consts,
-                                                                   l.padded, arrays);
-  FG_CUDA_TRY(cudaGetLastError());
   MmaArgs a = {};
   a.unscale = sizeof(T) == 4 ? &consts->unscale : nullptr;
   a.row_bias = arrays.row_bias;
@@ -1174,25 +1240,24 @@ int grad_mma(const Batch& b, const XentLayout& l, char* ws, const float* loss_gr
   a.partial = reinterpret_cast<float*>(ws + l.partial);
   a.status = status;
   auto join = [&](const Cut& cut, int64_t rows, const float* row_factor, const int32_t* row_label,
-                  const float* out_scale, T* out) {
-    if (cut.splits == 1) return;
-    const int64_t threads = rows * (l.out_cols / 4);
-    join_partial_kernel<T><<<(unsigned)((threads + 255) / 256), 256, 0, s>>>(
-        a.partial, cut.splits, rows, l.out_cols, (int)b.feat_len, row_factor, row_label, out_scale, out);
+                  const float* out_scale, T* out) -> cudaError_t {
+    if (cut.splits == 1) return cudaSuccess;
+    const int64_t quads = rows * (l.out_cols / 4), per_block = 256 / kJoinParts;
+    return launch(true, join_partial_kernel<T>, (unsigned)((quads + per_block - 1) / per_block), 256, 0, s,
+                  a.partial, cut.splits, rows, l.out_cols, (int)b.feat_len, row_factor, row_label,
+                  out_scale, out);
   };
   if (feat_grad) {
     a.out = feat_grad;
     a.out_scale = &consts->out_feat;
-    if (int rc = launch_mma<kFeatGrad, T>(b, l, o, l.feat, a, s)) return rc;
-    join(l.feat, b.n, arrays.row_factor, arrays.label, a.out_scale, feat_grad);
-    FG_CUDA_TRY(cudaGetLastError());
+    if (int rc = launch_mma<kFeatGrad, T>(b, l, o, l.feat, a, true, s)) return rc;
+    FG_CUDA_TRY(join(l.feat, b.n, arrays.row_factor, arrays.label, a.out_scale, feat_grad));
   }
   if (weight_grad) {
     a.out = weight_grad;
     a.out_scale = &consts->out_weight;
-    if (int rc = launch_mma<kWeightGrad, T>(b, l, o, l.weight, a, s)) return rc;
-    join(l.weight, b.vocab, nullptr, nullptr, a.out_scale, weight_grad);
-    FG_CUDA_TRY(cudaGetLastError());
+    if (int rc = launch_mma<kWeightGrad, T>(b, l, o, l.weight, a, true, s)) return rc;
+    FG_CUDA_TRY(join(l.weight, b.vocab, nullptr, nullptr, a.out_scale, weight_grad));
   }
   return FG_OK;
 }
