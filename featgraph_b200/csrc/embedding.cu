@@ -13,11 +13,12 @@
 namespace fg {
 namespace {
 
-__device__ __forceinline__ int64_t load_index(const void* ids, int wide, int64_t i) {
-  return wide ? __ldg(static_cast<const long long*>(ids) + i)
-              : (int64_t)__ldg(static_cast<const int*>(ids) + i);
+// The ids' type is a template parameter wherever a thread loads several: a choice at every load
+// makes each wait for the one before (5003 ids by 512 threads: 8000 cycles instead of 2000).
+template <typename I>
+__device__ __forceinline__ I load_id(const void* ids, int64_t i) {
+  return __ldg(static_cast<const I*>(ids) + i);
 }
-
 // ------------------------------------------------------------------ lookup --
 // A group of `lanes` (a power of two, at most 32) lanes copies kLookupRows consecutive rows side
 // by side, so that a lane has that many loads of up to 16 bytes in flight, and has the ids of
@@ -25,30 +26,30 @@ __device__ __forceinline__ int64_t load_index(const void* ids, int wide, int64_t
 constexpr int kLookupThreads = 256;
 constexpr int kLookupRows = 8;
 
-template <typename T, int N>
+template <typename T, int N, typename I>
 __global__ void __launch_bounds__(kLookupThreads)
 lookup_kernel(const T* __restrict__ table, int64_t table_ld, int64_t n_vertices,
-              const void* __restrict__ ids, int wide, int64_t n_ids, int feat_len, float scale,
+              const void* __restrict__ ids, int64_t n_ids, int feat_len, float scale,
               T* __restrict__ out, int64_t out_ld, int log_lanes, int32_t* status) {
   const int lanes = 1 << log_lanes;
   const int64_t group = ((int64_t)blockIdx.x * kLookupThreads + threadIdx.x) >> log_lanes;
   const int lane = threadIdx.x & (lanes - 1);
   const int64_t stride = (((int64_t)gridDim.x * kLookupThreads) >> log_lanes) * kLookupRows;
   int64_t first = group * kLookupRows;
-  int64_t id[kLookupRows];
+  I id[kLookupRows];
 #pragma unroll
   for (int u = 0; u < kLookupRows; ++u)
-    id[u] = first + u < n_ids ? load_index(ids, wide, first + u) : 0;
+    id[u] = first + u < n_ids ? load_id<I>(ids, first + u) : 0;
   for (; first < n_ids; first += stride) {
     bool ok[kLookupRows];
     int64_t from[kLookupRows];
 #pragma unroll
     for (int u = 0; u < kLookupRows; ++u) {
       const bool in = first + u < n_ids;
-      ok[u] = in && (uint64_t)id[u] < (uint64_t)n_vertices;
+      ok[u] = in && (uint64_t)(int64_t)id[u] < (uint64_t)n_vertices;
       if (in && !ok[u] && lane == 0) *status = FG_STATUS_BAD_INDEX;
       from[u] = id[u] * table_ld;
-      id[u] = first + stride + u < n_ids ? load_index(ids, wide, first + stride + u) : 0;
+      id[u] = first + stride + u < n_ids ? load_id<I>(ids, first + stride + u) : 0;
     }
     for (int c = lane * N; c < feat_len; c += lanes * N) {
       Vec<T, N> row[kLookupRows];
@@ -72,25 +73,36 @@ lookup_kernel(const T* __restrict__ table, int64_t table_ld, int64_t n_vertices,
 // The key of position i: its id, or n_vertices for a row that gets no gradient (the padding
 // id, or an id out of range), which sorts behind every vertex.
 struct KeySource {
-  const void* ids;           // first pass: the caller's ids
-  const uint2* pairs;        // later passes: (key, position) as the pass before left them
-  int wide;
+  const void* from;          // the caller's ids, or the pairs of the pass before
   int64_t n_vertices;
   int64_t padding;           // -1: none
   int32_t* status;
 };
-// What a key is made of, as it lies in memory, and the key.  Apart, so that a thread can have
-// all its loads on the way before it looks at the first (and may have to report it).
-__device__ __forceinline__ int64_t load_source(const KeySource& s, int64_t i) {
-  return s.pairs ? (int64_t)s.pairs[i].x : load_index(s.ids, s.wide, i);
+// What keys are made of as it lies in memory (S: int, long long, or uint2 for pairs), and the
+// pair it makes.  Apart, so that a thread has all its loads on the way before it looks at the
+// first (and may have to report it).
+template <typename S>
+__device__ __forceinline__ S load_source(const KeySource& s, int64_t i) {
+  if constexpr (std::is_same<S, uint2>::value)
+    return static_cast<const uint2*>(s.from)[i];
+  else
+    return load_id<S>(s.from, i);
 }
-__device__ __forceinline__ uint32_t make_key(const KeySource& s, int64_t id) {
-  if (s.pairs) return (uint32_t)id;
-  if ((uint64_t)id >= (uint64_t)s.n_vertices) {
-    *s.status = FG_STATUS_BAD_INDEX;
-    return (uint32_t)s.n_vertices;
+template <typename S>
+__device__ __forceinline__ uint2 make_pair(const KeySource& s, S id, int64_t i) {
+  if constexpr (std::is_same<S, uint2>::value) {
+    return id;
+  } else {
+    const int64_t v = id;
+    uint32_t key = (uint32_t)v;
+    if ((uint64_t)v >= (uint64_t)s.n_vertices) {
+      *s.status = FG_STATUS_BAD_INDEX;
+      key = (uint32_t)s.n_vertices;
+    } else if (v == s.padding) {
+      key = (uint32_t)s.n_vertices;
+    }
+    return make_uint2(key, (uint32_t)i);
   }
-  return id == s.padding ? (uint32_t)s.n_vertices : (uint32_t)id;
 }
 
 // The table's gradient starts as zeros: spare CTAs of the sort's kernels write a part of them
@@ -125,6 +137,7 @@ constexpr int kMaxDigitBits = 9;
 constexpr int kMaxBins = 1 << kMaxDigitBits;
 static_assert(kMaxBins == kSortThreads, "one thread per digit");
 
+template <typename S>
 __global__ void __launch_bounds__(kSortThreads)
 sort_count_kernel(KeySource src, int64_t n, int shift, int bits, uint32_t* __restrict__ counts,
                   int sort_blocks, ZeroFill zero) {
@@ -136,18 +149,18 @@ sort_count_kernel(KeySource src, int64_t n, int shift, int bits, uint32_t* __res
   __shared__ uint32_t hist[kMaxBins];
   const int bins = 1 << bits;
   const int64_t base = (int64_t)blockIdx.x * kSortTile;
-  int64_t id[kSortItems];
+  S id[kSortItems];
 #pragma unroll
   for (int k = 0; k < kSortItems; ++k) {
     const int64_t i = base + k * kSortThreads + threadIdx.x;
-    id[k] = i < n ? load_source(src, i) : 0;
+    id[k] = i < n ? load_source<S>(src, i) : S();
   }
   hist[threadIdx.x] = 0;
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kSortItems; ++k)
     if (base + k * kSortThreads + threadIdx.x < n)
-      atomicAdd(&hist[(make_key(src, id[k]) >> shift) & (bins - 1)], 1u);
+      atomicAdd(&hist[(make_pair<S>(src, id[k], 0).x >> shift) & (bins - 1)], 1u);
   __syncthreads();
   if ((int)threadIdx.x < bins) counts[(int64_t)threadIdx.x * sort_blocks + blockIdx.x] = hist[threadIdx.x];
 }
@@ -190,6 +203,7 @@ struct PlaceShared {
   uint32_t warp_sum[2][kSortWarps];
 };
 
+template <typename S>
 __global__ void __launch_bounds__(kSortThreads)
 sort_place_kernel(KeySource src, int64_t n, int shift, int bits,
                   const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals,
@@ -206,25 +220,17 @@ sort_place_kernel(KeySource src, int64_t n, int shift, int bits,
   const int64_t block_first = (int64_t)blockIdx.x * kSortTile;
   // each warp takes kSortItems * 32 consecutive keys, 32 at a time and in order
   const int64_t first = block_first + warp * (kSortItems * 32);
+  S id[kSortItems];
   uint2 pair[kSortItems];
-  if (src.pairs) {
 #pragma unroll
-    for (int k = 0; k < kSortItems; ++k) {
-      const int64_t i = first + k * 32 + lane;
-      pair[k] = i < n ? src.pairs[i] : make_uint2(0, 0);
-    }
-  } else {
-    int64_t id[kSortItems];
+  for (int k = 0; k < kSortItems; ++k) {
+    const int64_t i = first + k * 32 + lane;
+    id[k] = i < n ? load_source<S>(src, i) : S();
+  }
 #pragma unroll
-    for (int k = 0; k < kSortItems; ++k) {
-      const int64_t i = first + k * 32 + lane;
-      id[k] = i < n ? load_source(src, i) : 0;
-    }
-#pragma unroll
-    for (int k = 0; k < kSortItems; ++k) {
-      const int64_t i = first + k * 32 + lane;
-      pair[k] = i < n ? make_uint2(make_key(src, id[k]), (uint32_t)i) : make_uint2(0, 0);
-    }
+  for (int k = 0; k < kSortItems; ++k) {
+    const int64_t i = first + k * 32 + lane;
+    pair[k] = i < n ? make_pair<S>(src, id[k], i) : make_uint2(0, 0);
   }
   // a thread per digit: what it takes in all, and in the blocks before
   const int digit_here = threadIdx.x;
@@ -671,6 +677,8 @@ constexpr int kSliceBits = 7;
 constexpr int kSlices = 1 << kSliceBits;
 constexpr int kSliceThreads = 512;
 constexpr int kSliceAhead = 8;
+constexpr int kSliceChunks = (int)(kFewIds / kSliceThreads);
+constexpr int kSliceParts = 8;
 constexpr int kSliceAlone = 32;   // rows that one group of lanes sums alone
 constexpr int kSliceRank = 64;   // rows that are ranked by comparing each with each
 
@@ -683,7 +691,7 @@ __device__ __forceinline__ uint32_t slice_of(uint32_t v) {
 
 inline size_t slice_shared_bytes(int64_t n) { return (size_t)((n + 31) / 32 * 32) * 12; }
 
-template <typename T, int N>
+template <typename T, int N, typename I>
 __global__ void __launch_bounds__(kSliceThreads)
 slice_kernel(KeySource src, int n, const T* __restrict__ out_grad, int64_t out_grad_ld, int feat_len,
              float scale, int accumulate, T* __restrict__ grad, int log_lanes) {
@@ -694,26 +702,30 @@ slice_kernel(KeySource src, int n, const T* __restrict__ out_grad, int64_t out_g
   uint16_t* found = reinterpret_cast<uint16_t*>(mine + room);   // their positions
   uint16_t* sorted = found + room;                              // and these by (vertex, position)
   __shared__ int warp_count[kSliceThreads / 32];
-  __shared__ int n_long, long_start[kFewIds / kSliceAlone];
-  __shared__ float sums[kSliceThreads * N];
+  __shared__ int n_long, long_run[kFewIds / kSliceAlone];
+  __shared__ float sums[kSliceThreads * N], part_sums[kSliceParts * 32 * N];
   const int warp = threadIdx.x >> 5, lane32 = threadIdx.x & 31;
   const int lanes = 1 << log_lanes, groups = kSliceThreads >> log_lanes;
   const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> log_lanes;
   const int c = ((int)blockIdx.y * lanes + lane) * N;
   const bool in = c < feat_len;
 
-  for (int i0 = threadIdx.x; i0 < room; i0 += kSliceThreads * 8) {
-    int64_t id[8];
+  // every CTA begins with another stretch, so that they do not all ask for the same lines
+  {
+    const int chunks = (room + kSliceThreads - 1) / kSliceThreads;   // kSliceChunks at most
+    I id[kSliceChunks];
+    int place[kSliceChunks];
+    int chunk = (blockIdx.x + blockIdx.y) % chunks;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int i = i0 + k * kSliceThreads;
-      id[k] = i < n ? load_source(src, i) : -1;
+    for (int k = 0; k < kSliceChunks; ++k) {
+      place[k] = k < chunks ? chunk * kSliceThreads + threadIdx.x : room;
+      id[k] = place[k] < n ? load_source<I>(src, place[k]) : I();
+      if (++chunk == chunks) chunk = 0;
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int i = i0 + k * kSliceThreads;
-      if (i < room) keys[i] = i < n ? make_key(src, id[k]) : (uint32_t)src.n_vertices;
-    }
+    for (int k = 0; k < kSliceChunks; ++k)
+      if (place[k] < room)
+        keys[place[k]] = place[k] < n ? make_pair<I>(src, id[k], 0).x : (uint32_t)src.n_vertices;
   }
   // zeros first; the sums overwrite them behind the barriers below
   if (!accumulate && in) {
@@ -734,9 +746,14 @@ slice_kernel(KeySource src, int n, const T* __restrict__ out_grad, int64_t out_g
   auto is_mine = [&](uint32_t key) {
     return key < (uint32_t)src.n_vertices && slice_of(key) == blockIdx.x;
   };
+  uint32_t hits[kSliceChunks];
   int count = 0;
-  for (int i = from + lane32; i < to; i += 32)
-    count += __popc(__ballot_sync(0xffffffffu, is_mine(keys[i])));
+#pragma unroll
+  for (int k = 0; k < kSliceChunks; ++k) {
+    const int i = from + k * 32 + lane32;
+    hits[k] = __ballot_sync(0xffffffffu, i < to && is_mine(keys[min(i, room - 1)]));
+    count += __popc(hits[k]);
+  }
   if (lane32 == 0) warp_count[warp] = count;
   __syncthreads();
   int at = 0, m = 0;
@@ -746,17 +763,17 @@ slice_kernel(KeySource src, int n, const T* __restrict__ out_grad, int64_t out_g
     m += warp_count[w];
   }
   if (m == 0) return;
-  for (int i = from + lane32; i < to; i += 32) {
-    const uint32_t key = keys[i];
-    const uint32_t hits = __ballot_sync(0xffffffffu, is_mine(key));
-    if (is_mine(key)) {
-      const int e = at + __popc(hits & ((1u << lane32) - 1));
+#pragma unroll
+  for (int k = 0; k < kSliceChunks; ++k) {
+    if (hits[k] >> lane32 & 1) {
+      const int i = from + k * 32 + lane32, e = at + __popc(hits[k] & ((1u << lane32) - 1));
       found[e] = (uint16_t)i;
-      mine[e] = key;
+      mine[e] = keys[i];
     }
-    at += __popc(hits);
+    at += __popc(hits[k]);
   }
   __syncthreads();
+  uint32_t* sorted_keys = keys;        // all that is needed of the others has been found
   // While there are many: the rows of one vertex of theirs after the other are taken out, in
   // order.  The vertex in the middle of the list is most likely the one that has most rows.
   int left = m, out = 0;
@@ -787,7 +804,10 @@ slice_kernel(KeySource src, int n, const T* __restrict__ out_grad, int64_t out_g
         kept += warp_count[w];
       }
       const uint32_t below = (1u << lane32) - 1;
-      if (take >> lane32 & 1) sorted[to_taken + __popc(take & below)] = position;
+      if (take >> lane32 & 1) {
+        sorted[to_taken + __popc(take & below)] = position;
+        sorted_keys[to_taken + __popc(take & below)] = key;
+      }
       if (keep >> lane32 & 1) {
         mine[to_kept + __popc(keep & below)] = key;
         found[to_kept + __popc(keep & below)] = position;
@@ -802,17 +822,34 @@ slice_kernel(KeySource src, int n, const T* __restrict__ out_grad, int64_t out_g
     int rank = 0;
     for (int f = 0; f < left; ++f) rank += mine[f] < key + (f < e);
     sorted[out + rank] = found[e];
+    sorted_keys[out + rank] = key;
   }
   __syncthreads();
-  // a run per vertex: short ones to a group of lanes each
+  // a run per vertex; where they start, in order
+  uint16_t* starts = found;
+  int n_runs = 0;
+  for (int e0 = 0; e0 < m; e0 += kSliceThreads) {
+    const int e = e0 + threadIdx.x;
+    const bool start = e < m && (e == 0 || sorted_keys[e - 1] != sorted_keys[e]);
+    const uint32_t all = __ballot_sync(0xffffffffu, start);
+    if (lane32 == 0) warp_count[warp] = __popc(all);
+    __syncthreads();
+    int to_start = n_runs;
+#pragma unroll
+    for (int w = 0; w < kSliceThreads / 32; ++w) {
+      if (w < warp) to_start += warp_count[w];
+      n_runs += warp_count[w];
+    }
+    if (start) starts[to_start + __popc(all & ((1u << lane32) - 1))] = (uint16_t)e;
+    __syncthreads();
+  }
+  // short runs to a group of lanes each
   auto row_of = [&](int e) { return out_grad + (int64_t)sorted[e] * out_grad_ld + c; };
-  for (int e = group; e < m; e += groups) {
-    const uint32_t key = keys[sorted[e]];
-    if (e > 0 && keys[sorted[e - 1]] == key) continue;
-    int end = e + 1;
-    while (end < m && end - e <= kSliceAlone && keys[sorted[end]] == key) ++end;
+  for (int q = group; q < n_runs; q += groups) {
+    const int e = starts[q], end = q + 1 < n_runs ? starts[q + 1] : m;
+    const uint32_t key = sorted_keys[e];
     if (end - e > kSliceAlone) {
-      if (lane == 0) long_start[atomicAdd(&n_long, 1)] = e;
+      if (lane == 0) long_run[atomicAdd(&n_long, 1)] = q;
       continue;
     }
     if (!in) continue;
@@ -838,13 +875,8 @@ slice_kernel(KeySource src, int n, const T* __restrict__ out_grad, int64_t out_g
   __syncthreads();
   // long ones to all groups, a stretch each, and their sums added up in order
   for (int q = 0; q < n_long; ++q) {
-    const int e = long_start[q];
-    const uint32_t key = keys[sorted[e]];
-    int lo = e + kSliceAlone, hi = m;
-    while (lo < hi) {  // the first behind the run
-      const int mid = (lo + hi) >> 1;
-      if (keys[sorted[mid]] == key) lo = mid + 1; else hi = mid;
-    }
+    const int run = long_run[q], e = starts[run], lo = run + 1 < n_runs ? starts[run + 1] : m;
+    const uint32_t key = sorted_keys[e];
     const int stretch = (lo - e + groups - 1) / groups;
     const int j0 = min(lo, e + group * stretch), j1 = min(lo, j0 + stretch);
     float acc[N];
@@ -868,10 +900,21 @@ slice_kernel(KeySource src, int n, const T* __restrict__ out_grad, int64_t out_g
 #pragma unroll
     for (int k = 0; k < N; ++k) sums[threadIdx.x * N + k] = acc[k];
     __syncthreads();
+    // kSliceParts threads a column, each kSliceParts-th group; then one of them
+    const int width = lanes * N;
+    for (int i = threadIdx.x; i < width * kSliceParts; i += kSliceThreads) {
+      float total = 0.f;
+      for (int g = i / width; g < groups; g += kSliceParts) total += sums[g * width + i % width];
+      part_sums[i] = total;
+    }
+    __syncthreads();
     if (group == 0 && in) {
-      for (int g = 1; g < groups; ++g)
 #pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] += sums[((g << log_lanes) + lane) * N + k];
+      for (int k = 0; k < N; ++k) {
+        acc[k] = part_sums[lane * N + k];
+#pragma unroll
+        for (int g = 1; g < kSliceParts; ++g) acc[k] += part_sums[g * width + lane * N + k];
+      }
       store_grad_row<T, N>(grad + (int64_t)key * feat_len + c, acc, scale, accumulate);
     }
     __syncthreads();
@@ -966,11 +1009,19 @@ extern "C" int fg_embedding_lookup(const void* table_dev, int32_t dtype, int64_t
   const int64_t want = (n_ids + groups_per_block * kLookupRows - 1) / (groups_per_block * kLookupRows);
   const int grid = (int)std::min<int64_t>(std::max<int64_t>(want, 1), 148 * 4);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-#define FG_LOOKUP(T, N)                                                                        \
-  lookup_kernel<T, N><<<grid, kLookupThreads, 0, s>>>(                                         \
-      static_cast<const T*>(table_dev), table_ld, n_vertices, ids_dev,                         \
-      index_type == FG_INDEX_INT64, n_ids, (int)feat_len, scale, static_cast<T*>(out_dev),     \
-      out_ld, log_lanes, status_dev)
+#define FG_LOOKUP(T, N)                                                                         \
+  {                                                                                             \
+    const T* table = static_cast<const T*>(table_dev);                                          \
+    T* out = static_cast<T*>(out_dev);                                                          \
+    if (index_type == FG_INDEX_INT64)                                                           \
+      lookup_kernel<T, N, long long><<<grid, kLookupThreads, 0, s>>>(                           \
+          table, table_ld, n_vertices, ids_dev, n_ids, (int)feat_len, scale, out, out_ld,       \
+          log_lanes, status_dev);                                                               \
+    else                                                                                        \
+      lookup_kernel<T, N, int><<<grid, kLookupThreads, 0, s>>>(                                 \
+          table, table_ld, n_vertices, ids_dev, n_ids, (int)feat_len, scale, out, out_ld,       \
+          log_lanes, status_dev);                                                               \
+  }
 #define FG_LOOKUP_T(T)                                                    \
   switch (vb / (int)sizeof(T)) {                                          \
     case 8: if constexpr (sizeof(T) == 2) FG_LOOKUP(T, 8 / (sizeof(T) / 2)); break; \
@@ -1039,8 +1090,8 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
   char* ws = static_cast<char*>(workspace_dev);
   uint2* pairs[2] = {reinterpret_cast<uint2*>(ws + l.pairs[0]), reinterpret_cast<uint2*>(ws + l.pairs[1])};
   float* partial = reinterpret_cast<float*>(ws + l.partial);
-  KeySource src = {ids_dev, nullptr, index_type == FG_INDEX_INT64, n_vertices,
-                   padding_id < 0 ? -1 : padding_id, status_dev};
+  KeySource src = {ids_dev, n_vertices, padding_id < 0 ? -1 : padding_id, status_dev};
+  const bool wide = index_type == FG_INDEX_INT64;
   const int per_row = (int)((feat_len * es + vb - 1) / vb);
   if (l.few) {
     // slabs of 256 bytes where the rows allow 16-byte accesses: a popular vertex of long rows is
@@ -1052,11 +1103,12 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
     const dim3 grid(kSlices, (unsigned)slabs);
 #define FG_SLICE(T, N)                                                                             \
   {                                                                                                \
-    FG_CUDA_TRY(cudaFuncSetAttribute(slice_kernel<T, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
+    auto kernel = wide ? slice_kernel<T, N, long long> : slice_kernel<T, N, int>;                  \
+    FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,          \
                                      (int)slice_shared_bytes(kFewIds)));                           \
-    slice_kernel<T, N><<<grid, kSliceThreads, smem, s>>>(                                          \
-        src, (int)n_ids, static_cast<const T*>(out_grad_dev), out_grad_ld, (int)feat_len, scale,   \
-        accumulate, static_cast<T*>(grad_dev), log_lanes);                                         \
+    kernel<<<grid, kSliceThreads, smem, s>>>(src, (int)n_ids, static_cast<const T*>(out_grad_dev), \
+                                             out_grad_ld, (int)feat_len, scale, accumulate,        \
+                                             static_cast<T*>(grad_dev), log_lanes);                \
   }
 #define FG_SLICE_T(T)                                                       \
   switch (vb / (int)sizeof(T)) {                                            \
@@ -1074,20 +1126,22 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
   uint32_t* counts = reinterpret_cast<uint32_t*>(ws + l.counts);
   uint32_t* totals = reinterpret_cast<uint32_t*>(ws + l.totals);
   const int bins = 1 << l.digit_bits, blocks = (int)l.blocks;
-  FG_CUDA_TRY(cudaFuncSetAttribute(sort_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   (int)sizeof(PlaceShared)));
   for (int pass = 0; pass < l.passes; ++pass) {
     const int shift = pass * l.digit_bits;
     const ZeroFill z0 = zero_part(2 * pass, 2 * l.passes), z1 = zero_part(2 * pass + 1, 2 * l.passes);
-    FG_CUDA_TRY(launch(pass > 0, sort_count_kernel, blocks + zero_blocks(z0), kSortThreads, 0, s, src, n_ids,
+    auto count = pass > 0 ? sort_count_kernel<uint2> : wide ? sort_count_kernel<long long> : sort_count_kernel<int>;
+    auto place = pass > 0 ? sort_place_kernel<uint2> : wide ? sort_place_kernel<long long> : sort_place_kernel<int>;
+    FG_CUDA_TRY(cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)sizeof(PlaceShared)));
+    FG_CUDA_TRY(launch(pass > 0, count, blocks + zero_blocks(z0), kSortThreads, 0, s, src, n_ids,
                        shift, l.digit_bits, counts, blocks, z0));
     FG_CUDA_TRY(launch(true, sort_scan_kernel, (bins + kSortWarps - 1) / kSortWarps, kSortThreads, 0, s,
                        counts, blocks, bins, totals));
-    FG_CUDA_TRY(launch(true, sort_place_kernel, blocks + zero_blocks(z1), kSortThreads, sizeof(PlaceShared),
+    FG_CUDA_TRY(launch(true, place, blocks + zero_blocks(z1), kSortThreads, sizeof(PlaceShared),
                        s, src, n_ids, shift, l.digit_bits, counts, totals, pairs[pass & 1], blocks, z1));
-    src.pairs = pairs[pass & 1];
+    src.from = pairs[pass & 1];
   }
-  const Runs runs = {src.pairs, n_ids, (uint32_t)n_vertices};
+  const Runs runs = {static_cast<const uint2*>(src.from), n_ids, (uint32_t)n_vertices};
   const int log_lanes = std::max(ceil_log2(kSumLeastLanes), std::min(5, ceil_log2(per_row)));
   const int64_t slabs = (per_row + (1 << log_lanes) - 1) >> log_lanes;
   const int64_t pieces = (n_ids + kSumPiece - 1) / kSumPiece;

@@ -728,7 +728,7 @@ struct Consts {
 constexpr int kMaxPartials = 592;
 
 // Largest finite magnitude per CTA of the rows that take part, for both float32 operands
-// (blockIdx.y).  A warp a row, four loads a lane ahead.
+// (blockIdx.y).
 __global__ void __launch_bounds__(256)
 abs_max_kernel(Batch b, const float* __restrict__ feat, int64_t feat_ld,
                const float* __restrict__ weight, int64_t weight_ld, float* __restrict__ partial) {
@@ -736,7 +736,20 @@ abs_max_kernel(Batch b, const float* __restrict__ feat, int64_t feat_ld,
   float top = 0.f;
   const bool second = blockIdx.y == 1;
   const float* p = second ? weight : feat;
-  const int64_t rows = second ? b.vocab : b.n, ld = second ? weight_ld : feat_ld;
+  int64_t rows = second ? b.vocab : b.n;
+  const int64_t ld = second ? weight_ld : feat_ld;
+  if (second && ld == b.feat_len) {  // no gaps and no rows to leave out: one long array
+    const int64_t total = rows * ld, step = (int64_t)gridDim.x * 256;
+    for (int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x; i0 < total; i0 += step * 8) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = i0 + k * step < total ? fabsf(p[i0 + k * step]) : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (v[k] < INFINITY) top = fmaxf(top, v[k]);
+    }
+    rows = 0;
+  }
   // 32 lanes take whole rows of up to 128 elements four at a time, longer rows one at a time
   const int per_row = (int)min((int64_t)4, (b.feat_len + 31) / 32), together = 4 / per_row;
   const int64_t warps = (int64_t)gridDim.x * 8;
