@@ -148,6 +148,24 @@ cudaError_t launch(bool chained, void (*kernel)(P...), dim3 grid, int threads, s
   return cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
 }
 
+// Lets a kernel use `bytes` of dynamic shared memory on a device.  Asking the runtime takes
+// microseconds, so each host thread remembers what it has set.
+inline cudaError_t allow_shared(const void* kernel, int bytes, int device) {
+  struct Known {
+    const void* kernel;
+    int bytes, device;
+  };
+  constexpr int kMost = 64;
+  static thread_local Known known[kMost];
+  static thread_local int n = 0;
+  for (int k = 0; k < n; ++k)
+    if (known[k].kernel == kernel && known[k].device == device && known[k].bytes == bytes) return cudaSuccess;
+  const cudaError_t err =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == cudaSuccess) known[n < kMost ? n++ : (n = 1) - 1] = {kernel, bytes, device};
+  return err;
+}
+
 #ifdef __CUDACC__
 __device__ __forceinline__ void begin_chained() {
   wait_for_prior_grids();

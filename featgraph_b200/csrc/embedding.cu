@@ -677,6 +677,7 @@ constexpr int kSliceBits = 7;
 constexpr int kSlices = 1 << kSliceBits;
 constexpr int kSliceThreads = 512;
 constexpr int kSliceAhead = 8;
+constexpr int kSliceWarps = kSliceThreads / 32;
 constexpr int kSliceChunks = (int)(kFewIds / kSliceThreads);
 constexpr int kSliceParts = 8;
 constexpr int kSliceAlone = 32;   // rows that one group of lanes sums alone
@@ -697,11 +698,12 @@ slice_kernel(KeySource src, int n, const T* __restrict__ out_grad, int64_t out_g
              float scale, int accumulate, T* __restrict__ grad, int log_lanes) {
   extern __shared__ __align__(16) uint8_t raw[];
   const int room = (n + 31) / 32 * 32;
-  uint32_t* keys = reinterpret_cast<uint32_t*>(raw);            // of all ids
-  uint32_t* mine = keys + room;                                 // of this slice's, in order
-  uint16_t* found = reinterpret_cast<uint16_t*>(mine + room);   // their positions
-  uint16_t* sorted = found + room;                              // and these by (vertex, position)
-  __shared__ int warp_count[kSliceThreads / 32];
+  uint32_t* mine = reinterpret_cast<uint32_t*>(raw);            // this slice's keys, in order
+  uint32_t* sorted_keys = mine + room;                          // the same, vertex by vertex
+  uint16_t* found = reinterpret_cast<uint16_t*>(sorted_keys + room);  // their positions
+  uint16_t* sorted = found + room;                              // the same, vertex by vertex
+  __shared__ uint16_t before[kSliceChunks * kSliceWarps];
+  __shared__ int warp_count[kSliceWarps];
   __shared__ int n_long, long_run[kFewIds / kSliceAlone];
   __shared__ float sums[kSliceThreads * N], part_sums[kSliceParts * 32 * N];
   const int warp = threadIdx.x >> 5, lane32 = threadIdx.x & 31;
@@ -710,22 +712,30 @@ slice_kernel(KeySource src, int n, const T* __restrict__ out_grad, int64_t out_g
   const int c = ((int)blockIdx.y * lanes + lane) * N;
   const bool in = c < feat_len;
 
-  // every CTA begins with another stretch, so that they do not all ask for the same lines
+  // Looks through the ids, kSliceThreads at a time, and notes which are this slice's: bit k of
+  // `is_mine` the thread's own of stretch k, hits[k] its warp's.  Every CTA begins with another
+  // stretch, so that they do not all ask for the same lines.
+  const int stretches = (n + kSliceThreads - 1) / kSliceThreads;   // kSliceChunks at most
+  const int rotate = (blockIdx.x + blockIdx.y) % stretches;
+  uint32_t key[kSliceChunks], hits[kSliceChunks];
   {
-    const int chunks = (room + kSliceThreads - 1) / kSliceThreads;   // kSliceChunks at most
     I id[kSliceChunks];
-    int place[kSliceChunks];
-    int chunk = (blockIdx.x + blockIdx.y) % chunks;
 #pragma unroll
     for (int k = 0; k < kSliceChunks; ++k) {
-      place[k] = k < chunks ? chunk * kSliceThreads + threadIdx.x : room;
-      id[k] = place[k] < n ? load_source<I>(src, place[k]) : I();
-      if (++chunk == chunks) chunk = 0;
+      const int stretch = k + rotate < stretches ? k + rotate : k + rotate - stretches;
+      const int i = stretch * kSliceThreads + threadIdx.x;
+      id[k] = k < stretches && i < n ? load_source<I>(src, i) : I();
     }
 #pragma unroll
-    for (int k = 0; k < kSliceChunks; ++k)
-      if (place[k] < room)
-        keys[place[k]] = place[k] < n ? make_pair<I>(src, id[k], 0).x : (uint32_t)src.n_vertices;
+    for (int k = 0; k < kSliceChunks; ++k) {
+      hits[k] = 0;
+      if (k >= stretches) continue;
+      const int stretch = k + rotate < stretches ? k + rotate : k + rotate - stretches;
+      const int i = stretch * kSliceThreads + threadIdx.x;
+      key[k] = i < n ? make_pair<I>(src, id[k], 0).x : (uint32_t)src.n_vertices;
+      hits[k] = __ballot_sync(0xffffffffu, key[k] < (uint32_t)src.n_vertices && slice_of(key[k]) == blockIdx.x);
+      if (lane32 == 0) before[stretch * kSliceWarps + warp] = (uint16_t)__popc(hits[k]);
+    }
   }
   // zeros first; the sums overwrite them behind the barriers below
   if (!accumulate && in) {
@@ -740,40 +750,40 @@ slice_kernel(KeySource src, int n, const T* __restrict__ out_grad, int64_t out_g
   }
   if (threadIdx.x == 0) n_long = 0;
   __syncthreads();
-  // each warp looks through a stretch of whole 32s
-  const int per = (room / 32 + kSliceThreads / 32 - 1) / (kSliceThreads / 32) * 32;
-  const int from = min(room, warp * per), to = min(room, from + per);
-  auto is_mine = [&](uint32_t key) {
-    return key < (uint32_t)src.n_vertices && slice_of(key) == blockIdx.x;
-  };
-  uint32_t hits[kSliceChunks];
-  int count = 0;
+  // counts of the warps' stretches, in the order of positions, become those in front of them
+  int m;
+  {
+    const int total = stretches * kSliceWarps;   // at most kSliceChunks * kSliceWarps
+    static_assert(kSliceChunks * kSliceWarps <= kSliceThreads, "a thread each");
+    const int count = (int)threadIdx.x < total ? before[threadIdx.x] : 0;
+    int incl = count;
 #pragma unroll
-  for (int k = 0; k < kSliceChunks; ++k) {
-    const int i = from + k * 32 + lane32;
-    hits[k] = __ballot_sync(0xffffffffu, i < to && is_mine(keys[min(i, room - 1)]));
-    count += __popc(hits[k]);
-  }
-  if (lane32 == 0) warp_count[warp] = count;
-  __syncthreads();
-  int at = 0, m = 0;
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane32 >= d) incl += up;
+    }
+    if (lane32 == 31) warp_count[warp] = incl;
+    __syncthreads();
+    m = 0;
+    int ahead = 0;
 #pragma unroll
-  for (int w = 0; w < kSliceThreads / 32; ++w) {
-    if (w == warp) at = m;
-    m += warp_count[w];
+    for (int w = 0; w < kSliceWarps; ++w) {
+      if (w < warp) ahead += warp_count[w];
+      m += warp_count[w];
+    }
+    if ((int)threadIdx.x < total) before[threadIdx.x] = (uint16_t)(ahead + incl - count);
+    __syncthreads();
   }
   if (m == 0) return;
 #pragma unroll
   for (int k = 0; k < kSliceChunks; ++k) {
-    if (hits[k] >> lane32 & 1) {
-      const int i = from + k * 32 + lane32, e = at + __popc(hits[k] & ((1u << lane32) - 1));
-      found[e] = (uint16_t)i;
-      mine[e] = keys[i];
-    }
-    at += __popc(hits[k]);
+    if (!(hits[k] >> lane32 & 1)) continue;
+    const int stretch = k + rotate < stretches ? k + rotate : k + rotate - stretches;
+    const int e = before[stretch * kSliceWarps + warp] + __popc(hits[k] & ((1u << lane32) - 1));
+    found[e] = (uint16_t)(stretch * kSliceThreads + threadIdx.x);
+    mine[e] = key[k];
   }
   __syncthreads();
-  uint32_t* sorted_keys = keys;        // all that is needed of the others has been found
   // While there are many: the rows of one vertex of theirs after the other are taken out, in
   // order.  The vertex in the middle of the list is most likely the one that has most rows.
   int left = m, out = 0;
@@ -1104,8 +1114,7 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
 #define FG_SLICE(T, N)                                                                             \
   {                                                                                                \
     auto kernel = wide ? slice_kernel<T, N, long long> : slice_kernel<T, N, int>;                  \
-    FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,          \
-                                     (int)slice_shared_bytes(kFewIds)));                           \
+    FG_CUDA_TRY(allow_shared((const void*)kernel, (int)slice_shared_bytes(kFewIds), device));      \
     kernel<<<grid, kSliceThreads, smem, s>>>(src, (int)n_ids, static_cast<const T*>(out_grad_dev), \
                                              out_grad_ld, (int)feat_len, scale, accumulate,        \
                                              static_cast<T*>(grad_dev), log_lanes);                \
@@ -1131,8 +1140,7 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
     const ZeroFill z0 = zero_part(2 * pass, 2 * l.passes), z1 = zero_part(2 * pass + 1, 2 * l.passes);
     auto count = pass > 0 ? sort_count_kernel<uint2> : wide ? sort_count_kernel<long long> : sort_count_kernel<int>;
     auto place = pass > 0 ? sort_place_kernel<uint2> : wide ? sort_place_kernel<long long> : sort_place_kernel<int>;
-    FG_CUDA_TRY(cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     (int)sizeof(PlaceShared)));
+    FG_CUDA_TRY(allow_shared((const void*)place, (int)sizeof(PlaceShared), device));
     FG_CUDA_TRY(launch(pass > 0, count, blocks + zero_blocks(z0), kSortThreads, 0, s, src, n_ids,
                        shift, l.digit_bits, counts, blocks, z0));
     FG_CUDA_TRY(launch(true, sort_scan_kernel, (bins + kSortWarps - 1) / kSortWarps, kSortThreads, 0, s,

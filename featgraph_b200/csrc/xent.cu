@@ -1001,11 +1001,13 @@ struct Cut {
   int splits, steps_per_split;
 };
 Cut cut_steps(int64_t row_tiles, int64_t steps, int item_steps, int64_t most_steps) {
+  const int64_t least = (steps + most_steps - 1) / most_steps;
   Cut best = {1, (int)steps};
   int64_t best_time = INT64_MAX;
-  const int64_t least = (steps + most_steps - 1) / most_steps;
-  const int64_t most = std::max(least, std::min<int64_t>(steps, 4 * kSms / std::max<int64_t>(row_tiles, 1)));
-  for (int64_t s = least; s <= most; ++s) {
+  // of the counts that give as many waves, the largest ends first: five numbers of waves
+  const int64_t waves0 = std::max<int64_t>(1, (row_tiles * least + kSms - 1) / kSms);
+  for (int64_t w = waves0; w < waves0 + 5; ++w) {
+    const int64_t s = std::min(steps, std::max(least, w * kSms / std::max<int64_t>(row_tiles, 1)));
     const int64_t per = (steps + s - 1) / s, used = (steps + per - 1) / per;
     const int64_t waves = (row_tiles * used + kSms - 1) / kSms;
     const int64_t time = waves * (per + item_steps);
@@ -1152,7 +1154,7 @@ int prepare_operands(const Batch& b, const XentLayout& l, char* ws, const T* fea
 
 template <int MODE, typename T, bool STREAM>
 int launch_mma_as(const Batch& b, const XentLayout& l, const Operands& o, const Cut& cut, MmaArgs a,
-                  bool chained, cudaStream_t s) {
+                  bool chained, int device, cudaStream_t s) {
   using Shape = MmaShape<MODE, T, STREAM>;
   const bool rows_are_samples = MODE != kWeightGrad;
   const void* row_p = rows_are_samples ? o.feat : o.weight;
@@ -1189,7 +1191,7 @@ int launch_mma_as(const Batch& b, const XentLayout& l, const Operands& o, const 
   a.buffers = MODE != kLoss && !Shape::kSplit && l.out_cols <= 128 ? 3 : 2;
   a.chunks = MODE == kLoss ? 1 : (l.kb + Shape::kChunkTiles - 1) / Shape::kChunkTiles;
   auto kernel = xent_mma_kernel<MODE, T, STREAM>;
-  FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  FG_CUDA_TRY(allow_shared((const void*)kernel, (int)smem, device));
   const int64_t items = (int64_t)a.row_tiles * a.splits * a.chunks;
   if (items > INT32_MAX) return fail(FG_ERR_UNSUPPORTED, "too many tiles");
   FG_CUDA_TRY(launch(chained, kernel, (unsigned)std::min<int64_t>(items, kSms), Shape::kThreads, smem, s,
@@ -1199,15 +1201,15 @@ int launch_mma_as(const Batch& b, const XentLayout& l, const Operands& o, const 
 
 template <int MODE, typename T>
 int launch_mma(const Batch& b, const XentLayout& l, const Operands& o, const Cut& cut, const MmaArgs& a,
-               bool chained, cudaStream_t s) {
-  return l.tiles <= kMaxResidentTiles ? launch_mma_as<MODE, T, false>(b, l, o, cut, a, chained, s)
-                                      : launch_mma_as<MODE, T, true>(b, l, o, cut, a, chained, s);
+               bool chained, int device, cudaStream_t s) {
+  return l.tiles <= kMaxResidentTiles ? launch_mma_as<MODE, T, false>(b, l, o, cut, a, chained, device, s)
+                                      : launch_mma_as<MODE, T, true>(b, l, o, cut, a, chained, device, s);
 }
 
 template <typename T>
 int loss_mma(const Batch& b, const XentLayout& l, char* ws, const T* feat, int64_t feat_ld,
              const T* weight, int64_t weight_ld, int32_t dtype, float* loss, float* lse,
-             int32_t* status, cudaStream_t s) {
+             int32_t* status, int device, cudaStream_t s) {
   Operands o;
   SampleArrays none = {};
   none.hot = 1.f;
@@ -1218,7 +1220,7 @@ int loss_mma(const Batch& b, const XentLayout& l, char* ws, const T* feat, int64
   a.unscale = sizeof(T) == 4 ? &reinterpret_cast<Consts*>(ws + l.consts)->unscale : nullptr;
   a.stats = reinterpret_cast<float2*>(ws + l.stats);
   a.status = status;
-  if (int rc = launch_mma<kLoss, T>(b, l, o, l.loss, a, chained, s)) return rc;
+  if (int rc = launch_mma<kLoss, T>(b, l, o, l.loss, a, chained, device, s)) return rc;
   FG_CUDA_TRY(launch(true, join_loss_kernel<T>, (unsigned)((b.n + 7) / 8), 256, 0, s, b, feat, feat_ld,
                      weight, weight_ld, a.stats, l.loss.splits * kLossGroups, loss, lse, status));
   return FG_OK;
@@ -1227,7 +1229,7 @@ int loss_mma(const Batch& b, const XentLayout& l, char* ws, const T* feat, int64
 template <typename T>
 int grad_mma(const Batch& b, const XentLayout& l, char* ws, const float* loss_grad, const T* feat,
              int64_t feat_ld, const T* weight, int64_t weight_ld, int32_t dtype, const float* lse,
-             T* feat_grad, T* weight_grad, int32_t* status, cudaStream_t s) {
+             T* feat_grad, T* weight_grad, int32_t* status, int device, cudaStream_t s) {
   // fp16 holds down to 2^-24: a probability of 1 is held as 2^14, so that the smallest that
   // count are 2^-38
   const float hot = dtype == FG_BFLOAT16 ? 1.f : 16384.f;
@@ -1263,13 +1265,13 @@ int grad_mma(const Batch& b, const XentLayout& l, char* ws, const float* loss_gr
   if (feat_grad) {
     a.out = feat_grad;
     a.out_scale = &consts->out_feat;
-    if (int rc = launch_mma<kFeatGrad, T>(b, l, o, l.feat, a, true, s)) return rc;
+    if (int rc = launch_mma<kFeatGrad, T>(b, l, o, l.feat, a, true, device, s)) return rc;
     FG_CUDA_TRY(join(l.feat, b.n, arrays.row_factor, arrays.label, a.out_scale, feat_grad));
   }
   if (weight_grad) {
     a.out = weight_grad;
     a.out_scale = &consts->out_weight;
-    if (int rc = launch_mma<kWeightGrad, T>(b, l, o, l.weight, a, true, s)) return rc;
+    if (int rc = launch_mma<kWeightGrad, T>(b, l, o, l.weight, a, true, device, s)) return rc;
     FG_CUDA_TRY(join(l.weight, b.vocab, nullptr, nullptr, a.out_scale, weight_grad));
   }
   return FG_OK;
@@ -1308,7 +1310,7 @@ extern "C" int fg_softmax_xent(const void* feat_dev, int64_t feat_ld, const void
   int rc = FG_OK;
 #define FG_LOSS(T)                                                                               \
   rc = loss_mma<T>(b, l, ws, static_cast<const T*>(feat_dev), feat_ld,                           \
-                   static_cast<const T*>(weight_dev), weight_ld, dtype, loss_dev, lse_dev, status_dev, s)
+                   static_cast<const T*>(weight_dev), weight_ld, dtype, loss_dev, lse_dev, status_dev, device, s)
   FG_DISPATCH_DTYPE(dtype, FG_LOSS)
 #undef FG_LOSS
   return rc;
@@ -1350,7 +1352,7 @@ extern "C" int fg_softmax_xent_grad(const float* loss_grad_dev, const void* feat
 #define FG_GRAD(T)                                                                              \
   rc = grad_mma<T>(b, l, ws, loss_grad_dev, static_cast<const T*>(feat_dev), feat_ld,           \
                    static_cast<const T*>(weight_dev), weight_ld, dtype, lse_dev,                \
-                   static_cast<T*>(feat_grad_dev), static_cast<T*>(weight_grad_dev), status_dev, s)
+                   static_cast<T*>(feat_grad_dev), static_cast<T*>(weight_grad_dev), status_dev, device, s)
   FG_DISPATCH_DTYPE(dtype, FG_GRAD)
 #undef FG_GRAD
   return rc;
