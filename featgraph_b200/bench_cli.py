@@ -5,6 +5,8 @@
     python -m featgraph_b200.bench_cli --kernel sddmm --synthetic powerlaw --feat-len 128
     python -m featgraph_b200.bench_cli --kernel sddmm --synthetic powerlaw --heads 8 --head-dim 32
     torchrun --nproc-per-node 8 -m featgraph_b200.bench_cli --kernel spmm --synthetic rmat --feat-len 64
+    python -m featgraph_b200.bench_cli --kernel cross-entropy --feat-len 256 --samples 4096 --dtype bfloat16
+    python -m featgraph_b200.bench_cli --kernel train-step --feat-len 64 --samples 4096
 
 ``--dataset`` is a scipy ``save_npz`` file (CSR for SpMM, COO for SDDMM), as the reference's
 download script writes them; ``--synthetic`` generates one of the seeded graphs of
@@ -16,6 +18,12 @@ Under torchrun the graph is sharded over the ranks and the all-gather is inside 
 The features are seeded N(0,1) arrays (``graphs.normal_features`` with FEAT_SEED for the
 array indexed by column, FEAT2_SEED for the one indexed by row); ``--dump-output FILE``
 saves the last feature length's result as a ``.npy`` file so that it can be checked.
+
+The training operators (one GPU): ``--kernel lookup`` and ``lookup-grad`` take ``--samples``
+vertex ids of the graph, one per edge drawn, so that popular vertices come often;
+``cross-entropy`` scores ``--samples`` rows against every vertex, forward and both gradients;
+``clip`` bounds the gradient of the graph's embedding table; ``train-step`` runs them around
+the SpMM of the graph's first ``--samples`` rows (featgraph_b200.pipeline.VertexPrediction).
 """
 import argparse
 import json
@@ -26,6 +34,8 @@ import torch
 
 from . import _lib, graphs
 from .distributed import ShardedSDDMM, ShardedSpMM
+from .module.base import time_launches
+from .runtime import gpu
 
 NOMINAL_HBM_GBS = 8000.0
 
@@ -78,9 +88,93 @@ class _PartitionedSpMM(object):
         return self.module.device_status()
 
 
+def _lookup_case(args, g, f, device, table, ids, labels, feat):
+    from . import module, te
+    m = module.EmbeddingLookupcuda(device.index)
+    m.build([te.placeholder(tuple(table.shape), args.dtype), te.placeholder(tuple(ids.shape), "int32")],
+            {"scale": f ** 0.5, "with_grad": True}, {})
+    size = table.element_size()
+    n = ids.shape[0]
+    if args.kernel == "lookup":
+        return m, lambda: m.run([table, ids]), (2 * n * f * size, n * f)
+    return m, lambda: m.run_grad([feat, ids]), ((n + g.n_cols) * f * size, n * f)
+
+
+def _cross_entropy_case(args, g, f, device, table, ids, labels, feat):
+    from . import module, te
+    m = module.SoftmaxCrossEntropycuda(device.index)
+    m.build([te.placeholder(tuple(feat.shape), args.dtype), te.placeholder(tuple(table.shape), args.dtype),
+             te.placeholder(tuple(labels.shape), "int32")], {"scale": f ** -0.5, "with_grad": True}, {})
+    share = torch.full((labels.shape[0],), 1.0 / labels.shape[0], device=device)
+
+    def call():
+        loss, lse = m.run([feat, table, labels])
+        m.run_grad([share, feat, table, labels, lse])
+        return loss
+    n, v = feat.shape[0], table.shape[0]
+    return m, call, (2 * (n + v) * f * table.element_size(), 6 * n * v * f)
+
+
+def _clip_case(args, g, f, device, table, ids, labels, feat):
+    from . import module, te
+    m = module.GradientClipcuda(device.index)
+    m.build([te.placeholder(tuple(table.shape), args.dtype)], {"max_norm": 1.0}, {})
+    return m, lambda: m.run([table])[1][0], (2 * table.numel() * table.element_size(), 3 * table.numel())
+
+
+def _train_step_case(args, g, f, device, table, ids, labels, feat):
+    from .pipeline import VertexPrediction
+    if args.dtype != "float32":
+        raise SystemExit("--kernel train-step runs in float32, as the SpMM does")
+    n = min(args.samples, g.n_rows)
+    block = g.to_scipy()[:n]
+    step = VertexPrediction(block, g.n_cols, f, scale_out=f ** -0.5, max_norm=1.0,
+                            index_dtype="int32", device_id=device.index)
+    every = torch.arange(g.n_cols, dtype=torch.int32, device=device)
+    return (step, lambda: step.run(table, every, labels[:n])[2],
+            (4 * g.n_cols * f * table.element_size(), 6 * n * g.n_cols * f + 4 * block.nnz * f))
+
+
+TRAINING = {"lookup": _lookup_case, "lookup-grad": _lookup_case,
+            "cross-entropy": _cross_entropy_case, "clip": _clip_case,
+            "train-step": _train_step_case}
+
+
+def _run_training(args, g, source, device):
+    """The --kernel choices of TRAINING: one JSON line per feature length."""
+    dtype = getattr(torch, args.dtype)
+    gen = torch.Generator(device="cpu").manual_seed(graphs.FEAT_SEED)
+    draws = torch.randint(max(g.nnz, 1), (args.samples,), generator=gen)
+    ids = g.indices[draws.to(device)].to(torch.int32)
+    labels = torch.randint(g.n_cols, (args.samples,), generator=gen).to(torch.int32).to(device)
+    records = []
+    for f in (int(x) for x in args.feat_len.split(",")):
+        table = graphs.normal_features(g.n_cols, f, graphs.FEAT_SEED, device).to(dtype)
+        feat = graphs.normal_features(args.samples, f, graphs.FEAT2_SEED, device).to(dtype)
+        op, call, (nbytes, flops) = TRAINING[args.kernel](args, g, f, device, table, ids, labels, feat)
+        seconds = time_launches(gpu(device.index), call, args.num_runs)
+        result = call()
+        torch.cuda.synchronize(device)
+        op.device_status()
+        if args.dump_output:
+            result = result if isinstance(result, torch.Tensor) else result.torch
+            np.save(args.dump_output, result.float().cpu().numpy())
+        records.append({"kernel": args.kernel, "graph": source, "vertices": g.n_cols, "feat_len": f,
+                        "samples": args.samples, "dtype": args.dtype, "n_gpus": 1,
+                        "num_runs": args.num_runs, "ms": round(seconds * 1e3, 4),
+                        "tflops": round(flops / seconds / 1e12, 2),
+                        "alg_gbs": round(nbytes / seconds / 1e9, 1)})
+        print(json.dumps(records[-1]), flush=True)
+    return records
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__.split("\n\n")[0])
-    ap.add_argument("--kernel", choices=["spmm", "sddmm"], default="spmm")
+    ap.add_argument("--kernel", choices=["spmm", "sddmm"] + sorted(TRAINING), default="spmm")
+    ap.add_argument("--samples", type=int, default=4096,
+                    help="training operators: rows of the batch")
+    ap.add_argument("--dtype", choices=_lib.DTYPES, default="float32",
+                    help="training operators: type of the features")
     ap.add_argument("--dataset", type=str, default=None,
                     help="adjacency matrix stored as a scipy npz file")
     ap.add_argument("--synthetic", choices=["powerlaw", "rmat", "regular"], default="powerlaw")
@@ -124,6 +218,10 @@ def main(argv=None):
         dist.init_process_group("nccl", device_id=device)
 
     g, source = _load_graph(args, device)
+    if args.kernel in TRAINING:
+        if world > 1:
+            raise SystemExit("--kernel %s runs on one GPU" % args.kernel)
+        return _run_training(args, g, source, device)
     n = g.n_rows
     records = []
     # the cases of this run: (kernel, feat_len, heads)

@@ -203,7 +203,7 @@ extern "C" int fg_gradient_clip(const void* const* grads_host_array, void* const
   if (!(max_norm >= 0.0) || !(eps >= 0.0))
     return fail(FG_ERR_INVALID_ARGUMENT, "max_norm=%g and eps=%g must not be negative or NaN",
                 max_norm, eps);
-  if (!norm_dev || !workspace_dev || ((uintptr_t)workspace_dev & 7) != 0 ||
+  if (!norm_dev || ((uintptr_t)norm_dev & 3) != 0 || !workspace_dev || ((uintptr_t)workspace_dev & 7) != 0 ||
       workspace_bytes < fg_gradient_clip_workspace_bytes(n_tensors))
     return fail(FG_ERR_INVALID_ARGUMENT, "null norm_dev, or the workspace is smaller than %lld bytes",
                 (long long)fg_gradient_clip_workspace_bytes(n_tensors));

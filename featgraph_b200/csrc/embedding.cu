@@ -986,6 +986,8 @@ int check_common(const void* values, const void* ids, const int32_t* status, int
     return fail(FG_ERR_UNSUPPORTED, "n_vertices, n_ids must be below 2^31 - 1, feat_len at most 2^24");
   if (n_ids > 0 && (!values || !ids || !status))
     return fail(FG_ERR_INVALID_ARGUMENT, "null pointer");
+  if (((uintptr_t)ids & (index_type == FG_INDEX_INT64 ? 7 : 3)) != 0 || ((uintptr_t)status & 3) != 0)
+    return fail(FG_ERR_INVALID_ARGUMENT, "ids or status are not aligned to their type");
   return FG_OK;
 }
 

@@ -1093,6 +1093,8 @@ int check_xent(const void* feat, const void* weight, int32_t dtype, int64_t feat
   const size_t es = dtype_size(dtype);
   if (((uintptr_t)feat | (uintptr_t)weight) % es != 0)
     return fail(FG_ERR_INVALID_ARGUMENT, "a pointer is not aligned to its type");
+  if (((uintptr_t)labels & (index_type == FG_INDEX_INT64 ? 7 : 3)) != 0 || ((uintptr_t)status & 3) != 0)
+    return fail(FG_ERR_INVALID_ARGUMENT, "labels or status are not aligned to their type");
   return FG_OK;
 }
 
@@ -1258,6 +1260,7 @@ int grad_mma(const Batch& b, const XentLayout& l, char* ws, const float* loss_gr
                   const float* out_scale, T* out) -> cudaError_t {
     if (cut.splits == 1) return cudaSuccess;
     const int64_t quads = rows * (l.out_cols / 4), per_block = 256 / kJoinParts;
+    if ((quads + per_block - 1) / per_block > INT32_MAX) return cudaErrorInvalidConfiguration;
     return launch(true, join_partial_kernel<T>, (unsigned)((quads + per_block - 1) / per_block), 256, 0, s,
                   a.partial, cut.splits, rows, l.out_cols, (int)b.feat_len, row_factor, row_label,
                   out_scale, out);
@@ -1297,7 +1300,8 @@ extern "C" int fg_softmax_xent(const void* feat_dev, int64_t feat_ld, const void
                           n, vocab, feat_len, status_dev))
     return rc;
   if (n == 0) return FG_OK;
-  if (!loss_dev || !lse_dev) return fail(FG_ERR_INVALID_ARGUMENT, "null loss or lse");
+  if (!loss_dev || !lse_dev || (((uintptr_t)loss_dev | (uintptr_t)lse_dev) & 3) != 0)
+    return fail(FG_ERR_INVALID_ARGUMENT, "null loss or lse, or not aligned to float");
   const XentLayout l = xent_layout(dtype, n, vocab, feat_len, false);
   if (!workspace_dev || ((uintptr_t)workspace_dev & 255) != 0 || workspace_bytes < (int64_t)l.total)
     return fail(FG_ERR_INVALID_ARGUMENT, "the workspace needs %lld bytes at a 256-byte boundary",
@@ -1330,8 +1334,11 @@ extern "C" int fg_softmax_xent_grad(const float* loss_grad_dev, const void* feat
     return rc;
   if (!feat_grad_dev && !weight_grad_dev)
     return fail(FG_ERR_INVALID_ARGUMENT, "neither gradient is asked for");
+  if ((((uintptr_t)feat_grad_dev | (uintptr_t)weight_grad_dev) % dtype_size(dtype)) != 0)
+    return fail(FG_ERR_INVALID_ARGUMENT, "a gradient is not aligned to its type");
   if (n > 0) {
-    if (!loss_grad_dev || !lse_dev) return fail(FG_ERR_INVALID_ARGUMENT, "null loss_grad or lse");
+    if (!loss_grad_dev || !lse_dev || (((uintptr_t)loss_grad_dev | (uintptr_t)lse_dev) & 3) != 0)
+      return fail(FG_ERR_INVALID_ARGUMENT, "null loss_grad or lse, or not aligned to float");
     const int64_t need = fg_softmax_xent_workspace_bytes(dtype, n, vocab, feat_len, 1);
     if (!workspace_dev || ((uintptr_t)workspace_dev & 255) != 0 || workspace_bytes < need)
       return fail(FG_ERR_INVALID_ARGUMENT, "the workspace needs %lld bytes at a 256-byte boundary",

@@ -244,6 +244,8 @@ class EmbeddingLookupcuda(_TrainingOp):
             result, grad = self.grad_tvm, self.grad_tvm.torch
         else:
             result, grad = accumulate_into, self._tensor(accumulate_into, self._into)
+            if grad.untyped_storage().data_ptr() == dy.untyped_storage().data_ptr():
+                raise ValueError("OutGrad and accumulate_into share memory")
         n, vertices, feat_len, scale = self._sizes
         code = self._call(_lib.OP_LOOKUP_GRAD, _LOOKUP_GRAD.pack(
             dy.data_ptr(), self._codes[0], pitch, ids.data_ptr(), self._codes[1], n, vertices,

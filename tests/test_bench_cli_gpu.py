@@ -56,6 +56,34 @@ def test_sddmm_from_an_npz_file_keeps_the_stored_edge_order(tmp_path, oracle, he
     assert np.array_equal(bits(want.reshape(got.shape)), bits(got))
 
 
+@pytest.mark.parametrize("kernel, dtype", [("lookup", "bfloat16"), ("lookup-grad", "float32"),
+                                           ("cross-entropy", "float16"), ("clip", "bfloat16"),
+                                           ("train-step", "float32")])
+def test_training_operators(kernel, dtype):
+    recs = bench_cli.main(["--kernel", kernel, "--synthetic", "regular", "--vertices", "2048",
+                           "--feat-len", "32,64", "--samples", "300", "--dtype", dtype,
+                           "--num-runs", "2"])
+    assert [r["feat_len"] for r in recs] == [32, 64] and all(r["ms"] > 0 for r in recs)
+    assert recs[0]["kernel"] == kernel and recs[0]["vertices"] == 2048
+
+
+def test_lookup_result_of_the_command(tmp_path):
+    dump = str(tmp_path / "rows.npy")
+    bench_cli.main(["--kernel", "lookup", "--synthetic", "regular", "--vertices", "500",
+                    "--feat-len", "16", "--samples", "40", "--num-runs", "1", "--dump-output", dump])
+    table = graphs.normal_features(500, 16, graphs.FEAT_SEED, "cuda")
+    scaled = (table * np.float32(16 ** 0.5)).cpu().numpy()
+    rows = np.load(dump)
+    assert rows.shape == (40, 16)
+    assert all((scaled == r).all(1).any() for r in rows)    # every row is a scaled row of the table
+
+
+def test_train_step_is_refused_in_16_bits():
+    with pytest.raises(SystemExit, match="float32"):
+        bench_cli.main(["--kernel", "train-step", "--synthetic", "regular", "--vertices", "500",
+                        "--feat-len", "16", "--dtype", "bfloat16"])
+
+
 def test_the_x86_target_is_refused():
     with pytest.raises(SystemExit, match="cuda target only"):
         bench_cli.main(["--kernel", "spmm", "--synthetic", "regular", "--target", "x86"])

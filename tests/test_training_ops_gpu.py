@@ -196,6 +196,15 @@ def test_lookup_grad_without_ids():
     assert (keep == 1).all()
 
 
+def test_lookup_grad_refuses_to_accumulate_into_its_input():
+    ids = torch.arange(6, device="cuda")
+    dy = torch.ones((6, 4), device="cuda")
+    m = module.EmbeddingLookupcuda()
+    m.build([te.placeholder((6, 4))] + like(ids), {"with_grad": True}, {})
+    with pytest.raises(ValueError, match="share memory"):
+        m.run_grad([dy, ids], accumulate_into=dy)
+
+
 def test_lookup_grad_nan_reaches_only_its_vertex():
     ids = torch.arange(500, device="cuda") % 50
     dy = torch.ones((500, 16), device="cuda")
@@ -354,6 +363,25 @@ def test_cross_entropy_of_a_label_out_of_range():
 def test_cross_entropy_far_logits(dtype):
     # logits of a few hundred: exp of an unshifted logit would overflow
     feat, weight, labels, dloss = xent_inputs(90, 700, 64, dtype, 8, spread=60.0)
+    xent_check(xent_module(feat, weight, labels), feat, weight, labels, dloss)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("n, v", [(200, 40), (70, 3001)])
+@pytest.mark.parametrize("scale", [-0.5, 0.0, 3.0])
+def test_cross_entropy_signs(dtype, n, v, scale):
+    # negative and zero weights of the losses, negative and zero scales, sizes apart by 2^12
+    feat, weight, labels, dloss = xent_inputs(n, v, 72, dtype, 12)
+    dloss = dloss * torch.randn(n, generator=gen(13), device="cuda")
+    dloss[::9] = 0.0
+    dloss[4] *= 4096.0
+    xent_check(xent_module(feat, weight, labels, scale=scale), feat, weight, labels, dloss, scale)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_cross_entropy_one_gradient_alone_and_many_samples(dtype):
+    # more samples than the single-CTA preparation takes, few classes: the samples are split
+    feat, weight, labels, dloss = xent_inputs(8300, 17, 20, dtype, 14)
     xent_check(xent_module(feat, weight, labels), feat, weight, labels, dloss)
 
 
@@ -656,3 +684,37 @@ def test_a_training_step_of_a_layer():
           torch.float32)
     for m in (look, loss_op, spmm, back):
         assert m.device_status() == 0
+
+
+@pytest.mark.parametrize("index", ["int32", "int64"])
+def test_vertex_prediction_is_its_parts_and_follows_new_inputs(index):
+    # the composed step against 64-bit autograd of the formula: forward and backward are chains
+    # of sums whose terms' magnitudes the same formula gives with absolute values
+    from helpers import random_csr
+    from featgraph_b200.pipeline import VertexPrediction
+    v, f, n, cols = 300, 24, 90, 400
+    adj = random_csr(n, cols, 0.03, seed=4, empty_rows=(5, 6))
+    dense = torch.from_numpy(adj.toarray()).cuda().double()
+    step = VertexPrediction(adj, v, f, scale=2.0, scale_out=0.3, max_norm=0.2, index_dtype=index)
+    for seed in (1, 2):
+        g = gen(seed)
+        table = torch.randn((v, f), generator=g, device="cuda") * 0.3
+        ids = make_ids("skewed", cols, v, g).to(getattr(torch, index))
+        labels = torch.randint(v, (n,), generator=g, device="cuda").to(getattr(torch, index))
+        labels[::7] = -100
+        loss, norm, grad = step.run(table, ids, labels)
+        t = table.double().requires_grad_()
+        z = 0.3 * (dense @ (2.0 * t[ids.long()])) @ t.T
+        want = torch.nn.functional.cross_entropy(z, labels.long(), ignore_index=-100)
+        want.backward()
+        want = float(want.detach())
+        true = float(t.grad.norm())
+        # relative errors add up along the chain: lookup 1, SpMM degree (< 60), logits 2 (f + 8),
+        # softmax v + 64, two products 2 (v + 8), back through the SpMM 60 and the lookup 60;
+        # against a gradient that cancels by less than 20 in norm: 1500 u * 20
+        tol = 1500 * U * 20
+        assert abs(float(loss) - want) <= tol * abs(want)
+        assert abs(float(norm.torch) - true) <= tol * true
+        scaled = t.grad * (0.2 / (true + 1e-6))
+        assert float((grad.torch.double() - scaled).norm()) <= tol * float(scaled.norm())
+    assert step.device_status() == 0

@@ -178,3 +178,21 @@ def test_calls_by_words(lib):
     _refused(lib, lib.fg_training_call(_lib.OP_CLIP, clip, 13), 1, "-1.5")
     for op, fields in ((_lib.OP_LOOKUP_GRAD, 17), (_lib.OP_XENT, 19), (_lib.OP_XENT_GRAD, 21)):
         _refused(lib, lib.fg_training_call(op, words, 1), 1, "takes %d" % fields)
+
+
+def test_misaligned_pointers_are_refused(lib):
+    some, odd = ctypes.c_void_p(4096), ctypes.c_void_p(4098)
+    odd8 = ctypes.c_void_p(4100)
+    for index, ids in ((0, odd), (1, odd8)):
+        _refused(lib, lib.fg_embedding_lookup(some, 0, 8, 10, ids, index, 5, 8, 1.0, some, 8, some,
+                                              0, None), 1, "aligned")
+        _refused(lib, lib.fg_softmax_xent(some, 8, some, 8, 0, ids, index, 5, 10, 8, 1.0, -100, some,
+                                          some, some, 1 << 30, some, 0, None), 1, "aligned")
+    need = lib.fg_softmax_xent_workspace_bytes(0, 5, 10, 8, 1)
+    for place in range(4):
+        p = [odd if k == place else some for k in range(4)]     # loss_grad, lse and the gradients
+        _refused(lib, lib.fg_softmax_xent_grad(p[0], some, 8, some, 8, 0, some, 0, 5, 10, 8, 1.0,
+                                               -100, p[1], p[2], p[3], some, need, some, 0, None), 1,
+                 "aligned")
+    _refused(lib, lib.fg_softmax_xent(some, 8, some, 8, 0, some, 0, 5, 10, 8, 1.0, -100, odd, some,
+                                      some, 1 << 30, some, 0, None), 1, "aligned")
