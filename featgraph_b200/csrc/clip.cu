@@ -15,23 +15,28 @@ namespace fg {
 namespace {
 
 constexpr int kClipThreads = 256;
-constexpr int kClipTensors = 512;     // tensors a launch can name in its parameters
+// Tensors a launch can name in its parameters.  The launch copies them all, so a few tensors
+// take the short list (two tensors: 10.4 us a call with the long one).
+constexpr int kFewTensors = 32, kManyTensors = 512;
 constexpr int kClipMaxBlocks = 1184;  // CTAs (and partial norms) of one launch
 
 // One launch's tensors, in the kernel's parameters: the pointers change from call to call, and
 // parameters need no copy to the device and are recorded by a stream capture.
+template <int MOST>
 struct ClipTensors {
-  const void* in[kClipTensors];
-  void* out[kClipTensors];
-  int64_t size[kClipTensors];
-  int32_t first_chunk[kClipTensors + 1];  // chunks of kClipChunk elements, over all tensors
-  uint8_t dtype[kClipTensors];
-  uint8_t vector[kClipTensors];           // whether 16-byte accesses are aligned
+  static constexpr int kMost = MOST;
+  const void* in[MOST];
+  void* out[MOST];
+  int64_t size[MOST];
+  int32_t first_chunk[MOST + 1];  // chunks of kClipChunk elements, over all tensors
+  uint8_t dtype[MOST];
+  uint8_t vector[MOST];           // whether 16-byte accesses are aligned
   int n;
 };
 constexpr int kClipChunk = 8192;
 
-__device__ __forceinline__ int find_tensor(const ClipTensors& t, int chunk) {
+template <typename Tensors>
+__device__ __forceinline__ int find_tensor(const Tensors& t, int chunk) {
   int lo = 0, hi = t.n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -106,9 +111,9 @@ __device__ double block_norm(double v, double* shared) {
   return total;
 }
 
-template <bool MAX_NORM>
+template <bool MAX_NORM, typename Tensors>
 __global__ void __launch_bounds__(kClipThreads)
-partial_norm_kernel(const __grid_constant__ ClipTensors t, double* __restrict__ partial) {
+partial_norm_kernel(const __grid_constant__ Tensors t, double* __restrict__ partial) {
   begin_chained();
   __shared__ double shared[kClipThreads / 32];
   double acc = 0.0;
@@ -149,9 +154,9 @@ __device__ __forceinline__ void chunk_scale(const T* p, T* q, int count, bool ve
     q[i] = from_float<T>(to_float<T>(p[i]) * share);
 }
 
-template <bool MAX_NORM>
+template <bool MAX_NORM, typename Tensors>
 __global__ void __launch_bounds__(kClipThreads)
-scale_kernel(const __grid_constant__ ClipTensors t, const double* __restrict__ partial,
+scale_kernel(const __grid_constant__ Tensors t, const double* __restrict__ partial,
              int n_partial, double max_norm, double eps, float* __restrict__ norm_out) {
   begin_chained();
   __shared__ double shared[kClipThreads / 32];
@@ -182,12 +187,64 @@ scale_kernel(const __grid_constant__ ClipTensors t, const double* __restrict__ p
   }
 }
 
+// The two kernels over tensors of the C call, a launch per Tensors::kMost of them.
+struct ClipCall {
+  const void* const* grads;
+  void* const* outs;
+  const int64_t* sizes;
+  const int32_t* dtypes;
+  int32_t n_tensors;
+  bool max_abs_norm;
+  double max_norm, eps;
+  float* norm;
+  double* partial;
+};
+template <typename Tensors>
+int run_clip(const ClipCall& call, cudaStream_t s) {
+  Tensors t;
+  int grid = 1, n_partial = 0;
+  // the tensors from `first` on that one launch can name; returns the first one left
+  auto fill = [&](int32_t first) -> int32_t {
+    t.n = 0;
+    int64_t chunks = 0;
+    int32_t k = first;
+    for (; k < call.n_tensors && t.n < Tensors::kMost; ++k) {
+      t.in[t.n] = call.grads[k];
+      t.out[t.n] = call.outs[k];
+      t.size[t.n] = call.sizes[k];
+      t.dtype[t.n] = (uint8_t)call.dtypes[k];
+      t.vector[t.n] = (((uintptr_t)call.grads[k] | (uintptr_t)call.outs[k]) & 15) == 0;
+      t.first_chunk[t.n++] = (int32_t)chunks;
+      chunks += (call.sizes[k] + kClipChunk - 1) / kClipChunk;
+    }
+    t.first_chunk[t.n] = (int32_t)chunks;
+    grid = (int)std::max<int64_t>(1, std::min<int64_t>(chunks, kClipMaxBlocks));
+    return k;
+  };
+  int32_t next = 0;
+  do {
+    next = fill(next);
+    FG_CUDA_TRY(launch(n_partial > 0,
+                       call.max_abs_norm ? partial_norm_kernel<true, Tensors> : partial_norm_kernel<false, Tensors>,
+                       grid, kClipThreads, 0, s, t, call.partial + n_partial));
+    n_partial += grid;
+  } while (next < call.n_tensors);
+  const bool filled = next <= Tensors::kMost;   // one launch names them all: t is still right
+  next = filled ? call.n_tensors : 0;
+  do {
+    if (!filled) next = fill(next);
+    FG_CUDA_TRY(launch(true, call.max_abs_norm ? scale_kernel<true, Tensors> : scale_kernel<false, Tensors>,
+                       grid, kClipThreads, 0, s, t, call.partial, n_partial, call.max_norm, call.eps, call.norm));
+  } while (next < call.n_tensors);
+  return FG_OK;
+}
+
 }  // namespace
 }  // namespace fg
 
 extern "C" int64_t fg_gradient_clip_workspace_bytes(int32_t n_tensors) {
   if (n_tensors < 0) return 0;
-  const int64_t launches = (n_tensors + fg::kClipTensors - 1) / fg::kClipTensors;
+  const int64_t launches = (n_tensors + fg::kManyTensors - 1) / fg::kManyTensors;
   return std::max<int64_t>(launches, 1) * fg::kClipMaxBlocks * (int64_t)sizeof(double);
 }
 
@@ -225,41 +282,9 @@ extern "C" int fg_gradient_clip(const void* const* grads_host_array, void* const
                 (long long)all_chunks, kClipChunk);
   DeviceGuard guard(device);
   FG_CUDA_TRY(guard.status);
+  const ClipCall call = {grads_host_array, outs_host_array, sizes_host_array, dtypes_host_array, n_tensors,
+                         max_abs_norm != 0, max_norm, eps, norm_dev, static_cast<double*>(workspace_dev)};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  double* partial = static_cast<double*>(workspace_dev);
-  // the tensors from `first` on that one launch can name; returns the first one left
-  auto fill = [&](int32_t first, ClipTensors& t, int& grid) -> int32_t {
-    t.n = 0;
-    int64_t chunks = 0;
-    int32_t k = first;
-    for (; k < n_tensors && t.n < kClipTensors; ++k) {
-      const int64_t add = (sizes_host_array[k] + kClipChunk - 1) / kClipChunk;
-      t.in[t.n] = grads_host_array[k];
-      t.out[t.n] = outs_host_array[k];
-      t.size[t.n] = sizes_host_array[k];
-      t.dtype[t.n] = (uint8_t)dtypes_host_array[k];
-      t.vector[t.n] = (((uintptr_t)grads_host_array[k] | (uintptr_t)outs_host_array[k]) & 15) == 0;
-      t.first_chunk[t.n++] = (int32_t)chunks;
-      chunks += add;
-    }
-    t.first_chunk[t.n] = (int32_t)chunks;
-    grid = (int)std::max<int64_t>(1, std::min<int64_t>(chunks, kClipMaxBlocks));
-    return k;
-  };
-  ClipTensors t;
-  int grid = 1, n_partial = 0;
-  int32_t next = 0;
-  do {
-    next = fill(next, t, grid);
-    FG_CUDA_TRY(launch(n_partial > 0, max_abs_norm ? partial_norm_kernel<true> : partial_norm_kernel<false>,
-                       grid, kClipThreads, 0, s, t, partial + n_partial));
-    n_partial += grid;
-  } while (next < n_tensors);
-  next = 0;
-  do {
-    next = fill(next, t, grid);
-    FG_CUDA_TRY(launch(true, max_abs_norm ? scale_kernel<true> : scale_kernel<false>, grid, kClipThreads,
-                       0, s, t, partial, n_partial, max_norm, eps, norm_dev));
-  } while (next < n_tensors);
-  return FG_OK;
+  return n_tensors <= kFewTensors ? run_clip<ClipTensors<kFewTensors>>(call, s)
+                                  : run_clip<ClipTensors<kManyTensors>>(call, s);
 }
