@@ -145,24 +145,28 @@ cudaError_t launch(bool chained, void (*kernel)(P...), dim3 grid, int threads, s
   attr.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &attr;
   config.numAttrs = chained ? 1 : 0;
-  return cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
+  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
+  if (err != cudaSuccess) (void)cudaGetLastError();  // returned here, not to a later call
+  return err;
 }
 
-// Lets a kernel use `bytes` of dynamic shared memory on a device.  Asking the runtime takes
-// microseconds, so each host thread remembers what it has set.
-inline cudaError_t allow_shared(const void* kernel, int bytes, int device) {
+// Lets a kernel use up to `most` bytes of dynamic shared memory on a device: the most that any
+// call of it asks for, not this call's, since a later smaller limit would replace it.  Asking the
+// runtime takes microseconds, so each host thread remembers the kernels that have theirs.
+inline cudaError_t allow_shared(const void* kernel, int most, int device) {
   struct Known {
     const void* kernel;
-    int bytes, device;
+    int device;
   };
   constexpr int kMost = 64;
   static thread_local Known known[kMost];
   static thread_local int n = 0;
   for (int k = 0; k < n; ++k)
-    if (known[k].kernel == kernel && known[k].device == device && known[k].bytes == bytes) return cudaSuccess;
+    if (known[k].kernel == kernel && known[k].device == device) return cudaSuccess;
   const cudaError_t err =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (err == cudaSuccess) known[n < kMost ? n++ : (n = 1) - 1] = {kernel, bytes, device};
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (err == cudaSuccess && n < kMost) known[n++] = {kernel, device};
+  if (err != cudaSuccess) (void)cudaGetLastError();
   return err;
 }
 

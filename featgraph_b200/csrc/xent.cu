@@ -1193,7 +1193,7 @@ int launch_mma_as(const Batch& b, const XentLayout& l, const Operands& o, const 
   a.buffers = MODE != kLoss && !Shape::kSplit && l.out_cols <= 128 ? 3 : 2;
   a.chunks = MODE == kLoss ? 1 : (l.kb + Shape::kChunkTiles - 1) / Shape::kChunkTiles;
   auto kernel = xent_mma_kernel<MODE, T, STREAM>;
-  FG_CUDA_TRY(allow_shared((const void*)kernel, (int)smem, device));
+  FG_CUDA_TRY(allow_shared((const void*)kernel, room * kTileBytes + 1024, device));
   const int64_t items = (int64_t)a.row_tiles * a.splits * a.chunks;
   if (items > INT32_MAX) return fail(FG_ERR_UNSUPPORTED, "too many tiles");
   FG_CUDA_TRY(launch(chained, kernel, (unsigned)std::min<int64_t>(items, kSms), Shape::kThreads, smem, s,

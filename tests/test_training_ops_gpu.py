@@ -439,6 +439,26 @@ def test_cross_entropy_gradient_against_differences(along):
         assert slope > 3 * (e * e / 6 * third + noise / (2 * e) + own)
 
 
+def test_feature_lengths_in_any_order_in_a_fresh_process():
+    # the kernels' shared memory depends on the feature length: a shorter one in between must not
+    # take from a longer one what it was allowed before
+    import os
+    import subprocess
+    import sys
+    code = """
+import sys, torch
+sys.path[:0] = [%r, %r]
+import test_training_ops_gpu as t
+for dtype in sorted(t.TYPES):
+    for d in (128, 16, 128, 256, 40, 256, 70, 500, 20, 500):
+        feat, weight, labels, dloss = t.xent_inputs(40, 300, d, dtype, d)
+        t.xent_check(t.xent_module(feat, weight, labels), feat, weight, labels, dloss)
+""" % (os.path.dirname(os.path.abspath(__file__)),
+       os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
 def test_cross_entropy_of_nothing():
     m = module.SoftmaxCrossEntropycuda()
     feat = torch.empty((0, 8), device="cuda")
