@@ -67,6 +67,7 @@ struct MmaArgs {
   int row_tiles, splits, steps, steps_per_split;
   int chunks;             // pieces of at most kChunkTiles tiles that the results are cut into
   int slots;              // of the ring in shared memory
+  int paired;             // the second product takes two slots at a time (128 columns)
   int buffers;            // S tiles in TMEM
   int feat_len, out_cols; // out_cols: feat_len rounded up to 16
   int out_vec;            // bytes of an aligned access to the results' rows
@@ -436,12 +437,15 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
           tc::fence_after();
           const uint32_t p = tmem + o_buf.at * Shape::kCols;
           if (!STREAM) {
-            for (int q = 0; q < tiles; ++q) {
+            const int step_tiles = a.paired ? 2 : 1;
+            for (int q = 0; q < tiles; q += step_tiles) {
               const int t = q < a.kb ? q : q - a.kb;
-              product_o(t * 64, min(64, cols - t * 64), p,
+              product_o(t * 64, min(64 * step_tiles, cols - t * 64), p,
                         ring_desc_mn + o_slot.at * (kSlotBytes >> 4), q >= a.kb, begin);
-              tc::mma_commit(leader, empty + 8 * o_slot.at);
-              o_slot.next(a.slots);
+              for (int k = 0; k < step_tiles; ++k) {
+                tc::mma_commit(leader, empty + 8 * o_slot.at);
+                o_slot.next(a.slots);
+              }
             }
           } else {
             for (int plane = 0; plane < kPlanes; ++plane)
@@ -1007,7 +1011,9 @@ Cut cut_steps(int64_t row_tiles, int64_t steps, int item_steps, int64_t most_ste
   // of the counts that give as many waves, the largest ends first: five numbers of waves
   const int64_t waves0 = std::max<int64_t>(1, (row_tiles * least + kSms - 1) / kSms);
   for (int64_t w = waves0; w < waves0 + 5; ++w) {
-    const int64_t s = std::min(steps, std::max(least, w * kSms / std::max<int64_t>(row_tiles, 1)));
+    // but no more than four waves' worth: partial sums are written and read once more
+    const int64_t fit = std::min(w, (int64_t)4) * kSms / std::max<int64_t>(row_tiles, 1);
+    const int64_t s = std::min(steps, std::max({least, (int64_t)1, fit}));
     const int64_t per = (steps + s - 1) / s, used = (steps + per - 1) / per;
     const int64_t waves = (row_tiles * used + kSms - 1) / kSms;
     const int64_t time = waves * (per + item_steps);
@@ -1188,6 +1194,14 @@ int launch_mma_as(const Batch& b, const XentLayout& l, const Operands& o, const 
   const int room = MODE == kWeightGrad ? 13 : 14;
   const int resident = STREAM ? 0 : l.tiles;
   a.slots = std::min(kMaxSlots, (room - resident) / Shape::kSlotTiles);
+  // Two neighbouring slots are one operand of 128 columns where a step's tiles come in pairs and
+  // no pair goes around the end of the ring: half the mma of the second product (feat_grad of
+  // 4096 x 65 536 x 128: 131 -> 126 us).  Not where the odd slot that goes for it leaves less
+  // than half a step of lead (weight_grad at 256 columns: 226 us against 218), except float32,
+  // whose second product is three times as many mma (xent_train 2048 x 50 021 x 128: 418 -> 390).
+  a.paired = !STREAM && l.kb % 2 == 0 &&
+             (Shape::kSplit || (a.slots & ~1) * Shape::kSlotTiles >= 2 * l.tiles + 2);
+  if (a.paired) a.slots &= ~1;
   const size_t smem = (size_t)(resident + a.slots * Shape::kSlotTiles) * kTileBytes + 1024;
   // TMEM: 512 columns, two S tiles, three where the accumulators need only 128 columns
   a.buffers = MODE != kLoss && !Shape::kSplit && l.out_cols <= 128 ? 3 : 2;
