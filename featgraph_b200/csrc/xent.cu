@@ -797,7 +797,7 @@ __device__ __forceinline__ int operand_exponent(float top) {
   if (!(top > 0.f)) return 0;
   int e;
   frexpf(top, &e);
-  return min(60, max(-60, 13 - e));
+  return min(120, max(-120, 13 - e));
 }
 
 // What the gradients' kernels need of a sample, and of the padding up to a whole tile.
@@ -1083,7 +1083,9 @@ XentLayout xent_layout(int32_t dtype, int64_t n, int64_t vocab, int64_t feat_len
 
 int check_xent(const void* feat, const void* weight, int32_t dtype, int64_t feat_ld,
                int64_t weight_ld, const void* labels, int32_t index_type, int64_t n, int64_t vocab,
-               int64_t feat_len, const int32_t* status) {
+               int64_t feat_len, float scale, const int32_t* status) {
+  if (!std::isfinite(scale))
+    return fail(FG_ERR_INVALID_ARGUMENT, "scale=%g is not finite", (double)scale);
   if (!dtype_known(dtype) || !index_known(index_type))
     return fail(FG_ERR_INVALID_ARGUMENT, "unknown dtype=%d or index_type=%d", (int)dtype,
                 (int)index_type);
@@ -1311,7 +1313,7 @@ extern "C" int fg_softmax_xent(const void* feat_dev, int64_t feat_ld, const void
                                int32_t device, void* stream) {
   using namespace fg;
   if (int rc = check_xent(feat_dev, weight_dev, dtype, feat_ld, weight_ld, labels_dev, index_type,
-                          n, vocab, feat_len, status_dev))
+                          n, vocab, feat_len, scale, status_dev))
     return rc;
   if (n == 0) return FG_OK;
   if (!loss_dev || !lse_dev || (((uintptr_t)loss_dev | (uintptr_t)lse_dev) & 3) != 0)
@@ -1344,7 +1346,7 @@ extern "C" int fg_softmax_xent_grad(const float* loss_grad_dev, const void* feat
                                     int32_t* status_dev, int32_t device, void* stream) {
   using namespace fg;
   if (int rc = check_xent(feat_dev, weight_dev, dtype, feat_ld, weight_ld, labels_dev, index_type,
-                          n, vocab, feat_len, status_dev))
+                          n, vocab, feat_len, scale, status_dev))
     return rc;
   if (!feat_grad_dev && !weight_grad_dev)
     return fail(FG_ERR_INVALID_ARGUMENT, "neither gradient is asked for");

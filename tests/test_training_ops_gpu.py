@@ -643,6 +643,40 @@ def test_other_streams_and_captured_graphs_give_the_same_bits():
         assert all(torch.equal(a, b) for a, b in zip(want2, outs))
 
 
+def test_modules_side_by_side_on_streams_and_threads():
+    # each host thread with modules and a stream of its own; the tensor-core kernels of the
+    # others hold the machine in between
+    import threading
+    cases = []
+    for seed in (31, 32, 33):
+        call, _ = _operators(seed)
+        cases.append((call, [x.clone() for x in call()], torch.cuda.Stream(), []))
+    torch.cuda.synchronize()
+
+    def work(call, want, stream, wrong):
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got = call()
+                wrong.extend(not torch.equal(a, b) for a, b in zip(want, got))
+    threads = [threading.Thread(target=work, args=c) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert all(len(c[3]) == 20 * len(c[1]) and not any(c[3]) for c in cases)
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-4, 1e4, 1e15])
+def test_cross_entropy_float32_operands_of_any_size(size):
+    # the fp16 pieces are relative to the operands' largest values; scale brings the logits back
+    feat, weight, labels, dloss = xent_inputs(50, 400, 40, "float32", 15)
+    xent_check(xent_module(feat, weight * size, labels, scale=1.0 / size), feat, weight * size,
+               labels, dloss, 1.0 / size)
+    xent_check(xent_module(feat * size, weight, labels, scale=1.0 / size), feat * size, weight,
+               labels, dloss, 1.0 / size)
+
+
 def test_build_again_with_other_shapes():
     m = module.SoftmaxCrossEntropycuda()
     for n, v, d in ((5, 40, 8), (200, 30, 64), (3, 1000, 16)):

@@ -125,6 +125,9 @@ def test_xent_argument_errors(lib):
     _refused(lib, call(n=1 << 30), 3, "2^30")
     _refused(lib, call(feat=ctypes.c_void_p(4097)), 1, "aligned")
     assert call(n=0) == 0
+    for scale in (math.nan, math.inf):
+        _refused(lib, lib.fg_softmax_xent(some, 8, some, 8, 0, some, 0, 5, 10, 8, scale, -100, some,
+                                          some, some, need, some, 0, None), 1, "finite")
 
     def grad(dh=some, dw=some, size=need_grad, lse=some):
         return lib.fg_softmax_xent_grad(some, some, 8, some, 8, 0, some, 0, 5, 10, 8, 1.0, -100,
