@@ -824,22 +824,26 @@ __device__ __forceinline__ void sample(const Batch& b, const SampleArrays& s, fl
   s.col_bias[t] = weight == 0.f ? -INFINITY : bias + log2f(fabsf(weight));
 }
 
-// The scalars, by one CTA; it also makes the sample arrays of a batch of up to kSetupSamples.
+// The scalars, by one CTA of any size; it also makes the sample arrays of a batch of up to
+// kSetupSamples.
 constexpr int64_t kSetupSamples = 8192;
-__global__ void __launch_bounds__(1024)
-setup_kernel(Batch b, SampleArrays s, const float* __restrict__ abs_max, Consts* consts) {
-  begin_chained();
+__device__ __forceinline__ void setup(const Batch& b, const SampleArrays& s, const float* abs_max,
+                                      Consts* consts) {
   __shared__ float shared[32];
   float top = 0.f;
   if (s.loss_grad)
-    for (int64_t t = threadIdx.x; t < b.n; t += 1024)
+    for (int64_t t = threadIdx.x; t < b.n; t += blockDim.x)
       if (live_label(b, t) >= 0) top = fmaxf(top, fabsf(s.loss_grad[t]));
   top = block_max(top, shared);
   int ef = 0, ew = 0;
   if (abs_max) {
-    const bool in = threadIdx.x < kMaxPartials;
-    ef = operand_exponent(block_max(in ? abs_max[threadIdx.x] : 0.f, shared));
-    ew = operand_exponent(block_max(in ? abs_max[kMaxPartials + threadIdx.x] : 0.f, shared));
+    float top_feat = 0.f, top_weight = 0.f;
+    for (int k = threadIdx.x; k < kMaxPartials; k += blockDim.x) {
+      top_feat = fmaxf(top_feat, abs_max[k]);
+      top_weight = fmaxf(top_weight, abs_max[kMaxPartials + k]);
+    }
+    ef = operand_exponent(block_max(top_feat, shared));
+    ew = operand_exponent(block_max(top_weight, shared));
   }
   const float inv = top >= 1.17549435e-38f ? 1.f / top : 0.f;
   if (threadIdx.x == 0) {
@@ -853,7 +857,12 @@ setup_kernel(Batch b, SampleArrays s, const float* __restrict__ abs_max, Consts*
     *consts = c;
   }
   if (s.loss_grad && s.padded <= kSetupSamples)
-    for (int64_t t = threadIdx.x; t < s.padded; t += 1024) sample(b, s, inv, t);
+    for (int64_t t = threadIdx.x; t < s.padded; t += blockDim.x) sample(b, s, inv, t);
+}
+__global__ void __launch_bounds__(1024)
+setup_kernel(Batch b, SampleArrays s, const float* __restrict__ abs_max, Consts* consts) {
+  begin_chained();
+  setup(b, s, abs_max, consts);
 }
 __global__ void __launch_bounds__(256)
 sample_kernel(Batch b, SampleArrays s, const Consts* __restrict__ consts) {
@@ -865,7 +874,8 @@ sample_kernel(Batch b, SampleArrays s, const Consts* __restrict__ consts) {
 // Operands as the tensor maps want them: rows of `pitch` 16-bit elements, zero behind feat_len.
 // float32 becomes two fp16 pieces, the second behind the first.  A row whose label is out of
 // play (`masked`) becomes zero, whatever it held.  The first `blocks` CTAs pack one operand, the
-// others the second.
+// others the second; where packing needs none of the scalars (`with_setup`), the last CTA makes
+// these.
 template <typename T>
 struct PackJob {
   const T* from;
@@ -876,8 +886,13 @@ struct PackJob {
 };
 template <typename T>
 __global__ void __launch_bounds__(256)
-pack_kernel(Batch b, PackJob<T> first, PackJob<T> second, int64_t pitch) {
+pack_kernel(Batch b, PackJob<T> first, PackJob<T> second, int64_t pitch, int with_setup, SampleArrays s,
+            Consts* consts) {
   begin_chained();
+  if (with_setup && blockIdx.x == gridDim.x - 1) {
+    setup(b, s, nullptr, consts);
+    return;
+  }
   const bool is_second = (int)blockIdx.x >= first.blocks;
   const PackJob<T> j = is_second ? second : first;
   const int64_t block = is_second ? blockIdx.x - first.blocks : blockIdx.x;
@@ -1131,13 +1146,11 @@ int prepare_operands(const Batch& b, const XentLayout& l, char* ws, const T* fea
                        weight_ld, abs_max));
     *chained = true;
   }
-  if (sizeof(T) == 4 || grad) {
-    FG_CUDA_TRY(launch(*chained, setup_kernel, 1, 1024, 0, s, b, samples,
-                       sizeof(T) == 4 ? abs_max : nullptr, consts));
+  // 16-bit gradients always pack the features, and make the scalars beside that
+  const bool with_setup = sizeof(T) == 2 && grad;
+  if (sizeof(T) == 4) {
+    FG_CUDA_TRY(launch(*chained, setup_kernel, 1, 1024, 0, s, b, samples, abs_max, consts));
     *chained = true;
-    if (grad && samples.padded > kSetupSamples)
-      FG_CUDA_TRY(launch(true, sample_kernel, (unsigned)((samples.padded + 255) / 256), 256, 0, s, b, samples,
-                         consts));
   }
   *o = {feat, weight, feat_ld, weight_ld};
   auto blocks = [](int64_t rows) { return (int)std::min<int64_t>((rows + 7) / 8, 8 * kSms); };
@@ -1155,10 +1168,13 @@ int prepare_operands(const Batch& b, const XentLayout& l, char* ws, const T* fea
     o->weight_ld = l.pitch;
   }
   if (jobs[0].blocks + jobs[1].blocks > 0) {
-    FG_CUDA_TRY(launch(*chained, pack_kernel<T>, jobs[0].blocks + jobs[1].blocks, 256, 0, s, b, jobs[0],
-                       jobs[1], l.pitch));
+    FG_CUDA_TRY(launch(*chained, pack_kernel<T>, jobs[0].blocks + jobs[1].blocks + with_setup, 256, 0, s, b,
+                       jobs[0], jobs[1], l.pitch, with_setup, samples, consts));
     *chained = true;
   }
+  if (grad && samples.padded > kSetupSamples)
+    FG_CUDA_TRY(launch(true, sample_kernel, (unsigned)((samples.padded + 255) / 256), 256, 0, s, b, samples,
+                       consts));
   return FG_OK;
 }
 
