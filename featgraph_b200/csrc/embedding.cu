@@ -4,7 +4,9 @@
 //   grad[v, :] = scale * sum of out_grad[i, :] over the i with ids[i] = v, i ascending
 //
 // Both only move bytes: the lookup reads the rows it names and writes them once, the gradient
-// reads every row of out_grad once and writes every row of the table's gradient once.
+// reads every row of out_grad once and writes every row of the table's gradient once.  On one
+// B200, 1 048 576 rows of 256 bytes, a table of 232 965, skewed ids: lookup 67 us (4.9 TB/s),
+// gradient 144 us, of which 85 are the sums (3.4 TB/s of rows in random order) and 40 the sort.
 #include <algorithm>
 #include <cmath>
 
@@ -671,8 +673,8 @@ join_kernel(Runs r, int n_windows, int feat_len, float scale, int accumulate, T*
 // CTAs (times the slabs of columns): each looks through all ids for its own, keeps them in
 // order, ranks the few it has by (vertex, position), and sums.  A slice has one vertex of
 // every kSlices neighbours, at a place that changes from one such stretch to the next, so that neither
-// neighbouring nor evenly spaced popular vertices meet in one.  5003 skewed ids: the sort, sums
-// and join in launches of their own took 29 us.
+// neighbouring nor evenly spaced popular vertices meet in one.  5003 skewed ids of 400-byte rows:
+// 17 us; the sort, sums and join in launches of their own took 29.
 constexpr int64_t kFewIds = 8192;
 constexpr int kSliceBits = 7;
 constexpr int kSlices = 1 << kSliceBits;

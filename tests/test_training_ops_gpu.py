@@ -185,6 +185,54 @@ def test_lookup_grad_of_ids_that_meet_in_one_slice(n, distinct):
     check(m.run_grad([dy, ids]).torch, want, bound, dy.dtype)
 
 
+@pytest.mark.parametrize("n", [300, 9000])           # both forms of the gradient
+def test_lookup_and_its_gradient_beyond_32_bit_offsets(n):
+    v, f = (1 << 25) + 3, 72                            # 2.4e9 elements
+    g = gen(n)
+    table = torch.zeros((v, f), dtype=torch.float16, device="cuda")
+    ids = torch.randint(v - 1000, v, (n,), generator=g, device="cuda")
+    ids[:50] = torch.randint(v, (50,), generator=g, device="cuda")
+    table[ids] = torch.randn((n, f), generator=g, device="cuda").half()
+    m = module.EmbeddingLookupcuda()
+    m.build(like(table, ids), {"with_grad": True}, {})
+    assert torch.equal(m.run([table, ids]).torch, table[ids])
+    dy = torch.randn((n, f), generator=g, device="cuda").half()
+    m.grad_tvm.torch.fill_(1.0)
+    got = m.run_grad([dy, ids]).torch
+    rows, place = torch.unique(ids, return_inverse=True)
+    want, bound = grad_reference(dy, place, rows.shape[0], 1.0)
+    check(got[rows], want, bound, dy.dtype)
+    got[rows] = 0
+    assert not got.any()
+
+
+def test_cross_entropy_beyond_32_bit_offsets():
+    n, v, f = 3, (1 << 25) + 3, 72
+    g = gen(77)
+    feat = torch.randn((n, f), generator=g, device="cuda").half()
+    weight = torch.empty((v, f), dtype=torch.float16, device="cuda").normal_(generator=g) * 0.3
+    labels = torch.tensor([v - 1, 5, v // 2], device="cuda")
+    dloss = torch.tensor([1.0, -2.0, 0.5], device="cuda")
+    m = xent_module(feat, weight, labels)
+    loss, lse = m.run([feat, weight, labels])
+    dh, dw = m.run_grad([dloss, feat, weight, labels, lse])
+    # the sum of exponentials by pieces; what the other tests bound per element, here at a few rows
+    h = feat.double()
+    total = torch.full((n,), -math.inf, dtype=torch.float64, device="cuda")
+    for a in range(0, v, 1 << 22):
+        total = torch.logaddexp(total, torch.logsumexp(h @ weight[a:a + (1 << 22)].double().T, 1))
+    assert ((lse.torch.double() - total).abs() <= 2.0 ** -16).all()
+    z = (h * weight[labels].double()).sum(1)
+    assert ((loss.torch.double() - (total - z)).abs() <= 2.0 ** -15).all()
+    rows = torch.cat([labels, torch.randint(v, (200,), generator=g, device="cuda"),
+                      torch.arange(v - 200, v, device="cuda")])
+    p = torch.exp(h @ weight[rows].double().T - total[:, None]) * dloss[:, None].double()
+    p -= (labels[:, None] == rows[None]) * dloss[:, None].double()
+    want = p.T @ h
+    bound = (p.abs().T @ h.abs()) * 2.0 ** -10 + 2.0 ** -36 * h.abs().sum(0)
+    check(dw.torch[rows], want, bound, torch.float16)
+
+
 def test_lookup_grad_without_ids():
     m = module.EmbeddingLookupcuda()
     ids = torch.empty(0, dtype=torch.int64, device="cuda")
