@@ -725,6 +725,23 @@ def test_cross_entropy_float32_operands_of_any_size(size):
                labels, dloss, 1.0 / size)
 
 
+def test_the_rest_of_the_module_interface():
+    table = torch.randn((40, 8), device="cuda")
+    ids = torch.arange(20, device="cuda")
+    e, c, k = module.EmbeddingLookupcuda(), module.SoftmaxCrossEntropycuda(), module.GradientClipcuda()
+    e.build(like(table, ids), {}, {})
+    c.build(like(table[:20], table, ids), {}, {})
+    k.build(like(table), {"max_norm": 1.0, "in_place": True}, {})
+    for m, inputs in ((e, [table, ids]), (c, [table[:20], table, ids]), (k, [table.clone()])):
+        assert m.measure_average_time(inputs, 3) > 0
+        assert m.target == "cuda" and repr(m.ctx) == "gpu(0)" and m.device_status() == 0
+    text = c.lower_to_ir(like(table[:20], table, ids), {"with_grad": True}, {})
+    assert "softmax_cross_entropy" in text and "workspace" in text
+    with pytest.raises(RuntimeError, match="build"):
+        module.GradientClipcuda().run([table])
+    assert module.EmbeddingLookupcuda().device_status() == 0      # nothing built, nothing wrong
+
+
 def test_build_again_with_other_shapes():
     m = module.SoftmaxCrossEntropycuda()
     for n, v, d in ((5, 40, 8), (200, 30, 64), (3, 1000, 16)):
