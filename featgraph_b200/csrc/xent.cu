@@ -17,6 +17,10 @@
 //   weight_grad  rows = vocabulary, streamed = samples:   P^T H
 // so the logits are computed three times and never leave the SM.
 //
+// float32 runs as two fp16 pieces and three products.  Every row of either operand is scaled by a
+// power of two of its own, so that a masked, an infinite or a large row costs the others no bits
+// (2048 x 50 021 x 128: loss 80 us, gradients 339; with one scale per operand 74 and 278).
+//
 // 4096 samples x 232 965 vertices x 256, bfloat16, on one B200: loss 411 us (1190 TFLOP/s; 290 us
 // at the GEMM peak), loss and both gradients 1955 us (1250 TFLOP/s over the five products).  The
 // loss is bound by products and exponentials alike (both units 63 % busy), the gradients by the
@@ -78,7 +82,10 @@ struct MmaArgs {
   int out_vec;            // bytes of an aligned access to the results' rows
   int negate;             // a negative scale: |scale| with -A
   float logit_scale;      // |scale| * log2(e)
-  const float* unscale;   // float32: what undoes the operands' scaling; else null
+  // float32: what undoes the scaling of each row (a power of two; NaN: the row holds an infinity
+  // or a NaN), and the operands themselves, for the logits of such rows
+  const float *row_mul, *col_mul, *row_src, *col_src;
+  int64_t row_src_ld, col_src_ld;
   float2* stats;          // loss: (maximum, sum) per row, split and group of warps, base 2
   const float* row_bias;  // feat_grad: log2(hot) - lse * log2(e) of a row, -inf: takes no part
   const int32_t* row_label;
@@ -87,7 +94,8 @@ struct MmaArgs {
   const int32_t* col_label;
   float hot;              // what a probability of 1 is held as
   const float* row_factor;  // feat_grad: factor of a row of the results
-  const float* out_scale; // factor of all of them, on the device; null: 1
+  const float* out_scale; // weight_grad, 16 bits: factor of all of them, on the device
+  float out_factor;       // weight_grad, float32: the same
   void* out;              // one split: the results
   float* partial;         // several: a partial sum each, for join_partial_kernel
   int32_t* status;
@@ -100,18 +108,25 @@ struct MmaShape {
   static constexpr int kCols = MODE == kLoss ? 256 : 128;
   // Groups of four epilogue warps.  The loss only reads S, in 64 columns a group: with four
   // warps on every scheduler the exponentials' unit stays busy across the waits of each.  The
-  // gradients' groups hold twice the registers and take turns with the steps.
-  static constexpr int kGroups = MODE == kLoss ? 4 : 2;
+  // gradients' groups take turns with the steps: in 16 bits two that hold twice the registers, in
+  // float32 two pairs of which each group has half a step's columns (one group a step: 402 us for
+  // both gradients of 2048 x 50 021 x 128, with 36 % of the issue slots used).
+  static constexpr int kGroups = MODE == kLoss || kSplit ? 4 : 2;
+  static constexpr int kStepGroups = MODE == kLoss ? kGroups : kGroups / 2;  // those of one step
   static constexpr int kThreads = 32 * (kEpilogueWarp + 4 * kGroups);
   static constexpr int kChunkTiles = kSplit ? 2 : 4;
   // tiles of 16 KB that a slot of the ring holds: a tile of the streamed operand, with one of
   // the rows where these are streamed too (or, for the second product, two of the first)
   static constexpr int kSlotTiles = MODE == kLoss ? (STREAM ? 3 : 2) : (STREAM ? 2 : 1);
-  // float32: steps after which the accumulators are added up in registers.  tcgen05.mma adds
-  // to fp32 by cutting, about 2^-26 of the sum each time and always towards zero: 32 of these
-  // (eight a step) are 2^-21, several thousand were 1.1e-5.
-  static constexpr int kSegment = kSplit ? 4 : 1 << 30;
-  static constexpr int kLowOut = 128;             // the accumulators of float32's low products
+  // float32: steps after which the accumulators are added up in registers.  Every step has an
+  // exponent of its own (see the gradients' epilogue).  It also keeps the cutting small with which
+  // tcgen05.mma adds to fp32, about 2^-26 of the sum each time and always towards zero: several
+  // thousand additions were 1.1e-5.
+  static constexpr int kSegment = kSplit ? 1 : 1 << 30;
+  static constexpr int kHalfOut = 128;            // float32: the second half's accumulators
+  // What the epilogue warps keep of a step's columns in shared memory: arrays, and columns a warp.
+  static constexpr int kColArrays = kSplit ? (MODE == kLoss ? 1 : 2) : (MODE == kWeightGrad ? 1 : 0);
+  static constexpr int kMyCols = kCols / kStepGroups;
 };
 
 // Two probabilities in 16 bits each, the first in the low half.
@@ -131,22 +146,46 @@ __device__ __forceinline__ float2 unpack_half2(uint32_t r) {
 }
 
 // 32 columns of S become 32 k of P in 16 of the same columns.  Rounding P to the operands' type
-// (half a step, 2^-9 for bfloat16 and 2^-12 for float16) is what the second product's rate
-// costs; float32 keeps a second piece in the other 16 columns, together 2^-22.
+// (half a step: 2^-8 for bfloat16, 2^-11 for float16) is what the second product's rate costs.
 template <typename T>
 __device__ __forceinline__ void store_p(uint32_t at, const float (&p)[32]) {
   uint32_t r[16];
 #pragma unroll
   for (int k = 0; k < 16; ++k) r[k] = pack2<T>(p[2 * k], p[2 * k + 1]);
   tc::tmem_store16(at, r);
-  if (sizeof(T) == 4) {
+}
+// float32: 16 columns of S become 16 k of P in two pieces, eight columns each: together 2^-22.
+__device__ __forceinline__ void store_p_pieces(uint32_t at, const float (&p)[16]) {
+  uint32_t r[16];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const float2 hi = unpack_half2(r[k]);
-      r[k] = pack2<T>(p[2 * k] - hi.x, p[2 * k + 1] - hi.y);
-    }
-    tc::tmem_store16(at + 16, r);
+  for (int k = 0; k < 8; ++k) {
+    r[k] = pack2<float>(p[2 * k], p[2 * k + 1]);
+    const float2 rest = __ffma2_rn(unpack_half2(r[k]), make_float2(-1.f, -1.f),
+                                   make_float2(p[2 * k], p[2 * k + 1]));
+    r[8 + k] = pack2<float>(rest.x, rest.y);
   }
+  tc::tmem_store16(at, r);
+}
+
+// float32: factors that turn products of two scaled rows into logits in base 2.  `row` holds
+// |scale| log2(e) too.  Where the two powers of two together overflow, the products are 0 or their
+// logits far beyond what exp tells apart: the largest power does for both.  (It also stands for a
+// NaN, whose row gets its logits from plain_logit.)
+__device__ __forceinline__ float2 logit_factors(float row, float col0, float col1) {
+  const float2 m = __fmul2_rn(make_float2(row, row), make_float2(col0, col1));
+  return make_float2(fminf(m.x, 0x1p127f), fminf(m.y, 0x1p127f));
+}
+// The exponent of a power of two, 0 for NaN.
+__device__ __forceinline__ float exponent_of(float power) {
+  return power == power ? (float)((int)(__float_as_uint(power) >> 23) - 127) : 0.f;
+}
+// The product of two float32 rows of which one holds an infinity or a NaN.  In two pieces an
+// infinity would meet the zeros and the second pieces of the other row and become NaN.
+__device__ __noinline__ float plain_logit(const float* x, const float* y, int n) {
+  float z = 0.f;
+#pragma unroll 8
+  for (int c = 0; c < n; ++c) z = fmaf(__ldg(x + c), __ldg(y + c), z);
+  return z;
 }
 
 // One verdict for the whole warp: it either goes on together or gives up together.
@@ -229,7 +268,11 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
   extern __shared__ uint8_t raw_smem[];
   __shared__ uint64_t bars[2 * kMaxSlots + 2 * kMaxBuffers + 5];
   __shared__ uint32_t tmem_where;
-  __shared__ __align__(16) float col_bias_s[MODE == kWeightGrad ? 8 : 1][128];
+  constexpr int kColArrays = Shape::kColArrays > 0 ? Shape::kColArrays : 1;
+  constexpr int kColWarps = Shape::kColArrays > 0 ? 4 * Shape::kGroups : 1;
+  __shared__ __align__(16) float col_s[kColArrays][kColWarps][Shape::kMyCols];
+  // float32 gradients: what undoes a step's exponent, for every row of the last four steps
+  __shared__ float undo_s[Shape::kSplit && MODE != kLoss ? 4 : 1][2][kTileRows];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem = (smem_u32(raw_smem) + 1023) & ~1023u;
@@ -247,12 +290,12 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
     }
     for (int k = 0; k < a.buffers; ++k) {
       tc::bar_init(s_full + 8 * k, 1);
-      tc::bar_init(s_done + 8 * k, MODE == kLoss ? 128 * Shape::kGroups : 128);
+      tc::bar_init(s_done + 8 * k, 128 * Shape::kStepGroups);
     }
     tc::bar_init(rows_full, 1);
     tc::bar_init(rows_empty, 1);
     tc::bar_init(out_full, 1);
-    tc::bar_init(out_empty, 256);
+    tc::bar_init(out_empty, 128 * Shape::kGroups);
     tc::bar_init(drained, 1);
     tc::bar_init_fence();
     tc::prefetch_map(&row_map);
@@ -424,14 +467,18 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
           const uint32_t o_desc = tc::mma_desc(kBf16, n, false, true);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const uint32_t hi = p + 32 * (k >> 1) + 8 * (k & 1);
+            // 16 k are eight columns; float32's second pieces lie behind the first
+            const uint32_t hi = Shape::kSplit ? p + 16 * k : p + 32 * (k >> 1) + 8 * (k & 1);
             if (!Shape::kSplit) {
               tc::mma_ts(leader, d, hi, db + 128 * k, o_desc, !begin || k > 0);
-            } else if (!low) {             // high x high; low x high
-              tc::mma_ts(leader, d, hi, db + 128 * k, o_desc, !begin || k > 0);
-              tc::mma_ts(leader, d + Shape::kLowOut, hi + 16, db + 128 * k, o_desc, !begin || k > 0);
-            } else {                       // high x low
-              tc::mma_ts(leader, d + Shape::kLowOut, hi, db + 128 * k, o_desc, true);
+            } else {                       // each half of the k into accumulators of its own
+              const uint32_t dk = d + (k >> 2) * Shape::kHalfOut;
+              if (!low) {                  // high x high; low x high
+                tc::mma_ts(leader, dk, hi, db + 128 * k, o_desc, !begin || (k & 3) > 0);
+                tc::mma_ts(leader, dk, hi + 8, db + 128 * k, o_desc, true);
+              } else {                     // high x low
+                tc::mma_ts(leader, dk, hi, db + 128 * k, o_desc, true);
+              }
             }
           }
         };
@@ -485,7 +532,11 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
     const int group = (warp - kEpilogueWarp) >> 2;
     const int quarter = warp & 3;                         // TMEM lanes 32 * quarter ...
     const uint32_t lanes_at = (uint32_t)(quarter * 32) << 16;
-    const float scale = fmaxf(a.logit_scale * (a.unscale ? *a.unscale : 1.f), 1.17549435e-38f);
+    // float32 logits get their factors row by row and column by column instead
+    const float scale = Shape::kSplit ? 1.f : fmaxf(a.logit_scale, 1.17549435e-38f);
+    const int my_warp = Shape::kColArrays > 0 ? warp - kEpilogueWarp : 0;
+    auto& my_cols = col_s[0][my_warp];                  // float32: the factor of a column's scaling
+    auto& my_biases = col_s[kColArrays - 1][my_warp];   // gradients: what is added to its logits
     Place buf;
     uint32_t step = 0, segments = 0;
     bool ok = true;
@@ -493,6 +544,14 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
       const Item item = item_at(a, i);
       const int64_t row0 = (int64_t)item.row_tile * kTileRows;
       const int64_t row = row0 + quarter * 32 + lane;
+      float row_mul = 1.f;
+      bool row_odd = false;
+      if (Shape::kSplit && row < a.n_rows) {
+        row_mul = a.row_mul[row];
+        row_odd = row_mul != row_mul;
+        row_mul = fminf(row_mul * a.logit_scale, 0x1p127f);
+      }
+      const bool odd_rows = Shape::kSplit && MODE == kWeightGrad && __any_sync(0xffffffffu, row_odd);
       if (MODE == kLoss) {
         // Each group takes 64 of a step's 256 columns.  The exponentials are taken relative to
         // `top`, a value of the row that an earlier step had as its maximum, so that they do
@@ -501,7 +560,28 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
         constexpr int kMine = Shape::kCols / Shape::kGroups;
         const bool warp_live = row0 + quarter * 32 < a.n_rows;
         float top = -INFINITY, sum = 0.f;
+        // float32: the next step's factors are on the way while this one is worked on
+        float next_mul[Shape::kSplit ? kMine / 32 : 1];
+        auto fetch = [&](int j) {
+          const int64_t col = (int64_t)(item.first + j) * Shape::kCols + group * kMine + lane;
+#pragma unroll
+          for (int c = 0; c < kMine / 32; ++c)
+            next_mul[Shape::kSplit ? c : 0] = col + c * 32 < a.n_cols ? __ldg(a.col_mul + col + c * 32) : 1.f;
+        };
+        if (Shape::kSplit && warp_live) fetch(0);
         for (int j = 0; j < item.steps; ++j) {
+          uint32_t odd[kMine / 32] = {};   // columns that hold an infinity or a NaN
+          if (Shape::kSplit && warp_live) {
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < kMine / 32; ++c) {
+              const float m = next_mul[Shape::kSplit ? c : 0];
+              my_cols[c * 32 + lane] = m;
+              odd[c] = __ballot_sync(0xffffffffu, m != m);
+            }
+            __syncwarp();
+            if (j + 1 < item.steps) fetch(j + 1);
+          }
           if (!(ok = warp_wait(s_full + 8 * buf.at, buf.parity))) break;
           if (warp_live) {
             tc::fence_after();
@@ -517,6 +597,25 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
                 float v[32];
                 tc::tmem_load32(s_at + c * 32, v);
                 tc::wait_ld32(v);
+                if constexpr (Shape::kSplit) {
+                  for (uint32_t which = odd[c]; which; which &= which - 1) {
+                    const int from = __ffs(which) - 1;
+                    const int64_t col = (int64_t)(item.first + j) * Shape::kCols + group * kMine + c * 32 + from;
+                    float z = row < a.n_rows ? plain_logit(a.row_src + row * a.row_src_ld,
+                                                           a.col_src + col * a.col_src_ld, a.feat_len) : 0.f;
+                    if (a.negate) z = -z;
+#pragma unroll
+                    for (int k = 0; k < 32; ++k)
+                      if (k == from) v[k] = z;
+                  }
+#pragma unroll
+                  for (int k = 0; k < 32; k += 4) {
+                    const float4 e = *reinterpret_cast<const float4*>(&my_cols[c * 32 + k]);
+                    const float2 lo = __fmul2_rn(make_float2(v[k], v[k + 1]), logit_factors(row_mul, e.x, e.y));
+                    const float2 hi = __fmul2_rn(make_float2(v[k + 2], v[k + 3]), logit_factors(row_mul, e.z, e.w));
+                    v[k] = lo.x, v[k + 1] = lo.y, v[k + 2] = hi.x, v[k + 3] = hi.y;
+                  }
+                }
                 if (left < (c + 1) * 32) {
 #pragma unroll
                   for (int k = 0; k < 32; ++k)
@@ -559,9 +658,248 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
           tc::bar_arrive(s_done + 8 * buf.at);
           buf.next(a.buffers);
         }
+        if (row_odd) sum = __int_as_float(0x7fc00000);
         if (row < a.n_rows)
           a.stats[(row * a.splits + item.split) * Shape::kGroups + group] =
               make_float2(top == -INFINITY ? -INFINITY : top * scale, sum);
+      } else if constexpr (Shape::kSplit) {
+        // float32: the left operand of the second product is P times the power of two that the
+        // streamed row is scaled by, and those of rows far apart do not fit fp16 together.  So
+        // every row has an exponent that brings the largest of its entries so far to (2^13, 2^15].
+        // Where one would be larger, the exponent is lowered, and what has been stored of this step
+        // with it; each step's is undone when its products are added up.  An entry is off by 2^-22
+        // of itself and 2^-36 of the row's largest.
+        //
+        // A group has half of a step's columns, with exponents and accumulators of their own; two
+        // pairs of groups take turns with the steps.
+        constexpr int kMine = Shape::kMyCols;
+        const int pair = group >> 1, half = group & 1;
+        const int32_t warp_row0 = (int32_t)row0 + quarter * 32;
+        float bias = -INFINITY, factor = MODE == kFeatGrad ? 0.f : a.out_factor;
+        int32_t label = -1;
+        if (MODE == kFeatGrad && row < a.n_rows) {
+          bias = a.row_bias[row];
+          label = a.row_label[row];
+          factor = a.row_factor[row];
+        }
+        const bool live = MODE != kFeatGrad || label >= 0;
+        const int c0 = item.chunk * Shape::kChunkTiles * 64;
+        float acc[2][16];
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int k = 0; k < 16; ++k) acc[q][k] = 0.f;
+        // adds a step's accumulators up in registers and lets the tensor cores go on; a group takes
+        // every fourth 16-column piece
+        int flushed = 0;
+        auto flush = [&]() {
+          if (!(ok = warp_wait(out_full, segments & 1))) return;
+          tc::fence_after();
+          const float undo[2] = {undo_s[segments & 3][0][quarter * 32 + lane],
+                                 undo_s[segments & 3][1][quarter * 32 + lane]};
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const int c = group * 16 + q * 64;
+            if (c0 + c >= a.out_cols) break;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float v[16];
+              tc::tmem_load16(lanes_at + out_at + h * Shape::kHalfOut + c, v);
+              tc::wait_ld16(v);
+#pragma unroll
+              for (int k = 0; k < 16; k += 2) {
+                const float2 sum = __ffma2_rn(make_float2(v[k], v[k + 1]), make_float2(undo[h], undo[h]),
+                                              make_float2(acc[q][k], acc[q][k + 1]));
+                acc[q][k] = sum.x, acc[q][k + 1] = sum.y;
+              }
+            }
+          }
+          tc::fence_before();
+          tc::bar_arrive(out_empty);
+          ++segments;
+          ++flushed;
+        };
+        // What belongs to the group's columns, on the way before the step is: lane c fetches those
+        // of c and 32 + c.
+        float next_mul[2], next_bias[2], next_weight[2];
+        int32_t next_label[2];
+        auto fetch = [&](int j) {
+          const int64_t first = (int64_t)(item.first + j) * Shape::kCols + half * kMine + lane;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int64_t col = first + c * 32;
+            // behind the last column there is no probability, whatever lse
+            const bool in = col < a.n_cols;
+            next_mul[c] = in ? __ldg(a.col_mul + col) : 1.f;
+            next_bias[c] = in ? 0.f : -INFINITY;
+            if (MODE == kWeightGrad) {
+              next_bias[c] = a.col_bias[col];
+              next_weight[c] = a.col_weight[col];
+              next_label[c] = a.col_label[col];
+            }
+          }
+        };
+        float top = -1000.f;               // of the exponents of the row's entries; less counts as 0
+        int lift = 14 + 1000;
+        auto too_large = [&]() { return top + (float)lift > 15.f; };
+        auto fit = [&]() { lift = 14 - (int)ceilf(fminf(top, 1000.f)); };
+        bool fetched = false;
+        for (int j = 0; j < item.steps; ++j, ++step) {
+          const Place at = buf;
+          buf.next(a.buffers);
+          if ((step & 1) != pair) continue;
+          const int64_t col0 = (int64_t)(item.first + j) * Shape::kCols + half * kMine;
+          const int64_t hot_at = MODE == kFeatGrad ? label - col0 : -1;
+          const bool hot_here = hot_at >= 0 && hot_at < kMine;
+          // In `odd` the columns that hold an infinity or a NaN, in `hits` those whose label is one
+          // of this warp's rows, in `negative` those of a negative weight.
+          uint32_t odd[2] = {0, 0}, hits[2] = {0, 0}, negative[2] = {0, 0};
+          if (!fetched) fetch(j);
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float m = next_mul[c];
+            my_cols[c * 32 + lane] = m;
+            my_biases[c * 32 + lane] = next_bias[c] + exponent_of(m);
+            if (MODE == kFeatGrad) odd[c] = __ballot_sync(0xffffffffu, m != m);
+            if (MODE == kWeightGrad) {
+              hits[c] = __ballot_sync(0xffffffffu, next_label[c] >= warp_row0 && next_label[c] < warp_row0 + 32);
+              negative[c] = __ballot_sync(0xffffffffu, next_weight[c] < 0.f);
+            }
+          }
+          __syncwarp();
+          if (hot_here) top = fmaxf(top, my_biases[hot_at]);
+          const int hot_col = hot_here ? (int)hot_at : -1;
+          const bool any_hot = __any_sync(0xffffffffu, hot_here);
+          // weight_grad: which row the hit from column `from` is, and the label's 1 there
+          auto hit_row = [&](int c, int from) {
+            return a.col_label[col0 + c * 32 + from] - warp_row0;
+          };
+          auto hit_weight = [&](int c, int from) { return a.col_weight[col0 + c * 32 + from]; };
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            for (uint32_t left = hits[c]; left; left &= left - 1) {
+              const int from = __ffs(left) - 1;
+              if (lane == hit_row(c, from))
+                top = fmaxf(top, log2f(fabsf(hit_weight(c, from))) + exponent_of(my_cols[c * 32 + from]));
+            }
+          if (too_large()) fit();
+          if (!(ok = warp_wait(s_full + 8 * at.at, at.parity))) break;
+          tc::fence_after();
+          const uint32_t s_at = lanes_at + tmem + at.at * Shape::kCols + half * kMine;
+#pragma unroll 1
+          for (int c = 0; c < kMine / 16; ++c) {
+            float v[16];
+            tc::tmem_load16(s_at + c * 16, v);
+            tc::wait_ld16(v);
+            const int of32 = (c & 1) * 16, c32 = c >> 1;
+            uint32_t which = (c32 ? odd[1] : odd[0]) >> of32 & 0xffff;
+            if (odd_rows) which = 0xffff;
+            for (; which; which &= which - 1) {
+              const int from = __ffs(which) - 1;
+              // a sample that takes no part (or is none) is not looked at
+              const bool mine = row < a.n_rows && (MODE == kFeatGrad || row_odd);
+              float z = 0.f;
+              if (mine && my_biases[c * 16 + from] != -INFINITY)
+                z = plain_logit(a.row_src + row * a.row_src_ld,
+                                a.col_src + (col0 + c * 16 + from) * a.col_src_ld, a.feat_len);
+              if (a.negate) z = -z;
+#pragma unroll
+              for (int k = 0; k < 16; ++k)
+                if (k == from && mine) v[k] = z;
+            }
+            // the entries' logarithms
+            float largest = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 16; k += 4) {
+              const float4 m = *reinterpret_cast<const float4*>(&my_cols[c * 16 + k]);
+              const float4 e = *reinterpret_cast<const float4*>(&my_biases[c * 16 + k]);
+              float2 e0 = make_float2(e.x, e.y), e1 = make_float2(e.z, e.w);
+              if (MODE == kFeatGrad) {
+                e0 = __fadd2_rn(e0, make_float2(bias, bias));
+                e1 = __fadd2_rn(e1, make_float2(bias, bias));
+              }
+              const float2 q0 = __ffma2_rn(make_float2(v[k], v[k + 1]), logit_factors(row_mul, m.x, m.y), e0);
+              const float2 q1 = __ffma2_rn(make_float2(v[k + 2], v[k + 3]), logit_factors(row_mul, m.z, m.w), e1);
+              v[k] = q0.x, v[k + 1] = q0.y, v[k + 2] = q1.x, v[k + 3] = q1.y;
+              largest = fmaxf(largest, fmaxf(q0.x, q0.y));
+              largest = fmaxf(largest, fmaxf(q1.x, q1.y));
+            }
+            top = fmaxf(top, largest);
+            if (__any_sync(0xffffffffu, too_large())) {
+              const int before = lift;
+              if (too_large()) fit();
+              tc::wait_st();
+              const __half2 by = __float2half2_rn(ldexpf(1.f, max(lift - before, -126)));
+#pragma unroll 1
+              for (int done = 0; done < c; ++done) {
+                float r[16];
+                tc::tmem_load16(s_at + done * 16, r);
+                tc::wait_ld16(r);
+                uint32_t w[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                  w[k] = __float_as_uint(r[k]);
+                  __half2 h;
+                  memcpy(&h, &w[k], 4);
+                  h = __hmul2(h, by);
+                  memcpy(&w[k], &h, 4);
+                }
+                tc::tmem_store16(s_at + done * 16, w);
+              }
+            }
+            const float lifted = (float)lift;
+#pragma unroll
+            for (int k = 0; k < 16; k += 2) {
+              const float2 q = __fadd2_rn(make_float2(v[k], v[k + 1]), make_float2(lifted, lifted));
+              v[k] = exp2_fast(q.x), v[k + 1] = exp2_fast(q.y);
+            }
+            if (MODE == kFeatGrad) {
+              if (any_hot) {
+                const float hot = hot_here ? ldexpf(1.f, (int)my_biases[hot_col] + lift) : 0.f;
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                  if (hot_col == c * 16 + k) v[k] -= hot;
+              }
+            } else {
+              const uint32_t minus = (c32 ? negative[1] : negative[0]) >> of32 & 0xffff;
+              if (minus) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                  if (minus >> k & 1) v[k] = -v[k];
+              }
+              uint32_t left = (c32 ? hits[1] : hits[0]) >> of32 & 0xffff;
+              for (; left; left &= left - 1) {
+                const int from = __ffs(left) - 1;
+                const float weight = ldexpf(hit_weight(c32, of32 + from),
+                                            (int)exponent_of(my_cols[c * 16 + from]) + lift);
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                  if (k == from && lane == hit_row(c32, of32 + from)) v[k] -= weight;
+              }
+            }
+            store_p_pieces(s_at + c * 16, v);
+          }
+          float undo = ldexpf(factor, -lift);
+          // 0 times it stays 0 where the sums are beyond float32
+          if (isinf(undo) && !isinf(factor)) undo = copysignf(3.4028235e38f, factor);
+          undo_s[step & 3][half][quarter * 32 + lane] = undo;
+          tc::wait_st();
+          tc::fence_before();
+          tc::bar_arrive(s_done + 8 * at.at);
+          fetched = j + 2 < item.steps;
+          if (fetched) fetch(j + 2);
+          while (ok && flushed <= j) flush();
+          if (!ok) break;
+        }
+        if (!ok) break;
+        while (ok && flushed < item.steps) flush();
+        if (!ok) break;
+        if (row < a.n_rows) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            store_out<MODE, T>(a, item, row, c0 + group * 16 + q * 64, acc[q], 1.f, live);
+        }
       } else {
         // The groups take turns with the steps.
         const int32_t warp_row0 = (int32_t)row0 + quarter * 32;
@@ -574,37 +912,8 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
         const int c0 = item.chunk * Shape::kChunkTiles * 64;
         float factor = 0.f;
         if (a.splits == 1 && row < a.n_rows)
-          factor = (a.out_scale ? *a.out_scale : 1.f) * (MODE == kFeatGrad ? a.row_factor[row] : 1.f);
+          factor = MODE == kFeatGrad ? a.row_factor[row] : *a.out_scale;
         const bool live = MODE != kFeatGrad || label >= 0;
-        float acc[Shape::kSplit ? 4 : 1][16];
-#pragma unroll
-        for (int q = 0; q < (Shape::kSplit ? 4 : 1); ++q)
-#pragma unroll
-          for (int k = 0; k < 16; ++k) acc[q][k] = 0.f;
-        // adds a segment of accumulators up in registers and lets the tensor cores go on
-        int flushed = 0;
-        auto flush = [&]() {
-          if (!(ok = warp_wait(out_full, segments & 1))) return;
-          tc::fence_after();
-#pragma unroll
-          for (int q = 0; q < (Shape::kSplit ? 4 : 1); ++q) {
-            const int c = group * 16 + q * 32;
-            if (c0 + c >= a.out_cols) break;
-            float v[16];
-            tc::tmem_load16(lanes_at + out_at + c, v);
-            tc::wait_ld16(v);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) acc[q][k] += v[k];
-            tc::tmem_load16(lanes_at + out_at + Shape::kLowOut + c, v);
-            tc::wait_ld16(v);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) acc[q][k] += v[k];
-          }
-          tc::fence_before();
-          tc::bar_arrive(out_empty);
-          ++segments;
-          ++flushed;
-        };
         for (int j = 0; j < item.steps; ++j, ++step) {
           const Place at = buf;
           buf.next(a.buffers);
@@ -621,7 +930,7 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
             for (int c = 0; c < 4; ++c) {
               col_label[c] = a.col_label[col0 + c * 32 + lane];
               col_weight[c] = a.col_weight[col0 + c * 32 + lane];
-              col_bias_s[warp - kEpilogueWarp][c * 32 + lane] = a.col_bias[col0 + c * 32 + lane];
+              my_biases[c * 32 + lane] = a.col_bias[col0 + c * 32 + lane];
             }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -634,15 +943,13 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
           if (!(ok = warp_wait(s_full + 8 * at.at, at.parity))) break;
           tc::fence_after();
           const uint32_t s_at = lanes_at + tmem + at.at * Shape::kCols;
-          constexpr int kAhead = Shape::kSplit ? 1 : 2;  // float32 needs the registers
-          float x[kAhead][32];
-          if (kAhead == 2) tc::tmem_load32(s_at, x[0]);
+          float x[2][32];
+          tc::tmem_load32(s_at, x[0]);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            float(&v)[32] = x[c % kAhead];
-            if (kAhead == 1) tc::tmem_load32(s_at + c * 32, v);
+            float(&v)[32] = x[c & 1];
             tc::wait_ld32(v);
-            if (kAhead == 2 && c < 3) tc::tmem_load32(s_at + (c + 1) * 32, x[(c + 1) % kAhead]);
+            if (c < 3) tc::tmem_load32(s_at + (c + 1) * 32, x[(c + 1) & 1]);
             if (MODE == kFeatGrad) {
 #pragma unroll
               for (int k = 0; k < 32; ++k) v[k] = exp2_fast(fmaf(v[k], scale, bias));
@@ -660,8 +967,7 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
             } else {
 #pragma unroll
               for (int k = 0; k < 32; k += 4) {
-                const float4 e =
-                    *reinterpret_cast<const float4*>(&col_bias_s[warp - kEpilogueWarp][c * 32 + k]);
+                const float4 e = *reinterpret_cast<const float4*>(&my_biases[c * 32 + k]);
                 v[k] = exp2_fast(fmaf(v[k], scale, e.x));
                 v[k + 1] = exp2_fast(fmaf(v[k + 1], scale, e.y));
                 v[k + 2] = exp2_fast(fmaf(v[k + 2], scale, e.z));
@@ -686,36 +992,23 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
           tc::wait_st();
           tc::fence_before();
           tc::bar_arrive(s_done + 8 * at.at);
-          if (Shape::kSplit)
-            while (ok && (flushed + 1) * Shape::kSegment <= j + 1) flush();
-          if (!ok) break;
         }
         if (!ok) break;
-        if (Shape::kSplit) {
-          while (ok && flushed * Shape::kSegment < item.steps) flush();
-          if (!ok) break;
-          if (row < a.n_rows) {
-#pragma unroll
-            for (int q = 0; q < (Shape::kSplit ? 4 : 1); ++q)
-              store_out<MODE, T>(a, item, row, c0 + group * 16 + q * 32, acc[q], factor, live);
-          }
-        } else {
-          // the two groups take alternate 16-column pieces of the accumulators
-          if (!(ok = warp_wait(out_full, segments & 1))) break;
-          tc::fence_after();
-          ++segments;
-          const int cols = min(a.out_cols - c0, Shape::kChunkTiles * 64);
-          for (int c = group * 16; c < cols; c += 32) {
-            float v[16];
-            __syncwarp();
-            tc::tmem_load16(lanes_at + out_at + c, v);
-            tc::wait_ld16(v);
-            if (row < a.n_rows) store_out<MODE, T>(a, item, row, c0 + c, v, factor, live);
-          }
+        // the two groups take alternate 16-column pieces of the accumulators
+        if (!(ok = warp_wait(out_full, segments & 1))) break;
+        tc::fence_after();
+        ++segments;
+        const int cols = min(a.out_cols - c0, Shape::kChunkTiles * 64);
+        for (int c = group * 16; c < cols; c += 32) {
+          float v[16];
           __syncwarp();
-          tc::fence_before();
-          tc::bar_arrive(out_empty);
+          tc::tmem_load16(lanes_at + out_at + c, v);
+          tc::wait_ld16(v);
+          if (row < a.n_rows) store_out<MODE, T>(a, item, row, c0 + c, v, factor, live);
         }
+        __syncwarp();
+        tc::fence_before();
+        tc::bar_arrive(out_empty);
       }
     }
     if (!ok && lane == 0) *a.status = FG_STATUS_WAIT_EXPIRED;
@@ -727,66 +1020,11 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
 }
 
 // ------------------------------------------------------------ around the kernel --
-// Scalars of a call, on the device (setup_kernel).
+// Scalars of a call in 16 bits, on the device.
 struct Consts {
-  float scale_feat, scale_weight;   // powers of two that float32 operands are held with
-  float unscale;                    // 1 / (scale_feat * scale_weight), of the logits
-  float out_feat, out_weight;       // factors of the two gradients
+  float out_weight;                 // factor of weight_grad
   float inv_weight_max;             // 1 / the largest |loss_grad|
 };
-constexpr int kMaxPartials = 592;
-
-// Largest finite magnitude per CTA of the rows that take part, for both float32 operands
-// (blockIdx.y).
-__global__ void __launch_bounds__(256)
-abs_max_kernel(Batch b, const float* __restrict__ feat, int64_t feat_ld,
-               const float* __restrict__ weight, int64_t weight_ld, float* __restrict__ partial) {
-  begin_chained();
-  float top = 0.f;
-  const bool second = blockIdx.y == 1;
-  const float* p = second ? weight : feat;
-  int64_t rows = second ? b.vocab : b.n;
-  const int64_t ld = second ? weight_ld : feat_ld;
-  if (second && ld == b.feat_len) {  // no gaps and no rows to leave out: one long array
-    const int64_t total = rows * ld, step = (int64_t)gridDim.x * 256;
-    for (int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x; i0 < total; i0 += step * 8) {
-      float v[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = i0 + k * step < total ? fabsf(p[i0 + k * step]) : 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (v[k] < INFINITY) top = fmaxf(top, v[k]);
-    }
-    rows = 0;
-  }
-  // 32 lanes take whole rows of up to 128 elements four at a time, longer rows one at a time
-  const int per_row = (int)min((int64_t)4, (b.feat_len + 31) / 32), together = 4 / per_row;
-  const int64_t warps = (int64_t)gridDim.x * 8;
-  for (int64_t r0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * together; r0 < rows;
-       r0 += warps * together) {
-    for (int64_t c0 = threadIdx.x & 31; c0 < b.feat_len; c0 += 32 * per_row) {
-      float v[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int64_t r = r0 + k / per_row, c = c0 + (k % per_row) * 32;
-        const bool in = k < together * per_row && r < rows && c < b.feat_len;
-        v[k] = in ? fabsf(p[r * ld + c]) : 0.f;
-        if (!second && in && live_label(b, r) < 0) v[k] = 0.f;
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (v[k] < INFINITY) top = fmaxf(top, v[k]);
-    }
-  }
-  __shared__ float warps_top[8];
-  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  if ((threadIdx.x & 31) == 0) warps_top[threadIdx.x >> 5] = top;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 8; ++w) top = fmaxf(top, warps_top[w]);
-    partial[blockIdx.y * kMaxPartials + blockIdx.x] = top;
-  }
-}
 
 __device__ __forceinline__ float block_max(float v, float* shared) {
   for (int d = 16; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
@@ -796,13 +1034,13 @@ __device__ __forceinline__ float block_max(float v, float* shared) {
   for (int w = 0; w < (int)blockDim.x / 32; ++w) v = fmaxf(v, shared[w]);
   return v;
 }
-// The power of two that brings `top` to [2^12, 2^13): the two fp16 pieces of a value then end
-// at 2^-37 of the largest, and values up to 16 times the largest still fit.
-__device__ __forceinline__ int operand_exponent(float top) {
+// The power of two that brings `top`, the largest magnitude of a float32 row, to [2^12, 2^13): the
+// two fp16 pieces of a value are then off by 2^-22 of it and 2^-37 of the row's largest.
+__device__ __forceinline__ int row_exponent(float top) {
   if (!(top > 0.f)) return 0;
   int e;
   frexpf(top, &e);
-  return min(120, max(-120, 13 - e));
+  return min(126, 13 - e);
 }
 
 // What the gradients' kernels need of a sample, and of the padding up to a whole tile.
@@ -829,45 +1067,19 @@ __device__ __forceinline__ void sample(const Batch& b, const SampleArrays& s, fl
   s.col_bias[t] = weight == 0.f ? -INFINITY : bias + log2f(fabsf(weight));
 }
 
-// The scalars, by one CTA of any size; it also makes the sample arrays of a batch of up to
+// 16 bits: the scalars, by one CTA; it also makes the sample arrays of a batch of up to
 // kSetupSamples.
 constexpr int64_t kSetupSamples = 8192;
-__device__ __forceinline__ void setup(const Batch& b, const SampleArrays& s, const float* abs_max,
-                                      Consts* consts) {
+__device__ __forceinline__ void setup(const Batch& b, const SampleArrays& s, Consts* consts) {
   __shared__ float shared[32];
   float top = 0.f;
-  if (s.loss_grad)
-    for (int64_t t = threadIdx.x; t < b.n; t += blockDim.x)
-      if (live_label(b, t) >= 0) top = fmaxf(top, fabsf(s.loss_grad[t]));
+  for (int64_t t = threadIdx.x; t < b.n; t += blockDim.x)
+    if (live_label(b, t) >= 0) top = fmaxf(top, fabsf(s.loss_grad[t]));
   top = block_max(top, shared);
-  int ef = 0, ew = 0;
-  if (abs_max) {
-    float top_feat = 0.f, top_weight = 0.f;
-    for (int k = threadIdx.x; k < kMaxPartials; k += blockDim.x) {
-      top_feat = fmaxf(top_feat, abs_max[k]);
-      top_weight = fmaxf(top_weight, abs_max[kMaxPartials + k]);
-    }
-    ef = operand_exponent(block_max(top_feat, shared));
-    ew = operand_exponent(block_max(top_weight, shared));
-  }
   const float inv = top >= 1.17549435e-38f ? 1.f / top : 0.f;
-  if (threadIdx.x == 0) {
-    Consts c;
-    c.scale_feat = ldexpf(1.f, ef);
-    c.scale_weight = ldexpf(1.f, ew);
-    c.unscale = ldexpf(1.f, -ef - ew);
-    c.out_feat = ldexpf(1.f, -ew);
-    c.out_weight = top * b.scale / s.hot * ldexpf(1.f, -ef);
-    c.inv_weight_max = inv;
-    *consts = c;
-  }
-  if (s.loss_grad && s.padded <= kSetupSamples)
+  if (threadIdx.x == 0) *consts = {top * b.scale / s.hot, inv};
+  if (s.padded <= kSetupSamples)
     for (int64_t t = threadIdx.x; t < s.padded; t += blockDim.x) sample(b, s, inv, t);
-}
-__global__ void __launch_bounds__(1024)
-setup_kernel(Batch b, SampleArrays s, const float* __restrict__ abs_max, Consts* consts) {
-  begin_chained();
-  setup(b, s, abs_max, consts);
 }
 __global__ void __launch_bounds__(256)
 sample_kernel(Batch b, SampleArrays s, const Consts* __restrict__ consts) {
@@ -877,16 +1089,18 @@ sample_kernel(Batch b, SampleArrays s, const Consts* __restrict__ consts) {
 }
 
 // Operands as the tensor maps want them: rows of `pitch` 16-bit elements, zero behind feat_len.
-// float32 becomes two fp16 pieces, the second behind the first.  A row whose label is out of
-// play (`masked`) becomes zero, whatever it held.  The first `blocks` CTAs pack one operand, the
-// others the second; where packing needs none of the scalars (`with_setup`), the last CTA makes
-// these.
+// float32 becomes two fp16 pieces of the row scaled by its own power of two, the second behind the
+// first; `mul` gets what undoes the scaling, or NaN for a row with an infinity or a NaN, whose
+// pieces keep these in their places.  A row whose label is out of play (`masked`) becomes zero,
+// whatever it held.  The first `blocks` CTAs pack one operand, the others the second.  In 16 bits
+// the last CTA makes the scalars (`with_setup`); in float32 the samples' arrays need none and are
+// made along with the samples' rows.
 template <typename T>
 struct PackJob {
   const T* from;
   int64_t ld, rows;
   int blocks, masked;
-  const float* factor;
+  float* mul;
   uint16_t* to;
 };
 template <typename T>
@@ -895,27 +1109,49 @@ pack_kernel(Batch b, PackJob<T> first, PackJob<T> second, int64_t pitch, int wit
             Consts* consts) {
   begin_chained();
   if (with_setup && blockIdx.x == gridDim.x - 1) {
-    setup(b, s, nullptr, consts);
+    setup(b, s, consts);
     return;
   }
   const bool is_second = (int)blockIdx.x >= first.blocks;
   const PackJob<T> j = is_second ? second : first;
   const int64_t block = is_second ? blockIdx.x - first.blocks : blockIdx.x;
   const int64_t piece = sizeof(T) == 4 ? pitch / 2 : pitch;
-  const float f = sizeof(T) == 4 ? *j.factor : 1.f;
-  for (int64_t r = block * 8 + (threadIdx.x >> 5); r < j.rows; r += (int64_t)j.blocks * 8) {
+  const int lane = threadIdx.x & 31;
+  const bool with_samples = sizeof(T) == 4 && !is_second && s.loss_grad;
+  const int64_t rows = with_samples ? s.padded : j.rows;
+  for (int64_t r = block * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)j.blocks * 8) {
+    if (with_samples && lane == 0) sample(b, s, 1.f, r);
+    if (r >= j.rows) continue;
     const bool live = !j.masked || live_label(b, r) >= 0;
+    float f = 1.f;
+    if constexpr (sizeof(T) == 4) {
+      float top = 0.f;
+      bool odd = false;
+      if (live) {
+#pragma unroll 4
+        for (int64_t c = lane; c < b.feat_len; c += 32) {
+          const float x = fabsf(j.from[r * j.ld + c]);
+          if (x < INFINITY) top = fmaxf(top, x); else odd = true;
+        }
+      }
+      for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      odd = __any_sync(0xffffffffu, odd);
+      const int e = row_exponent(top);
+      f = ldexpf(1.f, e);
+      if (lane == 0) j.mul[r] = odd ? __int_as_float(0x7fc00000) : ldexpf(1.f, -e);
+    }
     // two neighbouring elements a lane, so that the 16-bit pieces are written as 32 bits
 #pragma unroll 2
-    for (int64_t c = (threadIdx.x & 31) * 2; c < piece; c += 64) {
+    for (int64_t c = lane * 2; c < piece; c += 64) {
       T x[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
         x[k] = live && c + k < b.feat_len ? j.from[r * j.ld + c + k] : from_float<T>(0.f);
       if constexpr (sizeof(T) == 4) {
-        const __half2 hi = __floats2half2_rn(x[0] * f, x[1] * f);
+        const float y0 = x[0] * f, y1 = x[1] * f;
+        const __half2 hi = __floats2half2_rn(y0, y1);
         const float2 back = __half22float2(hi);
-        const __half2 lo = __floats2half2_rn(x[0] * f - back.x, x[1] * f - back.y);
+        const __half2 lo = __floats2half2_rn(isinf(y0) ? 0.f : y0 - back.x, isinf(y1) ? 0.f : y1 - back.y);
         *reinterpret_cast<__half2*>(j.to + r * pitch + c) = hi;
         *reinterpret_cast<__half2*>(j.to + r * pitch + piece + c) = lo;
       } else {
@@ -1052,7 +1288,7 @@ struct XentLayout {
   int64_t t_tiles, v_tiles;
   int out_cols;
   Cut loss, feat, weight;
-  size_t consts, abs_max, packed_feat, packed_weight;
+  size_t consts, feat_mul, weight_mul, packed_feat, packed_weight;
   size_t stats, row_bias, row_factor, col_bias, col_weight, label, partial;
   size_t total;
 };
@@ -1082,7 +1318,10 @@ XentLayout xent_layout(int32_t dtype, int64_t n, int64_t vocab, int64_t feat_len
     return here;
   };
   l.consts = take(sizeof(Consts));
-  l.abs_max = take(2 * kMaxPartials * 4);
+  if (dtype == FG_FLOAT32) {
+    l.feat_mul = take((size_t)n * 4);
+    l.weight_mul = take((size_t)vocab * 4);
+  }
   l.packed_feat = take((size_t)n * l.pitch * 2);
   l.packed_weight = take((size_t)vocab * l.pitch * 2);
   l.stats = take((size_t)n * l.loss.splits * kLossGroups * sizeof(float2));
@@ -1137,37 +1376,27 @@ bool fits_map(int32_t dtype, const void* p, int64_t ld) {
   return dtype != FG_FLOAT32 && ((uintptr_t)p & 15) == 0 && ld % 8 == 0;
 }
 
-// Scalars, sample arrays (with loss_grad), scales of float32 operands, and packed copies where
-// they are needed.  `chained`: whether this call has launched something before.
+// Packed copies of the operands where they are needed and, with loss_grad, the samples' arrays
+// (in 16 bits the scalars too).  `chained`: whether this call has launched something.
 template <typename T>
 int prepare_operands(const Batch& b, const XentLayout& l, char* ws, const T* feat, int64_t feat_ld,
                      const T* weight, int64_t weight_ld, int32_t dtype, const SampleArrays& samples,
                      cudaStream_t s, Operands* o, bool* chained) {
   Consts* consts = reinterpret_cast<Consts*>(ws + l.consts);
-  float* abs_max = reinterpret_cast<float*>(ws + l.abs_max);
   const bool grad = samples.loss_grad != nullptr;
-  if constexpr (sizeof(T) == 4) {
-    FG_CUDA_TRY(launch(*chained, abs_max_kernel, dim3(kMaxPartials, 2), 256, 0, s, b, feat, feat_ld, weight,
-                       weight_ld, abs_max));
-    *chained = true;
-  }
-  // 16-bit gradients always pack the features, and make the scalars beside that
+  // gradients always pack the features, 16-bit ones make the scalars beside that
   const bool with_setup = sizeof(T) == 2 && grad;
-  if (sizeof(T) == 4) {
-    FG_CUDA_TRY(launch(*chained, setup_kernel, 1, 1024, 0, s, b, samples, abs_max, consts));
-    *chained = true;
-  }
   *o = {feat, weight, feat_ld, weight_ld};
   auto blocks = [](int64_t rows) { return (int)std::min<int64_t>((rows + 7) / 8, 8 * kSms); };
   PackJob<T> jobs[2] = {};
   if (grad || !fits_map(dtype, feat, feat_ld)) {
-    jobs[0] = {feat, feat_ld, b.n, blocks(b.n), grad, &consts->scale_feat,
+    jobs[0] = {feat, feat_ld, b.n, blocks(b.n), grad, reinterpret_cast<float*>(ws + l.feat_mul),
                reinterpret_cast<uint16_t*>(ws + l.packed_feat)};
     o->feat = ws + l.packed_feat;
     o->feat_ld = l.pitch;
   }
   if (!fits_map(dtype, weight, weight_ld)) {
-    jobs[1] = {weight, weight_ld, b.vocab, blocks(b.vocab), 0, &consts->scale_weight,
+    jobs[1] = {weight, weight_ld, b.vocab, blocks(b.vocab), 0, reinterpret_cast<float*>(ws + l.weight_mul),
                reinterpret_cast<uint16_t*>(ws + l.packed_weight)};
     o->weight = ws + l.packed_weight;
     o->weight_ld = l.pitch;
@@ -1177,10 +1406,27 @@ int prepare_operands(const Batch& b, const XentLayout& l, char* ws, const T* fea
                        jobs[0], jobs[1], l.pitch, with_setup, samples, consts));
     *chained = true;
   }
-  if (grad && samples.padded > kSetupSamples)
+  if (with_setup && samples.padded > kSetupSamples)
     FG_CUDA_TRY(launch(true, sample_kernel, (unsigned)((samples.padded + 255) / 256), 256, 0, s, b, samples,
                        consts));
   return FG_OK;
+}
+// float32: the rows' scalings and the operands they belong to, for the kernel.
+template <typename T>
+void set_row_scalings(MmaArgs* a, const XentLayout& l, char* ws, bool rows_are_samples, const T* feat,
+                      int64_t feat_ld, const T* weight, int64_t weight_ld) {
+  if constexpr (sizeof(T) == 4) {
+    const float* mul[2] = {reinterpret_cast<float*>(ws + l.feat_mul), reinterpret_cast<float*>(ws + l.weight_mul)};
+    const float* src[2] = {feat, weight};
+    const int64_t ld[2] = {feat_ld, weight_ld};
+    const int row = rows_are_samples ? 0 : 1;
+    a->row_mul = mul[row];
+    a->row_src = src[row];
+    a->row_src_ld = ld[row];
+    a->col_mul = mul[1 - row];
+    a->col_src = src[1 - row];
+    a->col_src_ld = ld[1 - row];
+  }
 }
 
 template <int MODE, typename T, bool STREAM>
@@ -1213,8 +1459,8 @@ int launch_mma_as(const Batch& b, const XentLayout& l, const Operands& o, const 
   a.negate = b.scale < 0.f;
   a.out_vec = common_vector_bytes({(uint64_t)(uintptr_t)a.out, (uint64_t)b.feat_len * sizeof(T)});
   a.logit_scale = std::fabs(b.scale) * kLog2e;
-  // shared memory: 14 tiles of 16 KB at most, 13 where the columns' biases need some of it
-  const int room = MODE == kWeightGrad ? 13 : 14;
+  // shared memory: 14 tiles of 16 KB at most, 13 where what belongs to columns needs some of it
+  const int room = Shape::kColArrays > 0 ? 13 : 14;
   const int resident = STREAM ? 0 : l.tiles;
   a.slots = std::min(kMaxSlots, (room - resident) / Shape::kSlotTiles);
   // Two neighbouring slots are one operand of 128 columns where a step's tiles come in pairs and
@@ -1256,7 +1502,7 @@ int loss_mma(const Batch& b, const XentLayout& l, char* ws, const T* feat, int64
   if (int rc = prepare_operands<T>(b, l, ws, feat, feat_ld, weight, weight_ld, dtype, none, s, &o, &chained))
     return rc;
   MmaArgs a = {};
-  a.unscale = sizeof(T) == 4 ? &reinterpret_cast<Consts*>(ws + l.consts)->unscale : nullptr;
+  set_row_scalings<T>(&a, l, ws, true, feat, feat_ld, weight, weight_ld);
   a.stats = reinterpret_cast<float2*>(ws + l.stats);
   a.status = status;
   if (int rc = launch_mma<kLoss, T>(b, l, o, l.loss, a, chained, device, s)) return rc;
@@ -1270,8 +1516,8 @@ int grad_mma(const Batch& b, const XentLayout& l, char* ws, const float* loss_gr
              int64_t feat_ld, const T* weight, int64_t weight_ld, int32_t dtype, const float* lse,
              T* feat_grad, T* weight_grad, int32_t* status, int device, cudaStream_t s) {
   // fp16 holds down to 2^-24: a probability of 1 is held as 2^14, so that the smallest that
-  // count are 2^-38
-  const float hot = dtype == FG_BFLOAT16 ? 1.f : 16384.f;
+  // count are 2^-38 (float32's have their own exponents)
+  const float hot = dtype == FG_FLOAT16 ? 16384.f : 1.f;
   const SampleArrays arrays = {lse, loss_grad,
                                reinterpret_cast<float*>(ws + l.row_bias),
                                reinterpret_cast<float*>(ws + l.row_factor),
@@ -1284,7 +1530,6 @@ int grad_mma(const Batch& b, const XentLayout& l, char* ws, const float* loss_gr
     return rc;
   Consts* consts = reinterpret_cast<Consts*>(ws + l.consts);
   MmaArgs a = {};
-  a.unscale = sizeof(T) == 4 ? &consts->unscale : nullptr;
   a.row_bias = arrays.row_bias;
   a.row_factor = arrays.row_factor;
   a.row_label = a.col_label = arrays.label;
@@ -1302,17 +1547,20 @@ int grad_mma(const Batch& b, const XentLayout& l, char* ws, const float* loss_gr
                   a.partial, cut.splits, rows, l.out_cols, (int)b.feat_len, row_factor, row_label,
                   out_scale, out);
   };
+  constexpr bool kSplit = sizeof(T) == 4;   // whose sums have their factors already
   if (feat_grad) {
     a.out = feat_grad;
-    a.out_scale = &consts->out_feat;
+    set_row_scalings<T>(&a, l, ws, true, feat, feat_ld, weight, weight_ld);
     if (int rc = launch_mma<kFeatGrad, T>(b, l, o, l.feat, a, true, device, s)) return rc;
-    FG_CUDA_TRY(join(l.feat, b.n, arrays.row_factor, arrays.label, a.out_scale, feat_grad));
+    FG_CUDA_TRY(join(l.feat, b.n, kSplit ? nullptr : arrays.row_factor, arrays.label, nullptr, feat_grad));
   }
   if (weight_grad) {
     a.out = weight_grad;
     a.out_scale = &consts->out_weight;
+    a.out_factor = b.scale;
+    set_row_scalings<T>(&a, l, ws, false, feat, feat_ld, weight, weight_ld);
     if (int rc = launch_mma<kWeightGrad, T>(b, l, o, l.weight, a, true, device, s)) return rc;
-    FG_CUDA_TRY(join(l.weight, b.vocab, nullptr, nullptr, a.out_scale, weight_grad));
+    FG_CUDA_TRY(join(l.weight, b.vocab, nullptr, nullptr, kSplit ? nullptr : a.out_scale, weight_grad));
   }
   return FG_OK;
 }

@@ -395,7 +395,10 @@ int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_t out_grad_
  *   lse[t] = log sum_v exp z[t, v],   loss[t] = lse[t] - z[t, labels[t]],
  * both fp32.  loss is 0 where labels[t] = ignore_index (lse is still that row's), NaN where
  * a label is out of range.  An infinite logit makes its row NaN, except -inf beside a
- * finite one. */
+ * finite one.
+ * float32 values are held relative to the largest finite magnitude of their own row of feat
+ * or weight: each is off by at most 2^-22 of itself and 2^-37 of that magnitude.  Rows that
+ * hold an infinity take no bits from others; a feat row with one gives that sample NaN. */
 int64_t fg_softmax_xent_workspace_bytes(int32_t dtype, int64_t n, int64_t vocab,
                                         int64_t feat_len, int32_t with_grad);
 int fg_softmax_xent(const void* feat_dev, int64_t feat_ld, const void* weight_dev,
@@ -410,7 +413,8 @@ int fg_softmax_xent(const void* feat_dev, int64_t feat_ld, const void* weight_de
  *   feat_grad = dz @ weight,  weight_grad = dz^T @ feat,
  * both in dtype, without gaps, every element overwritten; either may be NULL.  A row whose
  * label is ignore_index (or out of range) has dz = 0 whatever feat, lse and loss_grad hold
- * there. */
+ * there.  For the two products dz is rounded to dtype; float32 keeps two fp16 pieces of it,
+ * off by at most 2^-22 of an entry and 2^-35 of its row's largest contribution. */
 int fg_softmax_xent_grad(const float* loss_grad_dev, const void* feat_dev, int64_t feat_ld,
                          const void* weight_dev, int64_t weight_ld, int32_t dtype,
                          const void* labels_dev, int32_t index_type, int64_t n, int64_t vocab,

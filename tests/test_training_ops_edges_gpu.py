@@ -1,0 +1,199 @@
+"""Edges of the training operators on the GPU: operands whose rows lie far apart in size, masked
+and infinite rows, ignored rows.  Plain implementations in 64 bits, as in
+test_training_ops_gpu.py."""
+import math
+
+import pytest
+import torch
+
+import test_training_ops_gpu as t
+
+pytestmark = pytest.mark.gpu
+U = t.U
+
+
+# ------------------------------------- float32 cross entropy: rows of any size --
+def by_rows(feat, weight, labels, dloss, scale=1.0, ignore=-100):
+    """Losses and gradients in fp64 with the bounds of float32 held as two fp16 pieces relative to
+    the largest value of its OWN row.
+
+    An element x of a row whose largest magnitude is m is off by at most 2^-22 |x| + 2^-37 m (the
+    second piece is rounded to 2^-11 of the first's error, and ends at 2^-24 where m is at least
+    2^12); a product leaves out the two second pieces, 2^-22.  Sums as in xent_reference: 2 u a
+    term.  dz is held in two pieces relative to the largest entry of its row so far (probability
+    times the scale of the row that it multiplies), which is held as at least 2^13.  Each piece ends
+    at 2^-24, half a step of it is 2^-25, and where a larger entry comes both are rounded again at
+    half the size or less: 2^-23 in all.  The rows that they multiply are below 2^13, and the
+    largest contribution at least 2^13 2^12: k terms are off by k 2^-35 of that.  Nothing is
+    relative to the values of another row beside the largest contribution."""
+    h, w = feat.double(), weight.double()
+    n, d = h.shape
+    v = w.shape[0]
+    keep = labels != ignore
+    hm, wm = h.abs().amax(1, keepdim=True), w.abs().amax(1, keepdim=True)
+    z = scale * (h @ w.T)
+    ends = (h.abs().sum(1, keepdim=True) @ wm.T + hm @ w.abs().sum(1, keepdim=True).T) * 2.0 ** -37
+    ez = abs(scale) * ((h.abs() @ w.abs().T) * ((d + 8) * 2 * U + 2.0 ** -20) + ends)
+    lse = torch.logsumexp(z, 1)
+    p = torch.exp(z - lse[:, None])
+    # a logit's error counts by its probability, within the largest of those that count at all
+    far = z + ez < (z - ez).amax(1, keepdim=True) - 120
+    elz = torch.where(far, 0.0, ez).amax(1) + (v + 64) * U + lse.abs() * 4 * U
+    at = torch.where(keep, labels.long(), 0)[:, None]
+    loss = torch.where(keep, lse - z.gather(1, at)[:, 0], 0.0)
+    eloss = torch.where(keep, elz + ez.gather(1, at)[:, 0] + loss.abs() * 2 * U, 0.0)
+    g = torch.where(keep, dloss.double(), 0.0)[:, None]
+    hot = torch.zeros_like(p).scatter_(1, at, 1.0)
+    dz = (p - hot) * g * scale
+    ep = torch.where(far, 0.0, p * (torch.expm1(ez.clamp(max=300) + elz.clamp(max=300)[:, None]) + 16 * U))
+    ep = ep * (g * scale).abs()
+    edz = ep + (dz.abs() + ep) * 2.0 ** -20
+    unit = torch.maximum(p, hot) * (g * scale).abs()
+    hk = torch.where(keep[:, None], h, 0.0)
+    hmk = torch.where(keep[:, None], hm, 0.0)
+    size = dz.abs()
+    df = edz @ w.abs() + (size @ w.abs()) * ((v + 8) * 2 * U + 2.0 ** -20) + (size @ wm) * 2.0 ** -37
+    df = df + (unit * wm.T).amax(1, keepdim=True) * v * 2.0 ** -35
+    dw = edz.T @ hk.abs() + (size.T @ hk.abs()) * ((n + 8) * 2 * U + 2.0 ** -20) + (size.T @ hmk) * 2.0 ** -37
+    dw = dw + (unit * hmk).amax(0)[:, None] * n * 2.0 ** -35
+    return {"loss": (loss, eloss), "lse": (lse, elz),
+            "feat_grad": (torch.where(keep[:, None], dz @ w, 0.0), torch.where(keep[:, None], df, 0.0)),
+            "weight_grad": (dz.T @ hk, dw)}
+
+
+def run(m, feat, weight, labels, dloss):
+    loss, lse = m.run([feat, weight, labels])
+    dh, dw = m.run_grad([dloss, feat, weight, labels, lse])
+    return {"loss": loss.torch, "lse": lse.torch, "feat_grad": dh.torch, "weight_grad": dw.torch}
+
+
+def check_rows(feat, weight, labels, dloss, scale=1.0, rows=slice(None), vertices=slice(None)):
+    got = run(t.xent_module(feat, weight, labels, scale=scale), feat, weight, labels, dloss)
+    want = by_rows(feat, weight, labels, dloss, scale)
+    pick = {"loss": rows, "lse": rows, "feat_grad": rows, "weight_grad": vertices}
+    for key, (value, bound) in want.items():
+        t.check(got[key][pick[key]], value[pick[key]], bound[pick[key]], torch.float32)
+    return got
+
+
+SIZES = [(60, 400, 40), (150, 700, 128), (33, 300, 260)]      # one tile a row, two, streamed
+
+
+@pytest.mark.parametrize("n, v, d", SIZES)
+@pytest.mark.parametrize("mask", [-1e6, -1e9, torch.finfo(torch.float32).min])
+def test_float32_masked_table_rows_leave_the_others_alone(n, v, d, mask):
+    # a column of ones in the features carries the mask
+    feat, weight, labels, dloss = t.xent_inputs(n, v, d, "float32", n + d)
+    feat[:, 0] = 1.0
+    for row in (5, 133, v - 1):
+        weight[row] = 0.0
+        weight[row, 0] = mask
+        labels[labels == row] = 6
+    check_rows(feat, weight, labels, dloss)
+
+
+@pytest.mark.parametrize("n, v, d", SIZES)
+@pytest.mark.parametrize("size", [2.0 ** 24, 1e7, 1e-7])
+def test_float32_one_sample_of_another_size(n, v, d, size):
+    feat, weight, labels, dloss = t.xent_inputs(n, v, d, "float32", n + d + 1)
+    labels[7] = 3
+    feat[7] *= size
+    best = int((feat[7].double() @ weight.double().T).argmax())
+    rest = [i for i in range(n) if i != 7]
+    check_rows(feat, weight, labels, dloss, rows=rest,
+               vertices=[i for i in range(v) if i not in (3, best)])
+
+
+@pytest.mark.parametrize("n, v, d", SIZES)
+def test_float32_one_table_row_of_another_size(n, v, d):
+    # a large row that no sample comes near: its features point away from it
+    feat, weight, labels, dloss = t.xent_inputs(n, v, d, "float32", n + d + 2)
+    feat[:, 0] = 1.0 + feat[:, 0].abs()
+    weight[9, 0] = -2.0 ** 24
+    labels[labels == 9] = 10
+    weight[11] *= 2.0 ** -30
+    labels[0] = 11
+    check_rows(feat, weight, labels, dloss)
+
+
+@pytest.mark.parametrize("n, v, d", SIZES)
+@pytest.mark.parametrize("size", [100.0, 1e3, 1e6, 1e-6])
+def test_float32_lse_of_ignored_rows_is_theirs(n, v, d, size):
+    feat, weight, labels, dloss = t.xent_inputs(n, v, d, "float32", n + d + 3)
+    labels[4] = labels[20] = -100
+    feat[4] *= size
+    check_rows(feat, weight, labels, dloss)
+
+
+@pytest.mark.parametrize("size", [1e-6, 1e-5, 1e5, 1e6])
+def test_float32_lse_where_every_row_is_ignored(size):
+    feat, weight, labels, dloss = t.xent_inputs(70, 333, 48, "float32", 4)
+    labels.fill_(-100)
+    got = check_rows(feat * size, weight / size, labels, dloss)
+    assert not got["loss"].any() and not got["feat_grad"].any() and not got["weight_grad"].any()
+
+
+@pytest.mark.parametrize("n, v, d", SIZES)
+@pytest.mark.parametrize("scale", [1.0, -0.5])
+def test_float32_minus_infinity_in_table_rows(n, v, d, scale):
+    # such a vertex has probability 0: losses, the table's gradient and (but for the columns that
+    # hold an infinity, where 0 times it is NaN) the features' are those of the other vertices
+    feat, weight, labels, dloss = t.xent_inputs(n, v, d, "float32", n + d + 5)
+    feat[:, 0] = feat[:, 2] = math.copysign(1.0, scale)
+    gone = [5, 130, v - 1]
+    for row in gone:
+        labels[labels == row] = 6
+    kept = [i for i in range(v) if i not in gone]
+    place = torch.zeros(v, dtype=torch.int64, device="cuda")
+    place[kept] = torch.arange(len(kept), device="cuda")
+    small = torch.where(labels == -100, labels, place[labels.clamp(min=0)])
+    want = by_rows(feat, weight[kept], small, dloss, scale)
+    weight[5, 0] = weight[130, 2] = -math.inf
+    weight[v - 1, 0] = weight[v - 1, 2] = -math.inf
+    got = run(t.xent_module(feat, weight, labels, scale=scale), feat, weight, labels, dloss)
+    for key in ("loss", "lse"):
+        t.check(got[key], *want[key], torch.float32)
+    t.check(got["weight_grad"][kept], *want["weight_grad"], torch.float32)
+    assert not got["weight_grad"][gone].any()
+    cols = [c for c in range(d) if c not in (0, 2)]
+    t.check(got["feat_grad"][:, cols], want["feat_grad"][0][:, cols], want["feat_grad"][1][:, cols],
+            torch.float32)
+    dead = labels == -100
+    assert got["feat_grad"][~dead][:, [0, 2]].isnan().all() and not got["feat_grad"][dead].any()
+
+
+def test_float32_infinities_and_nan_stay_in_their_samples():
+    # a sample with an infinity or a NaN is NaN itself; a NaN in the table is everybody's
+    feat, weight, labels, dloss = t.xent_inputs(140, 300, 72, "float32", 21)
+    labels[3] = labels[4] = 8
+    clean = {k: x.clone() for k, x in run(t.xent_module(feat, weight, labels), feat, weight, labels,
+                                          dloss).items()}
+    feat[3, 5], feat[4, 70] = math.inf, math.nan
+    got = run(t.xent_module(feat, weight, labels), feat, weight, labels, dloss)
+    rest = [i for i in range(140) if i not in (3, 4)]
+    for key in ("loss", "lse", "feat_grad"):
+        assert got[key][[3, 4]].isnan().all() and torch.equal(got[key][rest], clean[key][rest])
+    assert got["weight_grad"].isnan().all()
+    labels[3] = labels[4] = -100
+    got = run(t.xent_module(feat, weight, labels), feat, weight, labels, dloss)
+    assert got["lse"][[3, 4]].isnan().all() and not got["weight_grad"].isnan().any()
+    weight[290, 1] = math.nan
+    got = run(t.xent_module(feat, weight, labels), feat, weight, labels, dloss)
+    assert got["lse"].isnan().all()
+
+
+def test_float32_loss_gradients_of_any_size():
+    # each sample's weight is its own: a large one takes nothing from the others' gradients
+    feat, weight, labels, dloss = t.xent_inputs(200, 500, 64, "float32", 22)
+    labels[9] = 17
+    dloss[9] = 1e9
+    feat[9] = 0.0
+    feat[9, 0] = 1.0
+    for row in (30, 31):
+        dloss[row] = 1e-12
+    want = by_rows(feat, weight, labels, dloss)
+    got = run(t.xent_module(feat, weight, labels), feat, weight, labels, dloss)
+    t.check(got["feat_grad"], *want["feat_grad"], torch.float32)
+    # the large sample has one feature only: the table's other columns are the others' alone
+    value, bound = want["weight_grad"]
+    t.check(got["weight_grad"], value, bound, torch.float32)
