@@ -1207,7 +1207,10 @@ join_loss_kernel(Batch b, const T* __restrict__ feat, int64_t feat_ld, const T* 
     *status = FG_STATUS_BAD_INDEX;
     loss[t] = __int_as_float(0x7fc00000);
   } else {
-    loss[t] = l - z * b.scale;
+    // not below zero: l is a sum that the tensor cores have cut, z one in another order, and where
+    // the label has all the probability their difference is the rounding of either sign
+    const float d = l - z * b.scale;
+    loss[t] = d < 0.f ? 0.f : d;
   }
 }
 

@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 
+from featgraph_b200 import _lib
 import test_training_ops_gpu as t
 
 pytestmark = pytest.mark.gpu
@@ -197,3 +198,22 @@ def test_float32_loss_gradients_of_any_size():
     # the large sample has one feature only: the table's other columns are the others' alone
     value, bound = want["weight_grad"]
     t.check(got["weight_grad"], value, bound, torch.float32)
+
+
+# ------------------------------------------------------------ losses below zero --
+@pytest.mark.parametrize("dtype", sorted(t.TYPES))
+@pytest.mark.parametrize("n, v, d, size", [(3000, 40, 64, 3.0), (600, 2000, 100, 2.0)])
+def test_no_loss_is_below_zero(dtype, n, v, d, size):
+    # samples that point at their own label's row: lse and the label's logit agree to the last bits
+    g = t.gen(n)
+    weight = torch.randn((v, d), generator=g, device="cuda").to(t.TYPES[dtype])
+    labels = torch.randint(v, (n,), generator=g, device="cuda")
+    feat = (weight[labels].float() * size).to(weight.dtype)
+    m = t.xent_module(feat, weight, labels)
+    loss = m.run([feat, weight, labels])[0].torch
+    assert not loss.isnan().any() and (loss >= 0).all() and (loss == 0).any()
+    labels[5] = v
+    loss = m.run([feat, weight, labels])[0].torch
+    assert loss[5].isnan() and int(loss.isnan().sum()) == 1
+    with pytest.raises(_lib.FeatGraphError, match="out of range"):
+        m.device_status()
