@@ -118,6 +118,9 @@ __device__ __forceinline__ void store_vec_stream(T* p, const Vec<T, N>& v) {
   __stcs(reinterpret_cast<typename Vec<T, N>::Raw*>(p), v.raw);
 }
 
+// Sets the status word; an expired wait, the larger code, is not hidden by an index out of range.
+__device__ __forceinline__ void report(int32_t* status, int32_t code) { atomicMax(status, code); }
+
 #endif  // __CUDACC__
 
 // CALL(T) for the element type `dtype`, already checked with dtype_known.

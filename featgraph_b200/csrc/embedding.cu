@@ -50,7 +50,7 @@ lookup_kernel(const T* __restrict__ table, int64_t table_ld, int64_t n_vertices,
     for (int u = 0; u < kLookupRows; ++u) {
       const bool in = first + u < n_ids;
       ok[u] = in && (uint64_t)(int64_t)id[u] < (uint64_t)n_vertices;
-      if (in && !ok[u] && lane == 0) *status = FG_STATUS_BAD_INDEX;
+      if (in && !ok[u] && lane == 0) report(status, FG_STATUS_BAD_INDEX);
       from[u] = id[u] * table_ld;
       id[u] = first + stride + u < n_ids ? load_id<I>(ids, first + stride + u) : 0;
     }
@@ -99,7 +99,7 @@ __device__ __forceinline__ uint2 make_pair(const KeySource& s, S id, int64_t i) 
     const int64_t v = id;
     uint32_t key = (uint32_t)v;
     if ((uint64_t)v >= (uint64_t)s.n_vertices) {
-      *s.status = FG_STATUS_BAD_INDEX;
+      report(s.status, FG_STATUS_BAD_INDEX);
       key = (uint32_t)s.n_vertices;
     } else if (v == s.padding) {
       key = (uint32_t)s.n_vertices;

@@ -385,7 +385,7 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
         }
       }
       if (!ok) {  // give up only once nothing is in flight into this CTA's shared memory
-        *a.status = FG_STATUS_WAIT_EXPIRED;
+        report(a.status, FG_STATUS_WAIT_EXPIRED);
         if (!STREAM) tc::bar_wait(rows_full, it & 1);
         for (uint32_t k = 0; k < min(loaded, (uint32_t)a.slots); ++k) {
           // the slots behind `slot.at` belong to the round before
@@ -527,7 +527,7 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
     }
     // the last barrier arrivals of the tensor cores land before this CTA's memory is freed
     tc::mma_commit(leader, drained);
-    if (!warp_wait(drained, 0) || !ok) *a.status = FG_STATUS_WAIT_EXPIRED;
+    if (!warp_wait(drained, 0) || !ok) report(a.status, FG_STATUS_WAIT_EXPIRED);
   } else if (warp >= kEpilogueWarp) {
     const int group = (warp - kEpilogueWarp) >> 2;
     const int quarter = warp & 3;                         // TMEM lanes 32 * quarter ...
@@ -1011,7 +1011,7 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
         tc::bar_arrive(out_empty);
       }
     }
-    if (!ok && lane == 0) *a.status = FG_STATUS_WAIT_EXPIRED;
+    if (!ok && lane == 0) report(a.status, FG_STATUS_WAIT_EXPIRED);
   }
   __syncwarp();
   tc::fence_before();
@@ -1204,7 +1204,7 @@ join_loss_kernel(Batch b, const T* __restrict__ feat, int64_t feat_ld, const T* 
   if (y == b.ignore_index) {
     loss[t] = 0.f;
   } else if ((uint64_t)y >= (uint64_t)b.vocab) {
-    *status = FG_STATUS_BAD_INDEX;
+    report(status, FG_STATUS_BAD_INDEX);
     loss[t] = __int_as_float(0x7fc00000);
   } else {
     // not below zero: l is a sum that the tensor cores have cut, z one in another order, and where

@@ -362,7 +362,7 @@ int fg_sddmm_describe(int64_t nnz, int32_t feat_len, int32_t num_heads,
  * overlap need two of them.  status_dev is an int32 that the caller zeroed: a kernel that
  * meets an id or a label out of range sets it (FG_STATUS_BAD_INDEX) and reads nothing
  * there; a kernel one of whose bounded waits gave up sets FG_STATUS_WAIT_EXPIRED, and the
- * call's results are then not to be used. */
+ * call's results are then not to be used.  The word keeps the larger code. */
 enum fg_dtype { FG_FLOAT32 = 0, FG_BFLOAT16 = 1, FG_FLOAT16 = 2 };
 enum fg_index_type { FG_INDEX_INT32 = 0, FG_INDEX_INT64 = 1 };
 enum { FG_STATUS_BAD_INDEX = 1, FG_STATUS_WAIT_EXPIRED = 2 };

@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from featgraph_b200 import _lib
+from featgraph_b200 import _lib, module
 import test_training_ops_gpu as t
 
 pytestmark = pytest.mark.gpu
@@ -217,3 +217,28 @@ def test_no_loss_is_below_zero(dtype, n, v, d, size):
     assert loss[5].isnan() and int(loss.isnan().sum()) == 1
     with pytest.raises(_lib.FeatGraphError, match="out of range"):
         m.device_status()
+
+
+# ------------------------------------------------------------------ the status word --
+def test_an_expired_wait_is_not_hidden_by_an_index_out_of_range():
+    # the word as a kernel leaves it that gave up a wait; every later call meets a bad index
+    table = torch.randn((10, 8), device="cuda")
+    bad = torch.tensor([3, 10, -1], device="cuda")
+    many = torch.full((9000,), 10, device="cuda")
+    e, big, c = (module.EmbeddingLookupcuda(), module.EmbeddingLookupcuda(),
+                 module.SoftmaxCrossEntropycuda())
+    e.build(t.like(table, bad), {"with_grad": True}, {})
+    big.build(t.like(table, many), {"with_grad": True}, {})
+    c.build(t.like(table[:3], table, bad), {"with_grad": True}, {})
+    loss = torch.zeros(3, device="cuda")
+    calls = [(e, lambda: e.run([table, bad])),
+             (e, lambda: e.run_grad([table[:3], bad])),
+             (big, lambda: big.run_grad([torch.ones((9000, 8), device="cuda"), many])),
+             (c, lambda: c.run([table[:3], table, bad])),
+             (c, lambda: c.run_grad([loss, table[:3], table, bad, loss]))]
+    for m, call in calls:
+        m._status.fill_(2)
+        call()
+        with pytest.raises(_lib.FeatGraphError, match="bounded wait"):
+            m.device_status()
+        assert m.device_status() == 0
