@@ -12,7 +12,7 @@ CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(CSRC, "libfeatgraph_b200.so")
 SOURCES = ["api.cu", "spmm.cu", "spmm_noalloc.cu", "sddmm.cu", "peer.cu",
            "embedding.cu", "xent.cu", "clip.cu"]
-HEADERS = ["common.cuh", "elem.cuh", "tensor.cuh", os.path.join("..", "..", "include", "featgraph_b200.h")]
+HEADERS = ["common.cuh", "elem.cuh", "ring.cuh", "tensor.cuh", os.path.join("..", "..", "include", "featgraph_b200.h")]
 
 NVCC_FLAGS = [
     "-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",

@@ -30,6 +30,7 @@
 #include <type_traits>
 
 #include "elem.cuh"
+#include "ring.cuh"
 #include "tensor.cuh"
 
 namespace fg {
@@ -193,17 +194,6 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
   return __all_sync(0xffffffffu, tc::bar_wait(bar, parity));
 }
 
-// A place in a ring of `n` slots or buffers and the parity of its current round.
-struct Place {
-  uint32_t at = 0, parity = 0;
-  __device__ __forceinline__ void next(uint32_t n) {
-    if (++at == n) {
-      at = 0;
-      parity ^= 1;
-    }
-  }
-};
-
 // What one item of a CTA's work is: a tile of the rows, a range of steps over the streamed
 // operand, and (for the gradients of wide rows) a piece of the results' columns.  Row tiles run
 // fastest: CTAs beside each other stream the same part.
@@ -314,6 +304,7 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
   if (warp == 0) {
     if (lane == 0) {
       Place slot;
+      Loads rows;                       // of the rows that stay
       uint32_t loaded = 0, it = 0;
       bool ok = tmem_where == tmem;
       // the next slot, free, with `n` tiles announced; 0 if the wait expired
@@ -340,6 +331,7 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
           tc::bar_expect(rows_full, tiles * kTileBytes);
           for (int q = 0; q < tiles; ++q)
             tc::load_tile(rows_at + q * kTileBytes, &row_map, q * 64, row0, rows_full);
+          ++rows.issued;
           for (int j = 0; ok && j < item.steps; ++j)
             for (int q = 0; q < tiles; ++q) {
               const uint32_t to = next_slot(Shape::kCols / 128);
@@ -386,12 +378,9 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
       }
       if (!ok) {  // give up only once nothing is in flight into this CTA's shared memory
         report(a.status, FG_STATUS_WAIT_EXPIRED);
-        if (!STREAM) tc::bar_wait(rows_full, it & 1);
-        for (uint32_t k = 0; k < min(loaded, (uint32_t)a.slots); ++k) {
-          // the slots behind `slot.at` belong to the round before
-          const uint32_t round = k < slot.at ? slot.parity : slot.parity ^ 1;
-          tc::bar_wait(full + 8 * k, round);
-        }
+        if (rows.any()) tc::bar_wait(rows_full, rows.last_parity());
+        for (uint32_t k = 0; k < min(loaded, (uint32_t)a.slots); ++k)
+          tc::bar_wait(full + 8 * k, last_round(slot, k));
       }
     }
   } else if (warp == 1) {
