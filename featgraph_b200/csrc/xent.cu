@@ -47,11 +47,14 @@ struct Batch {
   int64_t n, vocab, feat_len, ignore_index;
   float scale;
 };
-// The row's label, -1 if it takes no part.
-__device__ __forceinline__ int32_t live_label(const Batch& b, int64_t t) {
+// The row's label, -1 if it takes no part; `status`: reports one out of range.
+__device__ __forceinline__ int32_t live_label(const Batch& b, int64_t t, int32_t* status = nullptr) {
   if (t >= b.n) return -1;
   const int64_t y = load_label(b.labels, b.wide, t);
-  return y != b.ignore_index && (uint64_t)y < (uint64_t)b.vocab ? (int32_t)y : -1;
+  if (y == b.ignore_index) return -1;
+  if ((uint64_t)y < (uint64_t)b.vocab) return (int32_t)y;
+  if (status) report(status, FG_STATUS_BAD_INDEX);
+  return -1;
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -1039,10 +1042,11 @@ struct SampleArrays {
   int32_t* label;
   int64_t padded;
   float hot;
+  int32_t* status;
 };
 __device__ __forceinline__ void sample(const Batch& b, const SampleArrays& s, float inv_weight_max,
                                        int64_t t) {
-  const int32_t y = live_label(b, t);
+  const int32_t y = live_label(b, t, s.status);
   float bias = -INFINITY, weight = 0.f, g = 0.f;
   if (y >= 0) {
     g = s.loss_grad[t];
@@ -1515,7 +1519,7 @@ int grad_mma(const Batch& b, const XentLayout& l, char* ws, const float* loss_gr
                                reinterpret_cast<float*>(ws + l.row_factor),
                                reinterpret_cast<float*>(ws + l.col_bias),
                                reinterpret_cast<float*>(ws + l.col_weight),
-                               reinterpret_cast<int32_t*>(ws + l.label), l.padded, hot};
+                               reinterpret_cast<int32_t*>(ws + l.label), l.padded, hot, status};
   Operands o;
   bool chained = false;
   if (int rc = prepare_operands<T>(b, l, ws, feat, feat_ld, weight, weight_ld, dtype, arrays, s, &o, &chained))

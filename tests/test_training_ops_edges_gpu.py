@@ -242,3 +242,18 @@ def test_an_expired_wait_is_not_hidden_by_an_index_out_of_range():
         with pytest.raises(_lib.FeatGraphError, match="bounded wait"):
             m.device_status()
         assert m.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype, n", [("float32", 40), ("bfloat16", 40), ("float16", 9000)])
+def test_gradient_call_reports_a_label_out_of_range(dtype, n):
+    # both ways in which the samples' arrays are made: beside the packing, and (many) by themselves
+    feat, weight, labels, dloss = t.xent_inputs(n, 30, 16, dtype, 3)
+    m = t.xent_module(feat, weight, labels)
+    lse = m.run([feat, weight, labels])[1]
+    m.run_grad([dloss, feat, weight, labels, lse])
+    assert m.device_status() == 0                        # ignore_index is in range
+    for wrong in (30, -1):
+        labels[7] = wrong
+        m.run_grad([dloss, feat, weight, labels, lse])
+        with pytest.raises(_lib.FeatGraphError, match="out of range"):
+            m.device_status()
