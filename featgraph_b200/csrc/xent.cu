@@ -912,17 +912,20 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
           if ((step & 1) != group) continue;
           const int64_t col0 = (int64_t)(item.first + j) * Shape::kCols;
           // weight_grad: lane c holds columns c, 32 + c, ... of the step; in `hits` those whose
-          // label is one of this warp's rows, in `negative` those of a negative weight
+          // label is one of this warp's rows, in `negative` those of a negative weight, in `none`
+          // those that take no part: zeros, which meet an infinity of this lane's row as NaN
           int32_t col_label[4];
           float col_weight[4];
-          uint32_t hits[4] = {0, 0, 0, 0}, negative[4] = {0, 0, 0, 0};
+          uint32_t hits[4] = {0, 0, 0, 0}, negative[4] = {0, 0, 0, 0}, none[4] = {0, 0, 0, 0};
           if (MODE == kWeightGrad) {
             __syncwarp();
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               col_label[c] = a.col_label[col0 + c * 32 + lane];
               col_weight[c] = a.col_weight[col0 + c * 32 + lane];
-              my_biases[c * 32 + lane] = a.col_bias[col0 + c * 32 + lane];
+              const float col_bias = a.col_bias[col0 + c * 32 + lane];
+              my_biases[c * 32 + lane] = col_bias;
+              none[c] = __ballot_sync(0xffffffffu, col_bias == -INFINITY);
             }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -936,12 +939,14 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
           tc::fence_after();
           const uint32_t s_at = lanes_at + tmem + at.at * Shape::kCols;
           float x[2][32];
+          bool not_finite = false;   // a row that holds an infinity or a NaN has no finite logit
           tc::tmem_load32(s_at, x[0]);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             float(&v)[32] = x[c & 1];
             tc::wait_ld32(v);
             if (c < 3) tc::tmem_load32(s_at + (c + 1) * 32, x[(c + 1) & 1]);
+            if (MODE == kWeightGrad && c == 0) not_finite = __any_sync(0xffffffffu, !(fabsf(v[0]) < INFINITY));
             if (MODE == kFeatGrad) {
 #pragma unroll
               for (int k = 0; k < 32; ++k) v[k] = exp2_fast(fmaf(v[k], scale, bias));
@@ -964,6 +969,11 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
                 v[k + 1] = exp2_fast(fmaf(v[k + 1], scale, e.y));
                 v[k + 2] = exp2_fast(fmaf(v[k + 2], scale, e.z));
                 v[k + 3] = exp2_fast(fmaf(v[k + 3], scale, e.w));
+              }
+              if (not_finite && none[c]) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k)
+                  if (none[c] >> k & 1) v[k] = 0.f;
               }
               if (negative[c]) {
 #pragma unroll

@@ -257,3 +257,28 @@ def test_gradient_call_reports_a_label_out_of_range(dtype, n):
         m.run_grad([dloss, feat, weight, labels, lse])
         with pytest.raises(_lib.FeatGraphError, match="out of range"):
             m.device_status()
+
+
+# --------------------------------------- 16 bits: minus infinity in table rows --
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("n, v, d", [(40, 300, 16), (300, 90, 72), (70, 500, 320)])
+def test_16_bit_minus_infinity_leaves_the_tables_gradient_alone(dtype, n, v, d):
+    # ignored rows, and those behind the last one, meet the infinity as zeros
+    feat, weight, labels, dloss = t.xent_inputs(n, v, d, dtype, 9)
+    feat[:, 0] = 1.0
+    gone = [5, v - 1]
+    for row in gone:
+        labels[labels == row] = 6
+    labels[3] = -100
+    kept = [i for i in range(v) if i not in gone]
+    place = torch.zeros(v, dtype=torch.int64, device="cuda")
+    place[kept] = torch.arange(len(kept), device="cuda")
+    small = torch.where(labels == -100, labels, place[labels.clamp(min=0)])
+    want = t.xent_reference(feat, weight[kept], small, 1.0, -100, dloss)
+    weight[5, 0] = weight[v - 1, 0] = -math.inf
+    got = run(t.xent_module(feat, weight, labels), feat, weight, labels, dloss)
+    t.check(got["loss"], *want["loss"], torch.float32)
+    assert not got["weight_grad"][gone].any()
+    t.check(got["weight_grad"][kept], *want["weight_grad"], feat.dtype)
+    value, bound = want["feat_grad"]
+    t.check(got["feat_grad"][:, 1:], value[:, 1:], bound[:, 1:], feat.dtype)
