@@ -20,6 +20,7 @@ import torch
 from . import te
 from .module import (EmbeddingLookupcuda, GradientClipcuda, SoftmaxCrossEntropycuda,
                      VanillaSpMMcuda)
+from .runtime import NDArray
 
 
 class HostPair(object):
@@ -102,7 +103,8 @@ class VertexPrediction(object):
         x = self.lookup.run([table, ids])
         y = self.forward.run([x])
         losses, lse = self.loss.run([y, table, labels])
-        live = (labels != self.ignore_index).to(torch.float32)
+        wanted = labels.torch if isinstance(labels, NDArray) else labels
+        live = (wanted != self.ignore_index).to(torch.float32)
         share = live / live.sum().clamp(min=1.0)
         y_grad, grad = self.loss.run_grad([share, y, table, labels, lse])
         x_grad = self.backward.run([y_grad])

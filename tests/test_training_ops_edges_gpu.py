@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from featgraph_b200 import _lib, module
+from featgraph_b200 import _lib, module, nd
 import test_training_ops_gpu as t
 
 pytestmark = pytest.mark.gpu
@@ -282,3 +282,23 @@ def test_16_bit_minus_infinity_leaves_the_tables_gradient_alone(dtype, n, v, d):
     t.check(got["weight_grad"][kept], *want["weight_grad"], feat.dtype)
     value, bound = want["feat_grad"]
     t.check(got["feat_grad"][:, 1:], value[:, 1:], bound[:, 1:], feat.dtype)
+
+
+# ---------------------------------------------------------------- the whole step --
+def test_vertex_prediction_takes_arrays_of_the_framework():
+    from helpers import random_csr
+    from featgraph_b200.pipeline import VertexPrediction
+    v, f, n, cols = 120, 16, 50, 90
+    step = VertexPrediction(random_csr(n, cols, 0.1, seed=4), v, f, max_norm=0.2)
+    g = t.gen(8)
+    table = torch.randn((v, f), generator=g, device="cuda")
+    ids = torch.randint(v, (cols,), generator=g, device="cuda")
+    labels = torch.randint(v, (n,), generator=g, device="cuda")
+    labels[::5] = -100
+
+    def copy(out):
+        loss, norm, grad = out
+        return [x.torch.clone() if isinstance(x, nd.NDArray) else x.clone() for x in (loss, norm, grad)]
+    want = copy(step.run(table, ids, labels))
+    got = copy(step.run(nd.NDArray(table), nd.NDArray(ids), nd.NDArray(labels)))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
