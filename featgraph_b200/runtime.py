@@ -94,8 +94,10 @@ class NDArray(object):
         return str(self._t.dtype).replace("torch.", "")
 
     def asnumpy(self):
-        """Blocking copy to a new host array (synchronises the producing stream)."""
-        return self._t.detach().cpu().numpy()
+        """Blocking copy to a new host array (synchronises the producing stream); bfloat16, which
+        numpy lacks, as float32."""
+        t = self._t.detach().cpu()
+        return (t.float() if t.dtype == torch.bfloat16 else t).numpy()
 
     def copyfrom(self, source):
         src = source.torch if isinstance(source, NDArray) else torch.as_tensor(np.asarray(source))
