@@ -978,7 +978,9 @@ GradLayout grad_layout(int64_t n, int64_t n_vertices, int64_t feat_len) {
 }
 
 int check_common(const void* values, const void* ids, const int32_t* status, int32_t dtype,
-                 int32_t index_type, int64_t n_vertices, int64_t n_ids, int64_t feat_len) {
+                 int32_t index_type, int64_t n_vertices, int64_t n_ids, int64_t feat_len, float scale) {
+  if (!std::isfinite(scale))
+    return fail(FG_ERR_INVALID_ARGUMENT, "scale=%g is not finite", (double)scale);
   if (!dtype_known(dtype) || !index_known(index_type))
     return fail(FG_ERR_INVALID_ARGUMENT, "unknown dtype=%d or index_type=%d", (int)dtype,
                 (int)index_type);
@@ -1004,7 +1006,7 @@ extern "C" int fg_embedding_lookup(const void* table_dev, int32_t dtype, int64_t
                                    void* stream) {
   using namespace fg;
   if (int rc = check_common(out_dev, ids_dev, status_dev, dtype, index_type, n_vertices, n_ids,
-                            feat_len))
+                            feat_len, scale))
     return rc;
   if (table_ld < feat_len || out_ld < feat_len)
     return fail(FG_ERR_INVALID_ARGUMENT, "a row pitch is shorter than feat_len=%lld",
@@ -1065,7 +1067,7 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
                                  int32_t* status_dev, int32_t device, void* stream) {
   using namespace fg;
   if (int rc = check_common(out_grad_dev, ids_dev, status_dev, dtype, index_type, n_vertices,
-                            n_ids, feat_len))
+                            n_ids, feat_len, scale))
     return rc;
   if (out_grad_ld < feat_len)
     return fail(FG_ERR_INVALID_ARGUMENT, "a row pitch is shorter than feat_len=%lld",

@@ -33,6 +33,14 @@ def _finite(x, what):
     return x
 
 
+def _finite32(x, what):
+    """A number that reaches the kernels as float32."""
+    x = _finite(x, what)
+    if abs(x) >= 2.0 ** 128 - 2.0 ** 103:      # rounds to infinity there
+        raise ValueError("%s must be finite as float32, got %r" % (what, x))
+    return x
+
+
 def embedding_lookup(Table, Ids, scale=1.0, padding_idx=None, with_grad=False):
     """Out[i, f] = scale * Table[Ids[i], f], rounded once to the table's type.
 
@@ -51,7 +59,7 @@ def embedding_lookup(Table, Ids, scale=1.0, padding_idx=None, with_grad=False):
                              % (padding_idx, Table.shape[0]))
     return ComputeSpec("embedding_lookup", (Ids.shape[0], Table.shape[1]), Table.dtype,
                        (Table, Ids),
-                       {"scale": _finite(scale, "scale"), "padding_idx": padding_idx,
+                       {"scale": _finite32(scale, "scale"), "padding_idx": padding_idx,
                         "with_grad": bool(with_grad), "num_vertices": Table.shape[0],
                         "feat_len": Table.shape[1]})
 
@@ -79,9 +87,12 @@ def softmax_cross_entropy(Feat, Weight, Labels, scale=1.0, ignore_index=-100, wi
     assert Feat.shape[0] == Labels.shape[0], "dimension mismatch"
     if Weight.shape[0] < 1:
         raise ValueError("Weight needs at least one row")
+    ignore_index = int(ignore_index)
+    if not -2 ** 63 <= ignore_index < 2 ** 63:
+        raise ValueError("ignore_index %d does not fit 64 bits" % ignore_index)
     return ComputeSpec("softmax_cross_entropy", (Feat.shape[0],), "float32",
                        (Feat, Weight, Labels),
-                       {"scale": _finite(scale, "scale"), "ignore_index": int(ignore_index),
+                       {"scale": _finite32(scale, "scale"), "ignore_index": ignore_index,
                         "with_grad": bool(with_grad), "vocab": Weight.shape[0],
                         "feat_len": Feat.shape[1]})
 

@@ -357,7 +357,7 @@ int fg_sddmm_describe(int64_t nnz, int32_t feat_len, int32_t num_heads,
  * README.md:6 leaves the layers around its kernels to the caller).
  *
  * Rows are row-major with the last dimension contiguous; a *_ld is the distance between
- * two rows in elements.  All calls are asynchronous on `stream`, allocate nothing and keep
+ * two rows in elements.  A scale is finite.  All calls are asynchronous on `stream`, allocate nothing and keep
  * nothing between calls; the workspace is scratch of the call's own, so two calls that may
  * overlap need two of them.  status_dev is an int32 that the caller zeroed: a kernel that
  * meets an id or a label out of range sets it (FG_STATUS_BAD_INDEX) and reads nothing
