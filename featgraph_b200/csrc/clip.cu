@@ -9,6 +9,8 @@
 // tensors take 146 us, 1.02 GB at 7 TB/s with what L2 still holds of the first reading.
 #include <algorithm>
 #include <cmath>
+#include <memory>
+#include <new>
 
 #include "elem.cuh"
 
@@ -240,6 +242,33 @@ int run_clip(const ClipCall& call, cudaStream_t s) {
   return FG_OK;
 }
 
+// Whether an output shares memory with another output or with an input other than its own (which it
+// may be itself, but not in part).  `spans` has room for n_tensors.
+struct Span {
+  uint64_t begin, end;
+  int32_t tensor;
+};
+bool outputs_overlap(const ClipCall& call, Span* spans) {
+  int32_t n = 0;
+  for (int32_t k = 0; k < call.n_tensors; ++k) {
+    const uint64_t bytes = (uint64_t)call.sizes[k] * dtype_size(call.dtypes[k]);
+    const uint64_t at = (uint64_t)(uintptr_t)call.outs[k];
+    if (bytes > 0) spans[n++] = {at, at + bytes, k};
+  }
+  std::sort(spans, spans + n, [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  for (int32_t i = 1; i < n; ++i)
+    if (spans[i].begin < spans[i - 1].end) return true;
+  for (int32_t k = 0; k < call.n_tensors; ++k) {
+    const uint64_t bytes = (uint64_t)call.sizes[k] * dtype_size(call.dtypes[k]);
+    const uint64_t at = (uint64_t)(uintptr_t)call.grads[k];
+    if (bytes == 0 || call.grads[k] == call.outs[k]) continue;
+    // the first output that ends behind the input's begin
+    const Span* hit = std::lower_bound(spans, spans + n, at, [](const Span& s, uint64_t v) { return s.end <= v; });
+    if (hit != spans + n && hit->begin < at + bytes) return true;
+  }
+  return false;
+}
+
 }  // namespace
 }  // namespace fg
 
@@ -281,10 +310,18 @@ extern "C" int fg_gradient_clip(const void* const* grads_host_array, void* const
   if (all_chunks > INT32_MAX)
     return fail(FG_ERR_UNSUPPORTED, "%lld chunks of %d elements are too many",
                 (long long)all_chunks, kClipChunk);
-  DeviceGuard guard(device);
-  FG_CUDA_TRY(guard.status);
   const ClipCall call = {grads_host_array, outs_host_array, sizes_host_array, dtypes_host_array, n_tensors,
                          max_abs_norm != 0, max_norm, eps, norm_dev, static_cast<double*>(workspace_dev)};
+  Span some[kManyTensors];
+  std::unique_ptr<Span[]> more;
+  if (n_tensors > kManyTensors) {
+    more.reset(new (std::nothrow) Span[n_tensors]);
+    if (!more) return fail(FG_ERR_OUT_OF_MEMORY, "no host memory for %d tensors", (int)n_tensors);
+  }
+  if (outputs_overlap(call, more ? more.get() : some))
+    return fail(FG_ERR_INVALID_ARGUMENT, "an output shares memory with another tensor than its own input");
+  DeviceGuard guard(device);
+  FG_CUDA_TRY(guard.status);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return n_tensors <= kFewTensors ? run_clip<ClipTensors<kFewTensors>>(call, s)
                                   : run_clip<ClipTensors<kManyTensors>>(call, s);

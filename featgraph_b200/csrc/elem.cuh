@@ -23,6 +23,30 @@ inline int common_vector_bytes(std::initializer_list<uint64_t> things) {
   return (int)(all & (~all + 1));
 }
 
+// An array of a call: rows of `width` elements, `ld` from one to the next.  `overlap`: whether two
+// have a byte in common.  A kernel reads its inputs while it writes, in no order, so an output that
+// is also an input is refused.
+struct Array2d {
+  const void* at;
+  int64_t rows, width, ld;
+  size_t element;
+};
+inline bool overlap(const Array2d& a, const Array2d& b) {
+  if (!a.at || !b.at || a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+  typedef __int128 Wide;   // a product of the sizes may pass 64 bits
+  const Wide a0 = (Wide)(uintptr_t)a.at, b0 = (Wide)(uintptr_t)b.at;
+  const Wide a1 = a0 + ((Wide)(a.rows - 1) * a.ld + a.width) * (Wide)a.element;
+  const Wide b1 = b0 + ((Wide)(b.rows - 1) * b.ld + b.width) * (Wide)b.element;
+  if (a1 <= b0 || b1 <= a0) return false;
+  // columns of one array side by side
+  const Wide pitch = (Wide)(a.rows > 1 ? a.ld * (Wide)a.element : b.ld * (Wide)b.element);
+  if (a.rows > 1 && b.rows > 1 && (Wide)b.ld * (Wide)b.element != pitch) return true;
+  if (a.rows == 1 && b.rows == 1) return true;
+  const Wide apart = ((b0 - a0) % pitch + pitch) % pitch;   // where b's rows begin in a's pitch
+  return !(apart >= (Wide)a.width * (Wide)a.element && apart + (Wide)b.width * (Wide)b.element <= pitch);
+}
+inline Array2d array1d(const void* at, int64_t n, size_t element) { return {at, n > 0 ? 1 : 0, n, n, element}; }
+
 #ifdef __CUDACC__
 
 template <typename T>

@@ -1013,6 +1013,10 @@ extern "C" int fg_embedding_lookup(const void* table_dev, int32_t dtype, int64_t
                 (long long)feat_len);
   if (n_ids == 0) return FG_OK;
   if (n_vertices > 0 && !table_dev) return fail(FG_ERR_INVALID_ARGUMENT, "null table");
+  const Array2d out_array = {out_dev, n_ids, feat_len, out_ld, dtype_size(dtype)};
+  if (overlap(out_array, {table_dev, n_vertices, feat_len, table_ld, dtype_size(dtype)}) ||
+      overlap(out_array, array1d(ids_dev, n_ids, index_type == FG_INDEX_INT64 ? 8 : 4)))
+    return fail(FG_ERR_INVALID_ARGUMENT, "out shares memory with an input");
   DeviceGuard guard(device);
   FG_CUDA_TRY(guard.status);
   const size_t es = dtype_size(dtype);
@@ -1082,9 +1086,13 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
                     ((uintptr_t)workspace_dev & 15) != 0))
     return fail(FG_ERR_INVALID_ARGUMENT, "the workspace needs %lld bytes at a 16-byte boundary",
                 (long long)l.total);
+  const size_t es = dtype_size(dtype);
+  const Array2d grad_array = {grad_dev, n_vertices, feat_len, feat_len, es};
+  if (overlap(grad_array, {out_grad_dev, n_ids, feat_len, out_grad_ld, es}) ||
+      overlap(grad_array, array1d(ids_dev, n_ids, index_type == FG_INDEX_INT64 ? 8 : 4)))
+    return fail(FG_ERR_INVALID_ARGUMENT, "the gradient shares memory with an input");
   DeviceGuard guard(device);
   FG_CUDA_TRY(guard.status);
-  const size_t es = dtype_size(dtype);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int vb = common_vector_bytes({(uint64_t)(uintptr_t)out_grad_dev,
                                       (uint64_t)(uintptr_t)grad_dev, (uint64_t)(out_grad_ld * es),

@@ -1371,6 +1371,17 @@ int check_xent(const void* feat, const void* weight, int32_t dtype, int64_t feat
   return FG_OK;
 }
 
+// Whether one of the results shares memory with one of the inputs or another result.
+bool results_overlap(std::initializer_list<Array2d> results, std::initializer_list<Array2d> inputs) {
+  for (const Array2d* r = results.begin(); r != results.end(); ++r) {
+    for (const Array2d& in : inputs)
+      if (overlap(*r, in)) return true;
+    for (const Array2d* q = results.begin(); q != r; ++q)
+      if (overlap(*r, *q)) return true;
+  }
+  return false;
+}
+
 // The operands of one call as the tensor maps need them.
 struct Operands {
   const void *feat, *weight;
@@ -1597,6 +1608,11 @@ extern "C" int fg_softmax_xent(const void* feat_dev, int64_t feat_ld, const void
   if (!workspace_dev || ((uintptr_t)workspace_dev & 255) != 0 || workspace_bytes < (int64_t)l.total)
     return fail(FG_ERR_INVALID_ARGUMENT, "the workspace needs %lld bytes at a 256-byte boundary",
                 (long long)l.total);
+  const size_t es = dtype_size(dtype);
+  if (results_overlap({array1d(loss_dev, n, 4), array1d(lse_dev, n, 4)},
+                      {{feat_dev, n, feat_len, feat_ld, es}, {weight_dev, vocab, feat_len, weight_ld, es},
+                       array1d(labels_dev, n, index_type == FG_INDEX_INT64 ? 8 : 4)}))
+    return fail(FG_ERR_INVALID_ARGUMENT, "a result shares memory with an input or the other one");
   DeviceGuard guard(device);
   FG_CUDA_TRY(guard.status);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -1634,6 +1650,12 @@ extern "C" int fg_softmax_xent_grad(const float* loss_grad_dev, const void* feat
     if (!workspace_dev || ((uintptr_t)workspace_dev & 255) != 0 || workspace_bytes < need)
       return fail(FG_ERR_INVALID_ARGUMENT, "the workspace needs %lld bytes at a 256-byte boundary",
                   (long long)need);
+    const size_t es = dtype_size(dtype);
+    if (results_overlap({{feat_grad_dev, n, feat_len, feat_len, es}, {weight_grad_dev, vocab, feat_len, feat_len, es}},
+                        {{feat_dev, n, feat_len, feat_ld, es}, {weight_dev, vocab, feat_len, weight_ld, es},
+                         array1d(labels_dev, n, index_type == FG_INDEX_INT64 ? 8 : 4),
+                         array1d(loss_grad_dev, n, 4), array1d(lse_dev, n, 4)}))
+      return fail(FG_ERR_INVALID_ARGUMENT, "a result shares memory with an input or the other one");
   }
   DeviceGuard guard(device);
   FG_CUDA_TRY(guard.status);

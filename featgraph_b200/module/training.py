@@ -4,7 +4,9 @@ arrays every call): the vertex embedding lookup that feeds an SpMM, the softmax 
 that reads its output, and the gradient clip before the optimiser.  The reference has no
 counterpart (python/featgraph/module/__init__.py:1-2).
 
-A module's outputs and workspace are shared state: one call at a time per module.  A call on
+A module's outputs and workspace are shared state: one call at a time per module.  Its outputs
+are not its inputs: an array that shares memory with one is refused (a gradient clip takes the
+array that it writes to as its own input).  A call on
 another stream than the module's last one waits for that one first; while a stream is being
 captured nothing is waited for, so two graphs that hold calls of one module must not be
 replayed side by side.
@@ -141,6 +143,15 @@ class _TrainingOp(object):
                                  "strides %r" % (what, t.stride()))
         return t
 
+    @staticmethod
+    def _meet(a, b):
+        """Whether two tensors have memory in common (rows that lie apart count with their gaps)."""
+        def span(t):
+            last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
+            return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+        (a0, a1), (b0, b1) = span(a), span(b)
+        return a0 < b1 and b0 < a1
+
     def _rows(self, x, expected):
         """``_tensor`` and the distance between its rows in elements."""
         t = self._tensor(x, expected)
@@ -244,7 +255,7 @@ class EmbeddingLookupcuda(_TrainingOp):
             result, grad = self.grad_tvm, self.grad_tvm.torch
         else:
             result, grad = accumulate_into, self._tensor(accumulate_into, self._into)
-            if grad.untyped_storage().data_ptr() == dy.untyped_storage().data_ptr():
+            if self._meet(grad, dy):
                 raise ValueError("OutGrad and accumulate_into share memory")
         n, vertices, feat_len, scale = self._sizes
         code = self._call(_lib.OP_LOOKUP_GRAD, _LOOKUP_GRAD.pack(

@@ -357,7 +357,8 @@ int fg_sddmm_describe(int64_t nnz, int32_t feat_len, int32_t num_heads,
  * README.md:6 leaves the layers around its kernels to the caller).
  *
  * Rows are row-major with the last dimension contiguous; a *_ld is the distance between
- * two rows in elements.  A scale is finite.  All calls are asynchronous on `stream`, allocate nothing and keep
+ * two rows in elements.  A scale is finite.  A result that shares memory with an input or with
+ * another result is refused, but for the two uses that say so (accumulate, and clipping in place).  All calls are asynchronous on `stream`, allocate nothing and keep
  * nothing between calls; the workspace is scratch of the call's own, so two calls that may
  * overlap need two of them.  status_dev is an int32 that the caller zeroed: a kernel that
  * meets an id or a label out of range sets it (FG_STATUS_BAD_INDEX) and reads nothing
@@ -427,8 +428,7 @@ int fg_softmax_xent_grad(const float* loss_grad_dev, const void* feat_dev, int64
  *   norm = sqrt of the sum of all squares, or, with max_abs_norm != 0, the largest magnitude;
  *   out_k = grad_k * min(1, max_norm / (norm + eps)),
  * the norm summed in fp64 from fp32 pieces in a fixed order.  outs[k] may be grads[k] (in
- * place: then nothing is written when nothing has to be scaled), else the two do not
- * overlap.  The four arrays are host memory and are read before the call returns.  A NaN
+ * place: then nothing is written when nothing has to be scaled), else it overlaps no tensor.  The four arrays are host memory and are read before the call returns.  A NaN
  * norm makes every output NaN, an infinite one scales by zero, max_norm = +inf scales by 1. */
 int64_t fg_gradient_clip_workspace_bytes(int32_t n_tensors);
 int fg_gradient_clip(const void* const* grads_host_array, void* const* outs_host_array,

@@ -302,3 +302,30 @@ def test_vertex_prediction_takes_arrays_of_the_framework():
     want = copy(step.run(table, ids, labels))
     got = copy(step.run(nd.NDArray(table), nd.NDArray(ids), nd.NDArray(labels)))
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+# ---------------------------------------------------------- outputs as inputs --
+def test_modules_refuse_their_outputs_as_inputs():
+    table = torch.randn((6, 8), device="cuda")
+    ids = torch.tensor([5, 0, 3, 3, 1, 2], device="cuda")
+    e = module.EmbeddingLookupcuda()
+    e.build(t.like(table, ids), {"with_grad": True}, {})
+    out = e.run([table, ids])
+    with pytest.raises(_lib.FeatGraphError, match="shares memory"):
+        e.run([out, ids])
+    with pytest.raises(_lib.FeatGraphError, match="shares memory"):
+        e.run_grad([e.grad_tvm, ids])
+    # two parts of one storage are two arrays
+    both = torch.ones((12, 8), device="cuda")
+    assert e.run_grad([both[:6], ids], accumulate_into=both[6:]) is not None
+    assert torch.equal(both[:6], torch.ones((6, 8), device="cuda"))
+    assert both[6:, 0].tolist() == [2, 2, 2, 3, 1, 2]
+    k = module.GradientClipcuda()
+    grads = [torch.ones(50, device="cuda"), torch.full((50,), 2.0, device="cuda")]
+    k.build(t.like(*grads), {"max_norm": 1.0}, {})
+    _, clipped = k.run(grads)
+    with pytest.raises(_lib.FeatGraphError, match="shares memory"):
+        k.run([clipped[1], clipped[0]])
+    once = [x.torch.clone() for x in clipped]
+    _, again = k.run(clipped)                            # each its own: clipped once more
+    assert all(torch.allclose(a, b.torch) for a, b in zip(once, again))

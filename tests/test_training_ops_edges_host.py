@@ -54,3 +54,92 @@ def test_the_lookups_c_calls_refuse_a_scale_that_is_not_finite(lib):
                                              None), 1, "finite")
         refused(lib, lib.fg_embedding_grad(some, 0, 8, some, 0, 5, 10, 8, scale, -1, 0, some, some,
                                            1 << 20, some, 0, None), 1, "finite")
+
+
+# ------------------------------------------------- results that share memory with an input --
+# Addresses that are never read: every call below is refused before a launch.
+def at(x):
+    return ctypes.c_void_p(x)
+
+
+BASE, FAR = 1 << 20, 1 << 24
+
+
+def lookup(lib, table, ld, ids, out, out_ld, v=10, n=5, f=8):
+    return lib.fg_embedding_lookup(at(table), 0, ld, v, at(ids), 1, n, f, 1.0, at(out), out_ld,
+                                   at(FAR * 4), 99, None)
+
+
+def test_a_lookup_over_its_own_input_is_refused(lib):
+    table = 10 * 8 * 4
+    for out in (BASE, BASE + table - 32, BASE - 5 * 32 + 32):
+        refused(lib, lookup(lib, BASE, 8, FAR, out, 8), 1, "shares memory")
+    refused(lib, lookup(lib, FAR, 8, BASE, BASE + 32, 8), 1, "shares memory")          # the ids
+    # beside each other, also as columns of one array: the next check is the device's
+    for args in ((BASE, 8, FAR, BASE + table, 8), (BASE, 8, FAR, BASE - 5 * 32, 8),
+                 (BASE, 24, FAR, BASE + 32, 24), (BASE, 24, FAR, BASE + 64, 24)):
+        assert lookup(lib, *args) == 2
+    for args in ((BASE, 24, FAR, BASE + 28, 24), (BASE, 24, FAR, BASE + 68, 24),
+                 (BASE, 24, FAR, BASE + 32, 16)):
+        refused(lib, lookup(lib, *args), 1, "shares memory")
+
+
+def test_a_lookup_gradient_over_its_own_input_is_refused(lib):
+    def call(dy, ids, grad):
+        return lib.fg_embedding_grad(at(dy), 0, 8, at(ids), 1, 5, 10, 8, 1.0, -1, 0, at(grad), at(FAR * 2),
+                                     1 << 20, at(FAR * 4), 99, None)
+    for dy in (BASE, BASE + 320 - 4, BASE - 160 + 4):
+        refused(lib, call(dy, FAR, BASE), 1, "shares memory")
+    refused(lib, call(FAR, BASE + 8, BASE), 1, "shares memory")
+    assert call(BASE + 320, FAR, BASE) == 2
+
+
+def test_a_cross_entropy_over_its_own_input_is_refused(lib):
+    n, v, d = 5, 10, 8
+    need = lib.fg_softmax_xent_workspace_bytes(0, n, v, d, 1)
+    good = dict(feat=BASE, weight=BASE + 4096, labels=BASE + 8192, loss=BASE + 12288, lse=BASE + 16384,
+                dl=BASE + 20480, dh=BASE + 24576, dw=BASE + 28672)
+
+    def loss(**change):
+        a = dict(good, **change)
+        return lib.fg_softmax_xent(at(a["feat"]), d, at(a["weight"]), d, 0, at(a["labels"]), 1, n, v, d, 1.0,
+                                   -100, at(a["loss"]), at(a["lse"]), at(FAR), need, at(FAR * 2), 99, None)
+
+    def grad(**change):
+        a = dict(good, **change)
+        return lib.fg_softmax_xent_grad(at(a["dl"]), at(a["feat"]), d, at(a["weight"]), d, 0, at(a["labels"]),
+                                        1, n, v, d, 1.0, -100, at(a["lse"]), at(a["dh"]), at(a["dw"]), at(FAR),
+                                        need, at(FAR * 2), 99, None)
+    assert loss() == 2 and grad() == 2
+    for out in ("loss", "lse"):
+        for inp in ("feat", "weight", "labels"):
+            refused(lib, loss(**{out: good[inp]}), 1, "shares memory")
+    refused(lib, loss(loss=good["lse"]), 1, "shares memory")
+    for out in ("dh", "dw"):
+        for inp in ("feat", "weight", "labels", "dl", "lse"):
+            refused(lib, grad(**{out: good[inp] - 4 * (out == "dw")}), 1, "shares memory")
+    refused(lib, grad(dh=good["dw"]), 1, "shares memory")
+    assert grad(dl=good["lse"]) == 2                     # inputs may be one array
+
+
+@pytest.mark.parametrize("count", [3, 700])              # more than a launch's list too
+def test_clipping_over_another_tensor_is_refused(lib, count):
+    need = lib.fg_gradient_clip_workspace_bytes(count)
+
+    def call(ins, outs, sizes):
+        p = ctypes.c_void_p * count
+        return lib.fg_gradient_clip(p(*ins), p(*outs), (ctypes.c_int64 * count)(*sizes),
+                                    (ctypes.c_int32 * count)(), count, 0, 1.0, 0.0, at(FAR * 4), at(FAR * 2),
+                                    need, 99, None)
+    ins = [BASE + 400 * k for k in range(count)]
+    outs = [FAR + 400 * k for k in range(count)]
+    sizes = [100] * count
+    assert call(ins, outs, sizes) == 2 and call(ins, ins, sizes) == 2
+    swapped = outs[:]
+    swapped[0], swapped[1] = swapped[1], swapped[0]
+    refused(lib, call(outs, swapped, sizes), 1, "shares memory")       # each the other's input
+    refused(lib, call(ins, [outs[0]] * 2 + outs[2:], sizes), 1, "shares memory")
+    refused(lib, call(ins, [ins[0] + 4] + outs[1:], sizes), 1, "shares memory")   # its own in part
+    refused(lib, call([ins[1]] + ins[1:], [outs[0]] + ins[1:], sizes), 1, "shares memory")
+    assert call([ins[0]] * count, outs, sizes) == 2                    # inputs may be one array
+    assert call(ins, [outs[0]] * 2 + outs[2:], [100, 0] + sizes[2:]) == 2    # empty: nowhere
