@@ -82,6 +82,7 @@ struct DeviceGuard {
       status = cudaSetDevice(device);
       changed = (status == cudaSuccess);
     }
+    if (status != cudaSuccess) (void)cudaGetLastError();  // returned here, not to a later call
   }
   ~DeviceGuard() {
     if (changed) cudaSetDevice(prev);

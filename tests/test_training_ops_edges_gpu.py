@@ -329,3 +329,20 @@ def test_modules_refuse_their_outputs_as_inputs():
     once = [x.torch.clone() for x in clipped]
     _, again = k.run(clipped)                            # each its own: clipped once more
     assert all(torch.allclose(a, b.torch) for a, b in zip(once, again))
+
+
+def test_a_device_that_is_not_there_leaves_no_error_behind():
+    lib = _lib.load()
+    table = torch.randn((6, 8), device="cuda")
+    ids = torch.tensor([5, 0, 3], device="cuda")
+    out = torch.empty((3, 8), device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+
+    def call(device):
+        return lib.fg_embedding_lookup(table.data_ptr(), 0, 8, 6, ids.data_ptr(), 1, 3, 8, 1.0,
+                                       out.data_ptr(), 8, status.data_ptr(), device, None)
+    assert call(99) == 2 and "ordinal" in lib.fg_last_error_string().decode()
+    assert call(0) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(out, table[ids])
