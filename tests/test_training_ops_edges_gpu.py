@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from featgraph_b200 import _lib, module, nd
+from featgraph_b200 import _lib, module, nd, te
 import test_training_ops_gpu as t
 
 pytestmark = pytest.mark.gpu
@@ -346,3 +346,80 @@ def test_a_device_that_is_not_there_leaves_no_error_behind():
     assert call(0) == 0
     torch.cuda.synchronize()
     assert torch.equal(out, table[ids])
+
+
+# --------------------------------- the table's gradient of more ids than one launch takes --
+# 8193 ids and more are sorted; runs of more than 64 rows are cut into windows, those of more than
+# 32 parts joined by a whole CTA (60 000 ids of three vertices).
+MANY = [(8193, 300, 12), (9001, 97, 20), (30000, 11, 33), (60000, 3, 72)]
+
+
+@pytest.mark.parametrize("dtype", sorted(t.TYPES))
+@pytest.mark.parametrize("index", ["int32", "int64"])
+@pytest.mark.parametrize("n, v, f", MANY)
+def test_sorted_gradient_padding_accumulate_and_strides(dtype, index, n, v, f):
+    g = t.gen(n)
+    ids = t.make_ids("skewed", n, v, g).to(getattr(torch, index))
+    wide = torch.randn((n, f + 30), generator=g, device="cuda").to(t.TYPES[dtype])
+    dy = wide[:, 10:10 + f]
+    often = int(torch.bincount(ids.long()).argmax())
+    for padding in (None, often, v - 1):
+        m = module.EmbeddingLookupcuda()
+        m.build([te.placeholder((v, f), dtype)] + t.like(ids),
+                {"scale": 0.5, "padding_idx": padding, "with_grad": True}, {})
+        m.grad_tvm.torch.fill_(math.nan)
+        got = m.run_grad([dy, ids]).torch
+        t.check(got, *t.grad_reference(dy, ids, v, 0.5, padding), dy.dtype)
+        before = torch.randn((v, f), generator=g, device="cuda").to(t.TYPES[dtype])
+        into = before.clone()
+        assert m.run_grad([dy, ids], accumulate_into=into) is into
+        t.check(into, *t.grad_reference(dy, ids, v, 0.5, padding, before), dy.dtype)
+        if padding is not None:
+            assert not got[padding].any() and torch.equal(into[padding], before[padding])
+        again = before.clone()
+        m.run_grad([dy, ids], accumulate_into=again)
+        assert torch.equal(again, into) and m.device_status() == 0
+
+
+@pytest.mark.parametrize("index", ["int32", "int64"])
+@pytest.mark.parametrize("n, v, f", MANY)
+@pytest.mark.parametrize("wrong", [1, 63, 64, 700, 5000])
+def test_sorted_gradient_of_ids_out_of_range(index, n, v, f, wrong):
+    g = t.gen(n + wrong)
+    ids = t.make_ids("skewed", n, v, g).to(getattr(torch, index))
+    dy = torch.randn((n, f), generator=g, device="cuda")
+    at = torch.randperm(n, generator=g, device="cuda")[:wrong]
+    values = torch.tensor([v, -1, 2 ** 31 - 1, -2 ** 31], device="cuda")
+    bad = ids.clone()
+    bad[at] = values[torch.arange(wrong, device="cuda") % 4].to(bad.dtype)
+    dy[at] = math.nan                                  # and nothing of theirs is added
+    m = module.EmbeddingLookupcuda()
+    m.build([te.placeholder((v, f), "float32")] + t.like(ids), {"with_grad": True}, {})
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[at] = False
+    want, bound = t.grad_reference(dy[keep], ids[keep], v, 1.0)
+    t.check(m.run_grad([dy, bad]).torch, want, bound, torch.float32)
+    with pytest.raises(_lib.FeatGraphError, match="out of range"):
+        m.device_status()
+    before = torch.randn((v, f), generator=g, device="cuda")
+    into = before.clone()
+    m.run_grad([dy, bad], accumulate_into=into)
+    t.check(into, *t.grad_reference(dy[keep], ids[keep], v, 1.0, None, before), torch.float32)
+
+
+@pytest.mark.parametrize("dtype", sorted(t.TYPES))
+@pytest.mark.parametrize("n, v, d", [(20000, 41, 40), (40000, 300, 24), (140000, 41, 16)])
+def test_cross_entropy_of_many_samples_and_few_classes(dtype, n, v, d):
+    # the table's gradient of a class is a sum over every sample
+    feat, weight, labels, dloss = t.xent_inputs(n, v, d, dtype, n)
+    t.xent_check(t.xent_module(feat, weight, labels), feat, weight, labels, dloss)
+
+
+@pytest.mark.parametrize("dtype", sorted(t.TYPES))
+def test_cross_entropy_sums_of_one_sign(dtype):
+    # Nothing cancels in the gradients' sums, so that what the tensor cores cut adds up: features
+    # and weights of one sign.  At most 8192 additions go into one accumulator, each cut by at most
+    # 2^-23 of the sum in the worst case (the bound of xent_reference counts every term so).
+    feat, weight, labels, dloss = t.xent_inputs(30000, 70, 32, dtype, 5, spread=0.5)
+    feat, weight = feat.abs(), weight.abs()
+    t.xent_check(t.xent_module(feat, weight, labels), feat, weight, labels, dloss)
