@@ -1091,13 +1091,26 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
   if (overlap(grad_array, {out_grad_dev, n_ids, feat_len, out_grad_ld, es}) ||
       overlap(grad_array, array1d(ids_dev, n_ids, index_type == FG_INDEX_INT64 ? 8 : 4)))
     return fail(FG_ERR_INVALID_ARGUMENT, "the gradient shares memory with an input");
-  DeviceGuard guard(device);
-  FG_CUDA_TRY(guard.status);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int vb = common_vector_bytes({(uint64_t)(uintptr_t)out_grad_dev,
                                       (uint64_t)(uintptr_t)grad_dev, (uint64_t)(out_grad_ld * es),
                                       (uint64_t)(feat_len * es)});
   if (vb < (int)es) return fail(FG_ERR_INVALID_ARGUMENT, "a pointer is not aligned to its type");
+  // the launch shape of the sums; refused before anything is launched.  Few ids: slabs of 256 bytes
+  // where the rows allow 16-byte accesses, so that a popular vertex of long rows is the work of
+  // several CTAs
+  const int per_row = (int)((feat_len * es + vb - 1) / vb);
+  const int log_lanes = l.few ? std::min(vb == 16 ? 4 : 5, ceil_log2(per_row))
+                              : std::max(ceil_log2(kSumLeastLanes), std::min(5, ceil_log2(per_row)));
+  const int64_t slabs = (per_row + (1 << log_lanes) - 1) >> log_lanes;
+  const int64_t pieces = (n_ids + kSumPiece - 1) / kSumPiece;
+  const int64_t window_blocks = (l.windows + kSumWarps - 1) / kSumWarps;
+  const int64_t blocks_x = window_blocks + ((pieces << log_lanes) + kSumThreads - 1) / kSumThreads;
+  if (n_ids > 0 && (blocks_x > INT32_MAX || slabs > 65535))
+    return fail(FG_ERR_UNSUPPORTED, "n_ids=%lld x feat_len=%lld is too large", (long long)n_ids,
+                (long long)feat_len);
+  DeviceGuard guard(device);
+  FG_CUDA_TRY(guard.status);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
   const ZeroFill zero = {static_cast<uint8_t*>(grad_dev),
                          accumulate ? 0 : (int64_t)((size_t)n_vertices * feat_len * es)};
   if (n_ids == 0) {
@@ -1117,13 +1130,7 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
   float* partial = reinterpret_cast<float*>(ws + l.partial);
   KeySource src = {ids_dev, n_vertices, padding_id < 0 ? -1 : padding_id, status_dev};
   const bool wide = index_type == FG_INDEX_INT64;
-  const int per_row = (int)((feat_len * es + vb - 1) / vb);
   if (l.few) {
-    // slabs of 256 bytes where the rows allow 16-byte accesses: a popular vertex of long rows is
-    // then the work of several CTAs
-    const int log_lanes = std::min(vb == 16 ? 4 : 5, ceil_log2(per_row));
-    const int64_t slabs = (per_row + (1 << log_lanes) - 1) >> log_lanes;
-    if (slabs > 65535) return fail(FG_ERR_UNSUPPORTED, "feat_len is too large");
     const size_t smem = slice_shared_bytes(n_ids);
     const dim3 grid(kSlices, (unsigned)slabs);
 #define FG_SLICE(T, N)                                                                             \
@@ -1165,13 +1172,6 @@ extern "C" int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_
     src.from = pairs[pass & 1];
   }
   const Runs runs = {static_cast<const uint2*>(src.from), n_ids, (uint32_t)n_vertices};
-  const int log_lanes = std::max(ceil_log2(kSumLeastLanes), std::min(5, ceil_log2(per_row)));
-  const int64_t slabs = (per_row + (1 << log_lanes) - 1) >> log_lanes;
-  const int64_t pieces = (n_ids + kSumPiece - 1) / kSumPiece;
-  const int64_t window_blocks = (l.windows + kSumWarps - 1) / kSumWarps;
-  const int64_t blocks_x = window_blocks + ((pieces << log_lanes) + kSumThreads - 1) / kSumThreads;
-  if (blocks_x > INT32_MAX || slabs > 65535)
-    return fail(FG_ERR_UNSUPPORTED, "n_ids x feat_len is too large");
   const dim3 grid((unsigned)blocks_x, (unsigned)slabs);
 #define FG_SUM(T, N)                                                                             \
   FG_CUDA_TRY(launch(true, sum_kernel<T, N>, grid, kSumThreads, 0, s, runs, (int)l.windows,      \

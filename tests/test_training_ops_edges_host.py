@@ -143,3 +143,12 @@ def test_clipping_over_another_tensor_is_refused(lib, count):
     refused(lib, call([ins[1]] + ins[1:], [outs[0]] + ins[1:], sizes), 1, "shares memory")
     assert call([ins[0]] * count, outs, sizes) == 2                    # inputs may be one array
     assert call(ins, [outs[0]] * 2 + outs[2:], [100, 0] + sizes[2:]) == 2    # empty: nowhere
+
+
+@pytest.mark.parametrize("n", [100, 9000])               # both forms of the gradient
+def test_a_gradient_of_rows_too_long_is_refused_before_any_launch(lib, n):
+    f = 1 << 24
+    big = 1 << 44                                        # apart by more than the arrays' size
+    args = (at(big), 0, f, at(2 * big), 1, n, 10, f, 1.0, -1, 0, at(3 * big), at(4 * big), 1 << 44, at(FAR),
+            99, None)
+    refused(lib, lib.fg_embedding_grad(*args), 3, "too large")
