@@ -142,9 +142,12 @@ TRAINING = {"lookup": _lookup_case, "lookup-grad": _lookup_case,
 
 def _run_training(args, g, source, device):
     """The --kernel choices of TRAINING: one JSON line per feature length."""
+    if g.nnz < 1 or g.n_rows < 1:
+        raise SystemExit("--kernel %s draws its vertices from the graph's edges: there are none"
+                         % args.kernel)
     dtype = getattr(torch, args.dtype)
     gen = torch.Generator(device="cpu").manual_seed(graphs.FEAT_SEED)
-    draws = torch.randint(max(g.nnz, 1), (args.samples,), generator=gen)
+    draws = torch.randint(g.nnz, (args.samples,), generator=gen)
     ids = g.indices[draws.to(device)].to(torch.int32)
     labels = torch.randint(g.n_cols, (args.samples,), generator=gen).to(torch.int32).to(device)
     records = []
@@ -205,6 +208,8 @@ def main(argv=None):
     args = ap.parse_args(argv)
     if args.target != "cuda":
         raise SystemExit("this backend ships the cuda target only (no x86 code path)")
+    if args.kernel in TRAINING and args.samples < 1:
+        raise SystemExit("--samples must be at least 1")
 
     rank = int(os.environ.get("RANK", "0"))
     world = int(os.environ.get("WORLD_SIZE", "1"))

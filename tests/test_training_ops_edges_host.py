@@ -152,3 +152,17 @@ def test_a_gradient_of_rows_too_long_is_refused_before_any_launch(lib, n):
     args = (at(big), 0, f, at(2 * big), 1, n, 10, f, 1.0, -1, 0, at(3 * big), at(4 * big), 1 << 44, at(FAR),
             99, None)
     refused(lib, lib.fg_embedding_grad(*args), 3, "too large")
+
+
+# ------------------------------------------------------------------------ the command --
+@pytest.mark.parametrize("kernel", ["lookup", "lookup-grad", "cross-entropy", "clip", "train-step"])
+def test_the_command_refuses_an_empty_batch_and_a_graph_without_edges(kernel):
+    import types
+    from featgraph_b200 import bench_cli
+    for samples in ("0", "-3"):
+        with pytest.raises(SystemExit, match="at least 1"):
+            bench_cli.main(["--kernel", kernel, "--samples", samples])
+    args = types.SimpleNamespace(kernel=kernel, dtype="float32", samples=3, feat_len="8")
+    empty = types.SimpleNamespace(nnz=0, n_rows=5, n_cols=5, indices=torch.empty(0, dtype=torch.int32))
+    with pytest.raises(SystemExit, match="there are none"):
+        bench_cli._run_training(args, empty, "empty", torch.device("cpu"))
