@@ -27,6 +27,7 @@
 // products; the operands are read from DRAM once.
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <type_traits>
 
 #include "elem.cuh"
@@ -1475,7 +1476,7 @@ int launch_mma_as(const Batch& b, const XentLayout& l, const Operands& o, const 
   a.out_cols = l.out_cols;
   a.negate = b.scale < 0.f;
   a.out_vec = common_vector_bytes({(uint64_t)(uintptr_t)a.out, (uint64_t)b.feat_len * sizeof(T)});
-  a.logit_scale = std::fabs(b.scale) * kLog2e;
+  a.logit_scale = std::min(std::fabs(b.scale) * kLog2e, std::numeric_limits<float>::max());
   // shared memory: 14 tiles of 16 KB at most, 13 where what belongs to columns needs some of it
   const int room = Shape::kColArrays > 0 ? 13 : 14;
   const int resident = STREAM ? 0 : l.tiles;

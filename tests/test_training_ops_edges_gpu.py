@@ -423,3 +423,51 @@ def test_cross_entropy_sums_of_one_sign(dtype):
     feat, weight, labels, dloss = t.xent_inputs(30000, 70, 32, dtype, 5, spread=0.5)
     feat, weight = feat.abs(), weight.abs()
     t.xent_check(t.xent_module(feat, weight, labels), feat, weight, labels, dloss)
+
+
+@pytest.mark.parametrize("dtype", sorted(t.TYPES))
+@pytest.mark.parametrize("scale", [3e38, -3e38])
+def test_the_largest_scales_leave_zero_logits_zero(dtype, scale):
+    # |scale| log2(e) is beyond float32
+    feat = torch.zeros((40, 16), device="cuda", dtype=t.TYPES[dtype])
+    weight = torch.randn((300, 16), device="cuda").to(feat.dtype)
+    labels = torch.arange(40, device="cuda")
+    m = t.xent_module(feat, weight, labels, scale=scale)
+    loss, lse = m.run([feat, weight, labels])
+    want = math.log(300)
+    assert (loss.torch - want).abs().max() <= 400 * U and (lse.torch - want).abs().max() <= 400 * U
+
+
+# --------------------------------------------------------------- graphs and streams --
+def test_vertex_prediction_captured_and_on_another_stream():
+    from helpers import random_csr
+    from featgraph_b200.pipeline import VertexPrediction
+    v, f, n, cols = 200, 24, 60, 110
+    step = VertexPrediction(random_csr(n, cols, 0.1, seed=6, empty_rows=(2,)), v, f, scale=1.5, max_norm=0.3)
+
+    def inputs(seed):
+        g = t.gen(seed)
+        labels = torch.randint(v, (n,), generator=g, device="cuda")
+        labels[::4] = -100
+        return [torch.randn((v, f), generator=g, device="cuda"),
+                torch.randint(v, (cols,), generator=g, device="cuda"), labels]
+
+    def values(out):
+        return [out[0].clone(), out[1].torch.clone(), out[2].torch.clone()]
+    first, second = inputs(1), inputs(2)
+    want = [values(step.run(*x)) for x in (first, second)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = values(step.run(*first))
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want[0], got))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step.run(*first)
+    for x, y in zip(first, second):
+        x.copy_(y)
+    for _ in range(2):
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(want[1], values(out)))
+    assert all(torch.equal(a, b) for a, b in zip(want[1], values(step.run(*second))))
