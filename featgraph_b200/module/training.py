@@ -7,9 +7,11 @@ counterpart (python/featgraph/module/__init__.py:1-2).
 A module's outputs and workspace are shared state: one call at a time per module.  Its outputs
 are not its inputs: an array that shares memory with one is refused (a gradient clip takes the
 array that it writes to as its own input).  A call on
-another stream than the module's last one waits for that one first; while a stream is being
-captured nothing is waited for, so two graphs that hold calls of one module must not be
-replayed side by side.
+another stream than the module's last one waits for that one first.  While a stream is being
+captured nothing is waited for, and of a graph's replays a module knows nothing: two graphs that
+hold calls of one module must not be replayed side by side, nor a replay beside a call of the
+module on another stream, and a module that a graph holds calls of stays alive, and is not built
+again, until the graph is gone (its outputs and workspace are the module's memory).
 """
 import array
 import math
@@ -93,8 +95,9 @@ class _TrainingOp(object):
         return handle
 
     def _change_stream(self, handle):
-        if torch.cuda.is_current_stream_capturing():
-            return
+        with torch.cuda.device(self._device):       # whose current stream the handle is
+            if torch.cuda.is_current_stream_capturing():
+                return
         stream = torch.cuda.current_stream(self._device)
         stream.wait_stream(self._last_stream)
         for t in self._owned:
