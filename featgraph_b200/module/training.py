@@ -10,8 +10,8 @@ array that it writes to as its own input).  A call on
 another stream than the module's last one waits for that one first.  While a stream is being
 captured nothing is waited for, and of a graph's replays a module knows nothing: two graphs that
 hold calls of one module must not be replayed side by side, nor a replay beside a call of the
-module on another stream, and a module that a graph holds calls of stays alive, and is not built
-again, until the graph is gone (its outputs and workspace are the module's memory).
+module on another stream, and a module that a graph holds calls of stays alive until the graph is
+gone (its outputs and workspace are the module's memory; building the module again keeps them).
 """
 import array
 import math
@@ -51,6 +51,7 @@ class _TrainingOp(object):
         self._device = self._ctx.torch_device
         self._index = self._ctx.device_id
         self._spec = None
+        self._owned, self._captured, self._of_graphs = [], False, []
         self.out_tvm = None
 
     def _specialise(self, input_placeholders, compute_args, schedule_args):
@@ -61,7 +62,9 @@ class _TrainingOp(object):
         """Fix the static shapes; allocate the outputs and the workspace."""
         out, _ = self._specialise(input_placeholders, compute_args, schedule_args)
         self._spec = None
-        self._owned = []
+        if self._captured:
+            self._of_graphs.append(self._owned)     # replays still write there
+        self._owned, self._captured = [], False
         self._status = self._own(torch.zeros(1, dtype=torch.int32, device=self._device))
         self._allocate(out)
         size = max(self._workspace_bytes(out), 16)
@@ -90,14 +93,21 @@ class _TrainingOp(object):
     def _stream(self):
         """The current stream's handle, ordered behind the module's last call."""
         handle = torch._C._cuda_getCurrentRawStream(self._index)
+        if handle:                                  # 0: the default stream, which nothing captures
+            self._captured = self._captured or self._is_capturing()
         if handle != self._last_handle:
             self._change_stream(handle)
         return handle
 
-    def _change_stream(self, handle):
+    def _is_capturing(self):
+        if torch._C._cuda_getDevice() == self._index:
+            return torch._C._cuda_isCurrentStreamCapturing()
         with torch.cuda.device(self._device):       # whose current stream the handle is
-            if torch.cuda.is_current_stream_capturing():
-                return
+            return torch.cuda.is_current_stream_capturing()
+
+    def _change_stream(self, handle):
+        if handle and self._is_capturing():
+            return
         stream = torch.cuda.current_stream(self._device)
         stream.wait_stream(self._last_stream)
         for t in self._owned:

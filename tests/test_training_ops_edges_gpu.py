@@ -471,3 +471,31 @@ def test_vertex_prediction_captured_and_on_another_stream():
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(want[1], values(out)))
     assert all(torch.equal(a, b) for a, b in zip(want[1], values(step.run(*second))))
+
+
+@pytest.mark.parametrize("warm_up_there", [False, True])
+def test_a_graph_outlives_the_build_that_it_was_captured_with(warm_up_there):
+    feat, weight, labels, dloss = t.xent_inputs(60, 300, 32, "float32", 3)
+    m = t.xent_module(feat, weight, labels)
+    want = [x.clone() for x in run(m, feat, weight, labels, dloss).values()]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    if warm_up_there:                                  # the module's last stream is the captured one
+        with torch.cuda.stream(stream):
+            run(m, feat, weight, labels, dloss)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        outs = list(run(m, feat, weight, labels, dloss).values())
+    small = [x[:5] for x in (feat, weight, labels, dloss)]
+    small[2] = torch.tensor([0, 1, 2, 3, 4], device="cuda")
+    m.build(t.like(small[0], small[1], small[2]), {"with_grad": True}, {})
+    # what the allocator has left over goes to others now
+    others = [torch.full((size,), 7, dtype=torch.uint8, device="cuda")
+              for size in (512, 4096, 40000, 1 << 18, 1 << 20) for _ in range(40)]
+    for x in outs:
+        x.zero_()
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(want, outs))
+    assert all(bool((x == 7).all()) for x in others)
+    t.check(run(m, *small)["loss"], *t.xent_reference(*small[:3], 1.0, -100)["loss"], torch.float32)
