@@ -1297,7 +1297,7 @@ struct XentLayout {
   Cut loss, feat, weight;
   size_t consts, feat_mul, weight_mul, packed_feat, packed_weight;
   size_t stats, row_bias, row_factor, col_bias, col_weight, label, partial;
-  size_t total;
+  size_t total, total_in_place;
 };
 
 XentLayout xent_layout(int32_t dtype, int64_t n, int64_t vocab, int64_t feat_len, bool with_grad) {
@@ -1330,7 +1330,6 @@ XentLayout xent_layout(int32_t dtype, int64_t n, int64_t vocab, int64_t feat_len
     l.weight_mul = take((size_t)vocab * 4);
   }
   l.packed_feat = take((size_t)n * l.pitch * 2);
-  l.packed_weight = take((size_t)vocab * l.pitch * 2);
   l.stats = take((size_t)n * l.loss.splits * kLossGroups * sizeof(float2));
   if (with_grad) {
     l.row_bias = take((size_t)l.padded * 4);
@@ -1343,6 +1342,9 @@ XentLayout xent_layout(int32_t dtype, int64_t n, int64_t vocab, int64_t feat_len
     if (l.weight.splits > 1) rows = std::max(rows, (size_t)l.weight.splits * vocab);
     l.partial = take(rows * l.out_cols * 4);
   }
+  // last: a table that is read where it lies needs no room for it
+  l.total_in_place = at;
+  l.packed_weight = take((size_t)vocab * l.pitch * 2);
   l.total = at;
   return l;
 }
@@ -1589,7 +1591,8 @@ int grad_mma(const Batch& b, const XentLayout& l, char* ws, const float* loss_gr
 extern "C" int64_t fg_softmax_xent_workspace_bytes(int32_t dtype, int64_t n, int64_t vocab,
                                                    int64_t feat_len, int32_t with_grad) {
   if (n <= 0 || vocab < 1 || feat_len < 1) return 0;
-  return (int64_t)fg::xent_layout(dtype, n, vocab, feat_len, with_grad != 0).total;
+  const fg::XentLayout l = fg::xent_layout(dtype, n, vocab, feat_len, (with_grad & 1) != 0);
+  return (int64_t)((with_grad & FG_XENT_TABLE_IN_PLACE) && dtype != FG_FLOAT32 ? l.total_in_place : l.total);
 }
 
 extern "C" int fg_softmax_xent(const void* feat_dev, int64_t feat_ld, const void* weight_dev,
@@ -1606,9 +1609,10 @@ extern "C" int fg_softmax_xent(const void* feat_dev, int64_t feat_ld, const void
   if (!loss_dev || !lse_dev || (((uintptr_t)loss_dev | (uintptr_t)lse_dev) & 3) != 0)
     return fail(FG_ERR_INVALID_ARGUMENT, "null loss or lse, or not aligned to float");
   const XentLayout l = xent_layout(dtype, n, vocab, feat_len, false);
-  if (!workspace_dev || ((uintptr_t)workspace_dev & 255) != 0 || workspace_bytes < (int64_t)l.total)
+  const int64_t need = (int64_t)(fits_map(dtype, weight_dev, weight_ld) ? l.total_in_place : l.total);
+  if (!workspace_dev || ((uintptr_t)workspace_dev & 255) != 0 || workspace_bytes < need)
     return fail(FG_ERR_INVALID_ARGUMENT, "the workspace needs %lld bytes at a 256-byte boundary",
-                (long long)l.total);
+                (long long)need);
   const size_t es = dtype_size(dtype);
   if (results_overlap({array1d(loss_dev, n, 4), array1d(lse_dev, n, 4)},
                       {{feat_dev, n, feat_len, feat_ld, es}, {weight_dev, vocab, feat_len, weight_ld, es},
@@ -1647,7 +1651,8 @@ extern "C" int fg_softmax_xent_grad(const float* loss_grad_dev, const void* feat
   if (n > 0) {
     if (!loss_grad_dev || !lse_dev || (((uintptr_t)loss_grad_dev | (uintptr_t)lse_dev) & 3) != 0)
       return fail(FG_ERR_INVALID_ARGUMENT, "null loss_grad or lse, or not aligned to float");
-    const int64_t need = fg_softmax_xent_workspace_bytes(dtype, n, vocab, feat_len, 1);
+    const int64_t need = fg_softmax_xent_workspace_bytes(
+        dtype, n, vocab, feat_len, 1 | (fits_map(dtype, weight_dev, weight_ld) ? FG_XENT_TABLE_IN_PLACE : 0));
     if (!workspace_dev || ((uintptr_t)workspace_dev & 255) != 0 || workspace_bytes < need)
       return fail(FG_ERR_INVALID_ARGUMENT, "the workspace needs %lld bytes at a 256-byte boundary",
                   (long long)need);

@@ -67,14 +67,16 @@ class _TrainingOp(object):
         self._owned, self._captured = [], False
         self._status = self._own(torch.zeros(1, dtype=torch.int32, device=self._device))
         self._allocate(out)
-        size = max(self._workspace_bytes(out), 16)
-        self._workspace = self._own(torch.empty(size, dtype=torch.uint8, device=self._device))
-        self._workspace_size = size
-        self._workspace_at = self._workspace.data_ptr()
+        self._take_workspace(self._workspace_bytes(out))
         self._status_at = self._status.data_ptr()
         self._last_stream = torch.cuda.current_stream(self._device)
         self._last_handle = self._last_stream.cuda_stream
         self._spec = out
+
+    def _take_workspace(self, size):
+        size = max(size, 16)
+        workspace = self._own(torch.empty(size, dtype=torch.uint8, device=self._device))
+        self._workspace_size, self._workspace_at = size, workspace.data_ptr()
 
     def _own(self, tensor):
         self._owned.append(tensor)
@@ -311,17 +313,26 @@ class SoftmaxCrossEntropycuda(_TrainingOp):
         self._lse = (out.shape, torch.float32, "Lse", False)
         a = out.attrs
         self._sizes = (out.shape[0], a["vocab"], a["feat_len"], a["scale"], a["ignore_index"])
+        self._has_room = feat.dtype == "float32" or a["feat_len"] % 8 != 0   # for a packed table
         self._loss_at, self._lse_at = self.out_tvm.torch.data_ptr(), self.lse_tvm.torch.data_ptr()
 
-    def _workspace_bytes(self, out):
+    def _workspace_bytes(self, out, in_place=None):
+        """``in_place``: for a table that needs no packed copy; by default, whether a contiguous
+        table of these sizes is one."""
+        if in_place is None:
+            in_place = out.inputs[1].dtype != "float32" and out.attrs["feat_len"] % 8 == 0
         return int(_lib.load().fg_softmax_xent_workspace_bytes(
             _lib.DTYPES.index(out.inputs[0].dtype), out.shape[0], out.attrs["vocab"],
-            out.attrs["feat_len"], out.attrs["with_grad"]))
+            out.attrs["feat_len"], out.attrs["with_grad"] + (2 if in_place else 0)))
 
     def _checked_inputs(self, inputs):
         e = self._inputs
-        return (self._rows(inputs[0], e[0]) + self._rows(inputs[1], e[1])
-                + (self._tensor(inputs[2], e[2]),))
+        weight, pitch = self._rows(inputs[1], e[1])
+        if (pitch & 7 or weight.data_ptr() & 15) and not self._has_room:
+            self._stream()                     # ordered behind the calls that use the smaller one
+            self._take_workspace(self._workspace_bytes(self._spec, in_place=False))
+            self._has_room = True
+        return self._rows(inputs[0], e[0]) + (weight, pitch, self._tensor(inputs[2], e[2]))
 
     def _launch(self, feat, feat_pitch, weight, weight_pitch, labels):
         n, vocab, feat_len, scale, ignore = self._sizes

@@ -499,3 +499,24 @@ def test_a_graph_outlives_the_build_that_it_was_captured_with(warm_up_there):
     assert all(torch.equal(a, b) for a, b in zip(want, outs))
     assert all(bool((x == 7).all()) for x in others)
     t.check(run(m, *small)["loss"], *t.xent_reference(*small[:3], 1.0, -100)["loss"], torch.float32)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_a_table_read_where_it_lies_takes_no_workspace(dtype):
+    n, v, d = 40, 5000, 64
+    base = torch.zeros((v + 1) * (d + 8), dtype=t.TYPES[dtype], device="cuda")
+    feat, weight, labels, dloss = t.xent_inputs(n, v, d, dtype, 8)
+    m = t.xent_module(feat, weight, labels)
+    assert m._workspace_size < weight.numel() * 2
+    want = [x.clone() for x in run(m, feat, weight, labels, dloss).values()]
+    odd = base[1:1 + v * d].view(v, d)                 # off the 16-byte boundaries
+    apart = base[:v * (d + 1)].view(v, d + 1)[:, :d]
+    for place in (odd, apart, weight):
+        if place is not weight:
+            place.copy_(weight)
+        got = list(run(m, feat, place, labels, dloss).values())
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+        assert m._workspace_size > weight.numel() * 2
+    assert m.device_status() == 0
+    floats = t.xent_module(feat.float(), weight.float(), labels)
+    assert floats._workspace_size > weight.numel() * 4

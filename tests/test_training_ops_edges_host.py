@@ -154,6 +154,31 @@ def test_a_gradient_of_rows_too_long_is_refused_before_any_launch(lib, n):
     refused(lib, lib.fg_embedding_grad(*args), 3, "too large")
 
 
+@pytest.mark.parametrize("with_grad", [0, 1])
+def test_a_table_in_place_needs_no_room_but_one_that_is_packed_does(lib, with_grad):
+    n, v, d = 5, 1000, 64
+    for dtype in (0, 1, 2):
+        full = lib.fg_softmax_xent_workspace_bytes(dtype, n, v, d, with_grad)
+        less = lib.fg_softmax_xent_workspace_bytes(dtype, n, v, d, with_grad + 2)
+        assert less == full if dtype == 0 else full - less >= v * d * 2
+    full = lib.fg_softmax_xent_workspace_bytes(1, n, v, d, with_grad)
+    less = lib.fg_softmax_xent_workspace_bytes(1, n, v, d, with_grad + 2)
+
+    def call(weight, ld, size):
+        if with_grad:
+            return lib.fg_softmax_xent_grad(at(BASE), at(BASE + 64), d, at(weight), ld, 1, at(BASE + 8192), 0,
+                                            n, v, d, 1.0, -100, at(BASE + 12288), at(FAR * 5), at(FAR * 6),
+                                            at(FAR * 3), size, at(FAR * 4), 99, None)
+        return lib.fg_softmax_xent(at(BASE + 64), d, at(weight), ld, 1, at(BASE + 8192), 0, n, v, d, 1.0,
+                                   -100, at(BASE + 12288), at(BASE + 16384), at(FAR * 3), size, at(FAR * 4),
+                                   99, None)
+    assert call(FAR, 64, less) == 2 and call(FAR, 72, less) == 2 and call(FAR + 2, 64, full) == 2
+    refused(lib, call(FAR, 64, less - 1), 1, "workspace")
+    for weight, ld in ((FAR + 2, 64), (FAR + 8, 64), (FAR, 65), (FAR, 68)):
+        refused(lib, call(weight, ld, less), 1, "workspace")
+        refused(lib, call(weight, ld, full - 1), 1, "workspace")
+
+
 # ------------------------------------------------------------------------ the command --
 @pytest.mark.parametrize("kernel", ["lookup", "lookup-grad", "cross-entropy", "clip", "train-step"])
 def test_the_command_refuses_an_empty_batch_and_a_graph_without_edges(kernel):
