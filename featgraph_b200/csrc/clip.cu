@@ -48,8 +48,8 @@ __device__ __forceinline__ int find_tensor(const Tensors& t, int chunk) {
   return lo;
 }
 
-// Calls each(value, k) over one chunk.  Squares are summed in groups of at most eight in fp32
-// and the groups in fp64; a group whose fp32 sum leaves the range in which fp32 squares are
+// Adds one group of values to a thread's part of the norm.  Squares are summed in groups of at most
+// eight in fp32 and the groups in fp64; a group whose fp32 sum leaves the range in which fp32 squares are
 // exact enough (overflow, or below 2^-100) is summed again in fp64.
 template <bool MAX_NORM, int N>
 __device__ __forceinline__ void add_group(const float (&x)[N], double& acc, float& top, bool& nan) {

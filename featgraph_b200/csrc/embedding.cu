@@ -27,7 +27,7 @@ __device__ __forceinline__ I load_id(const void* ids, int64_t i) {
 // its next rows on the way meanwhile.
 constexpr int kLookupThreads = 256;
 constexpr int kLookupRows = 4;
-constexpr int kLookupBlocks = 4;   // CTAs on an SM: 1M rows of 256 bytes 63 us; 8 rows and 2 CTAs 72
+constexpr int kLookupBlocks = 4;   // CTAs on an SM: 1M rows of 256 bytes 67 us; 8 rows and 2 CTAs took 14 % more
 
 template <typename T, int N, typename I>
 __global__ void __launch_bounds__(kLookupThreads, kLookupBlocks)
@@ -715,9 +715,9 @@ slice_kernel(KeySource src, int n, const T* __restrict__ out_grad, int64_t out_g
   const int c = ((int)blockIdx.y * lanes + lane) * N;
   const bool in = c < feat_len;
 
-  // Looks through the ids, kSliceThreads at a time, and notes which are this slice's: bit k of
-  // `is_mine` the thread's own of stretch k, hits[k] its warp's.  Every CTA begins with another
-  // stretch, so that they do not all ask for the same lines.
+  // Looks through the ids, kSliceThreads at a time, and notes which are this slice's: key[k] is
+  // the thread's id of stretch k, hits[k] which lanes of its warp have one of the slice's.  Every
+  // CTA begins with another stretch, so that they do not all ask for the same lines.
   const int stretches = (n + kSliceThreads - 1) / kSliceThreads;   // kSliceChunks at most
   const int rotate = (blockIdx.x + blockIdx.y) % stretches;
   uint32_t key[kSliceChunks], hits[kSliceChunks];

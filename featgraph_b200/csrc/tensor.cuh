@@ -180,10 +180,10 @@ __host__ __device__ constexpr uint32_t mma_desc(bool bf16, int n, bool negate_a,
          (b_mn_major ? 1u : 0u) << 16 | (uint32_t)(n >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
 }
 // One lane of the (converged) warp: 1 there, 0 elsewhere.  The instructions below take it as
-// a predicate instead of standing in a branch of one lane: in a converged warp the compiler
-// keeps descriptors and addresses in uniform registers, and issuing a tcgen05.mma costs about a
-// quarter of what it costs behind `if (lane == 0)` (measured: 90 cycles each, which bounded the
-// kernels of xent.cu at half of the tensor cores' rate).
+// a predicate instead of standing in a branch of one lane: behind `if (lane == 0)` issuing a
+// tcgen05.mma took 90 cycles, which bounded the kernels of xent.cu at half of the tensor cores' rate;
+// issued by a converged warp it does not bound them (4096 x 232 965 x 256 bfloat16, loss and both
+// gradients: 2448 -> 2002 us).
 __device__ __forceinline__ uint32_t elect_one() {
   uint32_t leader;
   asm volatile(

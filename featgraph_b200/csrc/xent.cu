@@ -59,7 +59,9 @@ __device__ __forceinline__ int32_t live_label(const Batch& b, int64_t t, int32_t
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
-__device__ __forceinline__ float exp2_fast(float x) {  // results below 2^-126 are 0
+// Off by 2^-22 of the result (a term of a sum of probabilities, or one that is rounded to 16 bits);
+// results below 2^-126 are 0.
+__device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
@@ -1168,7 +1170,8 @@ pack_kernel(Batch b, PackJob<T> first, PackJob<T> second, int64_t pitch, int wit
 }
 
 // loss and lse of a sample from its partial maxima and sums (base 2); the label's logit is
-// computed here once more, one warp a sample.
+// computed here once more, one warp a sample, so that 16-bit and float32 samples alike lose nothing
+// of it to tensor core sums.
 template <typename T>
 __global__ void __launch_bounds__(256)
 join_loss_kernel(Batch b, const T* __restrict__ feat, int64_t feat_ld, const T* __restrict__ weight,
@@ -1263,7 +1266,7 @@ constexpr int kLossGroups = MmaShape<kLoss, float, false>::kGroups;
 constexpr int kSms = 148;  // the grids below are sized for B200's 148 SMs, one CTA each
 
 // How often the streamed operand is cut so that row_tiles x splits CTAs fill the machine: the
-// count that ends first when every item costs its steps plus kItemSteps of start and end.
+// count that ends first when every item costs its steps plus `item_steps` of start and end.
 struct Cut {
   int splits, steps_per_split;
 };
@@ -1311,7 +1314,8 @@ XentLayout xent_layout(int32_t dtype, int64_t n, int64_t vocab, int64_t feat_len
   l.padded = l.t_tiles * kTileRows;
   l.out_cols = (int)((feat_len + 15) / 16 * 16);
   // 1024 steps of the 16-bit gradients are 8192 additions into the same accumulators, which
-  // cut (see kSegment): 1e-4, half a step of float16; the pieces are joined in fp32
+  // cut (see kSegment) by 2^-26 of the sum: 1.2e-4 at most, a quarter of float16's half step
+  // (2^-11 = 4.9e-4); the pieces are joined in fp32
   const int64_t most_steps = dtype == FG_FLOAT32 ? INT32_MAX : 1024;
   const int chunk_tiles = dtype == FG_FLOAT32 ? 2 : 4;
   const int64_t chunks = (l.kb + chunk_tiles - 1) / chunk_tiles;
