@@ -1144,7 +1144,10 @@ pack_kernel(Batch b, PackJob<T> first, PackJob<T> second, int64_t pitch, int wit
       odd = __any_sync(0xffffffffu, odd);
       const int e = row_exponent(top);
       f = ldexpf(1.f, e);
-      if (lane == 0) j.mul[r] = odd ? __int_as_float(0x7fc00000) : ldexpf(1.f, -e);
+      // a row of zeros adds nothing, and its scaling is the least of all, so that its probabilities
+      // do not set the exponents of the second products
+      const float undo = top > 0.f ? ldexpf(1.f, -e) : 0x1p-126f;
+      if (lane == 0) j.mul[r] = odd ? __int_as_float(0x7fc00000) : undo;
     }
     // two neighbouring elements a lane, so that the 16-bit pieces are written as 32 bits
 #pragma unroll 2

@@ -396,7 +396,7 @@ int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_t out_grad_
  *   lse[t] = log sum_v exp z[t, v],   loss[t] = lse[t] - z[t, labels[t]],
  * both fp32.  loss is 0 where labels[t] = ignore_index (lse is still that row's), NaN where
  * a label is out of range.  An infinite logit makes its row NaN, except -inf beside a
- * finite one.
+ * finite one; where all are -inf, lse is -inf and loss NaN.
  * float32 values are held relative to the largest finite magnitude of their own row of feat
  * or weight: each is off by at most 2^-22 of itself and 2^-37 of that magnitude.  Rows that
  * hold an infinity take no bits from others; a feat row with one gives that sample NaN. */

@@ -183,6 +183,20 @@ def test_float32_infinities_and_nan_stay_in_their_samples():
     assert got["lse"].isnan().all()
 
 
+@pytest.mark.parametrize("n, v, d", SIZES)
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -40])
+def test_float32_rows_of_zeros_take_nothing_from_the_others(n, v, d, size):
+    # vertices that nothing has trained yet, samples without neighbours: their probabilities are as
+    # large as any, and what they multiply is zero
+    feat, weight, labels, dloss = t.xent_inputs(n, v, d, "float32", n + d + 6)
+    weight[::3] = 0.0
+    weight[v - 1] = 0.0
+    feat[::4] = 0.0
+    labels[1], labels[4] = 3, v - 1                       # also as labels
+    check_rows(feat, weight * size, labels, dloss, scale=1.0 / size)
+    check_rows(feat * size, weight, labels, dloss, scale=1.0 / size)
+
+
 def test_float32_loss_gradients_of_any_size():
     # each sample's weight is its own: a large one takes nothing from the others' gradients
     feat, weight, labels, dloss = t.xent_inputs(200, 500, 64, "float32", 22)
@@ -520,3 +534,14 @@ def test_a_table_read_where_it_lies_takes_no_workspace(dtype):
     assert m.device_status() == 0
     floats = t.xent_module(feat.float(), weight.float(), labels)
     assert floats._workspace_size > weight.numel() * 4
+
+
+@pytest.mark.parametrize("dtype", sorted(t.TYPES))
+def test_a_sample_whose_logits_are_all_minus_infinity(dtype):
+    feat, weight, labels, dloss = t.xent_inputs(40, 300, 16, dtype, 9)
+    feat[:, 0] = 1.0
+    weight[:, 0] = -math.inf
+    got = run(t.xent_module(feat, weight, labels), feat, weight, labels, dloss)
+    dead = labels == -100
+    assert (got["lse"] == -math.inf).all()
+    assert got["loss"][~dead].isnan().all() and not got["loss"][dead].any()
