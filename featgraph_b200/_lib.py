@@ -46,6 +46,7 @@ MSG_OPS = ("mul", "add", "sub", "div", "copy_lhs", "copy_rhs")    # enum fg_msg_
 REDUCE_OPS = ("sum", "max", "min")                                # enum fg_reduce_op
 DTYPES = ("float32", "bfloat16", "float16")                       # enum fg_dtype
 INDEX_TYPES = ("int32", "int64")                                  # enum fg_index_type
+XENT_TABLE_IN_PLACE = 256          # added to with_grad of fg_softmax_xent_workspace_bytes
 OP_LOOKUP, OP_LOOKUP_GRAD, OP_XENT, OP_XENT_GRAD, OP_CLIP = range(5)   # enum fg_training_op
 
 

@@ -1598,7 +1598,7 @@ int grad_mma(const Batch& b, const XentLayout& l, char* ws, const float* loss_gr
 extern "C" int64_t fg_softmax_xent_workspace_bytes(int32_t dtype, int64_t n, int64_t vocab,
                                                    int64_t feat_len, int32_t with_grad) {
   if (n <= 0 || vocab < 1 || feat_len < 1) return 0;
-  const fg::XentLayout l = fg::xent_layout(dtype, n, vocab, feat_len, (with_grad & 1) != 0);
+  const fg::XentLayout l = fg::xent_layout(dtype, n, vocab, feat_len, (with_grad & ~FG_XENT_TABLE_IN_PLACE) != 0);
   return (int64_t)((with_grad & FG_XENT_TABLE_IN_PLACE) && dtype != FG_FLOAT32 ? l.total_in_place : l.total);
 }
 

@@ -323,7 +323,7 @@ class SoftmaxCrossEntropycuda(_TrainingOp):
             in_place = out.inputs[1].dtype != "float32" and out.attrs["feat_len"] % 8 == 0
         return int(_lib.load().fg_softmax_xent_workspace_bytes(
             _lib.DTYPES.index(out.inputs[0].dtype), out.shape[0], out.attrs["vocab"],
-            out.attrs["feat_len"], out.attrs["with_grad"] + (2 if in_place else 0)))
+            out.attrs["feat_len"], out.attrs["with_grad"] + (_lib.XENT_TABLE_IN_PLACE if in_place else 0)))
 
     def _checked_inputs(self, inputs):
         e = self._inputs

@@ -401,9 +401,9 @@ int fg_embedding_grad(const void* out_grad_dev, int32_t dtype, int64_t out_grad_
  * or weight: each is off by at most 2^-22 of itself and 2^-37 of that magnitude.  Rows that
  * hold an infinity take no bits from others; a feat row with one gives that sample NaN. */
 /* The workspace has room for a packed copy of weight, except with FG_XENT_TABLE_IN_PLACE added to
- * with_grad (0 or 1): for 16-bit tables whose rows start on 16-byte boundaries, which are read
+ * with_grad: for 16-bit tables whose rows start on 16-byte boundaries, which are read
  * where they lie. */
-enum { FG_XENT_TABLE_IN_PLACE = 2 };
+enum { FG_XENT_TABLE_IN_PLACE = 256 };
 int64_t fg_softmax_xent_workspace_bytes(int32_t dtype, int64_t n, int64_t vocab,
                                         int64_t feat_len, int32_t with_grad);
 int fg_softmax_xent(const void* feat_dev, int64_t feat_ld, const void* weight_dev,

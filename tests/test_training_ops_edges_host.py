@@ -159,10 +159,13 @@ def test_a_table_in_place_needs_no_room_but_one_that_is_packed_does(lib, with_gr
     n, v, d = 5, 1000, 64
     for dtype in (0, 1, 2):
         full = lib.fg_softmax_xent_workspace_bytes(dtype, n, v, d, with_grad)
-        less = lib.fg_softmax_xent_workspace_bytes(dtype, n, v, d, with_grad + 2)
+        less = lib.fg_softmax_xent_workspace_bytes(dtype, n, v, d, with_grad + _lib.XENT_TABLE_IN_PLACE)
         assert less == full if dtype == 0 else full - less >= v * d * 2
+        if with_grad:                                     # any other value but 0 asks for the gradients
+            for other in (2, 3, 255, -1 - _lib.XENT_TABLE_IN_PLACE):
+                assert lib.fg_softmax_xent_workspace_bytes(dtype, n, v, d, other) == full
     full = lib.fg_softmax_xent_workspace_bytes(1, n, v, d, with_grad)
-    less = lib.fg_softmax_xent_workspace_bytes(1, n, v, d, with_grad + 2)
+    less = lib.fg_softmax_xent_workspace_bytes(1, n, v, d, with_grad + _lib.XENT_TABLE_IN_PLACE)
 
     def call(weight, ld, size):
         if with_grad:
