@@ -117,7 +117,8 @@ struct MmaShape {
   // warps on every scheduler the exponentials' unit stays busy across the waits of each.  The
   // gradients' groups take turns with the steps: in 16 bits two that hold twice the registers, in
   // float32 two pairs of which each group has half a step's columns (one group a step: 402 us for
-  // both gradients of 2048 x 50 021 x 128, with 36 % of the issue slots used).
+  // both gradients of 2048 x 50 021 x 128 instead of 339: a warp waits for one entry's chain of
+  // loads, factors and exponentials after the other, and only more warps hide that).
   static constexpr int kGroups = MODE == kLoss || kSplit ? 4 : 2;
   static constexpr int kStepGroups = MODE == kLoss ? kGroups : kGroups / 2;  // those of one step
   static constexpr int kThreads = 32 * (kEpilogueWarp + 4 * kGroups);
