@@ -242,8 +242,8 @@ int run_clip(const ClipCall& call, cudaStream_t s) {
   return FG_OK;
 }
 
-// Whether an output shares memory with another output or with an input other than its own (which it
-// may be itself, but not in part).  `spans` has room for n_tensors.
+// Whether an output (the norm too) shares memory with another output or with an input other than its
+// own (which it may be itself, but not in part).  `spans` has room for n_tensors.
 struct Span {
   uint64_t begin, end;
   int32_t tensor;
@@ -258,9 +258,11 @@ bool outputs_overlap(const ClipCall& call, Span* spans) {
   std::sort(spans, spans + n, [](const Span& a, const Span& b) { return a.begin < b.begin; });
   for (int32_t i = 1; i < n; ++i)
     if (spans[i].begin < spans[i - 1].end) return true;
+  const uint64_t norm = (uint64_t)(uintptr_t)call.norm;
   for (int32_t k = 0; k < call.n_tensors; ++k) {
     const uint64_t bytes = (uint64_t)call.sizes[k] * dtype_size(call.dtypes[k]);
-    const uint64_t at = (uint64_t)(uintptr_t)call.grads[k];
+    const uint64_t at = (uint64_t)(uintptr_t)call.grads[k], out = (uint64_t)(uintptr_t)call.outs[k];
+    if (bytes > 0 && ((norm < at + bytes && at < norm + 4) || (norm < out + bytes && out < norm + 4))) return true;
     if (bytes == 0 || call.grads[k] == call.outs[k]) continue;
     // the first output that ends behind the input's begin
     const Span* hit = std::lower_bound(spans, spans + n, at, [](const Span& s, uint64_t v) { return s.end <= v; });

@@ -1664,13 +1664,13 @@ extern "C" int fg_softmax_xent_grad(const float* loss_grad_dev, const void* feat
     if (!workspace_dev || ((uintptr_t)workspace_dev & 255) != 0 || workspace_bytes < need)
       return fail(FG_ERR_INVALID_ARGUMENT, "the workspace needs %lld bytes at a 256-byte boundary",
                   (long long)need);
-    const size_t es = dtype_size(dtype);
-    if (results_overlap({{feat_grad_dev, n, feat_len, feat_len, es}, {weight_grad_dev, vocab, feat_len, feat_len, es}},
-                        {{feat_dev, n, feat_len, feat_ld, es}, {weight_dev, vocab, feat_len, weight_ld, es},
-                         array1d(labels_dev, n, index_type == FG_INDEX_INT64 ? 8 : 4),
-                         array1d(loss_grad_dev, n, 4), array1d(lse_dev, n, 4)}))
-      return fail(FG_ERR_INVALID_ARGUMENT, "a result shares memory with an input or the other one");
   }
+  const size_t es = dtype_size(dtype);
+  if (results_overlap({{feat_grad_dev, n, feat_len, feat_len, es}, {weight_grad_dev, vocab, feat_len, feat_len, es}},
+                      {{feat_dev, n, feat_len, feat_ld, es}, {weight_dev, vocab, feat_len, weight_ld, es},
+                       array1d(labels_dev, n, index_type == FG_INDEX_INT64 ? 8 : 4),
+                       array1d(loss_grad_dev, n, 4), array1d(lse_dev, n, 4)}))
+    return fail(FG_ERR_INVALID_ARGUMENT, "a result shares memory with an input or the other one");
   DeviceGuard guard(device);
   FG_CUDA_TRY(guard.status);
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -120,16 +120,19 @@ def test_a_cross_entropy_over_its_own_input_is_refused(lib):
             refused(lib, grad(**{out: good[inp] - 4 * (out == "dw")}), 1, "shares memory")
     refused(lib, grad(dh=good["dw"]), 1, "shares memory")
     assert grad(dl=good["lse"]) == 2                     # inputs may be one array
+    # without samples the table's gradient is still written: with zeros
+    refused(lib, lib.fg_softmax_xent_grad(None, None, d, at(BASE), d, 0, None, 1, 0, v, d, 1.0, -100, None,
+                                          None, at(BASE + 32), None, 0, None, 99, None), 1, "shares memory")
 
 
 @pytest.mark.parametrize("count", [3, 700])              # more than a launch's list too
 def test_clipping_over_another_tensor_is_refused(lib, count):
     need = lib.fg_gradient_clip_workspace_bytes(count)
 
-    def call(ins, outs, sizes):
+    def call(ins, outs, sizes, norm=FAR * 4):
         p = ctypes.c_void_p * count
         return lib.fg_gradient_clip(p(*ins), p(*outs), (ctypes.c_int64 * count)(*sizes),
-                                    (ctypes.c_int32 * count)(), count, 0, 1.0, 0.0, at(FAR * 4), at(FAR * 2),
+                                    (ctypes.c_int32 * count)(), count, 0, 1.0, 0.0, at(norm), at(FAR * 2),
                                     need, 99, None)
     ins = [BASE + 400 * k for k in range(count)]
     outs = [FAR + 400 * k for k in range(count)]
@@ -142,6 +145,9 @@ def test_clipping_over_another_tensor_is_refused(lib, count):
     refused(lib, call(ins, [ins[0] + 4] + outs[1:], sizes), 1, "shares memory")   # its own in part
     refused(lib, call([ins[1]] + ins[1:], [outs[0]] + ins[1:], sizes), 1, "shares memory")
     assert call([ins[0]] * count, outs, sizes) == 2                    # inputs may be one array
+    for norm in (ins[2], ins[2] + 396, outs[1], outs[count - 1] + 396):
+        refused(lib, call(ins, outs, sizes, norm), 1, "shares memory")
+    assert call(ins, outs, sizes, outs[count - 1] + 400) == 2 and call(ins, outs, sizes, BASE - 4) == 2
     assert call(ins, [outs[0]] * 2 + outs[2:], [100, 0] + sizes[2:]) == 2    # empty: nowhere
 
 
