@@ -187,12 +187,19 @@ __device__ __forceinline__ float2 logit_factors(float row, float col0, float col
 __device__ __forceinline__ float exponent_of(float power) {
   return power == power ? (float)((int)(__float_as_uint(power) >> 23) - 127) : 0.f;
 }
-// The product of two float32 rows of which one holds an infinity or a NaN.  In two pieces an
-// infinity would meet the zeros and the second pieces of the other row and become NaN.
-__device__ __noinline__ float plain_logit(const float* x, const float* y, int n) {
+// A row that holds an infinity or a NaN has a NaN for its factor, whose low bits say where: the first
+// column, and whether it is the only one.
+constexpr uint32_t kOddNan = 0x7fc00000u, kOddAlone = 1u << 20, kOddColumn = kOddAlone - 1;
+constexpr int64_t kMostFeatures = kOddAlone;   // of a row
+// The product of two float32 rows of which one holds an infinity or a NaN, `mark` its factor: what
+// is finite does not count.  In two pieces an infinity would meet the zeros and the second pieces of
+// the other row and become NaN.  (Not unrolled and not a call: registers are short where it stands.)
+__device__ __forceinline__ float plain_logit(const float* x, const float* y, float mark, int n) {
+  int c = __float_as_uint(mark) & kOddColumn;
+  if (__float_as_uint(mark) & kOddAlone) n = c + 1;
   float z = 0.f;
-#pragma unroll 8
-  for (int c = 0; c < n; ++c) z = fmaf(__ldg(x + c), __ldg(y + c), z);
+#pragma unroll 1
+  do z = fmaf(__ldg(x + c), __ldg(y + c), z); while (++c < n && z == z);
   return z;
 }
 
@@ -597,8 +604,10 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
                   for (uint32_t which = odd[c]; which; which &= which - 1) {
                     const int from = __ffs(which) - 1;
                     const int64_t col = (int64_t)(item.first + j) * Shape::kCols + group * kMine + c * 32 + from;
-                    float z = row < a.n_rows ? plain_logit(a.row_src + row * a.row_src_ld,
-                                                           a.col_src + col * a.col_src_ld, a.feat_len) : 0.f;
+                    float z = 0.f;
+                    if (row < a.n_rows)
+                      z = plain_logit(a.row_src + row * a.row_src_ld, a.col_src + col * a.col_src_ld,
+                                      my_cols[c * 32 + from], a.feat_len);
                     if (a.negate) z = -z;
 #pragma unroll
                     for (int k = 0; k < 32; ++k)
@@ -797,8 +806,8 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
               const bool mine = row < a.n_rows && (MODE == kFeatGrad || row_odd);
               float z = 0.f;
               if (mine && my_biases[c * 16 + from] != -INFINITY)
-                z = plain_logit(a.row_src + row * a.row_src_ld,
-                                a.col_src + (col0 + c * 16 + from) * a.col_src_ld, a.feat_len);
+                z = plain_logit(a.row_src + row * a.row_src_ld, a.col_src + (col0 + c * 16 + from) * a.col_src_ld,
+                                MODE == kFeatGrad ? my_cols[c * 16 + from] : a.row_mul[row], a.feat_len);
               if (a.negate) z = -z;
 #pragma unroll
               for (int k = 0; k < 16; ++k)
@@ -1142,13 +1151,24 @@ pack_kernel(Batch b, PackJob<T> first, PackJob<T> second, int64_t pitch, int wit
         }
       }
       for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      odd = __any_sync(0xffffffffu, odd);
+      uint32_t mark = 0;                 // of a row with an infinity or a NaN
+      if (__any_sync(0xffffffffu, odd)) {
+        uint32_t first = kOddColumn, count = 0;
+        for (int64_t c = lane; c < b.feat_len; c += 32)
+          if (!(fabsf(j.from[r * j.ld + c]) < INFINITY)) {
+            first = min(first, (uint32_t)c);
+            ++count;
+          }
+        first = __reduce_min_sync(0xffffffffu, first);
+        count = __reduce_add_sync(0xffffffffu, count);
+        mark = kOddNan | first | (count == 1 ? kOddAlone : 0);
+      }
       const int e = row_exponent(top);
       f = ldexpf(1.f, e);
       // a row of zeros adds nothing, and its scaling is the least of all, so that its probabilities
       // do not set the exponents of the second products
       const float undo = top > 0.f ? ldexpf(1.f, -e) : 0x1p-126f;
-      if (lane == 0) j.mul[r] = odd ? __int_as_float(0x7fc00000) : undo;
+      if (lane == 0) j.mul[r] = mark ? __uint_as_float(mark) : undo;
     }
     // two neighbouring elements a lane, so that the 16-bit pieces are written as 32 bits
 #pragma unroll 2
@@ -1370,7 +1390,7 @@ int check_xent(const void* feat, const void* weight, int32_t dtype, int64_t feat
                 "bad shape: n=%lld vocab=%lld feat_len=%lld feat_ld=%lld weight_ld=%lld",
                 (long long)n, (long long)vocab, (long long)feat_len, (long long)feat_ld,
                 (long long)weight_ld);
-  if (n >= INT32_MAX / 2 || vocab >= INT32_MAX / 2 || feat_len > (1 << 20))
+  if (n >= INT32_MAX / 2 || vocab >= INT32_MAX / 2 || feat_len > kMostFeatures)
     return fail(FG_ERR_UNSUPPORTED, "n and vocab must be below 2^30, feat_len at most 2^20");
   if (!weight || (n > 0 && (!feat || !labels || !status)))
     return fail(FG_ERR_INVALID_ARGUMENT, "null pointer");

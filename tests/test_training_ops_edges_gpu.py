@@ -163,6 +163,32 @@ def test_float32_minus_infinity_in_table_rows(n, v, d, scale):
     assert got["feat_grad"][~dead][:, [0, 2]].isnan().all() and not got["feat_grad"][dead].any()
 
 
+@pytest.mark.parametrize("n, v, d", [(200, 900, 128), (70, 600, 260), (9, 300, 1)])
+@pytest.mark.parametrize("share", [0.1, 0.9])
+def test_float32_many_masked_vertices(n, v, d, share):
+    # candidates left out by one column, the last or another, or by a whole row
+    feat, weight, labels, dloss = t.xent_inputs(n, v, d, "float32", n + d + 7)
+    feat = feat.abs() + 0.1
+    g = t.gen(5)
+    gone = torch.rand(v, generator=g, device="cuda") < share
+    gone[0] = False
+    at = torch.randint(d, (v,), generator=g, device="cuda")
+    at[::3] = d - 1
+    whole = torch.rand(v, generator=g, device="cuda") < 0.2
+    labels = torch.where((labels >= 0) & gone[labels.clamp(min=0)], 0, labels)
+    kept = (~gone).nonzero()[:, 0]
+    place = torch.zeros(v, dtype=torch.int64, device="cuda")
+    place[kept] = torch.arange(len(kept), device="cuda")
+    want = by_rows(feat, weight[kept], torch.where(labels == -100, labels, place[labels.clamp(min=0)]), dloss)
+    weight[gone, at[gone]] = -math.inf
+    weight[gone & whole] = -math.inf
+    got = run(t.xent_module(feat, weight, labels), feat, weight, labels, dloss)
+    for key in ("loss", "lse"):
+        t.check(got[key], *want[key], torch.float32)
+    t.check(got["weight_grad"][kept], *want["weight_grad"], torch.float32)
+    assert not got["weight_grad"][gone].any()
+
+
 def test_float32_infinities_and_nan_stay_in_their_samples():
     # a sample with an infinity or a NaN is NaN itself; a NaN in the table is everybody's
     feat, weight, labels, dloss = t.xent_inputs(140, 300, 72, "float32", 21)
