@@ -19,10 +19,10 @@
 //
 // float32 runs as two fp16 pieces and three products.  Every row of either operand is scaled by a
 // power of two of its own, so that a masked, an infinite or a large row costs the others no bits
-// (2048 x 50 021 x 128: loss 80 us, gradients 339; with one scale per operand 74 and 278).
+// (2048 x 50 021 x 128: loss 81 us, gradients 325; with one scale per operand 74 and 278).
 //
-// 4096 samples x 232 965 vertices x 256, bfloat16, on one B200: loss 411 us (1190 TFLOP/s; 290 us
-// at the GEMM peak), loss and both gradients 1955 us (1250 TFLOP/s over the five products).  The
+// 4096 samples x 232 965 vertices x 256, bfloat16, on one B200: loss 416 us (1170 TFLOP/s; 290 us
+// at the GEMM peak), loss and both gradients 2000 us (1220 TFLOP/s over the five products).  The
 // loss is bound by products and exponentials alike (both units 63 % busy), the gradients by the
 // products; the operands are read from DRAM once.
 #include <algorithm>
@@ -925,20 +925,17 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
           if ((step & 1) != group) continue;
           const int64_t col0 = (int64_t)(item.first + j) * Shape::kCols;
           // weight_grad: lane c holds columns c, 32 + c, ... of the step; in `hits` those whose
-          // label is one of this warp's rows, in `negative` those of a negative weight, in `none`
-          // those that take no part: zeros, which meet an infinity of this lane's row as NaN
+          // label is one of this warp's rows, in `negative` those of a negative weight
           int32_t col_label[4];
           float col_weight[4];
-          uint32_t hits[4] = {0, 0, 0, 0}, negative[4] = {0, 0, 0, 0}, none[4] = {0, 0, 0, 0};
+          uint32_t hits[4] = {0, 0, 0, 0}, negative[4] = {0, 0, 0, 0};
           if (MODE == kWeightGrad) {
             __syncwarp();
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               col_label[c] = a.col_label[col0 + c * 32 + lane];
               col_weight[c] = a.col_weight[col0 + c * 32 + lane];
-              const float col_bias = a.col_bias[col0 + c * 32 + lane];
-              my_biases[c * 32 + lane] = col_bias;
-              none[c] = __ballot_sync(0xffffffffu, col_bias == -INFINITY);
+              my_biases[c * 32 + lane] = a.col_bias[col0 + c * 32 + lane];
             }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -983,10 +980,10 @@ xent_mma_kernel(const __grid_constant__ CUtensorMap row_map,
                 v[k + 2] = exp2_fast(fmaf(v[k + 2], scale, e.z));
                 v[k + 3] = exp2_fast(fmaf(v[k + 3], scale, e.w));
               }
-              if (not_finite && none[c]) {
+              if (not_finite) {  // samples that take no part are zeros, which meet an infinity as NaN
 #pragma unroll
                 for (int k = 0; k < 32; ++k)
-                  if (none[c] >> k & 1) v[k] = 0.f;
+                  if (my_biases[c * 32 + k] == -INFINITY) v[k] = 0.f;
               }
               if (negative[c]) {
 #pragma unroll
